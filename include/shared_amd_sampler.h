@@ -440,6 +440,121 @@ int sas_lm_head_sample(sas_sampler *s, const sas_lm_head *head, const sas_rows *
 int sas_lm_head_sample_step(sas_sampler *s, const sas_lm_head *head, const sas_rows *rows, const sas_step *step,
                             void *stream);
 
+/* ---- a shared projection with the low-rank adapters of many requests ----
+ *
+ * y[r] = cap(W x[r] + scale[a] * B[a] (A[a] x[r])), a = row_adapter[r], for
+ * any number of rows: a batch's decode head (the framework's fused head above
+ * takes up to 4 rows and no adapters) or another projection of the model.
+ * Rows whose row_adapter lies outside [0, adapters) have no adapter's term.
+ * Adapter a uses the first ranks[a] of its `rank` rows of A and columns of B;
+ * what lies behind them is never used, whatever it holds.  Products and sums
+ * are f32: bf16 products are exact in f32, f32 hidden states and the inner
+ * products A x (scaled) are carried as three bf16 pieces, 24 bits in all.
+ * A value that is not finite stays in its own row, weight row or adapter.
+ * cap(y) = softcap * tanh(y / softcap) in f32 when softcap > 0.
+ * No counterpart in the reference, whose head is one row's
+ * (lib/webgpu-llm/model.js:466-471). */
+#define SAS_TYPE_F32 0
+#define SAS_TYPE_BF16 1
+#define SAS_TYPE_F16 2
+/* Largest rank of an adapter pool. */
+#define SAS_MAX_RANK 256
+/* Largest number of rows of one sas_project call. */
+#define SAS_MAX_PROJECT_ROWS (1 << 19)
+
+typedef struct sas_projection {
+  const void *x;              /* device [rows][x_stride]: hidden states, 16-byte aligned */
+  int64_t x_stride;           /* elements between rows: >= dim, a multiple of 8 (f32: of 4) */
+  int32_t x_type;             /* SAS_TYPE_F32 or SAS_TYPE_BF16 */
+  int32_t rows;               /* >= 0 */
+  const void *weight;         /* device bf16 [out_dim][weight_stride], 16-byte aligned; NULL:
+                                 the adapters' terms alone (accumulate must be set) */
+  int64_t weight_stride;      /* elements: >= dim, a multiple of 8 */
+  int32_t dim;                /* a positive multiple of 8 */
+  int32_t out_dim;            /* >= 1 */
+  int32_t adapters;           /* adapters in the pool, 0: none (the fields below are unused) */
+  int32_t rank;               /* a multiple of 8 in [8, SAS_MAX_RANK] */
+  const void *a;              /* device bf16 [adapters][a_adapter_stride], rows of a_stride */
+  int64_t a_stride;           /* elements between A's rows: >= dim, a multiple of 8 */
+  int64_t a_adapter_stride;   /* elements between adapters: a multiple of 8 */
+  const void *b;              /* device bf16 [adapters][b_adapter_stride], rows of b_stride */
+  int64_t b_stride;           /* elements between B's rows: >= rank, a multiple of 8 */
+  int64_t b_adapter_stride;   /* elements between adapters: a multiple of 8 */
+  const float *scales;        /* device [adapters] or NULL (1) */
+  const int32_t *ranks;       /* device [adapters] or NULL (rank); clamped to [0, rank] */
+  const int32_t *row_adapter; /* device [rows] (required with adapters) */
+  void *out;                  /* device [rows][out_stride], aligned to its elements */
+  int64_t out_stride;         /* elements: >= out_dim */
+  int32_t out_type;           /* SAS_TYPE_F32 or SAS_TYPE_BF16 (rounded once, to nearest even) */
+  int32_t accumulate;         /* nonzero: y is added to what out holds (before the cap) */
+  float softcap;              /* 0 = off */
+} sas_projection;
+
+/* Stream-ordered on `stream`; no host synchronisation.  out must not overlap
+ * an input. */
+int sas_project(sas_sampler *s, const sas_projection *p, void *stream);
+
+/* Pre-size the handle's scratch for sas_project calls of at most these rows,
+ * dim and rank (rank 0: without adapters), so that they allocate nothing and
+ * can be captured into a HIP graph. */
+int sas_reserve_project(sas_sampler *s, int32_t rows, int32_t dim, int32_t rank);
+
+/* ---- sampling over the whole vocabulary: top-k, top-p, min-p ----
+ *
+ * Per row, v = the logit as f32, then sas_params' softcap (f32) and history
+ * penalties (in double, rounded once to f32).  Ids that the mask leaves out,
+ * NaN and -inf are no candidates.  With m the largest v, a candidate's mass
+ * is w = exp((v - m) / temperature) (1 where v = m, +inf included).  The
+ * candidates in the order (v descending, id ascending) are cut to
+ *   the first top_k (top_k <= 0: all),
+ *   the fewest of those, from the first on, whose mass is at least top_p of
+ *     theirs (top_p >= 1 or NaN: all; at least one),
+ *   those whose w is at least min_p (min_p <= 0 or NaN: all; min_p > 1 is 1),
+ * and the token is the first kept id, in ascending order, whose running mass
+ * exceeds U times the kept mass.  temperature <= 0 (or NaN) keeps the first
+ * candidate alone.  Masses are summed as integers of 2^-s, s = 62 -
+ * ceil(log2 vocab), so no sum depends on its order; an id whose mass is below
+ * half of 2^-s is not drawn.  The reference's sample()
+ * cuts to top_k <= 128 first and has no min-p (tokenizer.js:151-178). */
+typedef struct sas_filter_params {
+  double temperature;
+  double top_p;              /* 1 = off */
+  double min_p;              /* 0 = off */
+  double repetition_penalty; /* 1 = off; the penalties are sas_params' */
+  double presence_penalty;   /* 0 = off */
+  double frequency_penalty;  /* 0 = off */
+  float softcap;             /* 0 = off */
+  int32_t top_k;             /* 0 = off; any size */
+} sas_filter_params;
+
+typedef struct sas_filter_rows {
+  const void *logits;          /* device [rows][logits_stride], aligned to its elements */
+  int64_t logits_stride;       /* elements between rows, >= vocab */
+  int32_t logits_type;         /* SAS_TYPE_* */
+  int32_t vocab;               /* 1..SAS_MAX_VOCAB */
+  int32_t rows;                /* >= 0 */
+  const uint32_t *mask;        /* as in sas_rows */
+  int64_t mask_stride;
+  const uint32_t *hist_ids;    /* as in sas_rows */
+  const int32_t *hist_offsets;
+  int64_t hist_count;
+  const double *uniforms;      /* device [rows], U in [0, 1); may be NULL when every row is greedy */
+  sas_filter_params params;    /* used for every row unless row_params is set */
+  const sas_filter_params *row_params; /* device [rows] or NULL */
+  uint32_t *out_ids;           /* device [rows]: SAS_NO_TOKEN without a candidate */
+  double *out_probs;           /* device [rows] or NULL: the token's share of the kept mass
+                                  (0 without a candidate) */
+  int32_t *out_counts;         /* device [rows] or NULL: how many ids were kept */
+  uint32_t *out_flags;         /* device [rows] or NULL: SAS_FLAG_EMPTY_ROW */
+} sas_filter_rows;
+
+/* Samples one token per row, stream-ordered like sas_sample. */
+int sas_sample_filtered(sas_sampler *s, const sas_filter_rows *rows, void *stream);
+
+/* Pre-size the handle's scratch for sas_sample_filtered calls of at most
+ * these rows and this vocabulary. */
+int sas_reserve_filtered(sas_sampler *s, int32_t rows, int32_t vocab);
+
 /* Host: clamp parameters with the reference packer's rules
  * (model.js:418-423): non-finite or negative temperature -> 0 (greedy),
  * top_p -> [0, 1] (non-finite -> 1), presence -> [0, 10] (non-finite -> 0),

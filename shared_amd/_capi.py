@@ -41,6 +41,9 @@ FLAG_EMPTY_ROW, FLAG_TOPP_EDGE, FLAG_DRAW_EDGE, FLAG_SLOW_SELECT = 1, 2, 4, 8
 HINT_NO_SOFTCAP = 1
 HEAD_BF16, HEAD_Q8_0, HEAD_Q4_0, HEAD_Q6_K = 0, 1, 2, 3
 MASK_ALL, MASK_ALLOW, MASK_DENY = 0, 1, 2
+TYPE_F32, TYPE_BF16, TYPE_F16 = 0, 1, 2
+MAX_RANK = _header_define("SAS_MAX_RANK")
+MAX_PROJECT_ROWS = _header_define("SAS_MAX_PROJECT_ROWS")
 
 
 class SasParams(ctypes.Structure):
@@ -169,6 +172,70 @@ class SasLmHead(ctypes.Structure):
     ]
 
 
+class SasProjection(ctypes.Structure):
+    _fields_ = [
+        ("x", c_void_p),
+        ("x_stride", c_int64),
+        ("x_type", c_int32),
+        ("rows", c_int32),
+        ("weight", c_void_p),
+        ("weight_stride", c_int64),
+        ("dim", c_int32),
+        ("out_dim", c_int32),
+        ("adapters", c_int32),
+        ("rank", c_int32),
+        ("a", c_void_p),
+        ("a_stride", c_int64),
+        ("a_adapter_stride", c_int64),
+        ("b", c_void_p),
+        ("b_stride", c_int64),
+        ("b_adapter_stride", c_int64),
+        ("scales", c_void_p),
+        ("ranks", c_void_p),
+        ("row_adapter", c_void_p),
+        ("out", c_void_p),
+        ("out_stride", c_int64),
+        ("out_type", c_int32),
+        ("accumulate", c_int32),
+        ("softcap", c_float),
+    ]
+
+
+class SasFilterParams(ctypes.Structure):
+    _fields_ = [
+        ("temperature", c_double),
+        ("top_p", c_double),
+        ("min_p", c_double),
+        ("repetition_penalty", c_double),
+        ("presence_penalty", c_double),
+        ("frequency_penalty", c_double),
+        ("softcap", c_float),
+        ("top_k", c_int32),
+    ]
+
+
+class SasFilterRows(ctypes.Structure):
+    _fields_ = [
+        ("logits", c_void_p),
+        ("logits_stride", c_int64),
+        ("logits_type", c_int32),
+        ("vocab", c_int32),
+        ("rows", c_int32),
+        ("mask", c_void_p),
+        ("mask_stride", c_int64),
+        ("hist_ids", c_void_p),
+        ("hist_offsets", c_void_p),
+        ("hist_count", c_int64),
+        ("uniforms", c_void_p),
+        ("params", SasFilterParams),
+        ("row_params", c_void_p),
+        ("out_ids", c_void_p),
+        ("out_probs", c_void_p),
+        ("out_counts", c_void_p),
+        ("out_flags", c_void_p),
+    ]
+
+
 # name -> (restype, argtypes); every function declared in the header.
 SIGNATURES = {
     "sas_version": (c_char_p, []),
@@ -185,6 +252,10 @@ SIGNATURES = {
     "sas_spec_step": (c_int, [c_void_p, POINTER(SasSpecRows), POINTER(SasSpecState), c_void_p]),
     "sas_lm_head_sample": (c_int, [c_void_p, POINTER(SasLmHead), POINTER(SasRows), c_void_p]),
     "sas_lm_head_sample_step": (c_int, [c_void_p, POINTER(SasLmHead), POINTER(SasRows), POINTER(SasStep), c_void_p]),
+    "sas_project": (c_int, [c_void_p, POINTER(SasProjection), c_void_p]),
+    "sas_reserve_project": (c_int, [c_void_p, c_int32, c_int32, c_int32]),
+    "sas_sample_filtered": (c_int, [c_void_p, POINTER(SasFilterRows), c_void_p]),
+    "sas_reserve_filtered": (c_int, [c_void_p, c_int32, c_int32]),
     "sas_clamp_params": (c_int, [POINTER(SasParams), POINTER(SasParams)]),
     "sas_mask_from_ids": (c_int64, [c_int32, POINTER(c_uint32), c_size_t, c_int32, POINTER(c_uint32), c_int64]),
     "sas_pcg_uniform": (c_double, [c_uint32, c_uint32, c_uint32]),

@@ -190,4 +190,65 @@ size_t verify_scratch_bytes(int seqs, int L, int vocab);
 // The three verify launches, in stream order on `stream`.
 hipError_t launch_verify(const VerifyArgs &a, hipStream_t stream);
 
+// --------------------------------------------------------------- project --
+struct ProjArgs {
+  const void *x;
+  int64_t x_stride;
+  const void *weight;
+  int64_t weight_stride;
+  const void *a;
+  int64_t a_stride;
+  int64_t a_adapter_stride;
+  const void *b;
+  int64_t b_stride;
+  int64_t b_adapter_stride;
+  const float *scales;
+  const int32_t *ranks;
+  const int32_t *row_adapter;
+  void *out;
+  int64_t out_stride;
+  // Scratch: the rows' inner products h as pieces, bf16 [rows][3][rank] (rows
+  // without an adapter unwritten), and the hidden states' pieces, bf16
+  // [3][rows][dim] (null: bf16 hidden states, or no weight).
+  uint16_t *hp;
+  uint16_t *xp;
+  int32_t rows;
+  int32_t dim;
+  int32_t out_dim;
+  int32_t adapters;
+  int32_t rank;
+  float softcap;
+  bool x_f32;
+  bool out_bf16;
+  bool accumulate;
+  int32_t cus;
+};
+
+size_t proj_scratch_bytes(int rows, int dim, int rank, bool x_f32);
+hipError_t launch_project(const ProjArgs &a, hipStream_t stream);
+
+// ---------------------------------------------------------------- filter --
+struct FilterArgs {
+  const void *logits;
+  int64_t logits_stride;
+  const uint32_t *mask;
+  int64_t mask_stride;
+  const uint32_t *hist_ids;
+  const int32_t *hist_offsets;
+  int64_t hist_count;
+  const double *uniforms;
+  const sas_filter_params *row_params;
+  sas_filter_params params;
+  uint32_t *out_ids;
+  double *out_probs;
+  int32_t *out_counts;
+  uint32_t *out_flags;
+  int32_t type;   // SAS_TYPE_*
+  int32_t vocab;
+  int32_t rows;
+  int32_t shift;  // masses are integers of 2^-shift
+};
+
+hipError_t launch_filter(const FilterArgs &a, hipStream_t stream);
+
 }  // namespace sas

@@ -13,7 +13,8 @@ from typing import Optional, Sequence
 import numpy as np
 
 from . import _capi
-from ._capi import SasLmHead, SasParams, SasRows, SasSpecRows, SasVerifyRows, check, load
+from ._capi import (SasFilterParams, SasFilterRows, SasLmHead, SasParams, SasProjection, SasRows, SasSpecRows,
+                    SasVerifyRows, check, load)
 
 
 @dataclass
@@ -37,6 +38,62 @@ class Params:
         return {"temperature": self.temperature, "top_k": self.top_k, "top_p": self.top_p,
                 "repetition_penalty": self.repetition_penalty, "presence_penalty": self.presence_penalty,
                 "frequency_penalty": self.frequency_penalty, "softcap": self.softcap}
+
+
+@dataclass
+class FilterParams:
+    """One row's parameters of sample_filtered (sas_filter_params)."""
+
+    temperature: float = 0.0
+    top_p: float = 1.0
+    min_p: float = 0.0
+    repetition_penalty: float = 1.0
+    presence_penalty: float = 0.0
+    frequency_penalty: float = 0.0
+    softcap: float = 0.0
+    top_k: int = 0
+
+    def to_c(self) -> SasFilterParams:
+        return SasFilterParams(float(self.temperature), float(self.top_p), float(self.min_p),
+                               float(self.repetition_penalty), float(self.presence_penalty),
+                               float(self.frequency_penalty), float(self.softcap), int(self.top_k))
+
+
+FILTER_PARAMS_DTYPE = np.dtype([("temperature", "<f8"), ("top_p", "<f8"), ("min_p", "<f8"),
+                                ("repetition_penalty", "<f8"), ("presence_penalty", "<f8"),
+                                ("frequency_penalty", "<f8"), ("softcap", "<f4"), ("top_k", "<i4")])
+assert FILTER_PARAMS_DTYPE.itemsize == ctypes.sizeof(SasFilterParams)
+
+
+def pack_filter_params(rows: Sequence[FilterParams]) -> np.ndarray:
+    """Array of sas_filter_params (for sample_filtered's row_params)."""
+    out = np.zeros(len(rows), dtype=FILTER_PARAMS_DTYPE)
+    for i, p in enumerate(rows):
+        out[i] = (p.temperature, p.top_p, p.min_p, p.repetition_penalty, p.presence_penalty, p.frequency_penalty,
+                  p.softcap, p.top_k)
+    return out
+
+
+class Adapters:
+    """A pool of low-rank adapters for Sampler.project: a [n][rank][dim] and
+    b [n][out][rank] bf16 device tensors with unit element stride, and
+    optionally a scale (float32) and a used rank (int32) per adapter."""
+
+    def __init__(self, a, b, *, scales=None, ranks=None):
+        for name, t in (("a", a), ("b", b)):
+            if t.dim() != 3 or str(t.dtype) != "torch.bfloat16" or t.stride(2) != 1 or not t.is_cuda:
+                raise ValueError(f"{name} must be a 3-D bf16 device tensor with unit element stride")
+        if a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2]:
+            raise ValueError("a must be [n][rank][dim] and b [n][out][rank]")
+        n = a.shape[0]
+        for name, t in (("scales", scales), ("ranks", ranks)):
+            if t is not None and (t.dim() != 1 or t.shape[0] != n):
+                raise ValueError(f"{name} must hold one value per adapter")
+        self.a, self.b, self.scales, self.ranks = a, b, scales, ranks
+        self._scales, self._ranks = _ptr(scales, "f32", "scales"), _ptr(ranks, "i32", "ranks")
+
+    def __len__(self) -> int:
+        return self.a.shape[0]
 
 
 PARAMS_DTYPE = np.dtype([("temperature", "<f8"), ("top_p", "<f8"), ("repetition_penalty", "<f8"),
@@ -146,6 +203,26 @@ def _stream(stream):
             _current_stream = _find_current_stream()
         return ctypes.c_void_p(_current_stream())
     return ctypes.c_void_p(stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream))
+
+
+class _NoStream:
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_no_stream = _NoStream()
+
+
+def _on(stream):
+    """A context in which torch's allocations belong to `stream` (None: the
+    current one), so that their memory is not reused while it still runs."""
+    if stream is None:
+        return _no_stream
+    import torch
+    return torch.cuda.stream(stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(int(stream)))
 
 
 def rows_descriptor(logits, out_ids, *, vocab: Optional[int] = None, mask=None, hist_ids=None, hist_offsets=None,
@@ -417,6 +494,121 @@ class Sampler:
                                  out_probs=out.get("probs"), out_cand_ids=out.get("cand_ids"),
                                  out_counts=out.get("counts"), out_flags=out.get("flags"), **kw)
         return out if (full or logits) else out["ids"]
+
+    def project_into(self, x, weight, out, *, adapters: Optional[Adapters] = None, row_adapter=None,
+                     softcap: float = 0.0, accumulate: bool = False, stream=None) -> None:
+        """sas_project on caller-provided device buffers: out [rows][out]
+        (float32 or bfloat16) = x [rows][dim] (float32 or bfloat16) times
+        weight [out][dim] (bfloat16), plus each row's adapter's term, capped.
+        weight None: the adapters' terms alone, added to out (accumulate)."""
+        types = {"torch.float32": _capi.TYPE_F32, "torch.bfloat16": _capi.TYPE_BF16}
+        for name, t in (("x", x), ("weight", weight), ("out", out)):
+            if t is None and name == "weight":
+                continue
+            if t.dim() != 2 or t.stride(1) != 1 or not t.is_cuda:
+                raise ValueError(f"{name} must be a 2-D device tensor with unit element stride")
+            if str(t.dtype) not in types or (name == "weight" and t.dtype.itemsize != 2):
+                raise ValueError(f"{name} must hold {'bfloat16' if name == 'weight' else 'float32 or bfloat16'} elements")
+        rows, dim = x.shape
+        if out.shape[0] != rows or (weight is not None and tuple(weight.shape) != (out.shape[1], dim)):
+            raise ValueError("x [rows][dim], weight [out][dim] and out [rows][out] do not fit together")
+        d = SasProjection()
+        # (a tensor of one row may have any stride; its row is the whole of it)
+        d.x, d.x_stride, d.x_type = x.data_ptr(), x.stride(0) if rows > 1 else (dim + 7) // 8 * 8, types[str(x.dtype)]
+        d.rows, d.dim, d.out_dim = rows, dim, out.shape[1]
+        if weight is not None:
+            d.weight = weight.data_ptr()
+            d.weight_stride = weight.stride(0) if out.shape[1] > 1 else (dim + 7) // 8 * 8
+        if adapters is not None and len(adapters):
+            a, b = adapters.a, adapters.b
+            if a.shape[2] != dim or b.shape[1] != out.shape[1]:
+                raise ValueError("the adapters' dim or out differ from the projection's")
+            if row_adapter is None or row_adapter.dim() != 1 or row_adapter.shape[0] != rows:
+                raise ValueError("row_adapter must hold one adapter per row (-1: none)")
+            d.adapters, d.rank = len(adapters), a.shape[1]
+            d.a, d.a_stride, d.a_adapter_stride = a.data_ptr(), a.stride(1), a.stride(0)
+            d.b, d.b_stride, d.b_adapter_stride = b.data_ptr(), b.stride(1), b.stride(0)
+            d.scales, d.ranks = adapters._scales, adapters._ranks
+            d.row_adapter = _ptr(row_adapter, "i32", "row_adapter")
+        d.out, d.out_type = out.data_ptr(), types[str(out.dtype)]
+        d.out_stride = out.stride(0) if rows > 1 else out.shape[1]
+        d.softcap = float(softcap)
+        d.accumulate = 1 if accumulate else 0
+        check(self._lib.sas_project(self._h, ctypes.byref(d), _stream(stream)), self._h)
+
+    def project(self, x, weight, *, out_dtype=None, stream=None, **kw):
+        """Allocate out (float32 unless out_dtype is torch.bfloat16) and run
+        project_into; returns it."""
+        import torch
+        with _on(stream):
+            out = torch.empty((x.shape[0], weight.shape[0]), dtype=out_dtype or torch.float32, device=x.device)
+        self.project_into(x, weight, out, stream=stream, **kw)
+        return out
+
+    def reserve_project(self, rows: int, dim: int, *, rank: int = 0) -> None:
+        """Pre-size the scratch of project calls of at most these shapes."""
+        check(self._lib.sas_reserve_project(self._h, int(rows), int(dim), int(rank)), self._h)
+
+    def sample_filtered_into(self, logits, out_ids, *, vocab: Optional[int] = None, mask=None, hist_ids=None,
+                             hist_offsets=None, uniforms=None, params: Optional[FilterParams] = None, row_params=None,
+                             out_probs=None, out_counts=None, out_flags=None, stream=None) -> None:
+        """sas_sample_filtered on caller-provided device buffers: logits
+        [rows][>= vocab] float32, bfloat16 or float16 (no allocation, no
+        synchronisation: the kernels clamp the history offsets)."""
+        types = {"torch.float32": _capi.TYPE_F32, "torch.bfloat16": _capi.TYPE_BF16, "torch.float16": _capi.TYPE_F16}
+        if logits.dim() != 2 or logits.stride(1) != 1 or not logits.is_cuda or str(logits.dtype) not in types:
+            raise ValueError("logits must be a 2-D float32, bfloat16 or float16 device tensor with unit element stride")
+        rows = logits.shape[0]
+        d = SasFilterRows()
+        d.logits, d.logits_type = logits.data_ptr(), types[str(logits.dtype)]
+        d.rows, d.vocab = rows, int(vocab if vocab is not None else logits.shape[1])
+        d.logits_stride = logits.stride(0) if rows > 1 else max(logits.stride(0), logits.shape[1])
+        if d.vocab > logits.shape[1]:
+            raise ValueError("vocab exceeds the logits' columns")
+        if mask is not None:
+            words = (d.vocab + 31) // 32
+            if mask.dim() != 2 or mask.shape[0] not in (1, rows) or mask.shape[1] < words or mask.stride(1) != 1:
+                raise ValueError("mask must hold ceil(vocab / 32) words for every row, or one row for all")
+            d.mask = _ptr(mask, "i32", "mask")
+            d.mask_stride = mask.stride(0) if mask.shape[0] == rows and rows > 1 else 0
+        if hist_ids is not None and hist_ids.numel() > 0:
+            if hist_offsets is None or hist_offsets.numel() != rows + 1:
+                raise ValueError("hist_ids requires hist_offsets, rows + 1 of them")
+            d.hist_ids, d.hist_count = _ptr(hist_ids, "i32", "hist_ids"), hist_ids.numel()
+            d.hist_offsets = _ptr(hist_offsets, "i32", "hist_offsets")
+        d.params = (params or FilterParams()).to_c()
+        for name, t, kind, per_row in (("uniforms", uniforms, "f64", 1), ("out_ids", out_ids, "i32", 1),
+                                       ("out_probs", out_probs, "f64", 1), ("out_counts", out_counts, "i32", 1),
+                                       ("out_flags", out_flags, "i32", 1)):
+            if t is not None:
+                if t.numel() < rows * per_row:
+                    raise ValueError(f"{name} must hold one value per row")
+                setattr(d, name, _ptr(t, kind, name))
+        if row_params is not None:
+            if row_params.numel() * row_params.element_size() < rows * FILTER_PARAMS_DTYPE.itemsize:
+                raise ValueError("row_params must hold one sas_filter_params per row (pack_filter_params)")
+            d.row_params = _ptr(row_params)
+        check(self._lib.sas_sample_filtered(self._h, ctypes.byref(d), _stream(stream)), self._h)
+
+    def sample_filtered(self, logits, *, full: bool = False, stream=None, **kw):
+        """Allocate outputs and sample_filtered_into; returns ids, or with
+        full a dict of ids, probs (the token's share of the kept mass), counts
+        (ids kept) and flags."""
+        import torch
+        rows, dev = logits.shape[0], logits.device
+        with _on(stream):
+            out = {"ids": torch.empty(rows, dtype=torch.int32, device=dev)}
+            if full:
+                out["probs"] = torch.empty(rows, dtype=torch.float64, device=dev)
+                out["counts"] = torch.empty(rows, dtype=torch.int32, device=dev)
+                out["flags"] = torch.empty(rows, dtype=torch.int32, device=dev)
+        self.sample_filtered_into(logits, out["ids"], out_probs=out.get("probs"), out_counts=out.get("counts"),
+                                  out_flags=out.get("flags"), stream=stream, **kw)
+        return out if full else out["ids"]
+
+    def reserve_filtered(self, rows: int, vocab: int) -> None:
+        """Pre-size the scratch of sample_filtered calls of at most these shapes."""
+        check(self._lib.sas_reserve_filtered(self._h, int(rows), int(vocab)), self._h)
 
     def sample_step_into(self, logits, out_ids, state: DecodeState, *, stream=None, **kw) -> None:
         """One decode step with in-graph feedback (sas_sample_step): the
