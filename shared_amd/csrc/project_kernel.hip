@@ -9,9 +9,10 @@
 //      sum is the f32 value); f32 hidden states are stored as three pieces
 //      too.  Products of bf16 pieces are exact in the f32 sums of the matrix
 //      instructions, so f32 inputs keep all their bits.
-//   2. proj_rows_kernel: the rows' products with W, then with B of each
-//      adapter among a subtile's 16 rows, each adapter in sums of its own that
-//      only its rows add: a value that is not finite stays with its adapter.
+//   2. proj_wide_kernel or proj_split_kernel: the rows' products with W, then
+//      with B of each adapter among a tile's rows, each adapter in sums of its
+//      own that only its rows add: a value that is not finite stays with its
+//      adapter.
 #include "sas_device.h"
 #include "sas_launch.h"
 
@@ -89,28 +90,35 @@ __device__ __forceinline__ void each_adapter(int mine, F f) {
   }
 }
 
-// Block (subtile, slot): the slot-th adapter of the subtile's rows; its waves
-// split dim, their sums meet in LDS.  Blocks past the subtiles write the
-// pieces of f32 hidden states.
-__global__ __launch_bounds__(kThreads) void proj_inner_kernel(const ProjArgs a) {
+// Block (subtile, slot): the slot-th adapter of the subtile's rows.  Its
+// waves share out up to four rank tiles and, within each, the runs of 32 of
+// dim; the parts meet in LDS in a fixed order.  Blocks past the subtiles
+// write the pieces of f32 hidden states.
+constexpr int kInnerWaves = 16;
+constexpr int kInnerThreads = 64 * kInnerWaves;
+constexpr int kInnerDeep = 4;  // runs whose loads are in flight together
+
+template <bool kF32>
+__global__ __launch_bounds__(kInnerThreads) void proj_inner_kernel(const ProjArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int subs = (a.rows + kSub - 1) / kSub;
   if ((int)blockIdx.x >= subs) {
-    if (!a.xp) return;
-    // 8 values a thread
-    const int per = a.dim / 8;
-    const int64_t n = (int64_t)a.rows * per;
-    const int64_t step = (int64_t)(gridDim.x - subs) * gridDim.y * kThreads;
-    for (int64_t i = ((int64_t)(blockIdx.x - subs) * gridDim.y + blockIdx.y) * kThreads + tid; i < n; i += step) {
-      const int64_t row = i / per, c = i - row * per;
-      u32x4 p[3];
-      split8(static_cast<const float *>(a.x) + row * a.x_stride + 8 * c, p);
+    if constexpr (kF32) {
+      // 8 values a thread
+      const int per = a.dim / 8;
+      const int64_t n = (int64_t)a.rows * per;
+      const int64_t step = (int64_t)(gridDim.x - subs) * gridDim.y * kInnerThreads;
+      for (int64_t i = ((int64_t)(blockIdx.x - subs) * gridDim.y + blockIdx.y) * kInnerThreads + tid; i < n; i += step) {
+        const int64_t row = i / per, c = i - row * per;
+        u32x4 p[3];
+        split8(static_cast<const float *>(a.x) + row * a.x_stride + 8 * c, p);
 #pragma unroll
-      for (int k = 0; k < 3; ++k) *reinterpret_cast<u32x4 *>(a.xp + ((int64_t)k * a.rows + row) * a.dim + 8 * c) = p[k];
+        for (int k = 0; k < 3; ++k) *reinterpret_cast<u32x4 *>(a.xp + ((int64_t)k * a.rows + row) * a.dim + 8 * c) = p[k];
+      }
     }
     return;
   }
-  __shared__ f32x4 part[kWaves][64];
+  __shared__ f32x4 part[kInnerWaves][64];
   const int row = (int)blockIdx.x * kSub + (lane & 15);
   const int mine = adapter_of(a, row);
   int cur = -1, at = 0;
@@ -122,31 +130,41 @@ __global__ __launch_bounds__(kThreads) void proj_inner_kernel(const ProjArgs a) 
   const float scale = a.scales ? a.scales[cur] : 1.0f;
   const int xrow = min(row, a.rows - 1);
   const int kc = 8 * (lane >> 4);
-  // dim in runs of 32 for the waves to share
-  const int steps = (a.dim + 31) / 32, k0 = 32 * (steps * wave / kWaves), k1 = min(a.dim, 32 * (steps * (wave + 1) / kWaves));
+  const int tiles = (a.rank + kSub - 1) / kSub, group = min(tiles, 4), ks = kInnerWaves / group;
+  const int mytile = wave % group, myks = wave / group;
+  const int steps = (a.dim + 31) / 32;
+  const int g0 = myks < ks ? steps * myks / ks : 0, g1 = myks < ks ? steps * (myks + 1) / ks : 0;
   const uint16_t *A = static_cast<const uint16_t *>(a.a) + (int64_t)cur * a.a_adapter_stride;
-  for (int t = 0; t < a.rank; t += kSub) {
-    const uint16_t *ar = A + (int64_t)min(t + (lane & 15), a.rank - 1) * a.a_stride;
+  const u32x4 none = {0u, 0u, 0u, 0u};
+  for (int t0 = 0; t0 < tiles; t0 += group) {
+    const int t = kSub * (t0 + mytile);
+    const uint16_t *ar = A + (int64_t)min(t + (lane & 15), a.rank - 1) * a.a_stride + kc;
     f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int k = k0 + kc; k - kc < k1; k += 32) {
-      const bool in = k < k1;
-      const u32x4 none = {0u, 0u, 0u, 0u};
-      const u32x4 w = in ? *reinterpret_cast<const u32x4 *>(ar + k) : none;
-      if (a.x_f32) {
-        u32x4 p[3] = {none, none, none};
-        if (in) split8(static_cast<const float *>(a.x) + (int64_t)xrow * a.x_stride + k, p);
+    for (int g = g0; g < g1; g += kInnerDeep) {
+      u32x4 w[kInnerDeep], x[kInnerDeep][kF32 ? 3 : 1];
 #pragma unroll
-        for (int i = 0; i < 3; ++i) acc = mfma(w, p[i], acc);
-      } else {
-        const uint16_t *xr = static_cast<const uint16_t *>(a.x) + (int64_t)xrow * a.x_stride;
-        acc = mfma(w, in ? *reinterpret_cast<const u32x4 *>(xr + k) : none, acc);
+      for (int d = 0; d < kInnerDeep; ++d) {
+        const int k = 32 * (g + d);
+        const bool in = g + d < g1 && k + kc < a.dim;
+        w[d] = in ? *reinterpret_cast<const u32x4 *>(ar + k) : none;
+        if constexpr (kF32) {
+          if (in) split8(static_cast<const float *>(a.x) + (int64_t)xrow * a.x_stride + k + kc, x[d]);
+          else x[d][0] = x[d][1] = x[d][2] = none;
+        } else {
+          x[d][0] = in ? *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(a.x) + (int64_t)xrow * a.x_stride + k + kc) : none;
+        }
       }
+#pragma unroll
+      for (int d = 0; d < kInnerDeep; ++d)
+#pragma unroll
+        for (int i = 0; i < (kF32 ? 3 : 1); ++i) acc = mfma(w[d], x[d][i], acc);
     }
     part[wave][lane] = acc;
     __syncthreads();
-    if (wave == 0) {
+    if (wave < group) {
       // lane: row lane & 15, ranks t + 4 (lane / 16) ..
-      f32x4 h = (part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]);
+      f32x4 h = part[wave][lane];
+      for (int i = 1; i < ks; ++i) h = h + part[wave + i * group][lane];
       const int r0 = t + 4 * (lane >> 4);
       if (mine == cur && r0 < a.rank) {
         u16x4 p[3];
@@ -214,48 +232,282 @@ __device__ __forceinline__ void store4(const ProjArgs &a, int row, int n, f32x4 
   }
 }
 
-// Block (n, m): 64 outputs (16 a wave) of 16 rows.
-template <int P>
-__global__ __launch_bounds__(kThreads) void proj_rows_kernel(const ProjArgs a) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int row = (int)blockIdx.y * kSub + (lane & 15);
-  const int xrow = min(row, a.rows - 1);
-  const int kc = 8 * (lane >> 4);
-  const int n0 = ((int)blockIdx.x * kWaves + wave) * kSub;
-  if (n0 >= a.out_dim) return;
-  const int wrow = min(n0 + (lane & 15), a.out_dim - 1);
-  f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (a.weight) {
-    const uint16_t *w = static_cast<const uint16_t *>(a.weight) + (int64_t)wrow * a.weight_stride;
-    const uint16_t *x[P];
-#pragma unroll
-    for (int p = 0; p < P; ++p)
-      x[p] = P == 1 ? static_cast<const uint16_t *>(a.x) + (int64_t)xrow * a.x_stride
-                    : a.xp + ((int64_t)p * a.rows + xrow) * a.dim;
-    for (int k = kc; k - kc < a.dim; k += 32) {
-      const bool in = k < a.dim;
-      const u32x4 none = {0u, 0u, 0u, 0u};
-      const u32x4 wv = in ? *reinterpret_cast<const u32x4 *>(w + k) : none;
-#pragma unroll
-      for (int p = 0; p < P; ++p) acc = mfma(wv, in ? *reinterpret_cast<const u32x4 *>(x[p] + k) : none, acc);
-    }
+// The adapters among a tile's rows (16 MT, at most 128), one after another:
+// f(adapter, rows of the tile that use it as two masks of 64).
+template <int MT, typename F>
+__device__ __forceinline__ void each_tile_adapter(const ProjArgs &a, int tile0, F f) {
+  const int lane = threadIdx.x & 63;
+  const int lo = lane < 16 * MT ? adapter_of(a, tile0 + lane) : -1;
+  const int hi = MT > 4 && 64 + lane < 16 * MT ? adapter_of(a, tile0 + 64 + lane) : -1;
+  uint64_t l = __ballot(lo >= 0), h = MT > 4 ? __ballot(hi >= 0) : 0ull;
+  while (l | h) {
+    const int cur = l ? __builtin_amdgcn_readlane(lo, __builtin_ctzll(l)) : __builtin_amdgcn_readlane(hi, __builtin_ctzll(h));
+    const uint64_t ml = __ballot(lo == cur), mh = MT > 4 ? __ballot(hi == cur) : 0ull;
+    l &= ~ml;
+    h &= ~mh;
+    f(cur, ml, mh);
   }
-  const int mine = adapter_of(a, row);
-  each_adapter(mine, [&](int cur) {
-    const int used = rank_of(a, cur);
-    const uint16_t *b = static_cast<const uint16_t *>(a.b) + (int64_t)cur * a.b_adapter_stride + (int64_t)wrow * a.b_stride;
-    const uint16_t *h = a.hp + (int64_t)xrow * 3 * a.rank;
-    f32x4 ext = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int e = kc; e - kc < 3 * a.rank; e += 32) {
-      const u32x4 none = {0u, 0u, 0u, 0u};
+}
+
+// Adds adapter `cur`'s term to the sums of the rows of masks ml, mh: the
+// pieces of h (3 rank of them) times B's ranks, three times over, in sums of
+// their own.
+template <int MT, int NT>
+__device__ __forceinline__ void add_adapter(const ProjArgs &a, int cur, uint64_t ml, uint64_t mh, int tile0, int n0,
+                                            f32x4 (&acc)[MT][NT]) {
+  const int lane = threadIdx.x & 63, kc = 8 * (lane >> 4);
+  const int used = rank_of(a, cur);
+  const u32x4 none = {0u, 0u, 0u, 0u};
+  const uint16_t *b = static_cast<const uint16_t *>(a.b) + (int64_t)cur * a.b_adapter_stride;
+  const uint16_t *br[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) br[t] = b + (int64_t)min(n0 + 16 * t + (lane & 15), a.out_dim - 1) * a.b_stride;
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    const uint32_t users = (uint32_t)((m < 4 ? ml : mh) >> (16 * (m & 3))) & 0xFFFFu;
+    if (!users) continue;
+    const uint16_t *h = a.hp + (int64_t)min(tile0 + 16 * m + (lane & 15), a.rows - 1) * 3 * a.rank;
+    f32x4 ext[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) ext[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int e0 = 0; e0 < 3 * a.rank; e0 += 32) {
+      const int e = e0 + kc;
       const bool in = e < 3 * a.rank;
       const int r = e < a.rank ? e : e < 2 * a.rank ? e - a.rank : e - 2 * a.rank;
-      const u32x4 bv = in ? b_ranks(b, r, used) : none;
-      ext = mfma(bv, in ? *reinterpret_cast<const u32x4 *>(h + e) : none, ext);
+      const u32x4 hv = in ? *reinterpret_cast<const u32x4 *>(h + e) : none;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) ext[t] = mfma(in ? b_ranks(br[t], r, used) : none, hv, ext[t]);
     }
-    if (mine == cur) acc = acc + ext;
-  });
-  store4(a, row, n0 + 4 * (lane >> 4), acc);
+    const bool mine = (users >> (lane & 15)) & 1u;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+      if (mine) acc[m][t] = acc[m][t] + ext[t];
+  }
+}
+
+// Blocks in runs that one XCD's L2 serves: block i runs on XCD i % 8.
+__device__ __forceinline__ int xcd_run(int i, int n) {
+  const int per = n / 8, left = n % 8, x = i % 8;
+  return x * per + min(x, left) + i / 8;
+}
+
+// Many outputs: four waves share a tile's rows (16 MT) and take 64 outputs
+// each.  A wave's weight rows go from memory straight to its registers, kDeep
+// runs of 32 ahead (no other wave needs them); the hidden states go through
+// LDS in chunks of kSteps runs, laid out operand by operand (64 lanes x 16
+// bytes), so neither side of LDS has a conflict.
+template <int MT, int P>
+struct Wide {
+  static constexpr int kNT = 4;
+  static constexpr int kBlockOut = kWaves * 16 * kNT;
+  static constexpr int kSteps = MT * P >= 12 ? 2 : MT * P >= 6 ? 4 : MT * P >= 3 ? 8 : 16;  // runs of 32 a chunk
+  static constexpr int kDeep = MT >= 6 ? 2 : 4 < kSteps ? 4 : kSteps;
+  static constexpr int kFrags = kSteps * P * MT;  // operands of a chunk
+  static constexpr int kMine = (kFrags + kWaves - 1) / kWaves;
+};
+
+template <int MT, int P, bool kTail>
+__global__ __launch_bounds__(kThreads, 2) void proj_wide_kernel(const ProjArgs a) {
+  using C = Wide<MT, P>;
+  constexpr int NT = C::kNT;
+  __shared__ u32x4 xs[2][C::kFrags][64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int mtiles = (a.rows + 16 * MT - 1) / (16 * MT);
+  const int pos = xcd_run((int)blockIdx.x, (int)gridDim.x);
+  const int tile0 = (pos % mtiles) * 16 * MT, n0 = (pos / mtiles) * C::kBlockOut + wave * 16 * NT;
+  const int kc = 8 * (lane >> 4);
+  const u32x4 none = {0u, 0u, 0u, 0u};
+  f32x4 acc[MT][NT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int t = 0; t < NT; ++t) acc[m][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  if (a.weight) {
+    const int steps = (a.dim + 31) / 32, chunks = (steps + C::kSteps - 1) / C::kSteps;
+    const uint16_t *wr[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+      wr[t] = static_cast<const uint16_t *>(a.weight) + (int64_t)min(n0 + 16 * t + (lane & 15), a.out_dim - 1) * a.weight_stride + kc;
+    // run g of the weight rows (past the last: the last again)
+    auto load_w = [&](int g, u32x4 (&w)[NT]) __attribute__((always_inline)) {
+      const int k = 32 * min(g, steps - 1);
+      const bool in = !kTail || k + kc < a.dim;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        if constexpr (kTail) w[t] = in ? *reinterpret_cast<const u32x4 *>(wr[t] + k) : none;
+        else w[t] = *reinterpret_cast<const u32x4 *>(wr[t] + k);
+      }
+    };
+    // this wave's operands of chunk c: operand f = (step, piece, subtile)
+    auto load_x = [&](int c, u32x4 (&x)[C::kMine]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < C::kMine; ++i) {
+        const int f = min(wave + kWaves * i, C::kFrags - 1);
+        const int m = f % MT, p = (f / MT) % P, k = 32 * (min(c, chunks - 1) * C::kSteps + f / (MT * P)) + kc;
+        const int64_t row = min(tile0 + 16 * m + (lane & 15), a.rows - 1);
+        const uint16_t *src = P == 1 ? static_cast<const uint16_t *>(a.x) + row * a.x_stride
+                                     : a.xp + ((int64_t)p * a.rows + row) * a.dim;
+        if constexpr (kTail) x[i] = k < a.dim ? *reinterpret_cast<const u32x4 *>(src + k) : none;
+        else x[i] = *reinterpret_cast<const u32x4 *>(src + k);
+      }
+    };
+    auto store_x = [&](int buf, const u32x4 (&x)[C::kMine]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < C::kMine; ++i)
+        if (C::kFrags % kWaves == 0 || wave + kWaves * i < C::kFrags) xs[buf][wave + kWaves * i][lane] = x[i];
+    };
+    u32x4 w[C::kDeep][NT], x[C::kMine];
+    load_x(0, x);
+#pragma unroll
+    for (int d = 0; d < C::kDeep; ++d) load_w(d, w[d]);
+    store_x(0, x);
+    load_x(1, x);
+    lds_barrier();
+    for (int c = 0; c < chunks; ++c) {
+#pragma unroll
+      for (int s = 0; s < C::kSteps; ++s) {
+        constexpr int D = C::kDeep;
+        u32x4 cur[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) cur[t] = w[s % D][t];
+        load_w(c * C::kSteps + s + D, w[s % D]);
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int p = 0; p < P; ++p) {
+            const u32x4 xv = xs[c & 1][(s * P + p) * MT + m][lane];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) acc[m][t] = mfma(cur[t], xv, acc[m][t]);
+          }
+      }
+      if (c + 1 < chunks) {
+        store_x((c + 1) & 1, x);
+        load_x(c + 2, x);
+        lds_barrier();
+      }
+    }
+  }
+  if (n0 >= a.out_dim) return;
+  if (a.adapters > 0)
+    each_tile_adapter<MT>(a, tile0, [&](int cur, uint64_t ml, uint64_t mh) { add_adapter<MT, NT>(a, cur, ml, mh, tile0, n0, acc); });
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int t = 0; t < NT; ++t) store4(a, tile0 + 16 * m + (lane & 15), n0 + 16 * t + 4 * (lane >> 4), acc[m][t]);
+}
+
+// Few outputs: eight waves split dim (and the tile's adapters) for the same
+// 16 NT outputs of 16 MT rows; their sums meet in LDS in a fixed order.  No
+// two waves need the same operand, so all go straight to registers.
+constexpr int kSplitWaves = 8;
+
+template <int MT, int NT, int P>
+__global__ __launch_bounds__(64 * kSplitWaves) void proj_split_kernel(const ProjArgs a) {
+  __shared__ f32x4 part[kSplitWaves][MT * NT][64];
+  constexpr int U = MT * P >= 8 ? 1 : MT * P >= 4 ? 2 : 4;  // runs of 32 whose loads are in flight together
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int mtiles = (a.rows + 16 * MT - 1) / (16 * MT);
+  const int pos = xcd_run((int)blockIdx.x, (int)gridDim.x);
+  const int tile0 = (pos % mtiles) * 16 * MT, n0 = (pos / mtiles) * 16 * NT;
+  const int kc = 8 * (lane >> 4);
+  const u32x4 none = {0u, 0u, 0u, 0u};
+  f32x4 acc[MT][NT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int t = 0; t < NT; ++t) acc[m][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  if (a.weight) {
+    const int steps = (a.dim + 31) / 32, g0 = steps * wave / kSplitWaves, g1 = steps * (wave + 1) / kSplitWaves;
+    const uint16_t *wr[NT], *xr[MT][P];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+      wr[t] = static_cast<const uint16_t *>(a.weight) + (int64_t)min(n0 + 16 * t + (lane & 15), a.out_dim - 1) * a.weight_stride + kc;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const int64_t row = min(tile0 + 16 * m + (lane & 15), a.rows - 1);
+#pragma unroll
+      for (int p = 0; p < P; ++p)
+        xr[m][p] = (P == 1 ? static_cast<const uint16_t *>(a.x) + row * a.x_stride : a.xp + ((int64_t)p * a.rows + row) * a.dim) + kc;
+    }
+    for (int g = g0; g < g1; g += U) {
+      u32x4 w[U][NT], x[U][MT][P];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int k = 32 * (g + u);
+        const bool in = g + u < g1 && k + kc < a.dim;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) w[u][t] = in ? *reinterpret_cast<const u32x4 *>(wr[t] + k) : none;
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int p = 0; p < P; ++p) x[u][m][p] = in ? *reinterpret_cast<const u32x4 *>(xr[m][p] + k) : none;
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int p = 0; p < P; ++p)
+#pragma unroll
+            for (int t = 0; t < NT; ++t) acc[m][t] = mfma(w[u][t], x[u][m][p], acc[m][t]);
+    }
+  }
+  if (a.adapters > 0) {
+    int at = 0;
+    each_tile_adapter<MT>(a, tile0, [&](int cur, uint64_t ml, uint64_t mh) {
+      if (at++ % kSplitWaves == wave) add_adapter<MT, NT>(a, cur, ml, mh, tile0, n0, acc);
+    });
+  }
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int t = 0; t < NT; ++t) part[wave][m * NT + t][lane] = acc[m][t];
+  __syncthreads();
+  for (int i = wave; i < MT * NT; i += kSplitWaves) {
+    f32x4 v = part[0][i][lane];
+#pragma unroll
+    for (int w = 1; w < kSplitWaves; ++w) v = v + part[w][i][lane];
+    store4(a, tile0 + 16 * (i / NT) + (lane & 15), n0 + 16 * (i % NT) + 4 * (lane >> 4), v);
+  }
+}
+
+template <int MT, int P>
+void launch_wide(const ProjArgs &a, hipStream_t stream) {
+  using C = Wide<MT, P>;
+  const int blocks = ((a.rows + 16 * MT - 1) / (16 * MT)) * ((a.out_dim + C::kBlockOut - 1) / C::kBlockOut);
+  if (a.dim % (32 * C::kSteps) == 0) proj_wide_kernel<MT, P, false><<<blocks, kThreads, 0, stream>>>(a);
+  else proj_wide_kernel<MT, P, true><<<blocks, kThreads, 0, stream>>>(a);
+}
+
+template <int MT, int NT, int P>
+void launch_split(const ProjArgs &a, hipStream_t stream) {
+  const int blocks = ((a.rows + 16 * MT - 1) / (16 * MT)) * ((a.out_dim + 16 * NT - 1) / (16 * NT));
+  proj_split_kernel<MT, NT, P><<<blocks, 64 * kSplitWaves, 0, stream>>>(a);
+}
+
+template <int P>
+void launch_rows(const ProjArgs &a, hipStream_t stream) {
+  const int subs = (a.rows + kSub - 1) / kSub;
+  // subtiles a tile of the wide kernel: as few tiles as 8 allow, evenly
+  const int tiles = (subs + 7) / 8, mt = (subs + tiles - 1) / tiles;
+  if ((int64_t)tiles * ((a.out_dim + 255) / 256) >= a.cus) {
+    switch (mt) {
+      case 1: return launch_wide<1, P>(a, stream);
+      case 2: return launch_wide<2, P>(a, stream);
+      case 3: return launch_wide<3, P>(a, stream);
+      case 4: return launch_wide<4, P>(a, stream);
+      case 5: return launch_wide<5, P>(a, stream);
+      case 6: return launch_wide<6, P>(a, stream);
+      case 7: return launch_wide<7, P>(a, stream);
+      default: return launch_wide<8, P>(a, stream);
+    }
+  }
+  if (subs == 1) {
+    if (a.out_dim <= 32 * a.cus) return launch_split<1, 1, P>(a, stream);
+    return launch_split<1, 2, P>(a, stream);
+  }
+  if (subs <= 2) return launch_split<2, 2, P>(a, stream);
+  launch_split<4, 2, P>(a, stream);
 }
 
 }  // namespace
@@ -268,13 +520,14 @@ size_t proj_scratch_bytes(int rows, int dim, int rank, bool x_f32) {
 hipError_t launch_project(const ProjArgs &a, hipStream_t stream) {
   const int subs = (a.rows + kSub - 1) / kSub;
   if (a.adapters > 0 || a.xp) {
-    const int split = a.xp ? (int)(((int64_t)a.rows * (a.dim / 8) + kSub * kThreads - 1) / (kSub * kThreads)) : 0;
-    proj_inner_kernel<<<dim3(subs + (split > 1024 ? 1024 : split), kSub), kThreads, 0, stream>>>(a);
+    const int split = a.xp ? (int)(((int64_t)a.rows * (a.dim / 8) + kSub * kInnerThreads - 1) / (kSub * kInnerThreads)) : 0;
+    const dim3 grid(subs + (split > 1024 ? 1024 : split), kSub);
+    if (a.x_f32) proj_inner_kernel<true><<<grid, kInnerThreads, 0, stream>>>(a);
+    else proj_inner_kernel<false><<<grid, kInnerThreads, 0, stream>>>(a);
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   }
-  const dim3 grid((a.out_dim + kWaves * kSub - 1) / (kWaves * kSub), subs);
-  if (a.xp) proj_rows_kernel<3><<<grid, kThreads, 0, stream>>>(a);
-  else proj_rows_kernel<1><<<grid, kThreads, 0, stream>>>(a);
+  if (a.xp) launch_rows<3>(a, stream);
+  else launch_rows<1>(a, stream);
   return hipGetLastError();
 }
 
