@@ -291,31 +291,47 @@ __device__ __forceinline__ int xcd_run(int i, int n) {
   return x * per + min(x, left) + i / 8;
 }
 
-// Many outputs: four waves share a tile's rows (16 MT) and take 64 outputs
-// each.  A wave's weight rows go from memory straight to its registers, kDeep
-// runs of 32 ahead (no other wave needs them); the hidden states go through
-// LDS in chunks of kSteps runs, laid out operand by operand (64 lanes x 16
-// bytes), so neither side of LDS has a conflict.
-template <int MT, int P>
+// An operand of 16 rows x 64 values (2 KB): loaded eight lanes a row, whole
+// 128-byte lines (memory serves lines 10 % faster than the matrix layout's 64
+// bytes a row), and turned into the matrix layout through LDS, where value
+// octet o of row r sits in 16-byte slot 8 r + (o ^ r / 2): the eight lanes
+// that write a row, and the 16 rows that read an octet, meet every bank once.
+constexpr int kRun = 64;          // values of dim in an operand
+constexpr int kSlots = 128;       // 16-byte slots of an operand
+__device__ __forceinline__ int put_slot(int j) {  // of lane's load j (rows 8 j ..)
+  const int lane = threadIdx.x & 63, r = 8 * j + (lane >> 3);
+  return 8 * r + ((lane & 7) ^ (r >> 1));
+}
+__device__ __forceinline__ int get_slot(int h) {  // half h: values 32 h ..
+  const int lane = threadIdx.x & 63, r = lane & 15;
+  return 8 * r + ((4 * h + (lane >> 4)) ^ (r >> 1));
+}
+
+// Many outputs: eight waves share a tile's rows (16 MT) and take 16 NT outputs
+// each.  A wave's weight rows go through LDS of its own, kDeep runs ahead in
+// registers, so that a block alone keeps enough of memory in flight; the hidden
+// states' chunks of kSteps runs are staged for all waves.
+constexpr int kWideWaves = 8;
+constexpr int kWideThreads = 64 * kWideWaves;
+template <int MT, int NT, int P>
 struct Wide {
-  static constexpr int kNT = 4;
-  static constexpr int kBlockOut = kWaves * 16 * kNT;
-  static constexpr int kSteps = MT * P >= 12 ? 2 : MT * P >= 6 ? 4 : MT * P >= 3 ? 8 : 16;  // runs of 32 a chunk
-  static constexpr int kDeep = MT >= 6 ? 2 : 4 < kSteps ? 4 : kSteps;
-  static constexpr int kFrags = kSteps * P * MT;  // operands of a chunk
-  static constexpr int kMine = (kFrags + kWaves - 1) / kWaves;
+  static constexpr int kBlockOut = kWideWaves * 16 * NT;
+  static constexpr int kSteps = MT * P >= 4 ? 1 : MT * P >= 2 ? 2 : 4;  // runs a chunk
+  static constexpr int kDeep = NT == 1 ? 4 : 2;
+  static constexpr int kUnroll = kDeep > kSteps ? kDeep / kSteps : 1;   // chunks a turn of the loop
+  static constexpr int kTiles = kSteps * P * MT;                        // operands of a chunk
+  static constexpr int kMine = (2 * kTiles + kWideWaves - 1) / kWideWaves;  // a wave's loads of them
 };
 
-template <int MT, int P, bool kTail>
-__global__ __launch_bounds__(kThreads, 2) void proj_wide_kernel(const ProjArgs a) {
-  using C = Wide<MT, P>;
-  constexpr int NT = C::kNT;
-  __shared__ u32x4 xs[2][C::kFrags][64];
+template <int MT, int NT, int P>
+__global__ __launch_bounds__(kWideThreads, 2) void proj_wide_kernel(const ProjArgs a) {
+  using C = Wide<MT, NT, P>;
+  __shared__ u32x4 xs[2][C::kTiles][kSlots];
+  __shared__ u32x4 ws[kWideWaves][NT][kSlots];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int mtiles = (a.rows + 16 * MT - 1) / (16 * MT);
   const int pos = xcd_run((int)blockIdx.x, (int)gridDim.x);
   const int tile0 = (pos % mtiles) * 16 * MT, n0 = (pos / mtiles) * C::kBlockOut + wave * 16 * NT;
-  const int kc = 8 * (lane >> 4);
   const u32x4 none = {0u, 0u, 0u, 0u};
   f32x4 acc[MT][NT];
 #pragma unroll
@@ -323,67 +339,109 @@ __global__ __launch_bounds__(kThreads, 2) void proj_wide_kernel(const ProjArgs a
 #pragma unroll
     for (int t = 0; t < NT; ++t) acc[m][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   if (a.weight) {
-    const int steps = (a.dim + 31) / 32, chunks = (steps + C::kSteps - 1) / C::kSteps;
-    const uint16_t *wr[NT];
+    const int runs = (a.dim + kRun - 1) / kRun, chunks = (runs + C::kSteps - 1) / C::kSteps;
+    const int oct = 8 * (lane & 7);
+    const bool once = mtiles == 1;
+    const uint16_t *wr[NT][2];
 #pragma unroll
     for (int t = 0; t < NT; ++t)
-      wr[t] = static_cast<const uint16_t *>(a.weight) + (int64_t)min(n0 + 16 * t + (lane & 15), a.out_dim - 1) * a.weight_stride + kc;
-    // run g of the weight rows (past the last: the last again)
-    auto load_w = [&](int g, u32x4 (&w)[NT]) __attribute__((always_inline)) {
-      const int k = 32 * min(g, steps - 1);
-      const bool in = !kTail || k + kc < a.dim;
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        if constexpr (kTail) w[t] = in ? *reinterpret_cast<const u32x4 *>(wr[t] + k) : none;
-        else w[t] = *reinterpret_cast<const u32x4 *>(wr[t] + k);
+      for (int j = 0; j < 2; ++j)
+        wr[t][j] = static_cast<const uint16_t *>(a.weight) +
+                   (int64_t)min(n0 + 16 * t + 8 * j + (lane >> 3), a.out_dim - 1) * a.weight_stride + oct;
+    // run g of the weight rows (past the last: the last again)
+    auto load_w = [&](int g, u32x4 (&w)[NT][2]) __attribute__((always_inline)) {
+      const int k = kRun * min(g, runs - 1);
+      if (k + kRun > a.dim) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) w[t][j] = k + oct < a.dim ? *reinterpret_cast<const u32x4 *>(wr[t][j] + k) : none;
+      } else if (once) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) w[t][j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(wr[t][j] + k));
+      } else {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) w[t][j] = *reinterpret_cast<const u32x4 *>(wr[t][j] + k);
       }
     };
-    // this wave's operands of chunk c: operand f = (step, piece, subtile)
+    // this wave's loads of chunk c: load f is half f % 2 of operand f / 2 =
+    // (step, piece, subtile); operands past dim (a last chunk's) are zero
+    const uint16_t *xr[C::kMine];
+#pragma unroll
+    for (int i = 0; i < C::kMine; ++i) {
+      const int f = min(wave + kWideWaves * i, 2 * C::kTiles - 1), m = (f / 2) % MT, p = (f / 2 / MT) % P;
+      const int64_t row = min(tile0 + 16 * m + 8 * (f & 1) + (lane >> 3), a.rows - 1);
+      xr[i] = (P == 1 ? static_cast<const uint16_t *>(a.x) + row * a.x_stride : a.xp + ((int64_t)p * a.rows + row) * a.dim) +
+              kRun * (f / 2 / MT / P) + oct;
+    }
     auto load_x = [&](int c, u32x4 (&x)[C::kMine]) __attribute__((always_inline)) {
+      const int k = kRun * C::kSteps * min(c, chunks - 1);
 #pragma unroll
       for (int i = 0; i < C::kMine; ++i) {
-        const int f = min(wave + kWaves * i, C::kFrags - 1);
-        const int m = f % MT, p = (f / MT) % P, k = 32 * (min(c, chunks - 1) * C::kSteps + f / (MT * P)) + kc;
-        const int64_t row = min(tile0 + 16 * m + (lane & 15), a.rows - 1);
-        const uint16_t *src = P == 1 ? static_cast<const uint16_t *>(a.x) + row * a.x_stride
-                                     : a.xp + ((int64_t)p * a.rows + row) * a.dim;
-        if constexpr (kTail) x[i] = k < a.dim ? *reinterpret_cast<const u32x4 *>(src + k) : none;
-        else x[i] = *reinterpret_cast<const u32x4 *>(src + k);
+        const int f = min(wave + kWideWaves * i, 2 * C::kTiles - 1), at = k + kRun * (f / 2 / MT / P);
+        if (at + kRun > a.dim) x[i] = at + oct < a.dim ? *reinterpret_cast<const u32x4 *>(xr[i] + k) : none;
+        else x[i] = *reinterpret_cast<const u32x4 *>(xr[i] + k);
       }
     };
     auto store_x = [&](int buf, const u32x4 (&x)[C::kMine]) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < C::kMine; ++i)
-        if (C::kFrags % kWaves == 0 || wave + kWaves * i < C::kFrags) xs[buf][wave + kWaves * i][lane] = x[i];
+      for (int i = 0; i < C::kMine; ++i) {
+        const int f = wave + kWideWaves * i;
+        if (2 * C::kTiles % kWideWaves == 0 || f < 2 * C::kTiles) xs[buf][f / 2][put_slot(f & 1)] = x[i];
+      }
     };
-    u32x4 w[C::kDeep][NT], x[C::kMine];
+    u32x4 w[C::kDeep][NT][2], x[C::kMine];
     load_x(0, x);
 #pragma unroll
     for (int d = 0; d < C::kDeep; ++d) load_w(d, w[d]);
     store_x(0, x);
     load_x(1, x);
     lds_barrier();
-    for (int c = 0; c < chunks; ++c) {
+    for (int c0 = 0; c0 < chunks; c0 += C::kUnroll) {
 #pragma unroll
-      for (int s = 0; s < C::kSteps; ++s) {
-        constexpr int D = C::kDeep;
-        u32x4 cur[NT];
+      for (int v = 0; v < C::kUnroll; ++v) {
+        const int c = c0 + v;
+        if (c >= chunks) break;
 #pragma unroll
-        for (int t = 0; t < NT; ++t) cur[t] = w[s % D][t];
-        load_w(c * C::kSteps + s + D, w[s % D]);
+        for (int s = 0; s < C::kSteps; ++s) {
+          constexpr int D = C::kDeep;
+          const int slot = (v * C::kSteps + s) % D;
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+          for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int p = 0; p < P; ++p) {
-            const u32x4 xv = xs[c & 1][(s * P + p) * MT + m][lane];
+            for (int j = 0; j < 2; ++j) ws[wave][t][put_slot(j)] = w[slot][t][j];
+          // the loads stay here: left to itself the compiler moves them down to
+          // where they are used, and every run waits for memory
+          load_w(c * C::kSteps + s + D, w[slot]);
+          wave_lds_sync();
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int t = 0; t < NT; ++t) acc[m][t] = mfma(cur[t], xv, acc[m][t]);
+          for (int h = 0; h < 2; ++h) {
+            u32x4 wv[NT];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) wv[t] = ws[wave][t][get_slot(h)];
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+              for (int p = 0; p < P; ++p) {
+                const u32x4 xv = xs[c & 1][(s * P + p) * MT + m][get_slot(h)];
+#pragma unroll
+                for (int t = 0; t < NT; ++t) acc[m][t] = mfma(wv[t], xv, acc[m][t]);
+              }
           }
-      }
-      if (c + 1 < chunks) {
-        store_x((c + 1) & 1, x);
-        load_x(c + 2, x);
-        lds_barrier();
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        if (c + 1 < chunks) {
+          store_x((c + 1) & 1, x);
+          load_x(c + 2, x);
+          __builtin_amdgcn_sched_barrier(0);
+          lds_barrier();
+        }
       }
     }
   }
@@ -471,12 +529,11 @@ __global__ __launch_bounds__(64 * kSplitWaves) void proj_split_kernel(const Proj
   }
 }
 
-template <int MT, int P>
+template <int MT, int NT, int P>
 void launch_wide(const ProjArgs &a, hipStream_t stream) {
-  using C = Wide<MT, P>;
+  using C = Wide<MT, NT, P>;
   const int blocks = ((a.rows + 16 * MT - 1) / (16 * MT)) * ((a.out_dim + C::kBlockOut - 1) / C::kBlockOut);
-  if (a.dim % (32 * C::kSteps) == 0) proj_wide_kernel<MT, P, false><<<blocks, kThreads, 0, stream>>>(a);
-  else proj_wide_kernel<MT, P, true><<<blocks, kThreads, 0, stream>>>(a);
+  proj_wide_kernel<MT, NT, P><<<blocks, kWideThreads, 0, stream>>>(a);
 }
 
 template <int MT, int NT, int P>
@@ -492,14 +549,14 @@ void launch_rows(const ProjArgs &a, hipStream_t stream) {
   const int tiles = (subs + 7) / 8, mt = (subs + tiles - 1) / tiles;
   if ((int64_t)tiles * ((a.out_dim + 255) / 256) >= a.cus) {
     switch (mt) {
-      case 1: return launch_wide<1, P>(a, stream);
-      case 2: return launch_wide<2, P>(a, stream);
-      case 3: return launch_wide<3, P>(a, stream);
-      case 4: return launch_wide<4, P>(a, stream);
-      case 5: return launch_wide<5, P>(a, stream);
-      case 6: return launch_wide<6, P>(a, stream);
-      case 7: return launch_wide<7, P>(a, stream);
-      default: return launch_wide<8, P>(a, stream);
+      case 1: return launch_wide<1, 1, P>(a, stream);
+      case 2: return launch_wide<2, 1, P>(a, stream);
+      case 3: return launch_wide<3, 2, P>(a, stream);
+      case 4: return launch_wide<4, 2, P>(a, stream);
+      case 5: return launch_wide<5, 2, P>(a, stream);
+      case 6: return launch_wide<6, 2, P>(a, stream);
+      case 7: return launch_wide<7, 2, P>(a, stream);
+      default: return launch_wide<8, 2, P>(a, stream);
     }
   }
   if (subs == 1) {
