@@ -461,6 +461,8 @@ int sas_lm_head_sample_step(sas_sampler *s, const sas_lm_head *head, const sas_r
 #define SAS_MAX_RANK 256
 /* Largest number of rows of one sas_project call. */
 #define SAS_MAX_PROJECT_ROWS (1 << 19)
+/* Largest weight_stride of sas_project. */
+#define SAS_MAX_PROJECT_STRIDE (1 << 24)
 
 typedef struct sas_projection {
   const void *x;              /* device [rows][x_stride]: hidden states, 16-byte aligned */
@@ -469,7 +471,7 @@ typedef struct sas_projection {
   int32_t rows;               /* >= 0 */
   const void *weight;         /* device bf16 [out_dim][weight_stride], 16-byte aligned; NULL:
                                  the adapters' terms alone (accumulate must be set) */
-  int64_t weight_stride;      /* elements: >= dim, a multiple of 8 */
+  int64_t weight_stride;      /* elements: >= dim, a multiple of 8, <= SAS_MAX_PROJECT_STRIDE */
   int32_t dim;                /* a positive multiple of 8 */
   int32_t out_dim;            /* >= 1 */
   int32_t adapters;           /* adapters in the pool, 0: none (the fields below are unused) */

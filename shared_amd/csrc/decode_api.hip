@@ -54,8 +54,9 @@ const char *check_projection(const sas_projection *p) {
   if (p->out_stride < p->out_dim) return "out_stride < out_dim";
   if (!aligned(p->out, p->out_type == SAS_TYPE_F32 ? 4 : 2)) return "out must be aligned to its elements";
   if (p->weight) {
-    if (p->weight_stride < p->dim || p->weight_stride % 8 != 0)
-      return "weight_stride must be >= dim and a multiple of 8";
+    // (a wave's rows are addressed by 32-bit offsets from its first)
+    if (p->weight_stride < p->dim || p->weight_stride % 8 != 0 || p->weight_stride > SAS_MAX_PROJECT_STRIDE)
+      return "weight_stride must be >= dim, a multiple of 8 and <= SAS_MAX_PROJECT_STRIDE";
     if (!aligned(p->weight, 16)) return "weight must be 16-byte aligned";
   }
   if (p->adapters > 0) {
@@ -107,8 +108,9 @@ int sas_project(sas_sampler *s, const sas_projection *p, void *stream) {
     // the pieces of f32 hidden states serve the product with the weight
     const bool pieces = p->x_type == SAS_TYPE_F32 && p->weight;
     const int rank = p->adapters > 0 ? p->rank : 0;
-    if (int rc = grow(s, &s->proj, &s->proj_cap, proj_scratch_bytes(p->rows, p->dim, rank, pieces), stream, who))
-      return rc;
+    const ProjScratch at = proj_scratch(p->rows, p->dim, rank, pieces);
+    if (int rc = grow(s, &s->proj, &s->proj_cap, at.bytes, stream, who)) return rc;
+    char *scratch = static_cast<char *>(s->proj);
     ProjArgs a{};
     a.x = p->x;
     a.x_stride = p->x_stride;
@@ -125,9 +127,10 @@ int sas_project(sas_sampler *s, const sas_projection *p, void *stream) {
     a.row_adapter = p->row_adapter;
     a.out = p->out;
     a.out_stride = p->out_stride;
-    a.hp = static_cast<uint16_t *>(s->proj);
-    a.xp = pieces ? reinterpret_cast<uint16_t *>(static_cast<char *>(s->proj) + proj_scratch_bytes(p->rows, p->dim, rank, false))
-                  : nullptr;
+    // rows of one subtile, or of one adapter, need no order
+    a.perm = p->rows > 16 && p->adapters > 1 ? reinterpret_cast<int32_t *>(scratch) : nullptr;
+    a.hp = reinterpret_cast<uint16_t *>(scratch + at.hp);
+    a.xp = pieces ? reinterpret_cast<uint16_t *>(scratch + at.xp) : nullptr;
     a.rows = p->rows;
     a.dim = p->dim;
     a.out_dim = p->out_dim;
@@ -151,7 +154,7 @@ int sas_reserve_project(sas_sampler *s, int32_t rows, int32_t dim, int32_t rank)
                   "sas_reserve_project: rows must be in [0, SAS_MAX_PROJECT_ROWS], dim a positive multiple of 8, rank a "
                   "multiple of 8 in [0, SAS_MAX_RANK]");
     if (int rc = set_device(s)) return rc;
-    return grow(s, &s->proj, &s->proj_cap, proj_scratch_bytes(rows, dim, rank, true), nullptr, "sas_reserve_project");
+    return grow(s, &s->proj, &s->proj_cap, proj_scratch(rows, dim, rank, true).bytes, nullptr, "sas_reserve_project");
   });
 }
 

@@ -92,23 +92,61 @@ __device__ __forceinline__ void each_adapter(int mine, F f) {
 
 // Block (subtile, slot): the slot-th adapter of the subtile's rows.  Its
 // waves share out up to four rank tiles and, within each, the runs of 32 of
-// dim; the parts meet in LDS in a fixed order.  Blocks past the subtiles
-// write the pieces of f32 hidden states.
+// dim; the parts meet in LDS in a fixed order.  Of the blocks past the
+// subtiles the first puts the rows in order, the others write the pieces of
+// f32 hidden states.
 constexpr int kInnerWaves = 16;
 constexpr int kInnerThreads = 64 * kInnerWaves;
 constexpr int kInnerDeep = 4;  // runs whose loads are in flight together
+
+// The rows in the order of their adapters (rows without one last), so that a
+// tile holds few adapters: a counting sort by one block.  Adapters past the
+// bins share them, and rows of one bin come in any order; a row's result does
+// not depend on its place.
+constexpr int kOrderBins = 1024;
+__device__ void order_rows(const ProjArgs &a) {
+  __shared__ uint32_t bin[kOrderBins];
+  __shared__ uint32_t wsum[kInnerWaves];
+  const int tid = threadIdx.x, lane = tid & 63;
+  bin[tid] = 0u;
+  __syncthreads();
+  auto bin_of = [&](int row) {
+    const int n = adapter_of(a, row);
+    return n < 0 ? kOrderBins - 1 : n % (kOrderBins - 1);
+  };
+  for (int r = tid; r < a.rows; r += kInnerThreads) atomicAdd(&bin[bin_of(r)], 1u);
+  __syncthreads();
+  const uint32_t n = bin[tid];
+  uint32_t x = n;
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) {
+    const uint32_t y = (uint32_t)__shfl_up((int)x, s, 64);
+    if (lane >= s) x += y;
+  }
+  if (lane == 63) wsum[tid >> 6] = x;
+  __syncthreads();
+  for (int w = 0; w < (tid >> 6); ++w) x += wsum[w];
+  bin[tid] = x - n;
+  __syncthreads();
+  for (int r = tid; r < a.rows; r += kInnerThreads) a.perm[atomicAdd(&bin[bin_of(r)], 1u)] = r;
+}
+static_assert(kOrderBins == kInnerThreads, "a thread a bin");
 
 template <bool kF32>
 __global__ __launch_bounds__(kInnerThreads) void proj_inner_kernel(const ProjArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int subs = (a.rows + kSub - 1) / kSub;
-  if ((int)blockIdx.x >= subs) {
+  if ((int)blockIdx.x == subs) {
+    if (a.perm && blockIdx.y == 0) order_rows(a);
+    return;
+  }
+  if ((int)blockIdx.x > subs) {
     if constexpr (kF32) {
       // 8 values a thread
       const int per = a.dim / 8;
       const int64_t n = (int64_t)a.rows * per;
-      const int64_t step = (int64_t)(gridDim.x - subs) * gridDim.y * kInnerThreads;
-      for (int64_t i = ((int64_t)(blockIdx.x - subs) * gridDim.y + blockIdx.y) * kInnerThreads + tid; i < n; i += step) {
+      const int64_t step = (int64_t)(gridDim.x - subs - 1) * gridDim.y * kInnerThreads;
+      for (int64_t i = ((int64_t)(blockIdx.x - subs - 1) * gridDim.y + blockIdx.y) * kInnerThreads + tid; i < n; i += step) {
         const int64_t row = i / per, c = i - row * per;
         u32x4 p[3];
         split8(static_cast<const float *>(a.x) + row * a.x_stride + 8 * c, p);
@@ -200,7 +238,7 @@ __device__ __forceinline__ u32x4 b_ranks(const uint16_t *row, int r, int used) {
 
 // Four outputs from column n on of one row: added to, capped, rounded, stored.
 __device__ __forceinline__ void store4(const ProjArgs &a, int row, int n, f32x4 v) {
-  if (row >= a.rows || n >= a.out_dim) return;
+  if (n >= a.out_dim) return;
   const int left = min(a.out_dim - n, 4);
   const int64_t at = (int64_t)row * a.out_stride + n;
   float *of = static_cast<float *>(a.out) + at;
@@ -232,56 +270,123 @@ __device__ __forceinline__ void store4(const ProjArgs &a, int row, int n, f32x4 
   }
 }
 
-// The adapters among a tile's rows (16 MT, at most 128), one after another:
-// f(adapter, rows of the tile that use it as two masks of 64).
-template <int MT, typename F>
-__device__ __forceinline__ void each_tile_adapter(const ProjArgs &a, int tile0, F f) {
-  const int lane = threadIdx.x & 63;
-  const int lo = lane < 16 * MT ? adapter_of(a, tile0 + lane) : -1;
-  const int hi = MT > 4 && 64 + lane < 16 * MT ? adapter_of(a, tile0 + 64 + lane) : -1;
-  uint64_t l = __ballot(lo >= 0), h = MT > 4 ? __ballot(hi >= 0) : 0ull;
-  while (l | h) {
-    const int cur = l ? __builtin_amdgcn_readlane(lo, __builtin_ctzll(l)) : __builtin_amdgcn_readlane(hi, __builtin_ctzll(h));
-    const uint64_t ml = __ballot(lo == cur), mh = MT > 4 ? __ballot(hi == cur) : 0ull;
-    l &= ~ml;
-    h &= ~mh;
-    f(cur, ml, mh);
+// A tile of 16 MT rows (positions tile0 .. of the order in a.perm): its rows,
+// and its pairs (subtile, adapter) with the subtile's rows that use it.
+template <int MT>
+struct Tile {
+  int row[16 * MT];       // the row at a position; past the last row: the last row
+  int adapter[16 * MT];   // -1: none, or past the last row
+  int pairs;
+  int pair_adapter[16 * MT];
+  uint32_t pair_users[16 * MT];  // subtile << 16 | rows as bits
+};
+
+// Fills l (the block's threads; a barrier before it is read).
+template <int MT>
+__device__ __forceinline__ void tile_rows(const ProjArgs &a, int tile0, Tile<MT> &l) {
+  for (int i = threadIdx.x; i < 16 * MT; i += blockDim.x) {
+    const int at = tile0 + i, row = a.perm ? a.perm[min(at, a.rows - 1)] : min(at, a.rows - 1);
+    l.row[i] = row;
+    l.adapter[i] = at < a.rows ? adapter_of(a, row) : -1;
   }
 }
-
-// Adds adapter `cur`'s term to the sums of the rows of masks ml, mh: the
-// pieces of h (3 rank of them) times B's ranks, three times over, in sums of
-// their own.
-template <int MT, int NT>
-__device__ __forceinline__ void add_adapter(const ProjArgs &a, int cur, uint64_t ml, uint64_t mh, int tile0, int n0,
-                                            f32x4 (&acc)[MT][NT]) {
-  const int lane = threadIdx.x & 63, kc = 8 * (lane >> 4);
-  const int used = rank_of(a, cur);
-  const u32x4 none = {0u, 0u, 0u, 0u};
-  const uint16_t *b = static_cast<const uint16_t *>(a.b) + (int64_t)cur * a.b_adapter_stride;
-  const uint16_t *br[NT];
-#pragma unroll
-  for (int t = 0; t < NT; ++t) br[t] = b + (int64_t)min(n0 + 16 * t + (lane & 15), a.out_dim - 1) * a.b_stride;
-#pragma unroll
+template <int MT>
+__device__ __forceinline__ void tile_pairs(const ProjArgs &a, Tile<MT> &l) {
+  if (threadIdx.x >= 64 || a.adapters == 0) return;
+  const int lane = threadIdx.x;
+  int n = 0;
   for (int m = 0; m < MT; ++m) {
-    const uint32_t users = (uint32_t)((m < 4 ? ml : mh) >> (16 * (m & 3))) & 0xFFFFu;
-    if (!users) continue;
-    const uint16_t *h = a.hp + (int64_t)min(tile0 + 16 * m + (lane & 15), a.rows - 1) * 3 * a.rank;
-    f32x4 ext[NT];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) ext[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int e0 = 0; e0 < 3 * a.rank; e0 += 32) {
-      const int e = e0 + kc;
-      const bool in = e < 3 * a.rank;
-      const int r = e < a.rank ? e : e < 2 * a.rank ? e - a.rank : e - 2 * a.rank;
-      const u32x4 hv = in ? *reinterpret_cast<const u32x4 *>(h + e) : none;
-#pragma unroll
-      for (int t = 0; t < NT; ++t) ext[t] = mfma(in ? b_ranks(br[t], r, used) : none, hv, ext[t]);
+    const int mine = l.adapter[16 * m + (lane & 15)];
+    each_adapter(mine, [&](int cur) {
+      const uint32_t users = (uint32_t)__ballot(mine == cur) & 0xFFFFu;
+      if (lane == 0) {
+        l.pair_adapter[n] = cur;
+        l.pair_users[n] = (uint32_t)m << 16 | users;
+      }
+      ++n;
+    });
+  }
+  if (lane == 0) l.pairs = n;
+}
+
+// Adds the tile's adapters' terms, B times the pieces of h, 32 ranks an item,
+// an item's loads ahead of the products of the one before.  An item's sums are its own and
+// only the adapter's rows add them.  mine(adapter): whether this wave takes it.
+template <int MT, int NT, typename F>
+__device__ __forceinline__ void add_adapters(const ProjArgs &a, const Tile<MT> &l, int n0, F takes, f32x4 (&acc)[MT][NT]) {
+  const int lane = threadIdx.x & 63, q = lane >> 4;
+  const u32x4 none = {0u, 0u, 0u, 0u};
+  const int blocks = (a.rank + 31) / 32, pairs = l.pairs;
+  struct Item {
+    int m;          // subtile, -1: no item
+    uint32_t users;
+    int products;
+    u32x4 b[NT], h[3];
+  };
+  int at = -1, rb = blocks - 1, cur = 0, used = 0;
+  uint32_t mu = 0;
+  // the next item's loads
+  auto next = [&](Item &it) __attribute__((always_inline)) {
+    if (++rb == blocks) {
+      rb = 0;
+      do ++at;
+      while (at < pairs && !takes(l.pair_adapter[at]));
+      if (at < pairs) {
+        cur = __builtin_amdgcn_readfirstlane(l.pair_adapter[at]);
+        mu = __builtin_amdgcn_readfirstlane(l.pair_users[at]);
+        used = rank_of(a, cur);
+      }
     }
-    const bool mine = (users >> (lane & 15)) & 1u;
+    it.m = -1;
+    if (at >= pairs) {
+      rb = blocks - 1;  // (stays past the end)
+      return;
+    }
+    it.m = (int)(mu >> 16);
+    it.users = mu & 0xFFFFu;
+    const int r0 = 32 * rb, n = a.rank - r0;  // ranks from r0 on
+    // The four octets of an operand: of up to 8 ranks the three pieces (one
+    // product), of up to 16 two pieces and then the third (two), of more one
+    // piece after another (three).  B's octets repeat under them.
+    const int oct = n <= 8 ? 0 : n <= 16 ? q & 1 : q;
+    it.products = n <= 8 ? 1 : n <= 16 ? 2 : 3;
+    const uint16_t *b = static_cast<const uint16_t *>(a.b) + (int64_t)cur * a.b_adapter_stride;
 #pragma unroll
     for (int t = 0; t < NT; ++t)
-      if (mine) acc[m][t] = acc[m][t] + ext[t];
+      it.b[t] = b_ranks(b + (int64_t)min(n0 + 16 * t + (lane & 15), a.out_dim - 1) * a.b_stride, r0 + 8 * oct, used);
+    const uint16_t *h = a.hp + (int64_t)l.row[16 * it.m + (lane & 15)] * 3 * a.rank + r0 + 8 * oct;
+#pragma unroll
+    for (int j = 0; j < 3; ++j) {
+      const int piece = n <= 8 ? q : n <= 16 ? 2 * j + (q >> 1) : j;
+      it.h[j] = j < it.products && piece < 3 && r0 + 8 * oct < a.rank ? *reinterpret_cast<const u32x4 *>(h + piece * a.rank) : none;
+    }
+  };
+  auto add = [&](const Item &it) __attribute__((always_inline)) {
+    f32x4 ext[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) ext[t] = mfma(it.b[t], it.h[0], f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+#pragma unroll
+    for (int j = 1; j < 3; ++j)
+      if (j < it.products)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) ext[t] = mfma(it.b[t], it.h[j], ext[t]);
+    const bool mine = (it.users >> (lane & 15)) & 1u;
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+      if (m == it.m)
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[m][t][i] += mine ? ext[t][i] : 0.0f;
+  };
+  Item x, y;
+  next(x);
+  while (x.m >= 0) {
+    next(y);
+    add(x);
+    if (y.m < 0) return;
+    next(x);
+    add(y);
   }
 }
 
@@ -328,6 +433,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void proj_wide_kernel(const ProjAr
   using C = Wide<MT, NT, P>;
   __shared__ u32x4 xs[2][C::kTiles][kSlots];
   __shared__ u32x4 ws[kWideWaves][NT][kSlots];
+  __shared__ Tile<MT> tile;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int mtiles = (a.rows + 16 * MT - 1) / (16 * MT);
   const int pos = xcd_run((int)blockIdx.x, (int)gridDim.x);
@@ -338,35 +444,41 @@ __global__ __launch_bounds__(kWideThreads, 2) void proj_wide_kernel(const ProjAr
   for (int m = 0; m < MT; ++m)
 #pragma unroll
     for (int t = 0; t < NT; ++t) acc[m][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  tile_rows<MT>(a, tile0, tile);
+  __syncthreads();
+  tile_pairs<MT>(a, tile);
   if (a.weight) {
     const int runs = (a.dim + kRun - 1) / kRun, chunks = (runs + C::kSteps - 1) / C::kSteps;
     const int oct = 8 * (lane & 7);
     const bool once = mtiles == 1;
-    const uint16_t *wr[NT][2];
+    // byte offsets from the wave's first weight row
+    const int w0 = min(n0, a.out_dim - 1);
+    const char *wbase = static_cast<const char *>(a.weight) + (int64_t)w0 * a.weight_stride * 2;
+    uint32_t wr[NT][2];
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int j = 0; j < 2; ++j)
-        wr[t][j] = static_cast<const uint16_t *>(a.weight) +
-                   (int64_t)min(n0 + 16 * t + 8 * j + (lane >> 3), a.out_dim - 1) * a.weight_stride + oct;
+        wr[t][j] = ((uint32_t)(min(n0 + 16 * t + 8 * j + (lane >> 3), a.out_dim - 1) - w0) * (uint32_t)a.weight_stride + oct) * 2u;
     // run g of the weight rows (past the last: the last again)
     auto load_w = [&](int g, u32x4 (&w)[NT][2]) __attribute__((always_inline)) {
       const int k = kRun * min(g, runs - 1);
+      const char *wk = wbase + 2 * (int64_t)k;
       if (k + kRun > a.dim) {
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int j = 0; j < 2; ++j) w[t][j] = k + oct < a.dim ? *reinterpret_cast<const u32x4 *>(wr[t][j] + k) : none;
+          for (int j = 0; j < 2; ++j) w[t][j] = k + oct < a.dim ? *reinterpret_cast<const u32x4 *>(wk + wr[t][j]) : none;
       } else if (once) {
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int j = 0; j < 2; ++j) w[t][j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(wr[t][j] + k));
+          for (int j = 0; j < 2; ++j) w[t][j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(wk + wr[t][j]));
       } else {
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int j = 0; j < 2; ++j) w[t][j] = *reinterpret_cast<const u32x4 *>(wr[t][j] + k);
+          for (int j = 0; j < 2; ++j) w[t][j] = *reinterpret_cast<const u32x4 *>(wk + wr[t][j]);
       }
     };
     // this wave's loads of chunk c: load f is half f % 2 of operand f / 2 =
@@ -375,7 +487,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void proj_wide_kernel(const ProjAr
 #pragma unroll
     for (int i = 0; i < C::kMine; ++i) {
       const int f = min(wave + kWideWaves * i, 2 * C::kTiles - 1), m = (f / 2) % MT, p = (f / 2 / MT) % P;
-      const int64_t row = min(tile0 + 16 * m + 8 * (f & 1) + (lane >> 3), a.rows - 1);
+      const int64_t row = tile.row[16 * m + 8 * (f & 1) + (lane >> 3)];
       xr[i] = (P == 1 ? static_cast<const uint16_t *>(a.x) + row * a.x_stride : a.xp + ((int64_t)p * a.rows + row) * a.dim) +
               kRun * (f / 2 / MT / P) + oct;
     }
@@ -445,13 +557,15 @@ __global__ __launch_bounds__(kWideThreads, 2) void proj_wide_kernel(const ProjAr
       }
     }
   }
+  else __syncthreads();
   if (n0 >= a.out_dim) return;
-  if (a.adapters > 0)
-    each_tile_adapter<MT>(a, tile0, [&](int cur, uint64_t ml, uint64_t mh) { add_adapter<MT, NT>(a, cur, ml, mh, tile0, n0, acc); });
+  if (a.adapters > 0) add_adapters<MT, NT>(a, tile, n0, [](int) { return true; }, acc);
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
-    for (int t = 0; t < NT; ++t) store4(a, tile0 + 16 * m + (lane & 15), n0 + 16 * t + 4 * (lane >> 4), acc[m][t]);
+    for (int t = 0; t < NT; ++t)
+      if (tile0 + 16 * m + (lane & 15) < a.rows)
+        store4(a, tile.row[16 * m + (lane & 15)], n0 + 16 * t + 4 * (lane >> 4), acc[m][t]);
 }
 
 // Few outputs: eight waves split dim (and the tile's adapters) for the same
@@ -462,6 +576,7 @@ constexpr int kSplitWaves = 8;
 template <int MT, int NT, int P>
 __global__ __launch_bounds__(64 * kSplitWaves) void proj_split_kernel(const ProjArgs a) {
   __shared__ f32x4 part[kSplitWaves][MT * NT][64];
+  __shared__ Tile<MT> tile;
   constexpr int U = MT * P >= 8 ? 1 : MT * P >= 4 ? 2 : 4;  // runs of 32 whose loads are in flight together
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int mtiles = (a.rows + 16 * MT - 1) / (16 * MT);
@@ -474,6 +589,10 @@ __global__ __launch_bounds__(64 * kSplitWaves) void proj_split_kernel(const Proj
   for (int m = 0; m < MT; ++m)
 #pragma unroll
     for (int t = 0; t < NT; ++t) acc[m][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  tile_rows<MT>(a, tile0, tile);
+  __syncthreads();
+  tile_pairs<MT>(a, tile);
+  __syncthreads();
   if (a.weight) {
     const int steps = (a.dim + 31) / 32, g0 = steps * wave / kSplitWaves, g1 = steps * (wave + 1) / kSplitWaves;
     const uint16_t *wr[NT], *xr[MT][P];
@@ -482,7 +601,7 @@ __global__ __launch_bounds__(64 * kSplitWaves) void proj_split_kernel(const Proj
       wr[t] = static_cast<const uint16_t *>(a.weight) + (int64_t)min(n0 + 16 * t + (lane & 15), a.out_dim - 1) * a.weight_stride + kc;
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-      const int64_t row = min(tile0 + 16 * m + (lane & 15), a.rows - 1);
+      const int64_t row = tile.row[16 * m + (lane & 15)];
 #pragma unroll
       for (int p = 0; p < P; ++p)
         xr[m][p] = (P == 1 ? static_cast<const uint16_t *>(a.x) + row * a.x_stride : a.xp + ((int64_t)p * a.rows + row) * a.dim) + kc;
@@ -510,12 +629,9 @@ __global__ __launch_bounds__(64 * kSplitWaves) void proj_split_kernel(const Proj
             for (int t = 0; t < NT; ++t) acc[m][t] = mfma(w[u][t], x[u][m][p], acc[m][t]);
     }
   }
-  if (a.adapters > 0) {
-    int at = 0;
-    each_tile_adapter<MT>(a, tile0, [&](int cur, uint64_t ml, uint64_t mh) {
-      if (at++ % kSplitWaves == wave) add_adapter<MT, NT>(a, cur, ml, mh, tile0, n0, acc);
-    });
-  }
+  // (by the adapter, not its place in the tile: a row's sums then do not
+  // depend on the order of the rows)
+  if (a.adapters > 0) add_adapters<MT, NT>(a, tile, n0, [&](int cur) { return cur % kSplitWaves == wave; }, acc);
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -525,7 +641,8 @@ __global__ __launch_bounds__(64 * kSplitWaves) void proj_split_kernel(const Proj
     f32x4 v = part[0][i][lane];
 #pragma unroll
     for (int w = 1; w < kSplitWaves; ++w) v = v + part[w][i][lane];
-    store4(a, tile0 + 16 * (i / NT) + (lane & 15), n0 + 16 * (i % NT) + 4 * (lane >> 4), v);
+    const int at = 16 * (i / NT) + (lane & 15);
+    if (tile0 + at < a.rows) store4(a, tile.row[at], n0 + 16 * (i % NT) + 4 * (lane >> 4), v);
   }
 }
 
@@ -569,16 +686,21 @@ void launch_rows(const ProjArgs &a, hipStream_t stream) {
 
 }  // namespace
 
-size_t proj_scratch_bytes(int rows, int dim, int rank, bool x_f32) {
-  const size_t h = ((size_t)rows * 3 * rank * 2 + 255) & ~size_t(255);
-  return h + (x_f32 ? (size_t)rows * 3 * dim * 2 : 0);
+// The order of the rows, h, then the pieces of x.
+ProjScratch proj_scratch(int rows, int dim, int rank, bool x_f32) {
+  auto up = [](size_t n) { return (n + 255) & ~size_t(255); };
+  ProjScratch p;
+  p.hp = rank > 0 ? up((size_t)rows * 4) : 0;
+  p.xp = p.hp + up((size_t)rows * 3 * rank * 2);
+  p.bytes = p.xp + (x_f32 ? (size_t)rows * 3 * dim * 2 : 0);
+  return p;
 }
 
 hipError_t launch_project(const ProjArgs &a, hipStream_t stream) {
   const int subs = (a.rows + kSub - 1) / kSub;
   if (a.adapters > 0 || a.xp) {
     const int split = a.xp ? (int)(((int64_t)a.rows * (a.dim / 8) + kSub * kInnerThreads - 1) / (kSub * kInnerThreads)) : 0;
-    const dim3 grid(subs + (split > 1024 ? 1024 : split), kSub);
+    const dim3 grid(subs + 1 + (split > 1024 ? 1024 : split), kSub);
     if (a.x_f32) proj_inner_kernel<true><<<grid, kInnerThreads, 0, stream>>>(a);
     else proj_inner_kernel<false><<<grid, kInnerThreads, 0, stream>>>(a);
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;

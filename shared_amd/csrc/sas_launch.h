@@ -212,6 +212,7 @@ struct ProjArgs {
   // [3][rows][dim] (null: bf16 hidden states, or no weight).
   uint16_t *hp;
   uint16_t *xp;
+  int32_t *perm;  // the rows in the order of their adapters, or null (as they come)
   int32_t rows;
   int32_t dim;
   int32_t out_dim;
@@ -224,7 +225,11 @@ struct ProjArgs {
   int32_t cus;
 };
 
-size_t proj_scratch_bytes(int rows, int dim, int rank, bool x_f32);
+// Byte offsets in the scratch, and its size.
+struct ProjScratch {
+  size_t hp, xp, bytes;
+};
+ProjScratch proj_scratch(int rows, int dim, int rank, bool x_f32);
 hipError_t launch_project(const ProjArgs &a, hipStream_t stream);
 
 // ---------------------------------------------------------------- filter --
