@@ -13,6 +13,8 @@
 //      with B of each adapter among a tile's rows, each adapter in sums of its
 //      own that only its rows add: a value that is not finite stays with its
 //      adapter.
+#include <utility>
+
 #include "sas_device.h"
 #include "sas_launch.h"
 
@@ -236,37 +238,56 @@ __device__ __forceinline__ u32x4 b_ranks(const uint16_t *row, int r, int used) {
   return w;
 }
 
-// Four outputs from column n on of one row: added to, capped, rounded, stored.
-__device__ __forceinline__ void store4(const ProjArgs &a, int row, int n, f32x4 v) {
+// tanh within 1.4 ulp or so: below 0.625 x + x^3 P(x^2), P fitted to the
+// relative error (4.4e-9), above 1 - 2 / (e^2|x| + 1).  A third of tanhf's
+// instructions: 34 million capped values took 30 us of a call's 440.
+__device__ __forceinline__ float tanh_fast(float x) {
+  const float ax = fabsf(x), u = x * x;
+  float p = -0.005704975221306086f;
+  p = __builtin_fmaf(p, u, 0.020639074966311455f);
+  p = __builtin_fmaf(p, u, -0.05373971164226532f);
+  p = __builtin_fmaf(p, u, 0.13331441581249237f);
+  p = __builtin_fmaf(p, u, -0.3333328068256378f);
+  const float small = __builtin_fmaf(x * u, p, x);
+  const float e = __builtin_amdgcn_exp2f(fminf(ax, 16.0f) * 2.8853900817779268f);  // e^2|x|
+  const float large = copysignf(__builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(e + 1.0f), 1.0f), x);
+  return x != x ? x : ax < 0.625f ? small : large;
+}
+
+// The last steps of four sums of row `row`, outputs n .. n + 3: added to what
+// is there, capped, rounded, stored.  Nontemporal: the result is not read here
+// (128 x 262,144 f32: 312 -> 281 us a call, 268 with whole lines a row).
+__device__ __forceinline__ void finish4(const ProjArgs &a, int row, int n, f32x4 v) {
   if (n >= a.out_dim) return;
-  const int left = min(a.out_dim - n, 4);
+  const bool whole = n + 4 <= a.out_dim;
   const int64_t at = (int64_t)row * a.out_stride + n;
   float *of = static_cast<float *>(a.out) + at;
   uint16_t *ob = static_cast<uint16_t *>(a.out) + at;
   if (a.accumulate) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (i < left) v[i] += a.out_bf16 ? __uint_as_float((uint32_t)ob[i] << 16) : of[i];
+      if (n + i < a.out_dim) v[i] += a.out_bf16 ? __uint_as_float((uint32_t)ob[i] << 16) : of[i];
   }
   if (a.softcap > 0.0f) {
+    const float inv = 1.0f / a.softcap;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = a.softcap * tanhf(v[i] / a.softcap);
+    for (int i = 0; i < 4; ++i) v[i] = a.softcap * tanh_fast(v[i] * inv);
   }
   if (a.out_bf16) {
     const u16x4 p = {bf16_of(v[0]), bf16_of(v[1]), bf16_of(v[2]), bf16_of(v[3])};
-    if (left == 4) {
-      *reinterpret_cast<u16x4u *>(ob) = p;
+    if (whole) {
+      __builtin_nontemporal_store(p, reinterpret_cast<u16x4u *>(ob));
     } else {
 #pragma unroll
       for (int i = 0; i < 3; ++i)
-        if (i < left) ob[i] = p[i];
+        if (n + i < a.out_dim) ob[i] = p[i];
     }
-  } else if (left == 4) {
-    *reinterpret_cast<f32x4u *>(of) = v;
+  } else if (whole) {
+    __builtin_nontemporal_store(v, reinterpret_cast<f32x4u *>(of));
   } else {
 #pragma unroll
     for (int i = 0; i < 3; ++i)
-      if (i < left) of[i] = v[i];
+      if (n + i < a.out_dim) of[i] = v[i];
   }
 }
 
@@ -361,32 +382,37 @@ __device__ __forceinline__ void add_adapters(const ProjArgs &a, const Tile<MT> &
       it.h[j] = j < it.products && piece < 3 && r0 + 8 * oct < a.rank ? *reinterpret_cast<const u32x4 *>(h + piece * a.rank) : none;
     }
   };
-  auto add = [&](const Item &it) __attribute__((always_inline)) {
+  auto add = [&](const Item &it, f32x4 (&sum)[NT]) __attribute__((always_inline)) {
     f32x4 ext[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) ext[t] = mfma(it.b[t], it.h[0], f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+    // (operands past `products` are zero, but B's may hold what is not finite)
+    if (it.products > 1) {
 #pragma unroll
-    for (int j = 1; j < 3; ++j)
-      if (j < it.products)
+      for (int t = 0; t < NT; ++t) ext[t] = mfma(it.b[t], it.h[1], ext[t]);
+    }
+    if (it.products > 2) {
 #pragma unroll
-        for (int t = 0; t < NT; ++t) ext[t] = mfma(it.b[t], it.h[j], ext[t]);
+      for (int t = 0; t < NT; ++t) ext[t] = mfma(it.b[t], it.h[2], ext[t]);
+    }
     const bool mine = (it.users >> (lane & 15)) & 1u;
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
-      if (m == it.m)
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[m][t][i] += mine ? ext[t][i] : 0.0f;
+      for (int i = 0; i < 4; ++i) sum[t][i] += mine ? ext[t][i] : 0.0f;
   };
-  Item x, y;
+  // the pairs come subtile by subtile: the sums of each have a loop of their
+  // own (selecting them by a variable doubles the kernel's registers)
+  Item x;
   next(x);
-  while (x.m >= 0) {
-    next(y);
-    add(x);
-    if (y.m < 0) return;
-    next(x);
-    add(y);
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    while (x.m == m) {
+      Item y;
+      next(y);
+      add(x, acc[m]);
+      x = y;
+    }
   }
 }
 
@@ -394,6 +420,16 @@ __device__ __forceinline__ void add_adapters(const ProjArgs &a, const Tile<MT> &
 __device__ __forceinline__ int xcd_run(int i, int n) {
   const int per = n / 8, left = n % 8, x = i % 8;
   return x * per + min(x, left) + i / 8;
+}
+
+// f(integral_constant 0) .. f(integral_constant N - 1).
+template <int N, typename F, int... I>
+__device__ __forceinline__ void each_const_of(F f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void each_const(F f) {
+  each_const_of<N>(f, std::make_integer_sequence<int, N>{});
 }
 
 // An operand of 16 rows x 64 values (2 KB): loaded eight lanes a row, whole
@@ -421,24 +457,30 @@ constexpr int kWideThreads = 64 * kWideWaves;
 template <int MT, int NT, int P>
 struct Wide {
   static constexpr int kBlockOut = kWideWaves * 16 * NT;
-  static constexpr int kSteps = MT * P >= 4 ? 1 : MT * P >= 2 ? 2 : 4;  // runs a chunk
-  static constexpr int kDeep = NT == 1 ? 4 : 2;
-  static constexpr int kUnroll = kDeep > kSteps ? kDeep / kSteps : 1;   // chunks a turn of the loop
+  static constexpr int kSteps = MT * P >= 5 ? 1 : MT * P >= 2 ? 2 : 4;  // runs a chunk
+  static constexpr int kDeep = NT == 1 || (MT >= 7 && P == 1) ? 4 : 2;  // runs of the weight rows in registers
+  // Chunks of the hidden states in registers: as far ahead as the weight rows.
+  // Loads end in the order they began, so waiting for a younger chunk would
+  // wait for every weight row behind it (128 rows: 4 runs ahead were no
+  // faster than 2 until the hidden states were too).
+  static constexpr int kAhead = kDeep / kSteps > 2 ? kDeep / kSteps : 2;
+  static constexpr int kUnroll = kAhead;  // chunks a turn of the loop
   static constexpr int kTiles = kSteps * P * MT;                        // operands of a chunk
   static constexpr int kMine = (2 * kTiles + kWideWaves - 1) / kWideWaves;  // a wave's loads of them
 };
 
-template <int MT, int NT, int P>
-__global__ __launch_bounds__(kWideThreads, 2) void proj_wide_kernel(const ProjArgs a) {
+// kOnce: one tile holds all rows, so that no other block reads a weight row
+// again (nontemporal loads then: 6.2 -> 6.9 TB/s in a bare stream of a head).
+template <int MT, int NT, int P, bool kOnce>
+__global__ __launch_bounds__(kWideThreads, P == 1 && MT <= 6 ? 4 : 2) void proj_wide_kernel(const ProjArgs a) {
   using C = Wide<MT, NT, P>;
   __shared__ u32x4 xs[2][C::kTiles][kSlots];
   __shared__ u32x4 ws[kWideWaves][NT][kSlots];
   __shared__ Tile<MT> tile;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int mtiles = (a.rows + 16 * MT - 1) / (16 * MT);
+  const int mtiles = kOnce ? 1 : (a.rows + 16 * MT - 1) / (16 * MT);
   const int pos = xcd_run((int)blockIdx.x, (int)gridDim.x);
   const int tile0 = (pos % mtiles) * 16 * MT, n0 = (pos / mtiles) * C::kBlockOut + wave * 16 * NT;
-  const u32x4 none = {0u, 0u, 0u, 0u};
   f32x4 acc[MT][NT];
 #pragma unroll
   for (int m = 0; m < MT; ++m)
@@ -447,78 +489,74 @@ __global__ __launch_bounds__(kWideThreads, 2) void proj_wide_kernel(const ProjAr
   tile_rows<MT>(a, tile0, tile);
   __syncthreads();
   tile_pairs<MT>(a, tile);
+  // piece p of the hidden state at a position
+  auto x_row = [&](int p, int at) {
+    const int64_t row = tile.row[at];
+    return P == 1 ? static_cast<const uint16_t *>(a.x) + row * a.x_stride : a.xp + ((int64_t)p * a.rows + row) * a.dim;
+  };
   if (a.weight) {
-    const int runs = (a.dim + kRun - 1) / kRun, chunks = (runs + C::kSteps - 1) / C::kSteps;
-    const int oct = 8 * (lane & 7);
-    const bool once = mtiles == 1;
-    // byte offsets from the wave's first weight row
+    const int chunks = a.dim / (kRun * C::kSteps), runs = chunks * C::kSteps;  // whole ones
     const int w0 = min(n0, a.out_dim - 1);
-    const char *wbase = static_cast<const char *>(a.weight) + (int64_t)w0 * a.weight_stride * 2;
-    uint32_t wr[NT][2];
+    if (chunks > 0) {
+      // byte offsets from the wave's first weight row
+      const char *wbase = static_cast<const char *>(a.weight) + (int64_t)w0 * a.weight_stride * 2;
+      uint32_t wr[NT][2];
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
-        wr[t][j] = ((uint32_t)(min(n0 + 16 * t + 8 * j + (lane >> 3), a.out_dim - 1) - w0) * (uint32_t)a.weight_stride + oct) * 2u;
-    // run g of the weight rows (past the last: the last again)
-    auto load_w = [&](int g, u32x4 (&w)[NT][2]) __attribute__((always_inline)) {
-      const int k = kRun * min(g, runs - 1);
-      const char *wk = wbase + 2 * (int64_t)k;
-      if (k + kRun > a.dim) {
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) w[t][j] = k + oct < a.dim ? *reinterpret_cast<const u32x4 *>(wk + wr[t][j]) : none;
-      } else if (once) {
+        for (int j = 0; j < 2; ++j)
+          wr[t][j] = ((uint32_t)(min(n0 + 16 * t + 8 * j + (lane >> 3), a.out_dim - 1) - w0) * (uint32_t)a.weight_stride + 8 * (lane & 7)) * 2u;
+      // run g of the weight rows (past the last: the last again)
+      auto load_w = [&](int g, u32x4 (&w)[NT][2]) __attribute__((always_inline)) {
+        const char *wk = wbase + 2 * kRun * (int64_t)min(g, runs - 1);
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int j = 0; j < 2; ++j) w[t][j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(wk + wr[t][j]));
-      } else {
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) w[t][j] = *reinterpret_cast<const u32x4 *>(wk + wr[t][j]);
-      }
-    };
-    // this wave's loads of chunk c: load f is half f % 2 of operand f / 2 =
-    // (step, piece, subtile); operands past dim (a last chunk's) are zero
-    const uint16_t *xr[C::kMine];
-#pragma unroll
-    for (int i = 0; i < C::kMine; ++i) {
-      const int f = min(wave + kWideWaves * i, 2 * C::kTiles - 1), m = (f / 2) % MT, p = (f / 2 / MT) % P;
-      const int64_t row = tile.row[16 * m + 8 * (f & 1) + (lane >> 3)];
-      xr[i] = (P == 1 ? static_cast<const uint16_t *>(a.x) + row * a.x_stride : a.xp + ((int64_t)p * a.rows + row) * a.dim) +
-              kRun * (f / 2 / MT / P) + oct;
-    }
-    auto load_x = [&](int c, u32x4 (&x)[C::kMine]) __attribute__((always_inline)) {
-      const int k = kRun * C::kSteps * min(c, chunks - 1);
+          for (int j = 0; j < 2; ++j) {
+            const u32x4 *src = reinterpret_cast<const u32x4 *>(wk + wr[t][j]);
+            w[t][j] = kOnce ? __builtin_nontemporal_load(src) : *src;
+          }
+      };
+      // this wave's loads of chunk c: load f is half f % 2 of operand f / 2 =
+      // (step, piece, subtile)
+      const uint16_t *xr[C::kMine];
 #pragma unroll
       for (int i = 0; i < C::kMine; ++i) {
-        const int f = min(wave + kWideWaves * i, 2 * C::kTiles - 1), at = k + kRun * (f / 2 / MT / P);
-        if (at + kRun > a.dim) x[i] = at + oct < a.dim ? *reinterpret_cast<const u32x4 *>(xr[i] + k) : none;
-        else x[i] = *reinterpret_cast<const u32x4 *>(xr[i] + k);
+        const int f = min(wave + kWideWaves * i, 2 * C::kTiles - 1);
+        xr[i] = x_row((f / 2 / MT) % P, 16 * ((f / 2) % MT) + 8 * (f & 1) + (lane >> 3)) + kRun * (f / 2 / MT / P) + 8 * (lane & 7);
       }
-    };
-    auto store_x = [&](int buf, const u32x4 (&x)[C::kMine]) __attribute__((always_inline)) {
+      auto load_x = [&](int c, u32x4 (&x)[C::kMine]) __attribute__((always_inline)) {
+        const int64_t k = kRun * C::kSteps * (int64_t)min(c, chunks - 1);
 #pragma unroll
-      for (int i = 0; i < C::kMine; ++i) {
-        const int f = wave + kWideWaves * i;
-        if (2 * C::kTiles % kWideWaves == 0 || f < 2 * C::kTiles) xs[buf][f / 2][put_slot(f & 1)] = x[i];
+        for (int i = 0; i < C::kMine; ++i) x[i] = *reinterpret_cast<const u32x4 *>(xr[i] + k);
+      };
+      auto store_x = [&](int buf, const u32x4 (&x)[C::kMine]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < C::kMine; ++i) {
+          const int f = wave + kWideWaves * i;
+          if (2 * C::kTiles % kWideWaves == 0 || f < 2 * C::kTiles) xs[buf][f / 2][put_slot(f & 1)] = x[i];
+        }
+      };
+      u32x4 w[C::kDeep][NT][2], x[C::kAhead][C::kMine];
+      // in the order of their use (a wait in the loop covers the loop's first
+      // turn too)
+#pragma unroll
+      for (int d = 0; d < C::kAhead; ++d) {
+        load_x(d, x[d]);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int e = 0; e < C::kDeep; ++e)
+          if (e / C::kSteps == d || (d == C::kAhead - 1 && e / C::kSteps > d)) {
+            load_w(e, w[e]);
+            __builtin_amdgcn_sched_barrier(0);
+          }
       }
-    };
-    u32x4 w[C::kDeep][NT][2], x[C::kMine];
-    load_x(0, x);
-#pragma unroll
-    for (int d = 0; d < C::kDeep; ++d) load_w(d, w[d]);
-    store_x(0, x);
-    load_x(1, x);
-    lds_barrier();
-    for (int c0 = 0; c0 < chunks; c0 += C::kUnroll) {
-#pragma unroll
-      for (int v = 0; v < C::kUnroll; ++v) {
-        const int c = c0 + v;
-        if (c >= chunks) break;
+      store_x(0, x[0]);
+      lds_barrier();
+      // chunk c, the v-th of its turn, then the next one's hidden states (past
+      // the last the last again)
+      auto chunk = [&](int c, auto vt) __attribute__((always_inline)) {
+        constexpr int v = decltype(vt)::value;
 #pragma unroll
         for (int s = 0; s < C::kSteps; ++s) {
           constexpr int D = C::kDeep;
@@ -529,6 +567,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void proj_wide_kernel(const ProjAr
             for (int j = 0; j < 2; ++j) ws[wave][t][put_slot(j)] = w[slot][t][j];
           // the loads stay here: left to itself the compiler moves them down to
           // where they are used, and every run waits for memory
+          if (s == 0) load_x(c + C::kAhead, x[v]);
           load_w(c * C::kSteps + s + D, w[slot]);
           wave_lds_sync();
           __builtin_amdgcn_sched_barrier(0);
@@ -541,31 +580,70 @@ __global__ __launch_bounds__(kWideThreads, 2) void proj_wide_kernel(const ProjAr
             for (int m = 0; m < MT; ++m)
 #pragma unroll
               for (int p = 0; p < P; ++p) {
-                const u32x4 xv = xs[c & 1][(s * P + p) * MT + m][get_slot(h)];
+                const u32x4 xv = xs[v & 1][(s * P + p) * MT + m][get_slot(h)];
 #pragma unroll
                 for (int t = 0; t < NT; ++t) acc[m][t] = mfma(wv[t], xv, acc[m][t]);
               }
           }
           __builtin_amdgcn_sched_barrier(0);
         }
-        if (c + 1 < chunks) {
-          store_x((c + 1) & 1, x);
-          load_x(c + 2, x);
-          __builtin_amdgcn_sched_barrier(0);
-          lds_barrier();
-        }
-      }
+        store_x((v + 1) & 1, x[(v + 1) % C::kAhead]);
+        __builtin_amdgcn_sched_barrier(0);
+        lds_barrier();
+      };
+      // Whole turns first: the loop has no way out but its end (a way from its
+      // middle back to its head, even one never taken, would make the waits at
+      // the head cover the loads just begun).
+      int c = 0;
+      for (; c + C::kUnroll <= chunks; c += C::kUnroll) each_const<C::kUnroll>([&](auto v) { chunk(c + decltype(v)::value, v); });
+      each_const<C::kUnroll - 1>([&](auto v) {
+        if (c + decltype(v)::value < chunks) chunk(c + decltype(v)::value, v);
+      });
     }
-  }
-  else __syncthreads();
-  if (n0 >= a.out_dim) return;
-  if (a.adapters > 0) add_adapters<MT, NT>(a, tile, n0, [](int) { return true; }, acc);
+    if (chunks == 0) __syncthreads();
+    // what is left of dim, straight to registers
+    const u32x4 none = {0u, 0u, 0u, 0u};
+    for (int k0 = runs * kRun; k0 < a.dim; k0 += 32) {
+      const int k = k0 + 8 * (lane >> 4);
+      const bool in = k < a.dim;
+      u32x4 wv[NT];
 #pragma unroll
-  for (int m = 0; m < MT; ++m)
+      for (int t = 0; t < NT; ++t)
+        wv[t] = in ? *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(a.weight) +
+                                                      (int64_t)min(n0 + 16 * t + (lane & 15), a.out_dim - 1) * a.weight_stride + k)
+                   : none;
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+          const u32x4 xv = in ? *reinterpret_cast<const u32x4 *>(x_row(p, 16 * m + (lane & 15)) + k) : none;
+#pragma unroll
+          for (int t = 0; t < NT; ++t) acc[m][t] = mfma(wv[t], xv, acc[m][t]);
+        }
+    }
+  } else {
+    __syncthreads();
+  }
+  if (a.adapters > 0 && n0 < a.out_dim) add_adapters<MT, NT>(a, tile, n0, [](int) { return true; }, acc);
+  // A subtile's rows at a time through LDS, so that a row's outputs go out in
+  // whole lines (lane: outputs 4 l .. of a row).
+  constexpr int kPitch = C::kBlockOut + 4, kLanes = C::kBlockOut / 4, kRows = 64 / kLanes;
+  static_assert(16 * kPitch * 4 <= (int)sizeof(xs), "a subtile's sums fit");
+  float *stage = reinterpret_cast<float *>(&xs[0][0][0]);
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    lds_barrier();
 #pragma unroll
     for (int t = 0; t < NT; ++t)
-      if (tile0 + 16 * m + (lane & 15) < a.rows)
-        store4(a, tile.row[16 * m + (lane & 15)], n0 + 16 * t + 4 * (lane >> 4), acc[m][t]);
+      *reinterpret_cast<f32x4 *>(stage + (lane & 15) * kPitch + wave * 16 * NT + 16 * t + 4 * (lane >> 4)) = acc[m][t];
+    lds_barrier();
+#pragma unroll
+    for (int r = wave * kRows; r < 16; r += kWideWaves * kRows) {
+      const int at = 16 * m + r + lane / kLanes, col = 4 * (lane % kLanes);
+      const f32x4 v = *reinterpret_cast<const f32x4 *>(stage + (r + lane / kLanes) * kPitch + col);
+      if (tile0 + at < a.rows) finish4(a, tile.row[at], (pos / mtiles) * C::kBlockOut + col, v);
+    }
+  }
 }
 
 // Few outputs: eight waves split dim (and the tile's adapters) for the same
@@ -642,7 +720,7 @@ __global__ __launch_bounds__(64 * kSplitWaves) void proj_split_kernel(const Proj
 #pragma unroll
     for (int w = 1; w < kSplitWaves; ++w) v = v + part[w][i][lane];
     const int at = 16 * (i / NT) + (lane & 15);
-    if (tile0 + at < a.rows) store4(a, tile.row[at], n0 + 16 * (i % NT) + 4 * (lane >> 4), v);
+    if (tile0 + at < a.rows) finish4(a, tile.row[at], n0 + 16 * (i % NT) + 4 * (lane >> 4), v);
   }
 }
 
@@ -650,7 +728,9 @@ template <int MT, int NT, int P>
 void launch_wide(const ProjArgs &a, hipStream_t stream) {
   using C = Wide<MT, NT, P>;
   const int blocks = ((a.rows + 16 * MT - 1) / (16 * MT)) * ((a.out_dim + C::kBlockOut - 1) / C::kBlockOut);
-  proj_wide_kernel<MT, NT, P><<<blocks, kWideThreads, 0, stream>>>(a);
+  // a tile of up to four subtiles has all rows (launch_rows)
+  if (MT <= 4 || a.rows <= 16 * MT) proj_wide_kernel<MT, NT, P, true><<<blocks, kWideThreads, 0, stream>>>(a);
+  else proj_wide_kernel<MT, NT, P, MT <= 4><<<blocks, kWideThreads, 0, stream>>>(a);
 }
 
 template <int MT, int NT, int P>
