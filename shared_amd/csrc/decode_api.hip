@@ -183,6 +183,10 @@ int sas_sample_filtered(sas_sampler *s, const sas_filter_rows *r, void *stream) 
     a.vocab = r->vocab;
     a.rows = r->rows;
     a.shift = 62 - log2_ceil(r->vocab);
+    a.span = filter_span(r->rows, r->vocab, 2 * s->cus);
+    a.parts = (r->vocab + a.span - 1) / a.span;
+    if (int rc = grow(s, &s->filt, &s->filt_cap, filter_scratch_bytes(r->rows, a.parts), stream, "sas_sample_filtered")) return rc;
+    filter_scratch(s->filt, &a);
     hipError_t e = launch_filter(a, pick_stream(s, stream));
     return e == hipSuccess ? SAS_OK : hip_fail(s, e, "sas_sample_filtered launch");
   });
@@ -193,7 +197,16 @@ int sas_reserve_filtered(sas_sampler *s, int32_t rows, int32_t vocab) {
     if (!s) return fail(nullptr, SAS_ERR_INVALID, "sas_reserve_filtered: handle is NULL");
     if (rows < 0 || vocab < 1 || vocab > SAS_MAX_VOCAB)
       return fail(s, SAS_ERR_INVALID, "sas_reserve_filtered: rows must be >= 0 and vocab in [1, SAS_MAX_VOCAB]");
-    return SAS_OK;
+    if (int rc = set_device(s)) return rc;
+    // fewer rows may be cut into more parts (from 2 cus rows on no longer)
+    size_t bytes = 0;
+    auto shape = [&](int n) {
+      const int span = filter_span(n, vocab, 2 * s->cus);
+      bytes = std::max(bytes, filter_scratch_bytes(n, (vocab + span - 1) / span));
+    };
+    for (int n = 1; n <= std::min(rows, 2 * s->cus); ++n) shape(n);
+    if (rows > 0) shape(rows);
+    return grow(s, &s->filt, &s->filt_cap, bytes, nullptr, "sas_reserve_filtered");
   });
 }
 

@@ -25,6 +25,8 @@ constexpr int kRowThreads = 1024;
 constexpr int kRowWaves = kRowThreads / 64;
 constexpr int kSpan = 8192;                       // ids a block holds at once
 constexpr int kQuads = kSpan / (4 * kRowThreads); // quads of ids per thread
+constexpr int kMaxFilterParts = 2048;             // 2,048 ids a part: batches of up to 512 parts of 8,192
+constexpr int kEntries = 4096;                    // listed ids the merge takes
 constexpr int kBins = 512;                        // value ranges of (m - v) / T, 1/8 each; the last takes the rest
 constexpr uint32_t kNegInf = 0x007FFFFFu;         // okey(-inf): candidates lie above
 
@@ -42,12 +44,13 @@ __device__ __forceinline__ sas_filter_params load_filter_params(const FilterArgs
 }
 
 // Four logits from id `id` on (NaN past the row's end), as f32.
+template <int kType>
 __device__ __forceinline__ f32x4 load_logits(const FilterArgs &a, int64_t row0, int id) {
   const float nan = qnan();
   f32x4 v = {nan, nan, nan, nan};
   const int left = a.vocab - id;
   if (left <= 0) return v;
-  if (a.type == SAS_TYPE_F32) {
+  if constexpr (kType == SAS_TYPE_F32) {
     const float *p = static_cast<const float *>(a.logits) + row0 + id;
     if (left >= 4) return *reinterpret_cast<const f32x4u *>(p);
 #pragma unroll
@@ -66,7 +69,7 @@ __device__ __forceinline__ f32x4 load_logits(const FilterArgs &a, int64_t row0, 
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float f = a.type == SAS_TYPE_BF16 ? __uint_as_float((uint32_t)h[i] << 16)
+    const float f = kType == SAS_TYPE_BF16 ? __uint_as_float((uint32_t)h[i] << 16)
                                             : (float)__builtin_bit_cast(_Float16, (uint16_t)h[i]);
     v[i] = i < left ? f : nan;
   }
@@ -96,6 +99,228 @@ __device__ __forceinline__ float penalized(float v, uint32_t count, const sas_fi
   return (float)d;
 }
 
+// ---------------------------------------------------------------- parts --
+// A part's values on one grid of ranges of width 2^e, e = floor(log2(T / 8)):
+// 1/16 to 1/8 of (v - m) / T.  The grid is the same for every part of a row,
+// so their ranges add up, and scaling by a power of two is exact.
+struct Grid {
+  float inv_width;   // 2^-e
+  double per64;      // 64 / (T ln 2): exponentials count in 64ths of octaves
+  bool plain;        // T is in the grid's scope
+};
+__device__ __forceinline__ Grid grid_of(double temperature) {
+  Grid g;
+  const int e = (int)(((uint64_t)__double_as_longlong(temperature) >> 52) & 0x7FF) - 1023 - 3;
+  g.plain = temperature > 0.0 && e >= -24 && e <= 24;
+  g.inv_width = __uint_as_float((uint32_t)(127 - (g.plain ? e : 0)) << 23);
+  g.per64 = 92.33248261689366 / temperature;
+  return g;
+}
+// A value's range; exact below 2^22 ranges from zero (kFar otherwise).
+__device__ __forceinline__ float range_of(float v, const Grid &g) { return __builtin_floorf(v * g.inv_width); }
+constexpr float kFar = 4194304.0f;
+// A part's ranges sum masses as integers of 2^-kFilterShift: 8,192 of at most
+// e^(1/8) stay below 2^64.
+constexpr double kUnit = (double)(1ull << kFilterShift);
+
+// 2^(y / 64), -8192 <= y <= 64: the table's 2^(k / 64) times a Taylor series
+// in |r| <= 1/2 (2^(r / 64) to degree 5, 4e-17 short), the exponent added as
+// an integer: 13 double instructions, the longest part of the pass.
+__device__ __forceinline__ double exp64(double y, const double *tab) {
+  const double magic = 6755399441055744.0;
+  const double kf = y + magic;
+  const int k = (int)(uint32_t)(uint64_t)__double_as_longlong(kf);
+  const double r = y - (kf - magic);
+  const double t = tab[k & 63];
+  const double c1 = 0.010830424696249145, c2 = 5.864904955056169e-05, c3 = 2.1173137155464774e-07, c4 = 5.732851688640402e-10,
+               c5 = 1.2417843701716923e-12;
+  const double x = t * fma(fma(fma(fma(fma(r, c5, c4), r, c3), r, c2), r, c1), r, 1.0);
+  return __hiloint2double(__double2hiint(x) + ((k & ~63) << 14), __double2loint(x));
+}
+
+__device__ __forceinline__ bool filters(const sas_filter_params &p) {
+  return p.top_k > 0 || p.top_p < 1.0 || p.min_p > 0.0;
+}
+__device__ __forceinline__ bool greedy_row(const sas_filter_params &p) { return !(p.temperature > 0.0) || p.top_k == 1; }
+
+// The values of a span of ids as the operator takes them, -inf for what is no
+// candidate: quad j of thread t of kT holds ids id0 + 4 (j kT + t) ..
+template <int kT, int kType, bool kSoft, int Q>
+__device__ __forceinline__ void span_values(const FilterArgs &a, const sas_filter_params &p, int64_t row0, const uint32_t *mask,
+                                            const History &h, uint32_t *count, int id0, float (&v)[Q][4]) {
+  const float neg = -__builtin_inff();
+  uint32_t bits[Q];
+#pragma unroll
+  for (int j = 0; j < Q; ++j) {
+    const int id = id0 + 4 * (j * kT + (int)threadIdx.x);
+    const f32x4 x = load_logits<kType>(a, row0, id);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[j][i] = x[i];
+    bits[j] = !mask ? 0xFu : id < a.vocab ? mask[id >> 5] >> (id & 31) : 0u;
+  }
+  if (h.n) {
+    constexpr int kIds = 4 * kT * Q;
+    __syncthreads();
+    for (int i = threadIdx.x; i < kIds / 2; i += kT) count[i] = 0u;
+    __syncthreads();
+    for (int i = threadIdx.x; i < h.n; i += kT) {
+      const uint32_t at = h.ids[i] - (uint32_t)id0;
+      if (at < (uint32_t)kIds) atomicAdd(&count[at >> 1], 1u << (16 * (at & 1)));
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int j = 0; j < Q; ++j) {
+    // two counts a word; most quads have none
+    const int at = 4 * (j * kT + (int)threadIdx.x);
+    const uint32_t c0 = h.n ? count[at >> 1] : 0u, c1 = h.n ? count[(at >> 1) + 1] : 0u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float x = v[j][i];
+      if (kSoft && p.softcap > 0.0f) x = softcap_f32(x, p.softcap);
+      if (c0 | c1) {
+        const uint32_t c = ((i < 2 ? c0 : c1) >> (16 * (i & 1))) & 0xFFFFu;
+        if (c) x = penalized(x, c, p);
+      }
+      v[j][i] = ((bits[j] >> i) & 1u) && x > neg ? x : neg;
+    }
+  }
+}
+
+template <int kType, bool kSoft, int Q>
+__global__ __launch_bounds__(kThreads) void filter_parts_kernel(const FilterArgs a) {
+  constexpr int kIds = 4 * Q * kThreads;
+  constexpr int kList = kIds / 64 < 32 ? 32 : kIds / 64;  // ids the list takes
+  static_assert(kList <= kFilterList, "the list holds them");
+  __shared__ double tab[kExpTab];
+  __shared__ uint32_t count[kIds / 2];
+  __shared__ unsigned long long mass[kFilterRanges];
+  __shared__ uint32_t cnt[kFilterRanges];
+  __shared__ float wmax[kWaves];
+  __shared__ double wsum[kWaves];
+  __shared__ uint32_t wn[kWaves];
+  __shared__ uint32_t first, listed;
+  __shared__ int lowest;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
+  if (tid < kExpTab) tab[tid] = exp_tab_entry().x;
+  const sas_filter_params p = load_filter_params(a, row);
+  const int64_t row0 = (int64_t)row * a.logits_stride;
+  float v[Q][4];
+  span_values<kThreads, kType, kSoft, Q>(a, p, row0, a.mask ? a.mask + (int64_t)row * a.mask_stride : nullptr, history_of(a, row), count,
+                                         part * kIds, v);
+  if (tid < kFilterRanges) {
+    mass[tid] = 0ull;
+    cnt[tid] = 0u;
+  }
+  if (tid == 0) {
+    first = ~0u;
+    listed = 0u;
+  }
+  const float neg = -__builtin_inff();
+  float m = neg;
+#pragma unroll
+  for (int j = 0; j < Q; ++j) m = fmaxf(m, fmaxf(fmaxf(v[j][0], v[j][1]), fmaxf(v[j][2], v[j][3])));
+  m = wave_max(m);
+  if (lane == 0) wmax[wave] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(wmax[0], wmax[1]), fmaxf(wmax[2], wmax[3]));
+  const int64_t at = (int64_t)row * a.parts + part;
+  FilterPart *out = a.part + at;
+  const Grid g = grid_of(p.temperature);
+  const float top = range_of(m, g);
+  const bool greedy = greedy_row(p), ranged = !greedy && g.plain && fabsf(top) < kFar && m > neg;
+  const bool list = ranged && filters(p);
+  // masses are relative to the top of max's range, so that ranges of all parts
+  // share their edges; (-inf and what is 88 T below: e^-88)
+  const double ref = (double)top / (double)g.inv_width;
+  double sum[4] = {0.0, 0.0, 0.0, 0.0};
+  uint32_t n = 0, best = ~0u;
+#pragma unroll
+  for (int j = 0; j < Q; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float x = v[j][i];
+      n += x > neg ? 1u : 0u;
+      if (x == m) best = min(best, (uint32_t)(part * kIds + 4 * (j * kThreads + tid) + i));
+    }
+  if (ranged) {
+#pragma unroll
+    for (int j = 0; j < Q; ++j) {
+      double u[4];
+      float d[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        u[i] = exp64(fmax(((double)v[j][i] - ref) * g.per64, -8192.0), tab);
+        sum[i] += u[i];
+        d[i] = top - range_of(v[j][i], g);
+      }
+      if (list && fminf(fminf(d[0], d[1]), fminf(d[2], d[3])) < (float)kFilterRanges) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (d[i] < (float)kFilterRanges) {
+            // (a number below 2^51 in the low bits of its sum with 2^52)
+            const uint64_t whole = (uint64_t)__double_as_longlong(fma(u[i], kUnit, 4503599627370496.0)) & 0xFFFFFFFFFFFFFull;
+            atomicAdd(&mass[(int)d[i]], (unsigned long long)whole);
+            atomicAdd(&cnt[(int)d[i]], 1u);
+          }
+      }
+    }
+  }
+  if (best != ~0u && m > neg) atomicMin(&first, best);
+  const double s = wave_sum_d((sum[0] + sum[1]) + (sum[2] + sum[3]));
+  n = wave_reduce(n, [](uint32_t x, uint32_t y) { return x + y; });
+  if (lane == 0) {
+    wsum[wave] = s;
+    wn[wave] = n;
+  }
+  __syncthreads();
+  // the list takes whole ranges, the largest values first
+  if (list && wave == 0) {
+    const uint32_t c0 = cnt[2 * lane], c1 = cnt[2 * lane + 1];
+    uint32_t x = c0 + c1;
+#pragma unroll
+    for (int k = 1; k < 64; k <<= 1) {
+      const uint32_t y = (uint32_t)__shfl_up((int)x, k, 64);
+      if (lane >= k) x += y;
+    }
+    const uint64_t odd = __ballot(x <= (uint32_t)kList), even = __ballot(x - c1 <= (uint32_t)kList);
+    const int no = odd == ~0ull ? 64 : __builtin_ctzll(~odd), ne = even == ~0ull ? 64 : __builtin_ctzll(~even);
+    if (lane == 0) lowest = no + ne - 1;  // the last range whose running count fits, -1: none
+  }
+  if (list) {
+    __syncthreads();
+    for (int i = tid; i < kFilterRanges; i += kThreads) {
+      a.range_mass[at * kFilterRanges + i] = mass[i];
+      a.range_count[at * kFilterRanges + i] = cnt[i];
+    }
+  }
+  const float edge = list && lowest >= 0 ? (top - (float)lowest) / g.inv_width : __uint_as_float(0x7F800000u);
+  if (list && lowest >= 0) {
+#pragma unroll
+    for (int j = 0; j < Q; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (v[j][i] >= edge) {
+          const uint32_t to = atomicAdd(&listed, 1u);
+          a.list[at * kFilterList + to] =
+              (uint64_t)okey(v[j][i]) << 32 | (uint32_t) ~(uint32_t)(part * kIds + 4 * (j * kThreads + tid) + i);
+        }
+  }
+  __syncthreads();
+  if (tid == 0) {
+    FilterPart f;
+    f.max = m;
+    f.id = first;
+    f.count = (int32_t)(wn[0] + wn[1] + wn[2] + wn[3]);
+    f.listed = ranged ? (int32_t)listed : -1;
+    f.edge = edge;
+    f.top = ranged ? (int32_t)top : 0;
+    f.mass = ranged ? (wsum[0] + wsum[1]) + (wsum[2] + wsum[3]) : 0.0;
+    *out = f;
+  }
+}
+
 // (value range) of a key: 0 for m itself, kBins - 1 for the rest.
 struct Scale {
   double m, inv_t, per_bin;
@@ -114,6 +339,18 @@ __device__ __forceinline__ uint64_t units_of(double mass, const Scale &s) {
   return (uint64_t)__builtin_rint(__builtin_amdgcn_ldexp(mass, s.shift));
 }
 
+// The smallest key whose mass reaches min_p (the mass falls with the key).
+__device__ __forceinline__ uint32_t least_key(double min_p, uint32_t top, const Scale &s, const ExpTab &tab) {
+  const double least = fmin(min_p, 1.0);
+  uint32_t lo = kNegInf, hi = top;  // hi reaches it, lo does not (or is no candidate's)
+  while (hi - lo > 1) {
+    const uint32_t mid = lo + (hi - lo) / 2;
+    if (mass_of(mid, s, tab) >= least) hi = mid;
+    else lo = mid;
+  }
+  return hi;
+}
+
 // Every id of a larger key than `key`, and the first `take` of its own.
 struct Edge {
   uint32_t key;
@@ -127,7 +364,11 @@ struct RowShared {
   uint32_t cnt[kBins];
   unsigned long long red[kRowWaves][2];
   unsigned long long sel[4];
-  unsigned long long part[(SAS_MAX_VOCAB + kSpan - 1) / kSpan];
+  unsigned long long part[kMaxFilterParts];
+  unsigned long long ent[kEntries];   // listed ids: key << 32 | ~id
+  unsigned long long entm[kEntries];  // and their masses
+  uint32_t some[kRowThreads];         // entries under a closer look
+  uint32_t nent, nsome;
 };
 
 __device__ __forceinline__ uint64_t shfl_xor64(uint64_t x, int s) { return (uint64_t)__shfl_xor((unsigned long long)x, s, 64); }
@@ -175,6 +416,7 @@ __device__ __forceinline__ uint64_t block_scan(RowShared &l, uint64_t x, uint64_
 }
 
 // One row, one block.
+template <int kType, bool kSoft>
 struct Row {
   const FilterArgs &a;
   RowShared &l;
@@ -188,34 +430,12 @@ struct Row {
   // ids q * kSpan + (j * kRowThreads + threadIdx.x) * 4 ..
   __device__ __forceinline__ int id0(int q, int j) const { return q * kSpan + (j * kRowThreads + (int)threadIdx.x) * 4; }
   __device__ __forceinline__ void keys(int q, uint32_t (&key)[kQuads][4]) const {
-    if (h.n) {
-      __syncthreads();
-      for (int i = threadIdx.x; i < kSpan / 2; i += kRowThreads) l.count[i] = 0u;
-      __syncthreads();
-      for (int i = threadIdx.x; i < h.n; i += kRowThreads) {
-        const uint32_t at = h.ids[i] - (uint32_t)(q * kSpan);
-        if (at < (uint32_t)kSpan) atomicAdd(&l.count[at >> 1], 1u << (16 * (at & 1)));
-      }
-      __syncthreads();
-    }
+    float v[kQuads][4];
+    span_values<kRowThreads, kType, kSoft, kQuads>(a, p, row0, mask, h, l.count, q * kSpan, v);
 #pragma unroll
-    for (int j = 0; j < kQuads; ++j) {
-      const int id = id0(q, j);
-      const f32x4 v = load_logits(a, row0, id);
-      const uint32_t bits = !mask ? 0xFu : id < a.vocab ? mask[id >> 5] >> (id & 31) : 0u;
+    for (int j = 0; j < kQuads; ++j)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float x = v[i];
-        if (p.softcap > 0.0f) x = softcap_f32(x, p.softcap);
-        if (h.n) {
-          const uint32_t at = (uint32_t)(id + i - q * kSpan);
-          const uint32_t c = (l.count[at >> 1] >> (16 * (at & 1))) & 0xFFFFu;
-          if (c) x = penalized(x, c, p);
-        }
-        const uint32_t k = okey(x);
-        key[j][i] = ((bits >> i) & 1u) && k > kNegInf ? k : 0u;
-      }
-    }
+      for (int i = 0; i < 4; ++i) key[j][i] = v[j][i] > -__builtin_inff() ? okey(v[j][i]) : 0u;
   }
   __device__ __forceinline__ int spans() const { return (a.vocab + kSpan - 1) / kSpan; }
   template <typename F>
@@ -233,14 +453,14 @@ struct Row {
   // The first bin b (of n in l.mass / l.cnt) at which the running mass (or,
   // with by_count, count) reaches need; before: what lies above it.  Bins
   // rise from the largest keys on.
-  __device__ __forceinline__ int find(int n, bool by_count, uint64_t need, uint64_t *mass, uint64_t *count) const {
+  __device__ __forceinline__ int find(int n, bool by_count, uint64_t need, uint64_t *mass, uint64_t *count, int base = 0) const {
     __syncthreads();
     if (threadIdx.x < 64) {
       const int lane = threadIdx.x, per = n / 64;
       uint64_t m = 0, c = 0;
       for (int i = 0; i < per; ++i) {
-        m += l.mass[lane * per + i];
-        c += l.cnt[lane * per + i];
+        m += l.mass[base + lane * per + i];
+        c += l.cnt[base + lane * per + i];
       }
       uint64_t mi = m, ci = c;
 #pragma unroll
@@ -256,7 +476,7 @@ struct Row {
         uint64_t mm = mi - m, cc = ci - c;
         int i = 0;
         for (; i < per - 1; ++i) {
-          const uint64_t m1 = mm + l.mass[lane * per + i], c1 = cc + l.cnt[lane * per + i];
+          const uint64_t m1 = mm + l.mass[base + lane * per + i], c1 = cc + l.cnt[base + lane * per + i];
           if ((by_count ? c1 : m1) >= need) break;
           mm = m1;
           cc = c1;
@@ -340,58 +560,52 @@ struct Row {
   }
 };
 
-__global__ __launch_bounds__(kRowThreads) void filter_row_kernel(const FilterArgs a) {
-  __shared__ RowShared l;
-  const int row = blockIdx.x, tid = threadIdx.x;
-  l.tab.fill(exp_tab_entry());
-  __syncthreads();
-  const sas_filter_params p = load_filter_params(a, row);
-  Row r{a, l, p, (int64_t)row * a.logits_stride, a.mask ? a.mask + (int64_t)row * a.mask_stride : nullptr,
-        history_of(a, row), Scale{}};
-  // the best candidate, and how many there are
-  uint64_t best = 0, n = 0;
-  for (int q = 0; q < r.spans(); ++q) {
-    uint32_t key[kQuads][4];
-    r.keys(q, key);
-#pragma unroll
-    for (int j = 0; j < kQuads; ++j)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint64_t k = key[j][i] ? ((uint64_t)key[j][i] << 32) | (uint32_t)~(r.id0(q, j) + i) : 0ull;
-        best = max(best, k);
-        n += k ? 1 : 0;
-      }
-  }
-#pragma unroll
-  for (int s = 32; s > 0; s >>= 1) best = max(best, shfl_xor64(best, s));
-  __syncthreads();
-  if ((tid & 63) == 0) l.red[tid >> 6][0] = best;
-  __syncthreads();
-  for (int w = 0; w < kRowWaves; ++w) best = max(best, (uint64_t)l.red[w][0]);
-  uint64_t zero = 0;
-  block_sum2(l, n, zero);
-  auto done = [&](uint32_t id, double prob, uint64_t count) {
+// What a row's token is: written by one thread.
+struct Result {
+  const FilterArgs &a;
+  int row;
+  __device__ __forceinline__ void operator()(uint32_t id, double prob, uint64_t count) const {
     a.out_ids[row] = id;
     if (a.out_probs) a.out_probs[row] = prob;
     if (a.out_counts) a.out_counts[row] = (int32_t)count;
-    if (a.out_flags) a.out_flags[row] = best ? 0u : SAS_FLAG_EMPTY_ROW;
-  };
-  const bool greedy = !(p.temperature > 0.0) || p.top_k == 1;
-  if (best == 0 || greedy) {
-    if (tid == 0) done(best ? ~(uint32_t)best : SAS_NO_TOKEN, best ? 1.0 : 0.0, best ? 1 : 0);
-    return;
+    if (a.out_flags) a.out_flags[row] = count ? 0u : SAS_FLAG_EMPTY_ROW;
   }
-  const uint32_t top = (uint32_t)(best >> 32);
-  r.s = Scale{(double)fkey(top), 1.0 / p.temperature, 8.0 / p.temperature, a.shift};
+};
 
+// The part of a row (of n, their kept masses in l.part) in which the running
+// mass exceeds goal; before: what lies before it.
+__device__ __forceinline__ int part_of(RowShared &l, int n, uint64_t goal, uint64_t *before) {
+  const int per = (n + kRowThreads - 1) / kRowThreads, first = (int)threadIdx.x * per;
+  uint64_t mine = 0, all;
+  for (int i = first; i < min(first + per, n); ++i) mine += l.part[i];
+  uint64_t run = block_scan(l, mine, &all) - mine;
+  for (int i = first; i < min(first + per, n); ++i) {
+    if (run <= goal && goal < run + l.part[i]) {
+      l.sel[0] = (unsigned long long)i;
+      l.sel[1] = run;
+    }
+    run += l.part[i];
+  }
+  __syncthreads();
+  *before = l.sel[1];
+  return (int)l.sel[0];
+}
+
+// The row by its values alone, read as often as it takes: right for every
+// temperature, value and cut, and what the merge falls back on.
+template <int kType, bool kSoft>
+__device__ __forceinline__ void row_by_values(Row<kType, kSoft> &R, const FilterArgs &a, RowShared &l, const sas_filter_params &p, int row,
+                                           uint32_t top, uint64_t n, const Result &done) {
+  const int tid = threadIdx.x;
+  uint64_t zero = 0;
   Edge e{0u, 0u};  // no edge: every candidate
   uint64_t mass = 0, count = 0;
   if (p.top_k > 0 && (uint64_t)p.top_k < n) {
-    r.histogram();
-    e = r.edge(true, (uint64_t)p.top_k, &mass, &count);
+    R.histogram();
+    e = R.edge(true, (uint64_t)p.top_k, &mass, &count);
   }
   if (p.top_p < 1.0) {
-    r.histogram();
+    R.histogram();
     if (!e.key) {
       uint64_t all = 0;
       zero = 0;
@@ -400,26 +614,19 @@ __global__ __launch_bounds__(kRowThreads) void filter_row_kernel(const FilterArg
       mass = all;
     }
     const double need = ceil(fmax(p.top_p, 0.0) * (double)mass);
-    const Edge f = r.edge(false, min(max((uint64_t)need, (uint64_t)1), mass), &mass, &count);
+    const Edge f = R.edge(false, min(max((uint64_t)need, (uint64_t)1), mass), &mass, &count);
     if (!e.key || f.key > e.key || (f.key == e.key && f.take < e.take)) e = f;
   }
   if (p.min_p > 0.0) {
-    // the smallest key whose mass reaches min_p (the mass falls with the key)
-    const double least = fmin(p.min_p, 1.0);
-    uint32_t lo = kNegInf, hi = top;  // hi reaches it, lo does not (or is no candidate's)
-    while (hi - lo > 1) {
-      const uint32_t mid = lo + (hi - lo) / 2;
-      if (mass_of(mid, r.s, l.tab) >= least) hi = mid;
-      else lo = mid;
-    }
+    const uint32_t hi = least_key(p.min_p, top, R.s, l.tab);
     if (hi > e.key) e = Edge{hi, ~0u};
   }
   // what is kept of each span; the edge's ids count in ascending order
   uint64_t total = 0, kept = 0, ties = 0;
-  const uint64_t unit = e.key ? units_of(mass_of(e.key, r.s, l.tab), r.s) : 0;
-  for (int q = 0; q < r.spans(); ++q) {
+  const uint64_t unit = e.key ? units_of(mass_of(e.key, R.s, l.tab), R.s) : 0;
+  for (int q = 0; q < R.spans(); ++q) {
     uint32_t key[kQuads][4];
-    r.keys(q, key);
+    R.keys(q, key);
     uint64_t m = 0, c = 0;
 #pragma unroll
     for (int j = 0; j < kQuads; ++j)
@@ -427,7 +634,7 @@ __global__ __launch_bounds__(kRowThreads) void filter_row_kernel(const FilterArg
       for (int i = 0; i < 4; ++i) {
         const uint32_t k = key[j][i];
         if (k > e.key) {
-          m += units_of(mass_of(k, r.s, l.tab), r.s);
+          m += units_of(mass_of(k, R.s, l.tab), R.s);
           c += 1;
         } else if (k && k == e.key) {
           c += 1ull << 32;
@@ -448,13 +655,13 @@ __global__ __launch_bounds__(kRowThreads) void filter_row_kernel(const FilterArg
   goal = min(goal, total - 1);
   int q = 0;
   uint64_t before = 0;
-  while (q < r.spans() - 1 && before + l.part[q] <= goal) before += l.part[q++];
+  while (q < R.spans() - 1 && before + l.part[q] <= goal) before += l.part[q++];
   // the edge's ids in the spans before
   uint64_t tie0 = 0;
   if (e.key && e.take != ~0u) {
     for (int s = 0; s < q; ++s) {
       uint32_t key[kQuads][4];
-      r.keys(s, key);
+      R.keys(s, key);
 #pragma unroll
       for (int j = 0; j < kQuads; ++j)
 #pragma unroll
@@ -464,7 +671,7 @@ __global__ __launch_bounds__(kRowThreads) void filter_row_kernel(const FilterArg
     block_sum2(l, tie0, zero);
   }
   uint32_t key[kQuads][4];
-  r.keys(q, key);
+  R.keys(q, key);
   for (int j = 0; j < kQuads; ++j) {
     uint64_t t = 0, all = 0;
     uint64_t mine[4] = {0, 0, 0, 0};
@@ -478,7 +685,7 @@ __global__ __launch_bounds__(kRowThreads) void filter_row_kernel(const FilterArg
       const uint32_t k = key[j][i];
       bool in = k > e.key;
       if (k && k == e.key) in = tie++ < e.take;
-      mine[i] = in ? units_of(mass_of(k, r.s, l.tab), r.s) : 0;
+      mine[i] = in ? units_of(mass_of(k, R.s, l.tab), R.s) : 0;
       m += mine[i];
     }
     uint64_t run = before + block_scan(l, m, &all) - m;
@@ -486,7 +693,7 @@ __global__ __launch_bounds__(kRowThreads) void filter_row_kernel(const FilterArg
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if (run <= goal && goal < run + mine[i])
-          done((uint32_t)(r.id0(q, j) + i), mass_of(key[j][i], r.s, l.tab) / __builtin_amdgcn_ldexp((double)total, -a.shift), kept);
+          done((uint32_t)(R.id0(q, j) + i), mass_of(key[j][i], R.s, l.tab) / __builtin_amdgcn_ldexp((double)total, -a.shift), kept);
         run += mine[i];
       }
     }
@@ -494,11 +701,432 @@ __global__ __launch_bounds__(kRowThreads) void filter_row_kernel(const FilterArg
   }
 }
 
+// The entry that ends a prefix of the first c entries of l.ent, which rank by
+// (key, id): the one of rank need (by_count), else the first at which the
+// running mass reaches need.  Radix passes of 8 bits from the highest in which
+// the entries differ.  *mass, *count: of the entries up to it.
+template <typename R>
+__device__ __forceinline__ uint64_t end_of(const R &row, RowShared &l, int c, bool by_count, uint64_t need, uint64_t *mass, uint64_t *count) {
+  constexpr int kBase = 256;
+  const int tid = threadIdx.x;
+  uint64_t all = ~0ull, any = 0;
+  for (int i = tid; i < c; i += kRowThreads) {
+    all &= l.ent[i];
+    any |= l.ent[i];
+  }
+#pragma unroll
+  for (int s = 32; s > 0; s >>= 1) {
+    all &= shfl_xor64(all, s);
+    any |= shfl_xor64(any, s);
+  }
+  __syncthreads();
+  if ((tid & 63) == 0) {
+    l.red[tid >> 6][0] = all;
+    l.red[tid >> 6][1] = any;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kRowWaves; ++w) {
+    all &= l.red[w][0];
+    any |= l.red[w][1];
+  }
+  int sh = all == any ? 0 : max(63 - __builtin_clzll(all ^ any) - 7, 0);
+  uint64_t high = sh + 8 >= 64 ? 0ull : ~0ull << (sh + 8), at = all & high, m0 = 0, c0 = 0;
+  for (;;) {
+    __syncthreads();
+    if (tid < 256) {
+      l.mass[kBase + tid] = 0ull;
+      l.cnt[kBase + tid] = 0u;
+    }
+    __syncthreads();
+    for (int i = tid; i < c; i += kRowThreads) {
+      const uint64_t e = l.ent[i];
+      if ((e & high) != at) continue;
+      const int d = 255 - (int)((e >> sh) & 0xFFu);
+      atomicAdd(&l.mass[kBase + d], l.entm[i]);
+      atomicAdd(&l.cnt[kBase + d], 1u);
+    }
+    uint64_t m1, c1;
+    const int d = row.find(256, by_count, by_count ? need - c0 : need - m0, &m1, &c1, kBase);
+    m0 += m1;
+    c0 += c1;
+    at |= (uint64_t)(255 - d) << sh;
+    if (l.cnt[kBase + d] == 1u || sh == 0) {
+      // one entry (they differ): its low bits
+      const uint64_t low = ~0ull << sh;
+      __syncthreads();
+      for (int i = tid; i < c; i += kRowThreads)
+        if ((l.ent[i] & low) == at) {
+          l.sel[0] = l.ent[i];
+          l.sel[1] = l.entm[i];
+        }
+      __syncthreads();
+      *mass = m0 + l.sel[1];
+      *count = c0 + 1;
+      return l.sel[0];
+    }
+    const int down = min(sh, 8);
+    high = ~0ull << sh;
+    sh -= down;
+  }
+}
+
+// The row by what its parts left; false where that does not tell (*top, *n:
+// its best key and its candidates).
+template <int kType, bool kSoft>
+__device__ __forceinline__ bool row_by_parts(Row<kType, kSoft> &R, const FilterArgs &a, RowShared &l, const sas_filter_params &p, int row,
+                                             uint32_t *top_key, uint64_t *candidates, const Result &done) {
+  const int tid = threadIdx.x;
+  const FilterPart *parts = a.part + (int64_t)row * a.parts;
+  // the best candidate, how many there are, and from which value on all are listed
+  uint64_t best = 0, n = 0, zero = 0;
+  uint32_t edge = 0;  // okey
+  for (int i = tid; i < a.parts; i += kRowThreads) {
+    const FilterPart f = parts[i];
+    if (f.max > -__builtin_inff()) {
+      best = max(best, (uint64_t)okey(f.max) << 32 | (uint32_t)~f.id);
+      n += (uint64_t)f.count;
+      edge = max(edge, f.listed < 0 ? okey(f.max) + 1u : okey(f.edge));
+    }
+  }
+#pragma unroll
+  for (int s = 32; s > 0; s >>= 1) {
+    best = max(best, shfl_xor64(best, s));
+    edge = max(edge, (uint32_t)__shfl_xor((int)edge, s, 64));
+    n += shfl_xor64(n, s);
+  }
+  if ((tid & 63) == 0) {
+    l.red[tid >> 6][0] = best;
+    l.red[tid >> 6][1] = (uint64_t)edge << 32 | n;
+  }
+  __syncthreads();
+  n = 0;
+#pragma unroll
+  for (int w = 0; w < kRowWaves; ++w) {
+    best = max(best, (uint64_t)l.red[w][0]);
+    edge = max(edge, (uint32_t)(l.red[w][1] >> 32));
+    n += l.red[w][1] & 0xFFFFFFFFull;
+  }
+  if (best == 0 || greedy_row(p)) {
+    if (tid == 0) done(best ? ~(uint32_t)best : SAS_NO_TOKEN, best ? 1.0 : 0.0, best ? 1 : 0);
+    return true;
+  }
+  const uint32_t top = (uint32_t)(best >> 32);
+  const float m = fkey(top);
+  *top_key = top;
+  *candidates = n;
+  R.s = Scale{(double)m, 1.0 / p.temperature, 8.0 / p.temperature, a.shift};
+  const Grid g = grid_of(p.temperature);
+  const float mrange = range_of(m, g);
+  if (!g.plain || !(fabsf(mrange) < kFar)) return false;
+  const bool by_k = p.top_k > 0 && (uint64_t)p.top_k < n, by_p = p.top_p < 1.0, by_min = p.min_p > 0.0;
+  const bool cut = by_k || by_p || by_min;
+  // a part's factor to the row's units
+  auto scale_of = [&](const FilterPart &f) { return exp_sum(((double)f.top / (double)g.inv_width - R.s.m) * R.s.inv_t, l.tab); };
+  uint64_t all = 0;
+  for (int i = tid; i < a.parts; i += kRowThreads) {
+    const FilterPart f = parts[i];
+    uint64_t u = 0;
+    if (f.listed >= 0) u = (uint64_t)__builtin_rint(__builtin_amdgcn_ldexp(f.mass * scale_of(f), a.shift));
+    l.part[i] = u;
+    all += u;
+  }
+  zero = 0;
+  block_sum2(l, all, zero);
+  uint64_t last = 0;      // every id whose (key, ~id) reaches it is kept
+  uint64_t total = all, kept = n;
+  int entries = 0;        // what l.ent holds
+  bool listed = false;    // all that are kept
+  const int log_span = 31 - __builtin_clz(a.span);
+  if (cut) {
+    // the listed ids of the row's ranges, all that there are from `edge` on
+    for (int i = tid; i < kFilterRanges; i += kRowThreads) {
+      l.mass[i] = 0ull;
+      l.cnt[i] = 0u;
+    }
+    __syncthreads();
+    const uint64_t *lists = a.list + (int64_t)row * a.parts * kFilterList;
+    for (int i = tid; i < a.parts * kFilterList; i += kRowThreads) {
+      if (i % kFilterList >= max(parts[i / kFilterList].listed, 0)) continue;
+      const uint64_t e = lists[i];
+      const uint32_t key = (uint32_t)(e >> 32);
+      const float d = mrange - range_of(fkey(key), g);
+      if (key < edge || !(d < (float)kFilterRanges)) continue;
+      const uint32_t to = atomicAdd(&l.nent, 1u);
+      if (to >= (uint32_t)kEntries) continue;
+      const uint64_t u = units_of(mass_of(key, R.s, l.tab), R.s);
+      l.ent[to] = e;
+      l.entm[to] = u;
+      atomicAdd(&l.mass[(int)d], (unsigned long long)u);
+      atomicAdd(&l.cnt[(int)d], 1u);
+    }
+    __syncthreads();
+    entries = (int)min(l.nent, (uint32_t)kEntries);
+    uint64_t have = 0, havem = 0;
+    for (int i = tid; i < kFilterRanges; i += kRowThreads) {
+      have += l.cnt[i];
+      havem += l.mass[i];
+    }
+    block_sum2(l, have, havem);
+    const uint32_t least = by_min ? least_key(p.min_p, top, R.s, l.tab) : 0u;
+    const uint64_t of_p = by_p ? (uint64_t)ceil(fmax(p.top_p, 0.0) * (double)all) : 0ull;
+    // whether the lists hold the prefixes' ends (top-p's need is at most of_p)
+    listed = l.nent <= (uint32_t)kEntries && (!by_k || (uint64_t)p.top_k <= have) && (!by_p || (by_k && (uint64_t)p.top_k <= have) || of_p <= havem) &&
+             (by_k || by_p || (least >= edge && mrange - range_of(fkey(least), g) < (float)kFilterRanges));
+    if (!listed) {
+      // the ranges of all parts instead
+      __syncthreads();
+      for (int i = tid; i < kFilterRanges; i += kRowThreads) {
+        l.mass[i] = 0ull;
+        l.cnt[i] = 0u;
+      }
+      __syncthreads();
+      for (int i = tid; i < a.parts * kFilterRanges; i += kRowThreads) {
+        const FilterPart f = parts[i / kFilterRanges];
+        if (f.listed < 0 || !(f.max > -__builtin_inff())) continue;
+        const int64_t at = ((int64_t)row * a.parts) * kFilterRanges + i;
+        const uint32_t c = a.range_count[at];
+        const int d = (int)mrange - f.top + i % kFilterRanges;
+        if (c == 0u || d >= kFilterRanges) continue;
+        atomicAdd(&l.cnt[d], c);
+        atomicAdd(&l.mass[d], (unsigned long long)__builtin_rint(
+                                  __builtin_amdgcn_ldexp((double)a.range_mass[at] * scale_of(f), a.shift - kFilterShift)));
+      }
+      __syncthreads();
+      have = havem = 0;
+      for (int i = tid; i < kFilterRanges; i += kRowThreads) {
+        have += l.cnt[i];
+        havem += l.mass[i];
+      }
+      block_sum2(l, have, havem);
+    }
+    // The ids of range `bin` into l.ent: from the row's values, in the parts that
+    // have any there.
+    bool fits = true;
+    int held = -1;
+    auto gather = [&](int bin) {
+      if (held == bin) return;
+      held = bin;
+      __syncthreads();
+      if (tid == 0) l.nent = 0u;
+      __syncthreads();
+      for (int id0 = 0; id0 < a.vocab; id0 += kSpan) {
+        bool any = false;
+        for (int q = id0 >> log_span; q < min((id0 + kSpan) >> log_span, a.parts); ++q) {
+          const int i = bin - (int)mrange + parts[q].top;
+          any = any || (parts[q].listed >= 0 && i >= 0 && i < kFilterRanges && a.range_count[((int64_t)row * a.parts + q) * kFilterRanges + i] > 0u);
+        }
+        if (!any) continue;
+        float v[kQuads][4];
+        span_values<kRowThreads, kType, kSoft, kQuads>(a, p, R.row0, R.mask, R.h, l.count, id0, v);
+#pragma unroll
+        for (int j = 0; j < kQuads; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (mrange - range_of(v[j][i], g) == (float)bin) {
+              const uint32_t to = atomicAdd(&l.nent, 1u);
+              if (to < (uint32_t)kEntries) {
+                const uint32_t key = okey(v[j][i]);
+                l.ent[to] = (uint64_t)key << 32 | (uint32_t) ~(uint32_t)(id0 + 4 * (j * kRowThreads + tid) + i);
+                l.entm[to] = units_of(mass_of(key, R.s, l.tab), R.s);
+              }
+            }
+      }
+      __syncthreads();
+      fits = fits && l.nent <= (uint32_t)kEntries;
+      entries = (int)min(l.nent, (uint32_t)kEntries);
+    };
+    // the ends of the prefixes of top-k and top-p
+    bool known = true;
+    auto prefix = [&](bool by_count, uint64_t need, uint64_t *mass) {
+      if (need > (by_count ? have : havem)) {
+        known = false;
+        return;
+      }
+      uint64_t m0, c0, m1, c1;
+      const int bin = R.find(kFilterRanges, by_count, need, &m0, &c0);
+      if (!listed) {
+        gather(bin);
+        if (!fits) {
+          known = false;
+          return;
+        }
+        // (the range's mass was rounded as a whole, its ids' one by one)
+        uint64_t sum = 0;
+        zero = 0;
+        for (int i = tid; i < entries; i += kRowThreads) sum += l.entm[i];
+        block_sum2(l, sum, zero);
+        known = sum > 0;
+        if (!known) return;
+        last = max(last, end_of(R, l, entries, by_count, by_count ? need - c0 : min(need - m0, sum), &m1, &c1));
+        *mass = m0 + m1;
+      } else {
+        // (all entries: those of the ranges above rank before the end)
+        last = max(last, end_of(R, l, entries, by_count, need, mass, &c1));
+      }
+    };
+    uint64_t mass = all;
+    if (by_k) prefix(true, (uint64_t)p.top_k, &mass);
+    if (known && by_p) {
+      const uint64_t need = (uint64_t)ceil(fmax(p.top_p, 0.0) * (double)mass);
+      prefix(false, min(max(need, (uint64_t)1), mass), &mass);
+    }
+    if (known && by_min && (uint64_t)least << 32 > last) {
+      last = (uint64_t)least << 32;
+      known = mrange - range_of(fkey(least), g) < (float)kFilterRanges;
+    }
+    if (!known) return false;
+    // what is kept of each part: of the ranges above the end's all, of its own
+    // by its ids
+    const int bin = (int)(mrange - range_of(fkey((uint32_t)(last >> 32)), g));
+    if (!listed) {
+      gather(bin);
+      if (!fits) return false;
+    }
+    __syncthreads();
+    total = kept = 0;
+    for (int i = tid; i < a.parts; i += kRowThreads) {
+      uint64_t u = 0;
+      if (!listed) {
+        const FilterPart f = parts[i];
+        const int end = min(bin - (int)mrange + f.top, kFilterRanges);
+        const int64_t at = ((int64_t)row * a.parts + i) * kFilterRanges;
+        if (f.listed >= 0 && f.max > -__builtin_inff()) {
+          uint64_t w = 0;
+          for (int k = 0; k < end; ++k) {
+            w += a.range_mass[at + k];
+            kept += a.range_count[at + k];
+          }
+          u = (uint64_t)__builtin_rint(__builtin_amdgcn_ldexp((double)w * scale_of(f), a.shift - kFilterShift));
+        }
+      }
+      l.part[i] = u;
+      total += u;
+    }
+    __syncthreads();
+    for (int i = tid; i < entries; i += kRowThreads)
+      if (l.ent[i] >= last) {
+        total += l.entm[i];
+        ++kept;
+        atomicAdd(&l.part[~(uint32_t)l.ent[i] >> log_span], l.entm[i]);
+      }
+    block_sum2(l, total, kept);
+  }
+  // the draw: the part, then the id
+  uint64_t goal = (uint64_t)fmax(a.uniforms[row] * (double)total, 0.0), before;
+  goal = min(goal, total - 1);
+  const int q = part_of(l, a.parts, goal, &before);
+  const double whole = __builtin_amdgcn_ldexp((double)total, -a.shift);
+  if (cut && listed) {
+    if (tid == 0) l.nsome = 0u;
+    __syncthreads();
+    for (int i = tid; i < entries; i += kRowThreads)
+      if (l.ent[i] >= last && (int)(~(uint32_t)l.ent[i] >> log_span) == q) l.some[atomicAdd(&l.nsome, 1u)] = (uint32_t)i;  // (<= kFilterList)
+    __syncthreads();
+    if (tid < (int)l.nsome) {
+      const uint64_t mine = l.ent[l.some[tid]], own = l.entm[l.some[tid]];
+      uint64_t run = before;
+      for (int i = 0; i < (int)l.nsome; ++i)
+        if (~(uint32_t)l.ent[l.some[i]] < ~(uint32_t)mine) run += l.entm[l.some[i]];
+      if (run <= goal && goal < run + own) done(~(uint32_t)mine, mass_of((uint32_t)(mine >> 32), R.s, l.tab) / whole, kept);
+    }
+    return true;
+  }
+  // the part's values again: its kept ids' masses, and the goal as a share of them
+  float v[kQuads][4];
+  const int id0 = q * a.span;
+  span_values<kRowThreads, kType, kSoft, kQuads>(a, p, R.row0, R.mask, R.h, l.count, id0, v);
+  uint64_t u[kQuads][4], run[kQuads], sums = 0;
+#pragma unroll
+  for (int j = 0; j < kQuads; ++j) {
+    uint64_t sum = 0, of_all;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int at = 4 * (j * kRowThreads + tid) + i;
+      const uint32_t key = okey(v[j][i]);
+      const bool in = at < a.span && v[j][i] > -__builtin_inff() && ((uint64_t)key << 32 | (uint32_t) ~(uint32_t)(id0 + at)) >= last;
+      u[j][i] = in ? units_of(mass_of(key, R.s, l.tab), R.s) : 0ull;
+      sum += u[j][i];
+    }
+    run[j] = sums + block_scan(l, sum, &of_all) - sum;
+    sums += of_all;
+  }
+  uint64_t target = (uint64_t)((double)(goal - before) * ((double)sums / (double)l.part[q]));
+  target = min(target, sums - 1);
+#pragma unroll
+  for (int j = 0; j < kQuads; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (run[j] <= target && target < run[j] + u[j][i])
+        done((uint32_t)(id0 + 4 * (j * kRowThreads + tid) + i), mass_of(okey(v[j][i]), R.s, l.tab) / whole, kept);
+      run[j] += u[j][i];
+    }
+  return true;
+}
+
+template <int kType, bool kSoft>
+__global__ __launch_bounds__(kRowThreads) void filter_merge_kernel(const FilterArgs a) {
+  __shared__ RowShared l;
+  const int row = blockIdx.x;
+  l.tab.fill(exp_tab_entry());
+  if (threadIdx.x == 0) l.nent = 0u;
+  __syncthreads();
+  const sas_filter_params p = load_filter_params(a, row);
+  Row<kType, kSoft> R{a, l, p, (int64_t)row * a.logits_stride, a.mask ? a.mask + (int64_t)row * a.mask_stride : nullptr,
+                      history_of(a, row), Scale{}};
+  const Result done{a, row};
+  uint32_t top = 0;
+  uint64_t n = 0;
+  if (!row_by_parts<kType, kSoft>(R, a, l, p, row, &top, &n, done)) row_by_values<kType, kSoft>(R, a, l, p, row, top, n, done);
+}
+
+template <int kType, bool kSoft>
+hipError_t launch(const FilterArgs &a, hipStream_t stream) {
+  const int blocks = a.rows * a.parts;
+  switch (a.span) {
+    case 2048: filter_parts_kernel<kType, kSoft, 2><<<blocks, kThreads, 0, stream>>>(a); break;
+    case 4096: filter_parts_kernel<kType, kSoft, 4><<<blocks, kThreads, 0, stream>>>(a); break;
+    default: filter_parts_kernel<kType, kSoft, 8><<<blocks, kThreads, 0, stream>>>(a); break;
+  }
+  if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  filter_merge_kernel<kType, kSoft><<<a.rows, kRowThreads, 0, stream>>>(a);
+  return hipGetLastError();
+}
+template <int kType>
+hipError_t launch(const FilterArgs &a, bool soft, hipStream_t stream) {
+  return soft ? launch<kType, true>(a, stream) : launch<kType, false>(a, stream);
+}
+
 }  // namespace
 
+int filter_span(int rows, int vocab, int min_blocks) {
+  int span = kSpan;
+  while (span > 2048 && (int64_t)rows * ((vocab + span - 1) / span) < min_blocks) span /= 2;
+  return span;
+}
+
+// The parts, their lists, the masses and counts of their ranges.
+size_t filter_scratch_bytes(int rows, int parts) {
+  const size_t n = (size_t)rows * parts;
+  return n * (sizeof(FilterPart) + kFilterList * 8 + kFilterRanges * 12);
+}
+void filter_scratch(void *base, FilterArgs *a) {
+  const size_t n = (size_t)a->rows * a->parts;
+  static_assert(sizeof(FilterPart) % 8 == 0, "whole words");
+  char *at = static_cast<char *>(base);
+  a->part = reinterpret_cast<FilterPart *>(at);
+  a->list = reinterpret_cast<uint64_t *>(at += n * sizeof(FilterPart));
+  a->range_mass = reinterpret_cast<uint64_t *>(at += n * kFilterList * 8);
+  a->range_count = reinterpret_cast<uint32_t *>(at + n * kFilterRanges * 8);
+}
+
 hipError_t launch_filter(const FilterArgs &a, hipStream_t stream) {
-  filter_row_kernel<<<a.rows, kRowThreads, 0, stream>>>(a);
-  return hipGetLastError();
+  const bool soft = a.row_params || a.params.softcap > 0.0f;
+  switch (a.type) {
+    case SAS_TYPE_F32: return launch<SAS_TYPE_F32>(a, soft, stream);
+    case SAS_TYPE_BF16: return launch<SAS_TYPE_BF16>(a, soft, stream);
+    default: return launch<SAS_TYPE_F16>(a, soft, stream);
+  }
 }
 
 }  // namespace sas

@@ -248,12 +248,38 @@ struct FilterArgs {
   double *out_probs;
   int32_t *out_counts;
   uint32_t *out_flags;
+  // What the parts kernel leaves of each (row, part): FilterPart, the masses
+  // and counts of its value ranges, and its best ids as {id, key} pairs.
+  struct FilterPart *part;
+  uint64_t *range_mass;  // [rows][parts][kFilterRanges]
+  uint32_t *range_count;
+  uint64_t *list;        // [rows][parts][kFilterList]
   int32_t type;   // SAS_TYPE_*
   int32_t vocab;
   int32_t rows;
   int32_t shift;  // masses are integers of 2^-shift
+  int32_t span;   // ids a part, a power of two
+  int32_t parts;
 };
 
+constexpr int kFilterRanges = 128;
+constexpr int kFilterList = 128;
+struct FilterPart {
+  float max;        // the largest value (-inf: no candidate)
+  uint32_t id;      // its first id
+  int32_t count;    // candidates
+  int32_t listed;   // ids in the list, -1: the part's values are out of the ranges' scope
+  float edge;       // every candidate of at least this value is listed
+  int32_t top;      // the range of max: floor(max / width)
+  double mass;      // of all candidates, relative to e^(top width / T)
+};
+constexpr int kFilterShift = 50;
+
+// Ids a part: 8,192, or fewer (at least 2,048) where the grid would hold
+// fewer than `min_blocks` blocks.
+int filter_span(int rows, int vocab, int min_blocks);
+size_t filter_scratch_bytes(int rows, int parts);
+void filter_scratch(void *base, FilterArgs *a);
 hipError_t launch_filter(const FilterArgs &a, hipStream_t stream);
 
 }  // namespace sas
