@@ -187,10 +187,13 @@ __device__ __forceinline__ void span_values(const FilterArgs &a, const sas_filte
   }
 }
 
+// Ids a part of `ids` lists: 4,096 a row of 262,144.
+constexpr int list_size(int ids) { return ids / 64; }
+
 template <int kType, bool kSoft, int Q>
 __global__ __launch_bounds__(kThreads) void filter_parts_kernel(const FilterArgs a) {
   constexpr int kIds = 4 * Q * kThreads;
-  constexpr int kList = kIds / 64 < 32 ? 32 : kIds / 64;  // ids the list takes
+  constexpr int kList = list_size(kIds);
   static_assert(kList <= kFilterList, "the list holds them");
   __shared__ double tab[kExpTab];
   __shared__ uint32_t count[kIds / 2];
@@ -303,7 +306,7 @@ __global__ __launch_bounds__(kThreads) void filter_parts_kernel(const FilterArgs
       for (int i = 0; i < 4; ++i)
         if (v[j][i] >= edge) {
           const uint32_t to = atomicAdd(&listed, 1u);
-          a.list[at * kFilterList + to] =
+          a.list[at * kList + to] =
               (uint64_t)okey(v[j][i]) << 32 | (uint32_t) ~(uint32_t)(part * kIds + 4 * (j * kThreads + tid) + i);
         }
   }
@@ -592,7 +595,7 @@ __device__ __forceinline__ int part_of(RowShared &l, int n, uint64_t goal, uint6
 }
 
 // The row by its values alone, read as often as it takes: right for every
-// temperature, value and cut, and what the merge falls back on.
+// temperature, value and cut, and what the others fall back on.
 template <int kType, bool kSoft>
 __device__ __forceinline__ void row_by_values(Row<kType, kSoft> &R, const FilterArgs &a, RowShared &l, const sas_filter_params &p, int row,
                                            uint32_t top, uint64_t n, const Result &done) {
@@ -845,9 +848,10 @@ __device__ __forceinline__ bool row_by_parts(Row<kType, kSoft> &R, const FilterA
       l.cnt[i] = 0u;
     }
     __syncthreads();
-    const uint64_t *lists = a.list + (int64_t)row * a.parts * kFilterList;
-    for (int i = tid; i < a.parts * kFilterList; i += kRowThreads) {
-      if (i % kFilterList >= max(parts[i / kFilterList].listed, 0)) continue;
+    const int list = list_size(a.span);
+    const uint64_t *lists = a.list + (int64_t)row * a.parts * list;
+    for (int i = tid; i < a.parts * list; i += kRowThreads) {
+      if (i % list >= max(parts[i / list].listed, 0)) continue;
       const uint64_t e = lists[i];
       const uint32_t key = (uint32_t)(e >> 32);
       const float d = mrange - range_of(fkey(key), g);
@@ -1064,10 +1068,12 @@ __device__ __forceinline__ bool row_by_parts(Row<kType, kSoft> &R, const FilterA
   return true;
 }
 
+// The rows that the merge left.
 template <int kType, bool kSoft>
-__global__ __launch_bounds__(kRowThreads) void filter_merge_kernel(const FilterArgs a) {
+__global__ __launch_bounds__(kRowThreads) void filter_rest_kernel(const FilterArgs a) {
   __shared__ RowShared l;
   const int row = blockIdx.x;
+  if (!a.left[row]) return;
   l.tab.fill(exp_tab_entry());
   if (threadIdx.x == 0) l.nent = 0u;
   __syncthreads();
@@ -1080,16 +1086,331 @@ __global__ __launch_bounds__(kRowThreads) void filter_merge_kernel(const FilterA
   if (!row_by_parts<kType, kSoft>(R, a, l, p, row, &top, &n, done)) row_by_values<kType, kSoft>(R, a, l, p, row, top, n, done);
 }
 
+// ----------------------------------------------------------------- merge --
+// One row, four waves.  The lists' entries stay in registers; every wave
+// finds the same ends of the prefixes from the ranges' sums in LDS, so that
+// few barriers are left.  Rows whose ends the lists do not hold, or whose
+// values are out of the ranges' scope, are left to the rest kernel.
+constexpr int kMergeEntries = 16;                          // a thread's
+constexpr int kMergeMost = kMergeEntries * kThreads;       // entries of a row
+constexpr int kMergeSome = 512;                            // ids of one range, or of one part
+
+struct MergeShared {
+  double tab[kExpTab];
+  uint64_t red[kWaves][3];
+  unsigned long long mass[kFilterRanges];
+  uint32_t cnt[kFilterRanges];
+  unsigned long long part[kMaxFilterParts];
+  unsigned long long ent[kMergeSome], entm[kMergeSome];
+  uint32_t nsome;
+};
+
+template <typename Op>
+__device__ __forceinline__ uint64_t wave_reduce64(uint64_t x, Op op) {
+#pragma unroll
+  for (int s = 32; s > 0; s >>= 1) x = op(x, shfl_xor64(x, s));
+  return x;
+}
+__device__ __forceinline__ uint64_t wave_scan64(uint64_t x) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) {
+    const uint64_t y = (uint64_t)__shfl_up((unsigned long long)x, s, 64);
+    if (lane >= s) x += y;
+  }
+  return x;
+}
+__device__ __forceinline__ uint64_t lane64(uint64_t x, int lane) {
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), lane) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)x, lane);
+}
+
+template <int kType, bool kSoft, int Q>
+__global__ __launch_bounds__(kThreads) void filter_merge_kernel(const FilterArgs a) {
+  constexpr int kIds = 4 * Q * kThreads;
+  constexpr int kList = list_size(kIds);
+  constexpr int kLogIds = Q == 8 ? 13 : Q == 4 ? 12 : 11;
+  static_assert(kIds == 1 << kLogIds, "a power of two");
+  __shared__ MergeShared l;
+  __shared__ uint32_t hcount[kIds / 2];
+  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const FilterPart *parts = a.part + (int64_t)row * a.parts;
+  const uint64_t *lists = a.list + (int64_t)row * a.parts * kList;
+  const int slots = a.parts * kList;
+  // what the parts left: their entries (read before it is known how many hold)
+  uint64_t e[kMergeEntries];
+#pragma unroll
+  for (int i = 0; i < kMergeEntries; ++i) e[i] = i * kThreads + tid < slots ? lists[i * kThreads + tid] : 0ull;
+  const sas_filter_params p = load_filter_params(a, row);
+  if (tid < kExpTab) l.tab[tid] = exp_tab_entry().x;
+  if (tid < kFilterRanges) {
+    l.mass[tid] = 0ull;
+    l.cnt[tid] = 0u;
+  }
+  uint64_t best = 0, n = 0;
+  uint32_t edge = 0;
+  for (int i = tid; i < a.parts; i += kThreads) {
+    const FilterPart f = parts[i];
+    if (f.max > -__builtin_inff()) {
+      best = max(best, (uint64_t)okey(f.max) << 32 | (uint32_t)~f.id);
+      n += (uint64_t)f.count;
+      edge = max(edge, f.listed < 0 ? okey(f.max) + 1u : okey(f.edge));
+    }
+  }
+  auto more = [](uint64_t x, uint64_t y) { return x > y ? x : y; };
+  auto plus = [](uint64_t x, uint64_t y) { return x + y; };
+  best = wave_reduce64(best, more);
+  n = wave_reduce64(n, plus);
+  edge = wave_max_u32(edge);
+  if (lane == 0) {
+    l.red[wave][0] = best;
+    l.red[wave][1] = n;
+    l.red[wave][2] = edge;
+  }
+  __syncthreads();
+  best = n = 0;
+  edge = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    best = more(best, l.red[w][0]);
+    n += l.red[w][1];
+    edge = max(edge, (uint32_t)l.red[w][2]);
+  }
+  const Result done{a, row};
+  if (tid == 0) a.left[row] = 0u;
+  if (best == 0 || greedy_row(p)) {
+    if (tid == 0) done(best ? ~(uint32_t)best : SAS_NO_TOKEN, best ? 1.0 : 0.0, best ? 1 : 0);
+    return;
+  }
+  auto leave = [&]() {
+    if (tid == 0) a.left[row] = 1u;
+  };
+  const uint32_t top = (uint32_t)(best >> 32);
+  const double m = (double)fkey(top);
+  const Grid g = grid_of(p.temperature);
+  const float mrange = range_of((float)m, g);
+  if (!g.plain || !(fabsf(mrange) < kFar)) return leave();
+  auto mass_at = [&](double v) { return exp64(fmax((v - m) * g.per64, -8192.0), l.tab); };
+  auto units = [&](double mass) { return (uint64_t)__builtin_rint(__builtin_amdgcn_ldexp(mass, a.shift)); };
+  const bool by_k = p.top_k > 0 && (uint64_t)p.top_k < n, by_p = p.top_p < 1.0, by_min = p.min_p > 0.0;
+  const bool cut = by_k || by_p || by_min;
+  if (cut && slots > kMergeMost) return leave();
+  // the parts' masses in the row's units
+  uint64_t all = 0;
+  for (int i = tid; i < a.parts; i += kThreads) {
+    const FilterPart f = parts[i];
+    const uint64_t u = f.listed < 0 ? 0ull : units(f.mass * mass_at((double)f.top / (double)g.inv_width));
+    l.part[i] = cut ? 0ull : u;
+    all += u;
+  }
+  // the entries that count: all there are from `edge` on, within the ranges
+  uint64_t u[kMergeEntries];
+  if (cut) {
+#pragma unroll
+    for (int i = 0; i < kMergeEntries; ++i) {
+      const int at = i * kThreads + tid;
+      u[i] = 0ull;
+      if (at >= slots) continue;
+      const float v = fkey((uint32_t)(e[i] >> 32)), d = mrange - range_of(v, g);
+      const bool in = at % kList < max(parts[at / kList].listed, 0) && (uint32_t)(e[i] >> 32) >= edge && d < (float)kFilterRanges;
+      e[i] = in ? e[i] : 0ull;
+      if (!in) continue;
+      u[i] = units(mass_at((double)v));
+      atomicAdd(&l.mass[(int)d], (unsigned long long)u[i]);
+      atomicAdd(&l.cnt[(int)d], 1u);
+    }
+  }
+  all = wave_reduce64(all, plus);
+  __syncthreads();  // (red is read above)
+  if (lane == 0) l.red[wave][0] = all;
+  __syncthreads();
+  all = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) all += l.red[w][0];
+  uint64_t last = 0, total = all, kept = n;
+  if (cut) {
+    // the running sums over the ranges, two a lane
+    const uint64_t m0 = l.mass[2 * lane], m1 = l.mass[2 * lane + 1], c0 = l.cnt[2 * lane], c1 = l.cnt[2 * lane + 1];
+    const uint64_t mrun = wave_scan64(m0 + m1), crun = wave_scan64(c0 + c1);
+    const uint64_t havem = lane64(mrun, 63), have = lane64(crun, 63);
+    bool known = true;
+    uint64_t mass = all;
+    // the entry that ends a prefix: its range, then its place among the range's
+    auto prefix = [&](bool by_count, uint64_t need) {
+      if (need > (by_count ? have : havem)) {
+        known = false;
+        return;
+      }
+      const uint64_t run = by_count ? crun : mrun, second = by_count ? c1 : m1;
+      const int at = __builtin_ctzll(__ballot(run >= need));
+      const bool late = lane64(run, at) - lane64(second, at) < need;
+      const int bin = 2 * at + (late ? 1 : 0);
+      const uint64_t mb = lane64(mrun, at) - lane64(m1, at) - (late ? 0ull : lane64(m0, at));
+      const uint64_t cb = lane64(crun, at) - lane64(c1, at) - (late ? 0ull : lane64(c0, at));
+      if (l.cnt[bin] > (uint32_t)kMergeSome) {
+        known = false;
+        return;
+      }
+      __syncthreads();
+      if (tid == 0) l.nsome = 0u;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kMergeEntries; ++i)
+        if (e[i] && (int)(mrange - range_of(fkey((uint32_t)(e[i] >> 32)), g)) == bin) {
+          const uint32_t to = atomicAdd(&l.nsome, 1u);
+          l.ent[to] = e[i];
+          l.entm[to] = u[i];
+        }
+      __syncthreads();
+      const int c = (int)l.nsome;
+      const uint64_t rest = need - (by_count ? cb : mb);
+      for (int t0 = 0; t0 < c; t0 += 64) {
+        const uint64_t mine = t0 + lane < c ? l.ent[t0 + lane] : 0ull, own = t0 + lane < c ? l.entm[t0 + lane] : 0ull;
+        uint64_t before = 0, rank = 0;
+        for (int i = 0; i < c; ++i) {
+          const bool first = l.ent[i] > mine;
+          before += first ? l.entm[i] : 0ull;
+          rank += first ? 1 : 0;
+        }
+        const uint64_t hit = __ballot(mine && (by_count ? rank + 1 == rest : before < rest && rest <= before + own));
+        if (hit) {
+          const int w = __builtin_ctzll(hit);
+          last = more(last, lane64(mine, w));
+          mass = mb + lane64(before, w) + lane64(own, w);
+        }
+      }
+    };
+    if (by_k) prefix(true, (uint64_t)p.top_k);
+    if (known && by_p) {
+      const uint64_t need = (uint64_t)ceil(fmax(p.top_p, 0.0) * (double)mass);
+      prefix(false, min(max(need, (uint64_t)1), mass));
+    }
+    if (known && by_min) {
+      // the smallest key whose mass reaches min_p, 64 at a time
+      const double least = fmin(p.min_p, 1.0);
+      uint32_t lo = kNegInf, hi = top;
+      while (hi - lo > 1) {
+        const uint32_t step = max((hi - lo) / 65u, 1u), key = lo + step * (uint32_t)(lane + 1);
+        const uint64_t reach = __ballot(key >= hi || key < lo || mass_at((double)fkey(key)) >= least);
+        const int k = reach ? __builtin_ctzll(reach) : 64;
+        const uint32_t to = lo + step * (uint32_t)(k + 1);
+        if (k < 64 && to < hi && to > lo) hi = to;
+        lo = lo + step * (uint32_t)k;
+      }
+      if ((uint64_t)hi << 32 > last) {
+        last = (uint64_t)hi << 32;
+        known = hi >= edge && mrange - range_of(fkey(hi), g) < (float)kFilterRanges;
+      }
+    }
+    if (!known) return leave();
+    total = kept = 0;
+#pragma unroll
+    for (int i = 0; i < kMergeEntries; ++i)
+      if (e[i] && e[i] >= last) {
+        total += u[i];
+        ++kept;
+        atomicAdd(&l.part[~(uint32_t)e[i] >> kLogIds], (unsigned long long)u[i]);
+      }
+    total = wave_reduce64(total, plus);
+    kept = wave_reduce64(kept, plus);
+    __syncthreads();
+    if (lane == 0) {
+      l.red[wave][0] = total;
+      l.red[wave][1] = kept;
+    }
+    if (tid == 0) l.nsome = 0u;
+    __syncthreads();
+    total = kept = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      total += l.red[w][0];
+      kept += l.red[w][1];
+    }
+  }
+  // the draw: the part (every wave finds it), then the id
+  const double whole = __builtin_amdgcn_ldexp((double)total, -a.shift);
+  const uint64_t goal = min((uint64_t)fmax(a.uniforms[row] * (double)total, 0.0), total - 1);
+  uint64_t before = 0;
+  int q = a.parts - 1;
+  for (int i0 = 0; i0 < a.parts; i0 += 64) {
+    const uint64_t mine = i0 + lane < a.parts ? l.part[i0 + lane] : 0ull, run = before + wave_scan64(mine);
+    const uint64_t hit = __ballot(goal < run);
+    if (hit) {
+      const int w = __builtin_ctzll(hit);
+      q = i0 + w;
+      before = lane64(run, w) - lane64(mine, w);
+      break;
+    }
+    before = lane64(run, 63);
+  }
+  if (cut) {
+#pragma unroll
+    for (int i = 0; i < kMergeEntries; ++i)
+      if (e[i] && e[i] >= last && (int)(~(uint32_t)e[i] >> kLogIds) == q) {
+        const uint32_t to = atomicAdd(&l.nsome, 1u);  // (<= kList)
+        l.ent[to] = e[i];
+        l.entm[to] = u[i];
+      }
+    __syncthreads();
+    if (tid < (int)l.nsome) {
+      const uint32_t mine = ~(uint32_t)l.ent[tid];
+      uint64_t run = before;
+      for (int i = 0; i < (int)l.nsome; ++i) run += ~(uint32_t)l.ent[i] < mine ? l.entm[i] : 0ull;
+      if (run <= goal && goal < run + l.entm[tid]) done(mine, mass_at((double)fkey((uint32_t)(l.ent[tid] >> 32))) / whole, kept);
+    }
+    return;
+  }
+  // nothing is cut: the part's values again, the goal as a share of their masses
+  float v[Q][4];
+  span_values<kThreads, kType, kSoft, Q>(a, p, (int64_t)row * a.logits_stride, a.mask ? a.mask + (int64_t)row * a.mask_stride : nullptr,
+                                         history_of(a, row), hcount, q * kIds, v);
+  uint64_t sums = 0;
+  // (ids rise with the quad, then the thread: a quad's sums over the block first)
+  uint64_t quad[Q];
+#pragma unroll
+  for (int j = 0; j < Q; ++j) {
+    uint64_t s = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s += v[j][i] > -__builtin_inff() ? units(mass_at((double)v[j][i])) : 0ull;
+    quad[j] = wave_scan64(s);
+    if (lane == 63) l.mass[j * kWaves + wave] = quad[j];
+    quad[j] -= s;
+  }
+  __syncthreads();
+  for (int i = 0; i < Q * kWaves; ++i) sums += l.mass[i];
+  const uint64_t target = min((uint64_t)((double)(goal - before) * ((double)sums / (double)l.part[q])), sums - 1);
+  uint64_t base = 0;
+#pragma unroll
+  for (int j = 0; j < Q; ++j) {
+    for (int w = 0; w < wave; ++w) base += l.mass[j * kWaves + w];
+    uint64_t run = base + quad[j];
+    for (int w = wave; w < kWaves; ++w) base += l.mass[j * kWaves + w];
+    if (target < run) continue;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint64_t x = v[j][i] > -__builtin_inff() ? units(mass_at((double)v[j][i])) : 0ull;
+      if (run <= target && target < run + x) done((uint32_t)(q * kIds + 4 * (j * kThreads + tid) + i), mass_at((double)v[j][i]) / whole, kept);
+      run += x;
+    }
+  }
+}
+
 template <int kType, bool kSoft>
 hipError_t launch(const FilterArgs &a, hipStream_t stream) {
   const int blocks = a.rows * a.parts;
+  auto both = [&](auto parts_kernel, auto merge_kernel) {
+    parts_kernel<<<blocks, kThreads, 0, stream>>>(a);
+    if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    merge_kernel<<<a.rows, kThreads, 0, stream>>>(a);
+    return hipGetLastError();
+  };
+  hipError_t e;
   switch (a.span) {
-    case 2048: filter_parts_kernel<kType, kSoft, 2><<<blocks, kThreads, 0, stream>>>(a); break;
-    case 4096: filter_parts_kernel<kType, kSoft, 4><<<blocks, kThreads, 0, stream>>>(a); break;
-    default: filter_parts_kernel<kType, kSoft, 8><<<blocks, kThreads, 0, stream>>>(a); break;
+    case 2048: e = both(filter_parts_kernel<kType, kSoft, 2>, filter_merge_kernel<kType, kSoft, 2>); break;
+    case 4096: e = both(filter_parts_kernel<kType, kSoft, 4>, filter_merge_kernel<kType, kSoft, 4>); break;
+    default: e = both(filter_parts_kernel<kType, kSoft, 8>, filter_merge_kernel<kType, kSoft, 8>); break;
   }
-  if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-  filter_merge_kernel<kType, kSoft><<<a.rows, kRowThreads, 0, stream>>>(a);
+  if (e != hipSuccess) return e;
+  filter_rest_kernel<kType, kSoft><<<a.rows, kRowThreads, 0, stream>>>(a);
   return hipGetLastError();
 }
 template <int kType>
@@ -1108,7 +1429,7 @@ int filter_span(int rows, int vocab, int min_blocks) {
 // The parts, their lists, the masses and counts of their ranges.
 size_t filter_scratch_bytes(int rows, int parts) {
   const size_t n = (size_t)rows * parts;
-  return n * (sizeof(FilterPart) + kFilterList * 8 + kFilterRanges * 12);
+  return n * (sizeof(FilterPart) + kFilterList * 8 + kFilterRanges * 12) + (size_t)rows * 4;
 }
 void filter_scratch(void *base, FilterArgs *a) {
   const size_t n = (size_t)a->rows * a->parts;
@@ -1117,7 +1438,8 @@ void filter_scratch(void *base, FilterArgs *a) {
   a->part = reinterpret_cast<FilterPart *>(at);
   a->list = reinterpret_cast<uint64_t *>(at += n * sizeof(FilterPart));
   a->range_mass = reinterpret_cast<uint64_t *>(at += n * kFilterList * 8);
-  a->range_count = reinterpret_cast<uint32_t *>(at + n * kFilterRanges * 8);
+  a->range_count = reinterpret_cast<uint32_t *>(at += n * kFilterRanges * 8);
+  a->left = reinterpret_cast<uint32_t *>(at + n * kFilterRanges * 4);
 }
 
 hipError_t launch_filter(const FilterArgs &a, hipStream_t stream) {

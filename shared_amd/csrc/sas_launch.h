@@ -253,7 +253,8 @@ struct FilterArgs {
   struct FilterPart *part;
   uint64_t *range_mass;  // [rows][parts][kFilterRanges]
   uint32_t *range_count;
-  uint64_t *list;        // [rows][parts][kFilterList]
+  uint64_t *list;        // [rows][parts][span / 64]
+  uint32_t *left;        // [rows]: 1 where the merge leaves the row to the rest kernel
   int32_t type;   // SAS_TYPE_*
   int32_t vocab;
   int32_t rows;
