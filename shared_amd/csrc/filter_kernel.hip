@@ -21,9 +21,9 @@ namespace {
 typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
 typedef u16x4 u16x4u __attribute__((aligned(2)));
 
-constexpr int kRowThreads = 1024;
+constexpr int kRowThreads = 512;  // (1,024 would leave 128 registers a thread, and spill)
 constexpr int kRowWaves = kRowThreads / 64;
-constexpr int kSpan = 8192;                       // ids a block holds at once
+constexpr int kSpan = 16384;                      // ids a block of the rest kernel holds at once
 constexpr int kQuads = kSpan / (4 * kRowThreads); // quads of ids per thread
 constexpr int kMaxFilterParts = 2048;             // 2,048 ids a part: batches of up to 512 parts of 8,192
 constexpr int kEntries = 4096;                    // listed ids the merge takes
@@ -194,7 +194,7 @@ template <int kType, bool kSoft, int Q>
 __global__ __launch_bounds__(kThreads) void filter_parts_kernel(const FilterArgs a) {
   constexpr int kIds = 4 * Q * kThreads;
   constexpr int kList = list_size(kIds);
-  static_assert(kList <= kFilterList, "the list holds them");
+  static_assert(kList <= kFilterList && kList >= 8, "the list holds them");
   __shared__ double tab[kExpTab];
   __shared__ uint32_t count[kIds / 2];
   __shared__ unsigned long long mass[kFilterRanges];
@@ -202,7 +202,7 @@ __global__ __launch_bounds__(kThreads) void filter_parts_kernel(const FilterArgs
   __shared__ float wmax[kWaves];
   __shared__ double wsum[kWaves];
   __shared__ uint32_t wn[kWaves];
-  __shared__ uint32_t first, listed;
+  __shared__ uint32_t first, listed, reach[kWaves], deep[2];
   __shared__ int lowest;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
@@ -219,6 +219,7 @@ __global__ __launch_bounds__(kThreads) void filter_parts_kernel(const FilterArgs
   if (tid == 0) {
     first = ~0u;
     listed = 0u;
+    deep[0] = deep[1] = 0u;
   }
   const float neg = -__builtin_inff();
   float m = neg;
@@ -298,7 +299,40 @@ __global__ __launch_bounds__(kThreads) void filter_parts_kernel(const FilterArgs
       a.range_count[at * kFilterRanges + i] = cnt[i];
     }
   }
-  const float edge = list && lowest >= 0 ? (top - (float)lowest) / g.inv_width : __uint_as_float(0x7F800000u);
+  float edge = list && lowest >= 0 ? (top - (float)lowest) / g.inv_width : __uint_as_float(0x7F800000u);
+  if (list && p.top_k > 0 && lowest == kFilterRanges - 1) {
+    // The ranges leave room in the list and top-k may reach below them: down to
+    // a value that half a list of ids reaches, the smallest of the waves' J-th
+    // largest of their lanes' maxima; or to the largest, if that is too far.
+    constexpr int J = kList / 8;
+    float mine = neg;
+#pragma unroll
+    for (int j = 0; j < Q; ++j) mine = fmaxf(mine, fmaxf(fmaxf(v[j][0], v[j][1]), fmaxf(v[j][2], v[j][3])));
+    const uint32_t key = wave_jth_largest_key(mine > neg ? okey(mine) : 0u, J);
+    if (lane == 0) reach[wave] = key;
+    __syncthreads();
+    uint32_t t[2] = {~0u, 0u};
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      t[0] = min(t[0], reach[w]);
+      t[1] = max(t[1], reach[w]);
+    }
+    if (t[0] == 0u) t[0] = kNegInf + 1u;  // few candidates: all of them
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      uint32_t c = 0;
+      const float least = fkey(t[k]);
+#pragma unroll
+      for (int j = 0; j < Q; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c += t[k] && v[j][i] >= least ? 1u : 0u;
+      c = wave_reduce(c, [](uint32_t x, uint32_t y) { return x + y; });
+      if (lane == 0) atomicAdd(&deep[k], c);
+    }
+    __syncthreads();
+    const int k = deep[0] <= (uint32_t)kList ? 0 : 1;
+    if (t[k] && deep[k] <= (uint32_t)kList) edge = fminf(edge, fkey(t[k]));
+  }
   if (list && lowest >= 0) {
 #pragma unroll
     for (int j = 0; j < Q; ++j)
@@ -496,8 +530,8 @@ struct Row {
   }
 
   // The edge at which the running mass (count) of the order reaches need,
-  // from the histogram over bins in l.mass / l.cnt, which stays as it is only
-  // if `keep`.  *mass, *count: of the prefix up to the edge, its `take` in.
+  // from the histogram over bins in l.mass / l.cnt, which does not outlive it.
+  // *mass (not by_count), *count: of the prefix up to the edge, its `take` in.
   __device__ __forceinline__ Edge edge(bool by_count, uint64_t need, uint64_t *mass, uint64_t *count) {
     uint64_t m0, c0;
     const int bin = find(kBins, by_count, need, &m0, &c0);
@@ -533,8 +567,9 @@ struct Row {
     return Edge{top, (uint32_t)take};
   }
 
-  // The histogram of the row's candidates over the bins.
-  __device__ __forceinline__ void histogram() {
+  // The histogram over the bins of the row's candidates that rank up to `end`
+  // (key 0: all); by_count: without masses.
+  __device__ __forceinline__ void histogram(bool by_count, Edge end) {
     __syncthreads();
     for (int i = threadIdx.x; i < kBins; i += kRowThreads) {
       l.mass[i] = 0ull;
@@ -543,14 +578,14 @@ struct Row {
     __syncthreads();
     uint64_t rest = 0, nrest = 0;
     each([&](uint32_t k) {
-      if (!k) return;
+      if (!k || k <= end.key) return;
       const int b = bin_of(k, s);
-      const uint64_t u = units_of(mass_of(k, s, l.tab), s);
+      const uint64_t u = by_count ? 0ull : units_of(mass_of(k, s, l.tab), s);
       if (b == kBins - 1) {
         rest += u;
         ++nrest;
       } else {
-        atomicAdd(&l.mass[b], (unsigned long long)u);
+        if (!by_count) atomicAdd(&l.mass[b], (unsigned long long)u);
         atomicAdd(&l.cnt[b], 1u);
       }
     });
@@ -558,6 +593,11 @@ struct Row {
     if (threadIdx.x == 0) {
       l.mass[kBins - 1] = rest;
       l.cnt[kBins - 1] = (uint32_t)nrest;
+      if (end.key) {
+        const int b = bin_of(end.key, s);
+        l.mass[b] += end.take * units_of(mass_of(end.key, s, l.tab), s);
+        l.cnt[b] += end.take;
+      }
     }
     __syncthreads();
   }
@@ -604,18 +644,14 @@ __device__ __forceinline__ void row_by_values(Row<kType, kSoft> &R, const Filter
   Edge e{0u, 0u};  // no edge: every candidate
   uint64_t mass = 0, count = 0;
   if (p.top_k > 0 && (uint64_t)p.top_k < n) {
-    R.histogram();
+    R.histogram(true, e);
     e = R.edge(true, (uint64_t)p.top_k, &mass, &count);
   }
   if (p.top_p < 1.0) {
-    R.histogram();
-    if (!e.key) {
-      uint64_t all = 0;
-      zero = 0;
-      for (int i = tid; i < kBins; i += kRowThreads) all += l.mass[i];
-      block_sum2(l, all, zero);
-      mass = all;
-    }
+    R.histogram(false, e);
+    mass = zero = 0;
+    for (int i = tid; i < kBins; i += kRowThreads) mass += l.mass[i];
+    block_sum2(l, mass, zero);
     const double need = ceil(fmax(p.top_p, 0.0) * (double)mass);
     const Edge f = R.edge(false, min(max((uint64_t)need, (uint64_t)1), mass), &mass, &count);
     if (!e.key || f.key > e.key || (f.key == e.key && f.take < e.take)) e = f;
@@ -923,22 +959,39 @@ __device__ __forceinline__ bool row_by_parts(Row<kType, kSoft> &R, const FilterA
         if (!any) continue;
         float v[kQuads][4];
         span_values<kRowThreads, kType, kSoft, kQuads>(a, p, R.row0, R.mask, R.h, l.count, id0, v);
+        // a place for each of the wave's ids there, then the ids
+        uint32_t hits = 0;
 #pragma unroll
         for (int j = 0; j < kQuads; ++j)
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (mrange - range_of(v[j][i], g) == (float)bin) {
-              const uint32_t to = atomicAdd(&l.nent, 1u);
-              if (to < (uint32_t)kEntries) {
-                const uint32_t key = okey(v[j][i]);
-                l.ent[to] = (uint64_t)key << 32 | (uint32_t) ~(uint32_t)(id0 + 4 * (j * kRowThreads + tid) + i);
-                l.entm[to] = units_of(mass_of(key, R.s, l.tab), R.s);
+          for (int i = 0; i < 4; ++i) hits |= (mrange - range_of(v[j][i], g) == (float)bin ? 1u : 0u) << (4 * j + i);
+        const uint32_t mine = __popc(hits);
+        uint32_t upto = mine;
+#pragma unroll
+        for (int s = 1; s < 64; s <<= 1) {
+          const uint32_t y = (uint32_t)__shfl_up((int)upto, s, 64);
+          if ((tid & 63) >= s) upto += y;
+        }
+        uint32_t base = 0;
+        if ((tid & 63) == 63 && upto) base = atomicAdd(&l.nent, upto);
+        uint32_t to = (uint32_t)__builtin_amdgcn_readlane((int)base, 63) + upto - mine;
+        if (hits) {
+#pragma unroll
+          for (int j = 0; j < kQuads; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if ((hits >> (4 * j + i)) & 1u) {
+                if (to < (uint32_t)kEntries)
+                  l.ent[to] = (uint64_t)okey(v[j][i]) << 32 | (uint32_t) ~(uint32_t)(id0 + 4 * (j * kRowThreads + tid) + i);
+                ++to;
               }
-            }
+        }
       }
       __syncthreads();
       fits = fits && l.nent <= (uint32_t)kEntries;
       entries = (int)min(l.nent, (uint32_t)kEntries);
+      for (int i = tid; i < entries; i += kRowThreads) l.entm[i] = units_of(mass_of((uint32_t)(l.ent[i] >> 32), R.s, l.tab), R.s);
+      __syncthreads();
     };
     // the ends of the prefixes of top-k and top-p
     bool known = true;
@@ -989,24 +1042,20 @@ __device__ __forceinline__ bool row_by_parts(Row<kType, kSoft> &R, const FilterA
     }
     __syncthreads();
     total = kept = 0;
-    for (int i = tid; i < a.parts; i += kRowThreads) {
-      uint64_t u = 0;
-      if (!listed) {
-        const FilterPart f = parts[i];
-        const int end = min(bin - (int)mrange + f.top, kFilterRanges);
-        const int64_t at = ((int64_t)row * a.parts + i) * kFilterRanges;
-        if (f.listed >= 0 && f.max > -__builtin_inff()) {
-          uint64_t w = 0;
-          for (int k = 0; k < end; ++k) {
-            w += a.range_mass[at + k];
-            kept += a.range_count[at + k];
-          }
-          u = (uint64_t)__builtin_rint(__builtin_amdgcn_ldexp((double)w * scale_of(f), a.shift - kFilterShift));
-        }
+    for (int i = tid; i < a.parts; i += kRowThreads) l.part[i] = 0ull;
+    __syncthreads();
+    if (!listed)
+      for (int i = tid; i < a.parts * kFilterRanges; i += kRowThreads) {
+        const FilterPart f = parts[i / kFilterRanges];
+        if (f.listed < 0 || !(f.max > -__builtin_inff()) || (int)mrange - f.top + i % kFilterRanges >= bin) continue;
+        const int64_t at = (int64_t)row * a.parts * kFilterRanges + i;
+        const uint32_t c = a.range_count[at];
+        if (c == 0u) continue;
+        const uint64_t u = (uint64_t)__builtin_rint(__builtin_amdgcn_ldexp((double)a.range_mass[at] * scale_of(f), a.shift - kFilterShift));
+        total += u;
+        kept += c;
+        atomicAdd(&l.part[i / kFilterRanges], (unsigned long long)u);
       }
-      l.part[i] = u;
-      total += u;
-    }
     __syncthreads();
     for (int i = tid; i < entries; i += kRowThreads)
       if (l.ent[i] >= last) {
@@ -1102,6 +1151,7 @@ struct MergeShared {
   uint32_t cnt[kFilterRanges];
   unsigned long long part[kMaxFilterParts];
   unsigned long long ent[kMergeSome], entm[kMergeSome];
+  uint64_t end[2];
   uint32_t nsome;
 };
 
@@ -1122,6 +1172,11 @@ __device__ __forceinline__ uint64_t wave_scan64(uint64_t x) {
 }
 __device__ __forceinline__ uint64_t lane64(uint64_t x, int lane) {
   return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), lane) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)x, lane);
+}
+
+// The merge's bins: 96 ranges, then 32 of 16 ranges each, the last without end.
+__device__ __forceinline__ int merge_bin(float d) {
+  return d < 96.0f ? (int)d : d < 592.0f ? 96 + ((int)d - 96) / 16 : kFilterRanges - 1;
 }
 
 template <int kType, bool kSoft, int Q>
@@ -1202,7 +1257,7 @@ __global__ __launch_bounds__(kThreads) void filter_merge_kernel(const FilterArgs
     l.part[i] = cut ? 0ull : u;
     all += u;
   }
-  // the entries that count: all there are from `edge` on, within the ranges
+  // the entries that count: all there are from `edge` on
   uint64_t u[kMergeEntries];
   if (cut) {
 #pragma unroll
@@ -1211,12 +1266,12 @@ __global__ __launch_bounds__(kThreads) void filter_merge_kernel(const FilterArgs
       u[i] = 0ull;
       if (at >= slots) continue;
       const float v = fkey((uint32_t)(e[i] >> 32)), d = mrange - range_of(v, g);
-      const bool in = at % kList < max(parts[at / kList].listed, 0) && (uint32_t)(e[i] >> 32) >= edge && d < (float)kFilterRanges;
+      const bool in = at % kList < max(parts[at / kList].listed, 0) && (uint32_t)(e[i] >> 32) >= edge;
       e[i] = in ? e[i] : 0ull;
       if (!in) continue;
       u[i] = units(mass_at((double)v));
-      atomicAdd(&l.mass[(int)d], (unsigned long long)u[i]);
-      atomicAdd(&l.cnt[(int)d], 1u);
+      atomicAdd(&l.mass[merge_bin(d)], (unsigned long long)u[i]);
+      atomicAdd(&l.cnt[merge_bin(d)], 1u);
     }
   }
   all = wave_reduce64(all, plus);
@@ -1255,7 +1310,7 @@ __global__ __launch_bounds__(kThreads) void filter_merge_kernel(const FilterArgs
       __syncthreads();
 #pragma unroll
       for (int i = 0; i < kMergeEntries; ++i)
-        if (e[i] && (int)(mrange - range_of(fkey((uint32_t)(e[i] >> 32)), g)) == bin) {
+        if (e[i] && merge_bin(mrange - range_of(fkey((uint32_t)(e[i] >> 32)), g)) == bin) {
           const uint32_t to = atomicAdd(&l.nsome, 1u);
           l.ent[to] = e[i];
           l.entm[to] = u[i];
@@ -1263,21 +1318,23 @@ __global__ __launch_bounds__(kThreads) void filter_merge_kernel(const FilterArgs
       __syncthreads();
       const int c = (int)l.nsome;
       const uint64_t rest = need - (by_count ? cb : mb);
-      for (int t0 = 0; t0 < c; t0 += 64) {
-        const uint64_t mine = t0 + lane < c ? l.ent[t0 + lane] : 0ull, own = t0 + lane < c ? l.entm[t0 + lane] : 0ull;
+      for (int t = tid; t < c; t += kThreads) {
+        const uint64_t mine = l.ent[t], own = l.entm[t];
         uint64_t before = 0, rank = 0;
+#pragma unroll 4
         for (int i = 0; i < c; ++i) {
           const bool first = l.ent[i] > mine;
           before += first ? l.entm[i] : 0ull;
           rank += first ? 1 : 0;
         }
-        const uint64_t hit = __ballot(mine && (by_count ? rank + 1 == rest : before < rest && rest <= before + own));
-        if (hit) {
-          const int w = __builtin_ctzll(hit);
-          last = more(last, lane64(mine, w));
-          mass = mb + lane64(before, w) + lane64(own, w);
+        if (by_count ? rank + 1 == rest : before < rest && rest <= before + own) {
+          l.end[0] = mine;
+          l.end[1] = before + own;
         }
       }
+      __syncthreads();
+      last = more(last, l.end[0]);
+      mass = mb + l.end[1];
     };
     if (by_k) prefix(true, (uint64_t)p.top_k);
     if (known && by_p) {
@@ -1298,7 +1355,7 @@ __global__ __launch_bounds__(kThreads) void filter_merge_kernel(const FilterArgs
       }
       if ((uint64_t)hi << 32 > last) {
         last = (uint64_t)hi << 32;
-        known = hi >= edge && mrange - range_of(fkey(hi), g) < (float)kFilterRanges;
+        known = hi >= edge;
       }
     }
     if (!known) return leave();
@@ -1421,7 +1478,7 @@ hipError_t launch(const FilterArgs &a, bool soft, hipStream_t stream) {
 }  // namespace
 
 int filter_span(int rows, int vocab, int min_blocks) {
-  int span = kSpan;
+  int span = 8192;
   while (span > 2048 && (int64_t)rows * ((vocab + span - 1) / span) < min_blocks) span /= 2;
   return span;
 }
