@@ -404,9 +404,10 @@ struct RowShared {
   unsigned long long part[kMaxFilterParts];
   unsigned long long ent[kEntries];   // listed ids: key << 32 | ~id
   unsigned long long entm[kEntries];  // and their masses
-  uint32_t some[kRowThreads];         // entries under a closer look
-  uint32_t nent, nsome;
+  uint32_t some[kRowThreads];         // whether a span has ids of a range
+  uint32_t nent;
 };
+static_assert(SAS_MAX_VOCAB / kSpan <= kRowThreads, "a place for every span");
 
 __device__ __forceinline__ uint64_t shfl_xor64(uint64_t x, int s) { return (uint64_t)__shfl_xor((unsigned long long)x, s, 64); }
 
@@ -817,34 +818,30 @@ __device__ __forceinline__ bool row_by_parts(Row<kType, kSoft> &R, const FilterA
                                              uint32_t *top_key, uint64_t *candidates, const Result &done) {
   const int tid = threadIdx.x;
   const FilterPart *parts = a.part + (int64_t)row * a.parts;
-  // the best candidate, how many there are, and from which value on all are listed
+  // the best candidate, and how many there are
   uint64_t best = 0, n = 0, zero = 0;
-  uint32_t edge = 0;  // okey
   for (int i = tid; i < a.parts; i += kRowThreads) {
     const FilterPart f = parts[i];
     if (f.max > -__builtin_inff()) {
       best = max(best, (uint64_t)okey(f.max) << 32 | (uint32_t)~f.id);
       n += (uint64_t)f.count;
-      edge = max(edge, f.listed < 0 ? okey(f.max) + 1u : okey(f.edge));
     }
   }
 #pragma unroll
   for (int s = 32; s > 0; s >>= 1) {
     best = max(best, shfl_xor64(best, s));
-    edge = max(edge, (uint32_t)__shfl_xor((int)edge, s, 64));
     n += shfl_xor64(n, s);
   }
   if ((tid & 63) == 0) {
     l.red[tid >> 6][0] = best;
-    l.red[tid >> 6][1] = (uint64_t)edge << 32 | n;
+    l.red[tid >> 6][1] = n;
   }
   __syncthreads();
   n = 0;
 #pragma unroll
   for (int w = 0; w < kRowWaves; ++w) {
     best = max(best, (uint64_t)l.red[w][0]);
-    edge = max(edge, (uint32_t)(l.red[w][1] >> 32));
-    n += l.red[w][1] & 0xFFFFFFFFull;
+    n += l.red[w][1];
   }
   if (best == 0 || greedy_row(p)) {
     if (tid == 0) done(best ? ~(uint32_t)best : SAS_NO_TOKEN, best ? 1.0 : 0.0, best ? 1 : 0);
@@ -875,33 +872,25 @@ __device__ __forceinline__ bool row_by_parts(Row<kType, kSoft> &R, const FilterA
   uint64_t last = 0;      // every id whose (key, ~id) reaches it is kept
   uint64_t total = all, kept = n;
   int entries = 0;        // what l.ent holds
-  bool listed = false;    // all that are kept
   const int log_span = 31 - __builtin_clz(a.span);
   if (cut) {
-    // the listed ids of the row's ranges, all that there are from `edge` on
+    // the ranges of all parts, in the row's units
     for (int i = tid; i < kFilterRanges; i += kRowThreads) {
       l.mass[i] = 0ull;
       l.cnt[i] = 0u;
     }
     __syncthreads();
-    const int list = list_size(a.span);
-    const uint64_t *lists = a.list + (int64_t)row * a.parts * list;
-    for (int i = tid; i < a.parts * list; i += kRowThreads) {
-      if (i % list >= max(parts[i / list].listed, 0)) continue;
-      const uint64_t e = lists[i];
-      const uint32_t key = (uint32_t)(e >> 32);
-      const float d = mrange - range_of(fkey(key), g);
-      if (key < edge || !(d < (float)kFilterRanges)) continue;
-      const uint32_t to = atomicAdd(&l.nent, 1u);
-      if (to >= (uint32_t)kEntries) continue;
-      const uint64_t u = units_of(mass_of(key, R.s, l.tab), R.s);
-      l.ent[to] = e;
-      l.entm[to] = u;
-      atomicAdd(&l.mass[(int)d], (unsigned long long)u);
-      atomicAdd(&l.cnt[(int)d], 1u);
+    for (int i = tid; i < a.parts * kFilterRanges; i += kRowThreads) {
+      const FilterPart f = parts[i / kFilterRanges];
+      const int64_t at = (int64_t)row * a.parts * kFilterRanges + i;
+      const uint32_t c = a.range_count[at];
+      const uint64_t w = a.range_mass[at];
+      const int d = (int)mrange - f.top + i % kFilterRanges;
+      if (f.listed < 0 || !(f.max > -__builtin_inff()) || c == 0u || d >= kFilterRanges) continue;
+      atomicAdd(&l.cnt[d], c);
+      atomicAdd(&l.mass[d], (unsigned long long)__builtin_rint(__builtin_amdgcn_ldexp((double)w * scale_of(f), a.shift - kFilterShift)));
     }
     __syncthreads();
-    entries = (int)min(l.nent, (uint32_t)kEntries);
     uint64_t have = 0, havem = 0;
     for (int i = tid; i < kFilterRanges; i += kRowThreads) {
       have += l.cnt[i];
@@ -909,39 +898,8 @@ __device__ __forceinline__ bool row_by_parts(Row<kType, kSoft> &R, const FilterA
     }
     block_sum2(l, have, havem);
     const uint32_t least = by_min ? least_key(p.min_p, top, R.s, l.tab) : 0u;
-    const uint64_t of_p = by_p ? (uint64_t)ceil(fmax(p.top_p, 0.0) * (double)all) : 0ull;
-    // whether the lists hold the prefixes' ends (top-p's need is at most of_p)
-    listed = l.nent <= (uint32_t)kEntries && (!by_k || (uint64_t)p.top_k <= have) && (!by_p || (by_k && (uint64_t)p.top_k <= have) || of_p <= havem) &&
-             (by_k || by_p || (least >= edge && mrange - range_of(fkey(least), g) < (float)kFilterRanges));
-    if (!listed) {
-      // the ranges of all parts instead
-      __syncthreads();
-      for (int i = tid; i < kFilterRanges; i += kRowThreads) {
-        l.mass[i] = 0ull;
-        l.cnt[i] = 0u;
-      }
-      __syncthreads();
-      for (int i = tid; i < a.parts * kFilterRanges; i += kRowThreads) {
-        const FilterPart f = parts[i / kFilterRanges];
-        if (f.listed < 0 || !(f.max > -__builtin_inff())) continue;
-        const int64_t at = ((int64_t)row * a.parts) * kFilterRanges + i;
-        const uint32_t c = a.range_count[at];
-        const int d = (int)mrange - f.top + i % kFilterRanges;
-        if (c == 0u || d >= kFilterRanges) continue;
-        atomicAdd(&l.cnt[d], c);
-        atomicAdd(&l.mass[d], (unsigned long long)__builtin_rint(
-                                  __builtin_amdgcn_ldexp((double)a.range_mass[at] * scale_of(f), a.shift - kFilterShift)));
-      }
-      __syncthreads();
-      have = havem = 0;
-      for (int i = tid; i < kFilterRanges; i += kRowThreads) {
-        have += l.cnt[i];
-        havem += l.mass[i];
-      }
-      block_sum2(l, have, havem);
-    }
-    // The ids of range `bin` into l.ent: from the row's values, in the parts that
-    // have any there.
+    // The ids of range `bin` into l.ent: from the row's values, in the spans that
+    // have any there (l.some).
     bool fits = true;
     int held = -1;
     auto gather = [&](int bin) {
@@ -949,14 +907,16 @@ __device__ __forceinline__ bool row_by_parts(Row<kType, kSoft> &R, const FilterA
       held = bin;
       __syncthreads();
       if (tid == 0) l.nent = 0u;
+      for (int i = tid; i < R.spans(); i += kRowThreads) l.some[i] = 0u;
+      __syncthreads();
+      for (int q = tid; q < a.parts; q += kRowThreads) {
+        const int i = bin - (int)mrange + parts[q].top;
+        if (parts[q].listed >= 0 && i >= 0 && i < kFilterRanges && a.range_count[((int64_t)row * a.parts + q) * kFilterRanges + i] > 0u)
+          l.some[(q << log_span) / kSpan] = 1u;
+      }
       __syncthreads();
       for (int id0 = 0; id0 < a.vocab; id0 += kSpan) {
-        bool any = false;
-        for (int q = id0 >> log_span; q < min((id0 + kSpan) >> log_span, a.parts); ++q) {
-          const int i = bin - (int)mrange + parts[q].top;
-          any = any || (parts[q].listed >= 0 && i >= 0 && i < kFilterRanges && a.range_count[((int64_t)row * a.parts + q) * kFilterRanges + i] > 0u);
-        }
-        if (!any) continue;
+        if (!l.some[id0 / kSpan]) continue;
         float v[kQuads][4];
         span_values<kRowThreads, kType, kSoft, kQuads>(a, p, R.row0, R.mask, R.h, l.count, id0, v);
         // a place for each of the wave's ids there, then the ids
@@ -1002,25 +962,20 @@ __device__ __forceinline__ bool row_by_parts(Row<kType, kSoft> &R, const FilterA
       }
       uint64_t m0, c0, m1, c1;
       const int bin = R.find(kFilterRanges, by_count, need, &m0, &c0);
-      if (!listed) {
-        gather(bin);
-        if (!fits) {
-          known = false;
-          return;
-        }
-        // (the range's mass was rounded as a whole, its ids' one by one)
-        uint64_t sum = 0;
-        zero = 0;
-        for (int i = tid; i < entries; i += kRowThreads) sum += l.entm[i];
-        block_sum2(l, sum, zero);
-        known = sum > 0;
-        if (!known) return;
-        last = max(last, end_of(R, l, entries, by_count, by_count ? need - c0 : min(need - m0, sum), &m1, &c1));
-        *mass = m0 + m1;
-      } else {
-        // (all entries: those of the ranges above rank before the end)
-        last = max(last, end_of(R, l, entries, by_count, need, mass, &c1));
+      gather(bin);
+      if (!fits) {
+        known = false;
+        return;
       }
+      // (the range's mass was rounded as a whole, its ids' one by one)
+      uint64_t sum = 0;
+      zero = 0;
+      for (int i = tid; i < entries; i += kRowThreads) sum += l.entm[i];
+      block_sum2(l, sum, zero);
+      known = sum > 0;
+      if (!known) return;
+      last = max(last, end_of(R, l, entries, by_count, by_count ? need - c0 : min(need - m0, sum), &m1, &c1));
+      *mass = m0 + m1;
     };
     uint64_t mass = all;
     if (by_k) prefix(true, (uint64_t)p.top_k, &mass);
@@ -1036,26 +991,23 @@ __device__ __forceinline__ bool row_by_parts(Row<kType, kSoft> &R, const FilterA
     // what is kept of each part: of the ranges above the end's all, of its own
     // by its ids
     const int bin = (int)(mrange - range_of(fkey((uint32_t)(last >> 32)), g));
-    if (!listed) {
-      gather(bin);
-      if (!fits) return false;
-    }
+    gather(bin);
+    if (!fits) return false;
     __syncthreads();
     total = kept = 0;
     for (int i = tid; i < a.parts; i += kRowThreads) l.part[i] = 0ull;
     __syncthreads();
-    if (!listed)
-      for (int i = tid; i < a.parts * kFilterRanges; i += kRowThreads) {
-        const FilterPart f = parts[i / kFilterRanges];
-        if (f.listed < 0 || !(f.max > -__builtin_inff()) || (int)mrange - f.top + i % kFilterRanges >= bin) continue;
-        const int64_t at = (int64_t)row * a.parts * kFilterRanges + i;
-        const uint32_t c = a.range_count[at];
-        if (c == 0u) continue;
-        const uint64_t u = (uint64_t)__builtin_rint(__builtin_amdgcn_ldexp((double)a.range_mass[at] * scale_of(f), a.shift - kFilterShift));
-        total += u;
-        kept += c;
-        atomicAdd(&l.part[i / kFilterRanges], (unsigned long long)u);
-      }
+    for (int i = tid; i < a.parts * kFilterRanges; i += kRowThreads) {
+      const FilterPart f = parts[i / kFilterRanges];
+      if (f.listed < 0 || !(f.max > -__builtin_inff()) || (int)mrange - f.top + i % kFilterRanges >= bin) continue;
+      const int64_t at = (int64_t)row * a.parts * kFilterRanges + i;
+      const uint32_t c = a.range_count[at];
+      if (c == 0u) continue;
+      const uint64_t u = (uint64_t)__builtin_rint(__builtin_amdgcn_ldexp((double)a.range_mass[at] * scale_of(f), a.shift - kFilterShift));
+      total += u;
+      kept += c;
+      atomicAdd(&l.part[i / kFilterRanges], (unsigned long long)u);
+    }
     __syncthreads();
     for (int i = tid; i < entries; i += kRowThreads)
       if (l.ent[i] >= last) {
@@ -1070,21 +1022,6 @@ __device__ __forceinline__ bool row_by_parts(Row<kType, kSoft> &R, const FilterA
   goal = min(goal, total - 1);
   const int q = part_of(l, a.parts, goal, &before);
   const double whole = __builtin_amdgcn_ldexp((double)total, -a.shift);
-  if (cut && listed) {
-    if (tid == 0) l.nsome = 0u;
-    __syncthreads();
-    for (int i = tid; i < entries; i += kRowThreads)
-      if (l.ent[i] >= last && (int)(~(uint32_t)l.ent[i] >> log_span) == q) l.some[atomicAdd(&l.nsome, 1u)] = (uint32_t)i;  // (<= kFilterList)
-    __syncthreads();
-    if (tid < (int)l.nsome) {
-      const uint64_t mine = l.ent[l.some[tid]], own = l.entm[l.some[tid]];
-      uint64_t run = before;
-      for (int i = 0; i < (int)l.nsome; ++i)
-        if (~(uint32_t)l.ent[l.some[i]] < ~(uint32_t)mine) run += l.entm[l.some[i]];
-      if (run <= goal && goal < run + own) done(~(uint32_t)mine, mass_of((uint32_t)(mine >> 32), R.s, l.tab) / whole, kept);
-    }
-    return true;
-  }
   // the part's values again: its kept ids' masses, and the goal as a share of them
   float v[kQuads][4];
   const int id0 = q * a.span;
