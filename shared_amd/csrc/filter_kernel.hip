@@ -105,7 +105,7 @@ __device__ __forceinline__ float penalized(float v, uint32_t count, const sas_fi
 // so their ranges add up, and scaling by a power of two is exact.
 struct Grid {
   float inv_width;   // 2^-e
-  double per64;      // 64 / (T ln 2): exponentials count in 64ths of octaves
+  double per;        // 256 / (T ln 2): 256ths of an octave a unit of value
   bool plain;        // T is in the grid's scope
 };
 __device__ __forceinline__ Grid grid_of(double temperature) {
@@ -113,7 +113,7 @@ __device__ __forceinline__ Grid grid_of(double temperature) {
   const int e = (int)(((uint64_t)__double_as_longlong(temperature) >> 52) & 0x7FF) - 1023 - 3;
   g.plain = temperature > 0.0 && e >= -24 && e <= 24;
   g.inv_width = __uint_as_float((uint32_t)(127 - (g.plain ? e : 0)) << 23);
-  g.per64 = 92.33248261689366 / temperature;
+  g.per = 369.3299304675746 / temperature;
   return g;
 }
 // A value's range; exact below 2^22 ranges from zero (kFar otherwise).
@@ -123,20 +123,29 @@ constexpr float kFar = 4194304.0f;
 // e^(1/8) stay below 2^64.
 constexpr double kUnit = (double)(1ull << kFilterShift);
 
-// 2^(y / 64), -8192 <= y <= 64: the table's 2^(k / 64) times a Taylor series
-// in |r| <= 1/2 (2^(r / 64) to degree 5, 4e-17 short), the exponent added as
-// an integer: 13 double instructions, the longest part of the pass.
-__device__ __forceinline__ double exp64(double y, const double *tab) {
+// Masses are powers of two counted in 256ths of an octave.  2^(j / 256), j = 0
+// .. 255, within 1 ulp, a thread an entry (the block's first 256).
+constexpr int kTab = 256;
+__device__ __forceinline__ void fill_tab(double *tab) {
+  const int j = threadIdx.x & 3;
+  const double c = j == 0 ? 1.0 : j == 1 ? 0x1.00b1afa5abcbfp+0 : j == 2 ? 0x1.0163da9fb3335p+0 : 0x1.02168143b0281p+0;
+  if (threadIdx.x < kTab) tab[threadIdx.x] = kExp2Tab[threadIdx.x >> 2].x * c;
+}
+// 2^(y / 256), -32768 <= y <= 256: the table's 2^(k / 256) times a Taylor series
+// in |r| <= 1/2 (2^(r / 256) to degree 4, 4e-17 short), the exponent added as
+// an integer; within 3 ulp.  14 instructions a value, most of what the parts
+// kernel computes.
+__device__ __forceinline__ double exp256(double y, const double *tab) {
   const double magic = 6755399441055744.0;
   const double kf = y + magic;
   const int k = (int)(uint32_t)(uint64_t)__double_as_longlong(kf);
   const double r = y - (kf - magic);
-  const double t = tab[k & 63];
-  const double c1 = 0.010830424696249145, c2 = 5.864904955056169e-05, c3 = 2.1173137155464774e-07, c4 = 5.732851688640402e-10,
-               c5 = 1.2417843701716923e-12;
-  const double x = t * fma(fma(fma(fma(fma(r, c5, c4), r, c3), r, c2), r, c1), r, 1.0);
-  return __hiloint2double(__double2hiint(x) + ((k & ~63) << 14), __double2loint(x));
+  const double t = tab[k & (kTab - 1)];
+  const double c1 = 0.0027076061740622863, c2 = 3.665565596910106e-06, c3 = 3.308302680541371e-09, c4 = 2.239395190875157e-12;
+  const double x = t * fma(fma(fma(fma(r, c4, c3), r, c2), r, c1), r, 1.0);
+  return __hiloint2double(__double2hiint(x) + ((k >> 8) << 20), __double2loint(x));
 }
+constexpr double kLeast = -32768.0;  // (2^-128: nothing)
 
 __device__ __forceinline__ bool filters(const sas_filter_params &p) {
   return p.top_k > 0 || p.top_p < 1.0 || p.min_p > 0.0;
@@ -190,27 +199,27 @@ __device__ __forceinline__ void span_values(const FilterArgs &a, const sas_filte
 // Ids a part of `ids` lists: 4,096 a row of 262,144.
 constexpr int list_size(int ids) { return ids / 64; }
 
-template <int kType, bool kSoft, int Q>
-__global__ __launch_bounds__(kThreads) void filter_parts_kernel(const FilterArgs a) {
-  constexpr int kIds = 4 * Q * kThreads;
+template <int kType, bool kSoft, int kT, int Q>
+__global__ __launch_bounds__(kT) void filter_parts_kernel(const FilterArgs a) {
+  constexpr int kIds = 4 * Q * kT, kW = kT / 64;
   constexpr int kList = list_size(kIds);
   static_assert(kList <= kFilterList && kList >= 8, "the list holds them");
-  __shared__ double tab[kExpTab];
+  __shared__ double tab[kTab];
   __shared__ uint32_t count[kIds / 2];
   __shared__ unsigned long long mass[kFilterRanges];
   __shared__ uint32_t cnt[kFilterRanges];
-  __shared__ float wmax[kWaves];
-  __shared__ double wsum[kWaves];
-  __shared__ uint32_t wn[kWaves];
-  __shared__ uint32_t first, listed, reach[kWaves], deep[2];
+  __shared__ float wmax[kW];
+  __shared__ double wsum[kW];
+  __shared__ uint32_t wn[kW];
+  __shared__ uint32_t first, listed, reach[kW], deep[2];
   __shared__ int lowest;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
-  if (tid < kExpTab) tab[tid] = exp_tab_entry().x;
+  fill_tab(tab);
   const sas_filter_params p = load_filter_params(a, row);
   const int64_t row0 = (int64_t)row * a.logits_stride;
   float v[Q][4];
-  span_values<kThreads, kType, kSoft, Q>(a, p, row0, a.mask ? a.mask + (int64_t)row * a.mask_stride : nullptr, history_of(a, row), count,
+  span_values<kT, kType, kSoft, Q>(a, p, row0, a.mask ? a.mask + (int64_t)row * a.mask_stride : nullptr, history_of(a, row), count,
                                          part * kIds, v);
   if (tid < kFilterRanges) {
     mass[tid] = 0ull;
@@ -228,45 +237,50 @@ __global__ __launch_bounds__(kThreads) void filter_parts_kernel(const FilterArgs
   m = wave_max(m);
   if (lane == 0) wmax[wave] = m;
   __syncthreads();
-  m = fmaxf(fmaxf(wmax[0], wmax[1]), fmaxf(wmax[2], wmax[3]));
+  m = wmax[0];
+#pragma unroll
+  for (int w = 1; w < kW; ++w) m = fmaxf(m, wmax[w]);
   const int64_t at = (int64_t)row * a.parts + part;
   FilterPart *out = a.part + at;
   const Grid g = grid_of(p.temperature);
   const float top = range_of(m, g);
   const bool greedy = greedy_row(p), ranged = !greedy && g.plain && fabsf(top) < kFar && m > neg;
   const bool list = ranged && filters(p);
-  // masses are relative to the top of max's range, so that ranges of all parts
-  // share their edges; (-inf and what is 88 T below: e^-88)
-  const double ref = (double)top / (double)g.inv_width;
+  // Masses are relative to the lower edge of max's range.  (The edge's place is
+  // rounded as 256ths of an octave; the merge's arithmetic rounds it alike.)
+  const double ref = (double)top / (double)g.inv_width * g.per;
   double sum[4] = {0.0, 0.0, 0.0, 0.0};
   uint32_t n = 0, best = ~0u;
 #pragma unroll
   for (int j = 0; j < Q; ++j)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float x = v[j][i];
-      n += x > neg ? 1u : 0u;
-      if (x == m) best = min(best, (uint32_t)(part * kIds + 4 * (j * kThreads + tid) + i));
-    }
+    for (int i = 0; i < 4; ++i) n += v[j][i] > neg ? 1u : 0u;
+  if (greedy) {
+#pragma unroll
+    for (int j = 0; j < Q; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (v[j][i] == m) best = min(best, (uint32_t)(part * kIds + 4 * (j * kT + tid) + i));
+  }
   if (ranged) {
+    const float hot = list ? (top - (float)(kFilterRanges - 1)) / g.inv_width : __uint_as_float(0x7F800000u);
 #pragma unroll
     for (int j = 0; j < Q; ++j) {
       double u[4];
-      float d[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        u[i] = exp64(fmax(((double)v[j][i] - ref) * g.per64, -8192.0), tab);
+        u[i] = exp256(fmax(fma((double)v[j][i], g.per, -ref), kLeast), tab);
         sum[i] += u[i];
-        d[i] = top - range_of(v[j][i], g);
       }
-      if (list && fminf(fminf(d[0], d[1]), fminf(d[2], d[3])) < (float)kFilterRanges) {
+      if (fmaxf(fmaxf(v[j][0], v[j][1]), fmaxf(v[j][2], v[j][3])) >= hot) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (d[i] < (float)kFilterRanges) {
+          if (v[j][i] >= hot) {
+            const int d = (int)(top - range_of(v[j][i], g));
             // (a number below 2^51 in the low bits of its sum with 2^52)
             const uint64_t whole = (uint64_t)__double_as_longlong(fma(u[i], kUnit, 4503599627370496.0)) & 0xFFFFFFFFFFFFFull;
-            atomicAdd(&mass[(int)d[i]], (unsigned long long)whole);
-            atomicAdd(&cnt[(int)d[i]], 1u);
+            atomicAdd(&mass[d], (unsigned long long)whole);
+            atomicAdd(&cnt[d], 1u);
           }
       }
     }
@@ -294,7 +308,7 @@ __global__ __launch_bounds__(kThreads) void filter_parts_kernel(const FilterArgs
   }
   if (list) {
     __syncthreads();
-    for (int i = tid; i < kFilterRanges; i += kThreads) {
+    for (int i = tid; i < kFilterRanges; i += kT) {
       a.range_mass[at * kFilterRanges + i] = mass[i];
       a.range_count[at * kFilterRanges + i] = cnt[i];
     }
@@ -304,7 +318,7 @@ __global__ __launch_bounds__(kThreads) void filter_parts_kernel(const FilterArgs
     // The ranges leave room in the list and top-k may reach below them: down to
     // a value that half a list of ids reaches, the smallest of the waves' J-th
     // largest of their lanes' maxima; or to the largest, if that is too far.
-    constexpr int J = kList / 8;
+    constexpr int J = kList / 2 / kW;
     float mine = neg;
 #pragma unroll
     for (int j = 0; j < Q; ++j) mine = fmaxf(mine, fmaxf(fmaxf(v[j][0], v[j][1]), fmaxf(v[j][2], v[j][3])));
@@ -313,7 +327,7 @@ __global__ __launch_bounds__(kThreads) void filter_parts_kernel(const FilterArgs
     __syncthreads();
     uint32_t t[2] = {~0u, 0u};
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
+    for (int w = 0; w < kW; ++w) {
       t[0] = min(t[0], reach[w]);
       t[1] = max(t[1], reach[w]);
     }
@@ -341,7 +355,7 @@ __global__ __launch_bounds__(kThreads) void filter_parts_kernel(const FilterArgs
         if (v[j][i] >= edge) {
           const uint32_t to = atomicAdd(&listed, 1u);
           a.list[at * kList + to] =
-              (uint64_t)okey(v[j][i]) << 32 | (uint32_t) ~(uint32_t)(part * kIds + 4 * (j * kThreads + tid) + i);
+              (uint64_t)okey(v[j][i]) << 32 | (uint32_t) ~(uint32_t)(part * kIds + 4 * (j * kT + tid) + i);
         }
   }
   __syncthreads();
@@ -349,11 +363,17 @@ __global__ __launch_bounds__(kThreads) void filter_parts_kernel(const FilterArgs
     FilterPart f;
     f.max = m;
     f.id = first;
-    f.count = (int32_t)(wn[0] + wn[1] + wn[2] + wn[3]);
+    f.count = 0;
+    f.mass = 0.0;
+#pragma unroll
+    for (int w = 0; w < kW; ++w) {
+      f.count += (int32_t)wn[w];
+      f.mass += wsum[w];
+    }
+    if (!ranged) f.mass = 0.0;
     f.listed = ranged ? (int32_t)listed : -1;
     f.edge = edge;
     f.top = ranged ? (int32_t)top : 0;
-    f.mass = ranged ? (wsum[0] + wsum[1]) + (wsum[2] + wsum[3]) : 0.0;
     *out = f;
   }
 }
@@ -1082,7 +1102,7 @@ constexpr int kMergeMost = kMergeEntries * kThreads;       // entries of a row
 constexpr int kMergeSome = 512;                            // ids of one range, or of one part
 
 struct MergeShared {
-  double tab[kExpTab];
+  double tab[kTab];
   uint64_t red[kWaves][3];
   unsigned long long mass[kFilterRanges];
   uint32_t cnt[kFilterRanges];
@@ -1133,7 +1153,7 @@ __global__ __launch_bounds__(kThreads) void filter_merge_kernel(const FilterArgs
 #pragma unroll
   for (int i = 0; i < kMergeEntries; ++i) e[i] = i * kThreads + tid < slots ? lists[i * kThreads + tid] : 0ull;
   const sas_filter_params p = load_filter_params(a, row);
-  if (tid < kExpTab) l.tab[tid] = exp_tab_entry().x;
+  fill_tab(l.tab);
   if (tid < kFilterRanges) {
     l.mass[tid] = 0ull;
     l.cnt[tid] = 0u;
@@ -1177,11 +1197,13 @@ __global__ __launch_bounds__(kThreads) void filter_merge_kernel(const FilterArgs
     if (tid == 0) a.left[row] = 1u;
   };
   const uint32_t top = (uint32_t)(best >> 32);
-  const double m = (double)fkey(top);
   const Grid g = grid_of(p.temperature);
-  const float mrange = range_of((float)m, g);
+  const float mrange = range_of(fkey(top), g);
   if (!g.plain || !(fabsf(mrange) < kFar)) return leave();
-  auto mass_at = [&](double v) { return exp64(fmax((v - m) * g.per64, -8192.0), l.tab); };
+  // the mass of a value, and of a part's reference
+  const double m = (double)fkey(top) * g.per;
+  auto mass_at = [&](double v) { return exp256(fmax(fma(v, g.per, -m), kLeast), l.tab); };
+  auto mass_of_ref = [&](int t) { return exp256(fmax((double)t / (double)g.inv_width * g.per - m, kLeast), l.tab); };
   auto units = [&](double mass) { return (uint64_t)__builtin_rint(__builtin_amdgcn_ldexp(mass, a.shift)); };
   const bool by_k = p.top_k > 0 && (uint64_t)p.top_k < n, by_p = p.top_p < 1.0, by_min = p.min_p > 0.0;
   const bool cut = by_k || by_p || by_min;
@@ -1190,7 +1212,7 @@ __global__ __launch_bounds__(kThreads) void filter_merge_kernel(const FilterArgs
   uint64_t all = 0;
   for (int i = tid; i < a.parts; i += kThreads) {
     const FilterPart f = parts[i];
-    const uint64_t u = f.listed < 0 ? 0ull : units(f.mass * mass_at((double)f.top / (double)g.inv_width));
+    const uint64_t u = f.listed < 0 ? 0ull : units(f.mass * mass_of_ref(f.top));
     l.part[i] = cut ? 0ull : u;
     all += u;
   }
@@ -1391,17 +1413,17 @@ __global__ __launch_bounds__(kThreads) void filter_merge_kernel(const FilterArgs
 template <int kType, bool kSoft>
 hipError_t launch(const FilterArgs &a, hipStream_t stream) {
   const int blocks = a.rows * a.parts;
-  auto both = [&](auto parts_kernel, auto merge_kernel) {
-    parts_kernel<<<blocks, kThreads, 0, stream>>>(a);
+  auto both = [&](auto parts_kernel, int threads, auto merge_kernel) {
+    parts_kernel<<<blocks, threads, 0, stream>>>(a);
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     merge_kernel<<<a.rows, kThreads, 0, stream>>>(a);
     return hipGetLastError();
   };
   hipError_t e;
   switch (a.span) {
-    case 2048: e = both(filter_parts_kernel<kType, kSoft, 2>, filter_merge_kernel<kType, kSoft, 2>); break;
-    case 4096: e = both(filter_parts_kernel<kType, kSoft, 4>, filter_merge_kernel<kType, kSoft, 4>); break;
-    default: e = both(filter_parts_kernel<kType, kSoft, 8>, filter_merge_kernel<kType, kSoft, 8>); break;
+    case 2048: e = both(filter_parts_kernel<kType, kSoft, 256, 2>, 256, filter_merge_kernel<kType, kSoft, 2>); break;
+    case 4096: e = both(filter_parts_kernel<kType, kSoft, 256, 4>, 256, filter_merge_kernel<kType, kSoft, 4>); break;
+    default: e = both(filter_parts_kernel<kType, kSoft, 512, 4>, 512, filter_merge_kernel<kType, kSoft, 8>); break;
   }
   if (e != hipSuccess) return e;
   filter_rest_kernel<kType, kSoft><<<a.rows, kRowThreads, 0, stream>>>(a);

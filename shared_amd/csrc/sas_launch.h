@@ -267,12 +267,12 @@ constexpr int kFilterRanges = 128;
 constexpr int kFilterList = 128;
 struct FilterPart {
   float max;        // the largest value (-inf: no candidate)
-  uint32_t id;      // its first id
+  uint32_t id;      // its first id (greedy rows)
   int32_t count;    // candidates
   int32_t listed;   // ids in the list, -1: the part's values are out of the ranges' scope
   float edge;       // every candidate of at least this value is listed
   int32_t top;      // the range of max: floor(max / width)
-  double mass;      // of all candidates, relative to e^(top width / T)
+  double mass;      // of all candidates, relative to e^(top width / T), the range's lower edge
 };
 constexpr int kFilterShift = 50;
 
