@@ -216,6 +216,7 @@ __global__ __launch_bounds__(kT) void filter_parts_kernel(const FilterArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
   fill_tab(tab);
+  if (blockIdx.x == 0 && tid == 0) *a.nleft = 0u;
   const sas_filter_params p = load_filter_params(a, row);
   const int64_t row0 = (int64_t)row * a.logits_stride;
   float v[Q][4];
@@ -424,10 +425,7 @@ struct RowShared {
   unsigned long long part[kMaxFilterParts];
   unsigned long long ent[kEntries];   // listed ids: key << 32 | ~id
   unsigned long long entm[kEntries];  // and their masses
-  uint32_t some[kRowThreads];         // whether a span has ids of a range
-  uint32_t nent;
 };
-static_assert(SAS_MAX_VOCAB / kSpan <= kRowThreads, "a place for every span");
 
 __device__ __forceinline__ uint64_t shfl_xor64(uint64_t x, int s) { return (uint64_t)__shfl_xor((unsigned long long)x, s, 64); }
 
@@ -761,19 +759,20 @@ __device__ __forceinline__ void row_by_values(Row<kType, kSoft> &R, const Filter
   }
 }
 
-// The entry that ends a prefix of the first c entries of l.ent, which rank by
-// (key, id): the one of rank need (by_count), else the first at which the
+// The entry that ends a prefix of those of the first c entries of l.ent that
+// are `in`, ranked by (key, id): the one of rank need (by_count), else the first at which the
 // running mass reaches need.  Radix passes of 8 bits from the highest in which
 // the entries differ.  *mass, *count: of the entries up to it.
-template <typename R>
-__device__ __forceinline__ uint64_t end_of(const R &row, RowShared &l, int c, bool by_count, uint64_t need, uint64_t *mass, uint64_t *count) {
+template <typename R, typename In>
+__device__ __forceinline__ uint64_t end_of(const R &row, RowShared &l, int c, In in, bool by_count, uint64_t need, uint64_t *mass, uint64_t *count) {
   constexpr int kBase = 256;
   const int tid = threadIdx.x;
   uint64_t all = ~0ull, any = 0;
-  for (int i = tid; i < c; i += kRowThreads) {
-    all &= l.ent[i];
-    any |= l.ent[i];
-  }
+  for (int i = tid; i < c; i += kRowThreads)
+    if (in(l.ent[i])) {
+      all &= l.ent[i];
+      any |= l.ent[i];
+    }
 #pragma unroll
   for (int s = 32; s > 0; s >>= 1) {
     all &= shfl_xor64(all, s);
@@ -801,7 +800,7 @@ __device__ __forceinline__ uint64_t end_of(const R &row, RowShared &l, int c, bo
     __syncthreads();
     for (int i = tid; i < c; i += kRowThreads) {
       const uint64_t e = l.ent[i];
-      if ((e & high) != at) continue;
+      if ((e & high) != at || !in(e)) continue;
       const int d = 255 - (int)((e >> sh) & 0xFFu);
       atomicAdd(&l.mass[kBase + d], l.entm[i]);
       atomicAdd(&l.cnt[kBase + d], 1u);
@@ -816,7 +815,7 @@ __device__ __forceinline__ uint64_t end_of(const R &row, RowShared &l, int c, bo
       const uint64_t low = ~0ull << sh;
       __syncthreads();
       for (int i = tid; i < c; i += kRowThreads)
-        if ((l.ent[i] & low) == at) {
+        if ((l.ent[i] & low) == at && in(l.ent[i])) {
           l.sel[0] = l.ent[i];
           l.sel[1] = l.entm[i];
         }
@@ -834,7 +833,7 @@ __device__ __forceinline__ uint64_t end_of(const R &row, RowShared &l, int c, bo
 // The row by what its parts left; false where that does not tell (*top, *n:
 // its best key and its candidates).
 template <int kType, bool kSoft>
-__device__ __forceinline__ bool row_by_parts(Row<kType, kSoft> &R, const FilterArgs &a, RowShared &l, const sas_filter_params &p, int row,
+__device__ __forceinline__ bool row_by_parts(Row<kType, kSoft> &R, const FilterArgs &a, RowShared &l, const sas_filter_params &p, const FilterLeft &x, int row,
                                              uint32_t *top_key, uint64_t *candidates, const Result &done) {
   const int tid = threadIdx.x;
   const FilterPart *parts = a.part + (int64_t)row * a.parts;
@@ -874,7 +873,7 @@ __device__ __forceinline__ bool row_by_parts(Row<kType, kSoft> &R, const FilterA
   R.s = Scale{(double)m, 1.0 / p.temperature, 8.0 / p.temperature, a.shift};
   const Grid g = grid_of(p.temperature);
   const float mrange = range_of(m, g);
-  if (!g.plain || !(fabsf(mrange) < kFar)) return false;
+  if (!x.planned) return false;
   const bool by_k = p.top_k > 0 && (uint64_t)p.top_k < n, by_p = p.top_p < 1.0, by_min = p.min_p > 0.0;
   const bool cut = by_k || by_p || by_min;
   // a part's factor to the row's units
@@ -918,61 +917,17 @@ __device__ __forceinline__ bool row_by_parts(Row<kType, kSoft> &R, const FilterA
     }
     block_sum2(l, have, havem);
     const uint32_t least = by_min ? least_key(p.min_p, top, R.s, l.tab) : 0u;
-    // The ids of range `bin` into l.ent: from the row's values, in the spans that
-    // have any there (l.some).
-    bool fits = true;
-    int held = -1;
-    auto gather = [&](int bin) {
-      if (held == bin) return;
-      held = bin;
-      __syncthreads();
-      if (tid == 0) l.nent = 0u;
-      for (int i = tid; i < R.spans(); i += kRowThreads) l.some[i] = 0u;
-      __syncthreads();
-      for (int q = tid; q < a.parts; q += kRowThreads) {
-        const int i = bin - (int)mrange + parts[q].top;
-        if (parts[q].listed >= 0 && i >= 0 && i < kFilterRanges && a.range_count[((int64_t)row * a.parts + q) * kFilterRanges + i] > 0u)
-          l.some[(q << log_span) / kSpan] = 1u;
-      }
-      __syncthreads();
-      for (int id0 = 0; id0 < a.vocab; id0 += kSpan) {
-        if (!l.some[id0 / kSpan]) continue;
-        float v[kQuads][4];
-        span_values<kRowThreads, kType, kSoft, kQuads>(a, p, R.row0, R.mask, R.h, l.count, id0, v);
-        // a place for each of the wave's ids there, then the ids
-        uint32_t hits = 0;
-#pragma unroll
-        for (int j = 0; j < kQuads; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) hits |= (mrange - range_of(v[j][i], g) == (float)bin ? 1u : 0u) << (4 * j + i);
-        const uint32_t mine = __popc(hits);
-        uint32_t upto = mine;
-#pragma unroll
-        for (int s = 1; s < 64; s <<= 1) {
-          const uint32_t y = (uint32_t)__shfl_up((int)upto, s, 64);
-          if ((tid & 63) >= s) upto += y;
-        }
-        uint32_t base = 0;
-        if ((tid & 63) == 63 && upto) base = atomicAdd(&l.nent, upto);
-        uint32_t to = (uint32_t)__builtin_amdgcn_readlane((int)base, 63) + upto - mine;
-        if (hits) {
-#pragma unroll
-          for (int j = 0; j < kQuads; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if ((hits >> (4 * j + i)) & 1u) {
-                if (to < (uint32_t)kEntries)
-                  l.ent[to] = (uint64_t)okey(v[j][i]) << 32 | (uint32_t) ~(uint32_t)(id0 + 4 * (j * kRowThreads + tid) + i);
-                ++to;
-              }
-        }
-      }
-      __syncthreads();
-      fits = fits && l.nent <= (uint32_t)kEntries;
-      entries = (int)min(l.nent, (uint32_t)kEntries);
-      for (int i = tid; i < entries; i += kRowThreads) l.entm[i] = units_of(mass_of((uint32_t)(l.ent[i] >> 32), R.s, l.tab), R.s);
-      __syncthreads();
-    };
+    // the ids of the planned ranges
+    entries = (int)a.found[row];
+    if (entries > kEntries) return false;
+    for (int i = tid; i < entries; i += kRowThreads) {
+      const uint64_t e = a.ids[(int64_t)row * kEntries + i];
+      l.ent[i] = e;
+      l.entm[i] = units_of(mass_of((uint32_t)(e >> 32), R.s, l.tab), R.s);
+    }
+    __syncthreads();
+    auto planned = [&](int bin) { return bin < kFilterRanges && ((x.ranges[bin >> 5] >> (bin & 31)) & 1u) != 0u; };
+    auto bin_of_entry = [&](uint64_t e) { return (int)(mrange - range_of(fkey((uint32_t)(e >> 32)), g)); };
     // the ends of the prefixes of top-k and top-p
     bool known = true;
     auto prefix = [&](bool by_count, uint64_t need, uint64_t *mass) {
@@ -982,19 +937,17 @@ __device__ __forceinline__ bool row_by_parts(Row<kType, kSoft> &R, const FilterA
       }
       uint64_t m0, c0, m1, c1;
       const int bin = R.find(kFilterRanges, by_count, need, &m0, &c0);
-      gather(bin);
-      if (!fits) {
-        known = false;
-        return;
-      }
+      known = planned(bin);
+      if (!known) return;
       // (the range's mass was rounded as a whole, its ids' one by one)
       uint64_t sum = 0;
       zero = 0;
-      for (int i = tid; i < entries; i += kRowThreads) sum += l.entm[i];
+      for (int i = tid; i < entries; i += kRowThreads) sum += bin_of_entry(l.ent[i]) == bin ? l.entm[i] : 0ull;
       block_sum2(l, sum, zero);
       known = sum > 0;
       if (!known) return;
-      last = max(last, end_of(R, l, entries, by_count, by_count ? need - c0 : min(need - m0, sum), &m1, &c1));
+      last = max(last, end_of(R, l, entries, [&](uint64_t e) { return bin_of_entry(e) == bin; }, by_count,
+                              by_count ? need - c0 : min(need - m0, sum), &m1, &c1));
       *mass = m0 + m1;
     };
     uint64_t mass = all;
@@ -1011,9 +964,7 @@ __device__ __forceinline__ bool row_by_parts(Row<kType, kSoft> &R, const FilterA
     // what is kept of each part: of the ranges above the end's all, of its own
     // by its ids
     const int bin = (int)(mrange - range_of(fkey((uint32_t)(last >> 32)), g));
-    gather(bin);
-    if (!fits) return false;
-    __syncthreads();
+    if (!planned(bin)) return false;
     total = kept = 0;
     for (int i = tid; i < a.parts; i += kRowThreads) l.part[i] = 0ull;
     __syncthreads();
@@ -1030,7 +981,7 @@ __device__ __forceinline__ bool row_by_parts(Row<kType, kSoft> &R, const FilterA
     }
     __syncthreads();
     for (int i = tid; i < entries; i += kRowThreads)
-      if (l.ent[i] >= last) {
+      if (l.ent[i] >= last && bin_of_entry(l.ent[i]) == bin) {
         total += l.entm[i];
         ++kept;
         atomicAdd(&l.part[~(uint32_t)l.ent[i] >> log_span], l.entm[i]);
@@ -1078,10 +1029,10 @@ __device__ __forceinline__ bool row_by_parts(Row<kType, kSoft> &R, const FilterA
 template <int kType, bool kSoft>
 __global__ __launch_bounds__(kRowThreads) void filter_rest_kernel(const FilterArgs a) {
   __shared__ RowShared l;
-  const int row = blockIdx.x;
-  if (!a.left[row]) return;
+  if (blockIdx.x >= *a.nleft) return;
+  const FilterLeft x = a.left[blockIdx.x];
+  const int row = x.row;
   l.tab.fill(exp_tab_entry());
-  if (threadIdx.x == 0) l.nent = 0u;
   __syncthreads();
   const sas_filter_params p = load_filter_params(a, row);
   Row<kType, kSoft> R{a, l, p, (int64_t)row * a.logits_stride, a.mask ? a.mask + (int64_t)row * a.mask_stride : nullptr,
@@ -1089,7 +1040,7 @@ __global__ __launch_bounds__(kRowThreads) void filter_rest_kernel(const FilterAr
   const Result done{a, row};
   uint32_t top = 0;
   uint64_t n = 0;
-  if (!row_by_parts<kType, kSoft>(R, a, l, p, row, &top, &n, done)) row_by_values<kType, kSoft>(R, a, l, p, row, top, n, done);
+  if (!row_by_parts<kType, kSoft>(R, a, l, p, x, row, &top, &n, done)) row_by_values<kType, kSoft>(R, a, l, p, row, top, n, done);
 }
 
 // ----------------------------------------------------------------- merge --
@@ -1188,13 +1139,13 @@ __global__ __launch_bounds__(kThreads) void filter_merge_kernel(const FilterArgs
     edge = max(edge, (uint32_t)l.red[w][2]);
   }
   const Result done{a, row};
-  if (tid == 0) a.left[row] = 0u;
   if (best == 0 || greedy_row(p)) {
     if (tid == 0) done(best ? ~(uint32_t)best : SAS_NO_TOKEN, best ? 1.0 : 0.0, best ? 1 : 0);
     return;
   }
+  // leaves the row to the rest kernel, by its values alone
   auto leave = [&]() {
-    if (tid == 0) a.left[row] = 1u;
+    if (tid == 0) a.left[atomicAdd(a.nleft, 1u)] = FilterLeft{row, 0u, {0u, 0u, 0u, 0u}};
   };
   const uint32_t top = (uint32_t)(best >> 32);
   const Grid g = grid_of(p.temperature);
@@ -1207,7 +1158,6 @@ __global__ __launch_bounds__(kThreads) void filter_merge_kernel(const FilterArgs
   auto units = [&](double mass) { return (uint64_t)__builtin_rint(__builtin_amdgcn_ldexp(mass, a.shift)); };
   const bool by_k = p.top_k > 0 && (uint64_t)p.top_k < n, by_p = p.top_p < 1.0, by_min = p.min_p > 0.0;
   const bool cut = by_k || by_p || by_min;
-  if (cut && slots > kMergeMost) return leave();
   // the parts' masses in the row's units
   uint64_t all = 0;
   for (int i = tid; i < a.parts; i += kThreads) {
@@ -1218,7 +1168,8 @@ __global__ __launch_bounds__(kThreads) void filter_merge_kernel(const FilterArgs
   }
   // the entries that count: all there are from `edge` on
   uint64_t u[kMergeEntries];
-  if (cut) {
+  bool known = slots <= kMergeMost;
+  if (cut && known) {
 #pragma unroll
     for (int i = 0; i < kMergeEntries; ++i) {
       const int at = i * kThreads + tid;
@@ -1246,7 +1197,6 @@ __global__ __launch_bounds__(kThreads) void filter_merge_kernel(const FilterArgs
     const uint64_t m0 = l.mass[2 * lane], m1 = l.mass[2 * lane + 1], c0 = l.cnt[2 * lane], c1 = l.cnt[2 * lane + 1];
     const uint64_t mrun = wave_scan64(m0 + m1), crun = wave_scan64(c0 + c1);
     const uint64_t havem = lane64(mrun, 63), have = lane64(crun, 63);
-    bool known = true;
     uint64_t mass = all;
     // the entry that ends a prefix: its range, then its place among the range's
     auto prefix = [&](bool by_count, uint64_t need) {
@@ -1295,15 +1245,16 @@ __global__ __launch_bounds__(kThreads) void filter_merge_kernel(const FilterArgs
       last = more(last, l.end[0]);
       mass = mb + l.end[1];
     };
-    if (by_k) prefix(true, (uint64_t)p.top_k);
+    if (known && by_k) prefix(true, (uint64_t)p.top_k);
     if (known && by_p) {
       const uint64_t need = (uint64_t)ceil(fmax(p.top_p, 0.0) * (double)mass);
       prefix(false, min(max(need, (uint64_t)1), mass));
     }
-    if (known && by_min) {
+    uint32_t hi = top;
+    if (by_min) {
       // the smallest key whose mass reaches min_p, 64 at a time
       const double least = fmin(p.min_p, 1.0);
-      uint32_t lo = kNegInf, hi = top;
+      uint32_t lo = kNegInf;
       while (hi - lo > 1) {
         const uint32_t step = max((hi - lo) / 65u, 1u), key = lo + step * (uint32_t)(lane + 1);
         const uint64_t reach = __ballot(key >= hi || key < lo || mass_at((double)fkey(key)) >= least);
@@ -1312,12 +1263,73 @@ __global__ __launch_bounds__(kThreads) void filter_merge_kernel(const FilterArgs
         if (k < 64 && to < hi && to > lo) hi = to;
         lo = lo + step * (uint32_t)k;
       }
-      if ((uint64_t)hi << 32 > last) {
+      if (known && (uint64_t)hi << 32 > last) {
         last = (uint64_t)hi << 32;
         known = hi >= edge;
       }
     }
-    if (!known) return leave();
+    if (!known) {
+      // the ranges that the ends lie in, from the ranges of all parts
+      __syncthreads();
+      if (tid < kFilterRanges) {
+        l.mass[tid] = 0ull;
+        l.cnt[tid] = 0u;
+      }
+      __syncthreads();
+      for (int i = tid; i < a.parts * kFilterRanges; i += kThreads) {
+        const FilterPart f = parts[i / kFilterRanges];
+        const int64_t at = (int64_t)row * a.parts * kFilterRanges + i;
+        const uint32_t c = a.range_count[at];
+        const uint64_t w = a.range_mass[at];
+        const int d = (int)mrange - f.top + i % kFilterRanges;
+        if (f.listed < 0 || !(f.max > -__builtin_inff()) || c == 0u || d >= kFilterRanges) continue;
+        atomicAdd(&l.cnt[d], c);
+        atomicAdd(&l.mass[d], (unsigned long long)__builtin_rint(__builtin_amdgcn_ldexp((double)w * mass_of_ref(f.top), a.shift - kFilterShift)));
+      }
+      __syncthreads();
+      if (wave > 0) return;
+      const uint64_t rm0 = l.mass[2 * lane], rm1 = l.mass[2 * lane + 1], rc0 = l.cnt[2 * lane], rc1 = l.cnt[2 * lane + 1];
+      const uint64_t mr = wave_scan64(rm0 + rm1), cr = wave_scan64(rc0 + rc1);
+      // the range in which a running sum reaches need (kFilterRanges: none)
+      auto range_at = [&](uint64_t run, uint64_t second, uint64_t need) {
+        const uint64_t hit = __ballot(run >= need);
+        if (!hit) return (int)kFilterRanges;
+        const int at = __builtin_ctzll(hit);
+        return 2 * at + (lane64(run, at) - lane64(second, at) < need ? 1 : 0);
+      };
+      FilterLeft x{row, 0u, {0u, 0u, 0u, 0u}};
+      bool sure = true;
+      uint64_t ids = 0, low = all, high = all;
+      auto plan = [&](int bin) {
+        if (bin >= kFilterRanges) {
+          sure = false;
+          return;
+        }
+        if (!((x.ranges[bin >> 5] >> (bin & 31)) & 1u)) ids += l.cnt[bin];
+        x.ranges[bin >> 5] |= 1u << (bin & 31);
+      };
+      if (by_k) {
+        const int bin = range_at(cr, rc1, (uint64_t)p.top_k);
+        plan(bin);
+        if (sure) {
+          // top-p's share is of a mass between the ranges' above the end and with it
+          high = lane64(mr, bin >> 1) - (bin & 1 ? 0ull : lane64(rm1, bin >> 1));
+          low = high - l.mass[bin];
+        }
+      }
+      if (by_p && sure) {
+        auto share = [&](uint64_t of) { return max((uint64_t)ceil(fmax(p.top_p, 0.0) * (double)of), (uint64_t)1); };
+        const int from = range_at(mr, rm1, share(low)), to = range_at(mr, rm1, min(share(high), lane64(mr, 63)));
+        for (int bin = from; bin <= to && sure; ++bin) plan(bin);
+      }
+      if (by_min) plan((int)fminf(mrange - range_of(fkey(hi), g), (float)kFilterRanges));
+      if (sure && ids <= (uint64_t)kEntries) x.planned = 1u;
+      if (lane == 0) {
+        a.found[row] = 0u;
+        a.left[atomicAdd(a.nleft, 1u)] = x;
+      }
+      return;
+    }
     total = kept = 0;
 #pragma unroll
     for (int i = 0; i < kMergeEntries; ++i)
@@ -1410,20 +1422,92 @@ __global__ __launch_bounds__(kThreads) void filter_merge_kernel(const FilterArgs
   }
 }
 
+// The ids of the planned ranges of the rows left: a part at a time, on the
+// whole chip (one block a row read 16,384 ids in 5 us).
+template <int kType, bool kSoft, int Q>
+__global__ __launch_bounds__(kThreads) void filter_gather_kernel(const FilterArgs a) {
+  constexpr int kIds = 4 * Q * kThreads;
+  __shared__ uint32_t count[kIds / 2];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int items = (int)*a.nleft * a.parts;
+  for (int item = blockIdx.x; item < items; item += gridDim.x) {
+    const FilterLeft x = a.left[item / a.parts];
+    const int part = item % a.parts;
+    if (!x.planned) continue;
+    const FilterPart *parts = a.part + (int64_t)x.row * a.parts;
+    // the row's first range, as the merge has it
+    float m = -__builtin_inff();
+    for (int i = lane; i < a.parts; i += 64) m = fmaxf(m, parts[i].max);
+    m = wave_max(m);
+    const sas_filter_params p = load_filter_params(a, x.row);
+    const Grid g = grid_of(p.temperature);
+    const float mrange = range_of(m, g);
+    const FilterPart f = parts[part];
+    if (f.listed < 0 || !(f.max > -__builtin_inff())) continue;
+    bool any = false;
+    for (int d = lane; d < kFilterRanges; d += 64) {
+      const int i = d - (int)mrange + f.top;
+      any = any || ((x.ranges[d >> 5] >> (d & 31)) & 1u && i >= 0 && i < kFilterRanges &&
+                    a.range_count[((int64_t)x.row * a.parts + part) * kFilterRanges + i] > 0u);
+    }
+    if (!__ballot(any)) continue;  // (the same in every wave)
+    float v[Q][4];
+    __syncthreads();
+    span_values<kThreads, kType, kSoft, Q>(a, p, (int64_t)x.row * a.logits_stride,
+                                           a.mask ? a.mask + (int64_t)x.row * a.mask_stride : nullptr, history_of(a, x.row), count,
+                                           part * kIds, v);
+    uint32_t hits = 0;
+#pragma unroll
+    for (int j = 0; j < Q; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float d = mrange - range_of(v[j][i], g);
+        const int bin = d < (float)kFilterRanges ? (int)d : 0;
+        const uint32_t word = bin < 64 ? (bin < 32 ? x.ranges[0] : x.ranges[1]) : (bin < 96 ? x.ranges[2] : x.ranges[3]);
+        hits |= (d < (float)kFilterRanges ? (word >> (bin & 31)) & 1u : 0u) << (4 * j + i);
+      }
+    const uint32_t mine = __popc(hits);
+    uint32_t upto = mine;
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) {
+      const uint32_t y = (uint32_t)__shfl_up((int)upto, s, 64);
+      if (lane >= s) upto += y;
+    }
+    uint32_t base = 0;
+    if (lane == 63 && upto) base = atomicAdd(&a.found[x.row], upto);
+    uint32_t to = (uint32_t)__builtin_amdgcn_readlane((int)base, 63) + upto - mine;
+#pragma unroll
+    for (int j = 0; j < Q; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if ((hits >> (4 * j + i)) & 1u) {
+          if (to < (uint32_t)kEntries)
+            a.ids[(int64_t)x.row * kEntries + to] =
+                (uint64_t)okey(v[j][i]) << 32 | (uint32_t) ~(uint32_t)(part * kIds + 4 * (j * kThreads + tid) + i);
+          ++to;
+        }
+  }
+}
+
 template <int kType, bool kSoft>
 hipError_t launch(const FilterArgs &a, hipStream_t stream) {
   const int blocks = a.rows * a.parts;
-  auto both = [&](auto parts_kernel, int threads, auto merge_kernel) {
+  auto three = [&](auto parts_kernel, int threads, auto merge_kernel, auto gather_kernel) {
     parts_kernel<<<blocks, threads, 0, stream>>>(a);
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     merge_kernel<<<a.rows, kThreads, 0, stream>>>(a);
+    if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    gather_kernel<<<blocks < 1024 ? blocks : 1024, kThreads, 0, stream>>>(a);
     return hipGetLastError();
   };
   hipError_t e;
   switch (a.span) {
-    case 2048: e = both(filter_parts_kernel<kType, kSoft, 256, 2>, 256, filter_merge_kernel<kType, kSoft, 2>); break;
-    case 4096: e = both(filter_parts_kernel<kType, kSoft, 256, 4>, 256, filter_merge_kernel<kType, kSoft, 4>); break;
-    default: e = both(filter_parts_kernel<kType, kSoft, 512, 4>, 512, filter_merge_kernel<kType, kSoft, 8>); break;
+    case 2048: e = three(filter_parts_kernel<kType, kSoft, 256, 2>, 256, filter_merge_kernel<kType, kSoft, 2>,
+                               filter_gather_kernel<kType, kSoft, 2>); break;
+    case 4096: e = three(filter_parts_kernel<kType, kSoft, 256, 4>, 256, filter_merge_kernel<kType, kSoft, 4>,
+                               filter_gather_kernel<kType, kSoft, 4>); break;
+    default: e = three(filter_parts_kernel<kType, kSoft, 512, 4>, 512, filter_merge_kernel<kType, kSoft, 8>,
+                               filter_gather_kernel<kType, kSoft, 8>); break;
   }
   if (e != hipSuccess) return e;
   filter_rest_kernel<kType, kSoft><<<a.rows, kRowThreads, 0, stream>>>(a);
@@ -1445,7 +1529,7 @@ int filter_span(int rows, int vocab, int min_blocks) {
 // The parts, their lists, the masses and counts of their ranges.
 size_t filter_scratch_bytes(int rows, int parts) {
   const size_t n = (size_t)rows * parts;
-  return n * (sizeof(FilterPart) + kFilterList * 8 + kFilterRanges * 12) + (size_t)rows * 4;
+  return n * (sizeof(FilterPart) + kFilterList * 8 + kFilterRanges * 12) + (size_t)rows * (kEntries * 8 + sizeof(FilterLeft) + 4) + 8;
 }
 void filter_scratch(void *base, FilterArgs *a) {
   const size_t n = (size_t)a->rows * a->parts;
@@ -1455,7 +1539,10 @@ void filter_scratch(void *base, FilterArgs *a) {
   a->list = reinterpret_cast<uint64_t *>(at += n * sizeof(FilterPart));
   a->range_mass = reinterpret_cast<uint64_t *>(at += n * kFilterList * 8);
   a->range_count = reinterpret_cast<uint32_t *>(at += n * kFilterRanges * 8);
-  a->left = reinterpret_cast<uint32_t *>(at + n * kFilterRanges * 4);
+  a->ids = reinterpret_cast<uint64_t *>(at += n * kFilterRanges * 4);
+  a->left = reinterpret_cast<FilterLeft *>(at += (size_t)a->rows * kEntries * 8);
+  a->found = reinterpret_cast<uint32_t *>(at += (size_t)a->rows * sizeof(FilterLeft));
+  a->nleft = reinterpret_cast<uint32_t *>(at + (size_t)a->rows * 4);
 }
 
 hipError_t launch_filter(const FilterArgs &a, hipStream_t stream) {

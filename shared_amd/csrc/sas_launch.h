@@ -254,7 +254,12 @@ struct FilterArgs {
   uint64_t *range_mass;  // [rows][parts][kFilterRanges]
   uint32_t *range_count;
   uint64_t *list;        // [rows][parts][span / 64]
-  uint32_t *left;        // [rows]: 1 where the merge leaves the row to the rest kernel
+  // The rows that the merge leaves to the rest kernel, their number, and per row
+  // how many ids of its planned ranges were found, and which.
+  struct FilterLeft *left;
+  uint32_t *nleft;
+  uint32_t *found;
+  uint64_t *ids;         // [rows][4,096]
   int32_t type;   // SAS_TYPE_*
   int32_t vocab;
   int32_t rows;
@@ -273,6 +278,12 @@ struct FilterPart {
   float edge;       // every candidate of at least this value is listed
   int32_t top;      // the range of max: floor(max / width)
   double mass;      // of all candidates, relative to e^(top width / T), the range's lower edge
+};
+// A row left: by the ids of these of its ranges (planned), or by its values.
+struct FilterLeft {
+  int32_t row;
+  uint32_t planned;
+  uint32_t ranges[4];
 };
 constexpr int kFilterShift = 50;
 
