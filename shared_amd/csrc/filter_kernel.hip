@@ -899,16 +899,35 @@ __device__ __forceinline__ bool row_by_parts(Row<kType, kSoft> &R, const FilterA
       l.cnt[i] = 0u;
     }
     __syncthreads();
-    for (int i = tid; i < a.parts * kFilterRanges; i += kRowThreads) {
-      const FilterPart f = parts[i / kFilterRanges];
-      const int64_t at = (int64_t)row * a.parts * kFilterRanges + i;
-      const uint32_t c = a.range_count[at];
-      const uint64_t w = a.range_mass[at];
-      const int d = (int)mrange - f.top + i % kFilterRanges;
-      if (f.listed < 0 || !(f.max > -__builtin_inff()) || c == 0u || d >= kFilterRanges) continue;
+    // fn(part, range, count, mass in the row's units) of every range that has ids, four
+    // ranges' loads in flight together
+    auto each_range = [&](auto fn) {
+      for (int i0 = tid; i0 < a.parts * kFilterRanges; i0 += 4 * kRowThreads) {
+        uint32_t c[4];
+        uint64_t w[4];
+        FilterPart f[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int i = min(i0 + k * kRowThreads, a.parts * kFilterRanges - 1);
+          const int64_t at = (int64_t)row * a.parts * kFilterRanges + i;
+          c[k] = a.range_count[at];
+          w[k] = a.range_mass[at];
+          f[k] = parts[i / kFilterRanges];
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int i = i0 + k * kRowThreads;
+          const int d = (int)mrange - f[k].top + i % kFilterRanges;
+          if (i >= a.parts * kFilterRanges || f[k].listed < 0 || !(f[k].max > -__builtin_inff()) || c[k] == 0u || d >= kFilterRanges) continue;
+          fn(i / kFilterRanges, d, c[k],
+             (uint64_t)__builtin_rint(__builtin_amdgcn_ldexp((double)w[k] * scale_of(f[k]), a.shift - kFilterShift)));
+        }
+      }
+    };
+    each_range([&](int, int d, uint32_t c, uint64_t u) {
       atomicAdd(&l.cnt[d], c);
-      atomicAdd(&l.mass[d], (unsigned long long)__builtin_rint(__builtin_amdgcn_ldexp((double)w * scale_of(f), a.shift - kFilterShift)));
-    }
+      atomicAdd(&l.mass[d], (unsigned long long)u);
+    });
     __syncthreads();
     uint64_t have = 0, havem = 0;
     for (int i = tid; i < kFilterRanges; i += kRowThreads) {
@@ -968,17 +987,12 @@ __device__ __forceinline__ bool row_by_parts(Row<kType, kSoft> &R, const FilterA
     total = kept = 0;
     for (int i = tid; i < a.parts; i += kRowThreads) l.part[i] = 0ull;
     __syncthreads();
-    for (int i = tid; i < a.parts * kFilterRanges; i += kRowThreads) {
-      const FilterPart f = parts[i / kFilterRanges];
-      if (f.listed < 0 || !(f.max > -__builtin_inff()) || (int)mrange - f.top + i % kFilterRanges >= bin) continue;
-      const int64_t at = (int64_t)row * a.parts * kFilterRanges + i;
-      const uint32_t c = a.range_count[at];
-      if (c == 0u) continue;
-      const uint64_t u = (uint64_t)__builtin_rint(__builtin_amdgcn_ldexp((double)a.range_mass[at] * scale_of(f), a.shift - kFilterShift));
+    each_range([&](int part, int d, uint32_t c, uint64_t u) {
+      if (d >= bin) return;
       total += u;
       kept += c;
-      atomicAdd(&l.part[i / kFilterRanges], (unsigned long long)u);
-    }
+      atomicAdd(&l.part[part], (unsigned long long)u);
+    });
     __syncthreads();
     for (int i = tid; i < entries; i += kRowThreads)
       if (l.ent[i] >= last && bin_of_entry(l.ent[i]) == bin) {
@@ -994,12 +1008,13 @@ __device__ __forceinline__ bool row_by_parts(Row<kType, kSoft> &R, const FilterA
   const int q = part_of(l, a.parts, goal, &before);
   const double whole = __builtin_amdgcn_ldexp((double)total, -a.shift);
   // the part's values again: its kept ids' masses, and the goal as a share of them
-  float v[kQuads][4];
+  constexpr int kDraw = 8192 / (4 * kRowThreads);  // quads of the longest part
+  float v[kDraw][4];
   const int id0 = q * a.span;
-  span_values<kRowThreads, kType, kSoft, kQuads>(a, p, R.row0, R.mask, R.h, l.count, id0, v);
-  uint64_t u[kQuads][4], run[kQuads], sums = 0;
+  span_values<kRowThreads, kType, kSoft, kDraw>(a, p, R.row0, R.mask, R.h, l.count, id0, v);
+  uint64_t u[kDraw][4], run[kDraw], sums = 0;
 #pragma unroll
-  for (int j = 0; j < kQuads; ++j) {
+  for (int j = 0; j < kDraw; ++j) {
     uint64_t sum = 0, of_all;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -1015,7 +1030,7 @@ __device__ __forceinline__ bool row_by_parts(Row<kType, kSoft> &R, const FilterA
   uint64_t target = (uint64_t)((double)(goal - before) * ((double)sums / (double)l.part[q]));
   target = min(target, sums - 1);
 #pragma unroll
-  for (int j = 0; j < kQuads; ++j)
+  for (int j = 0; j < kDraw; ++j)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if (run[j] <= target && target < run[j] + u[j][i])
