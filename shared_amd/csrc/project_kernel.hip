@@ -92,9 +92,9 @@ __device__ __forceinline__ void each_adapter(int mine, F f) {
   }
 }
 
-// Block (subtile, slot): the slot-th adapter of the subtile's rows.  Its
-// waves share out up to four rank tiles and, within each, the runs of 32 of
-// dim; the parts meet in LDS in a fixed order.  Of the blocks past the
+// Block (subtile, slot, tile): 16 ranks of the slot-th adapter of the
+// subtile's rows.  Its waves share out the runs of 32 of dim; their parts meet
+// in LDS in a fixed order.  Of the blocks past the
 // subtiles the first puts the rows in order, the others write the pieces of
 // f32 hidden states.
 constexpr int kInnerWaves = 16;
@@ -138,6 +138,7 @@ template <bool kF32>
 __global__ __launch_bounds__(kInnerThreads) void proj_inner_kernel(const ProjArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int subs = (a.rows + kSub - 1) / kSub;
+  if ((int)blockIdx.x >= subs && blockIdx.z > 0) return;
   if ((int)blockIdx.x == subs) {
     if (a.perm && blockIdx.y == 0) order_rows(a);
     return;
@@ -170,56 +171,51 @@ __global__ __launch_bounds__(kInnerThreads) void proj_inner_kernel(const ProjArg
   const float scale = a.scales ? a.scales[cur] : 1.0f;
   const int xrow = min(row, a.rows - 1);
   const int kc = 8 * (lane >> 4);
-  const int tiles = (a.rank + kSub - 1) / kSub, group = min(tiles, 4), ks = kInnerWaves / group;
-  const int mytile = wave % group, myks = wave / group;
-  const int steps = (a.dim + 31) / 32;
-  const int g0 = myks < ks ? steps * myks / ks : 0, g1 = myks < ks ? steps * (myks + 1) / ks : 0;
+  const int t = kSub * (int)blockIdx.z;
+  const int steps = (a.dim + 31) / 32, g0 = steps * wave / kInnerWaves, g1 = steps * (wave + 1) / kInnerWaves;
   const uint16_t *A = static_cast<const uint16_t *>(a.a) + (int64_t)cur * a.a_adapter_stride;
   const u32x4 none = {0u, 0u, 0u, 0u};
-  for (int t0 = 0; t0 < tiles; t0 += group) {
-    const int t = kSub * (t0 + mytile);
-    const uint16_t *ar = A + (int64_t)min(t + (lane & 15), a.rank - 1) * a.a_stride + kc;
-    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int g = g0; g < g1; g += kInnerDeep) {
-      u32x4 w[kInnerDeep], x[kInnerDeep][kF32 ? 3 : 1];
+  const uint16_t *ar = A + (int64_t)min(t + (lane & 15), a.rank - 1) * a.a_stride + kc;
+  f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int g = g0; g < g1; g += kInnerDeep) {
+    u32x4 w[kInnerDeep], x[kInnerDeep][kF32 ? 3 : 1];
 #pragma unroll
-      for (int d = 0; d < kInnerDeep; ++d) {
-        const int k = 32 * (g + d);
-        const bool in = g + d < g1 && k + kc < a.dim;
-        w[d] = in ? *reinterpret_cast<const u32x4 *>(ar + k) : none;
-        if constexpr (kF32) {
-          if (in) split8(static_cast<const float *>(a.x) + (int64_t)xrow * a.x_stride + k + kc, x[d]);
-          else x[d][0] = x[d][1] = x[d][2] = none;
-        } else {
-          x[d][0] = in ? *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(a.x) + (int64_t)xrow * a.x_stride + k + kc) : none;
-        }
-      }
-#pragma unroll
-      for (int d = 0; d < kInnerDeep; ++d)
-#pragma unroll
-        for (int i = 0; i < (kF32 ? 3 : 1); ++i) acc = mfma(w[d], x[d][i], acc);
-    }
-    part[wave][lane] = acc;
-    __syncthreads();
-    if (wave < group) {
-      // lane: row lane & 15, ranks t + 4 (lane / 16) ..
-      f32x4 h = part[wave][lane];
-      for (int i = 1; i < ks; ++i) h = h + part[wave + i * group][lane];
-      const int r0 = t + 4 * (lane >> 4);
-      if (mine == cur && r0 < a.rank) {
-        u16x4 p[3];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint16_t q[3];
-          pieces_of(r0 + i < used ? h[i] * scale : 0.0f, q);
-#pragma unroll
-          for (int k = 0; k < 3; ++k) p[k][i] = q[k];
-        }
-#pragma unroll
-        for (int k = 0; k < 3; ++k) *reinterpret_cast<u16x4 *>(a.hp + ((int64_t)row * 3 + k) * a.rank + r0) = p[k];
+    for (int d = 0; d < kInnerDeep; ++d) {
+      const int k = 32 * (g + d);
+      const bool in = g + d < g1 && k + kc < a.dim;
+      w[d] = in ? *reinterpret_cast<const u32x4 *>(ar + k) : none;
+      if constexpr (kF32) {
+        if (in) split8(static_cast<const float *>(a.x) + (int64_t)xrow * a.x_stride + k + kc, x[d]);
+        else x[d][0] = x[d][1] = x[d][2] = none;
+      } else {
+        x[d][0] = in ? *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(a.x) + (int64_t)xrow * a.x_stride + k + kc) : none;
       }
     }
-    __syncthreads();
+#pragma unroll
+    for (int d = 0; d < kInnerDeep; ++d)
+#pragma unroll
+      for (int i = 0; i < (kF32 ? 3 : 1); ++i) acc = mfma(w[d], x[d][i], acc);
+  }
+  part[wave][lane] = acc;
+  __syncthreads();
+  if (wave == 0) {
+    // lane: row lane & 15, ranks t + 4 (lane / 16) ..
+    f32x4 h = part[0][lane];
+#pragma unroll
+    for (int i = 1; i < kInnerWaves; ++i) h = h + part[i][lane];
+    const int r0 = t + 4 * (lane >> 4);
+    if (mine == cur && r0 < a.rank) {
+      u16x4 p[3];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint16_t q[3];
+        pieces_of(r0 + i < used ? h[i] * scale : 0.0f, q);
+#pragma unroll
+        for (int k = 0; k < 3; ++k) p[k][i] = q[k];
+      }
+#pragma unroll
+      for (int k = 0; k < 3; ++k) *reinterpret_cast<u16x4 *>(a.hp + ((int64_t)row * 3 + k) * a.rank + r0) = p[k];
+    }
   }
 }
 
@@ -299,7 +295,7 @@ struct Tile {
   int adapter[16 * MT];   // -1: none, or past the last row
   int pairs;
   int pair_adapter[16 * MT];
-  uint32_t pair_users[16 * MT];  // subtile << 16 | rows as bits
+  uint32_t pair_users[16 * MT];  // rank in use << 20 | subtile << 16 | rows as bits
 };
 
 // Fills l (the block's threads; a barrier before it is read).
@@ -320,9 +316,10 @@ __device__ __forceinline__ void tile_pairs(const ProjArgs &a, Tile<MT> &l) {
     const int mine = l.adapter[16 * m + (lane & 15)];
     each_adapter(mine, [&](int cur) {
       const uint32_t users = (uint32_t)__ballot(mine == cur) & 0xFFFFu;
+      const int used = rank_of(a, cur);
       if (lane == 0) {
         l.pair_adapter[n] = cur;
-        l.pair_users[n] = (uint32_t)m << 16 | users;
+        l.pair_users[n] = (uint32_t)used << 20 | (uint32_t)m << 16 | users;
       }
       ++n;
     });
@@ -331,7 +328,7 @@ __device__ __forceinline__ void tile_pairs(const ProjArgs &a, Tile<MT> &l) {
 }
 
 // Adds the tile's adapters' terms, B times the pieces of h, 32 ranks an item,
-// an item's loads ahead of the products of the one before.  An item's sums are its own and
+// an item's loads two ahead of its products.  An item's sums are its own and
 // only the adapter's rows add them.  mine(adapter): whether this wave takes it.
 template <int MT, int NT, typename F>
 __device__ __forceinline__ void add_adapters(const ProjArgs &a, const Tile<MT> &l, int n0, F takes, f32x4 (&acc)[MT][NT]) {
@@ -355,7 +352,7 @@ __device__ __forceinline__ void add_adapters(const ProjArgs &a, const Tile<MT> &
       if (at < pairs) {
         cur = __builtin_amdgcn_readfirstlane(l.pair_adapter[at]);
         mu = __builtin_amdgcn_readfirstlane(l.pair_users[at]);
-        used = rank_of(a, cur);
+        used = (int)(mu >> 20);
       }
     }
     it.m = -1;
@@ -363,7 +360,7 @@ __device__ __forceinline__ void add_adapters(const ProjArgs &a, const Tile<MT> &
       rb = blocks - 1;  // (stays past the end)
       return;
     }
-    it.m = (int)(mu >> 16);
+    it.m = (int)(mu >> 16) & 15;
     it.users = mu & 0xFFFFu;
     const int r0 = 32 * rb, n = a.rank - r0;  // ranks from r0 on
     // The four octets of an operand: of up to 8 ranks the three pieces (one
@@ -403,15 +400,17 @@ __device__ __forceinline__ void add_adapters(const ProjArgs &a, const Tile<MT> &
   };
   // the pairs come subtile by subtile: the sums of each have a loop of their
   // own (selecting them by a variable doubles the kernel's registers)
-  Item x;
+  Item x, y;
   next(x);
+  next(y);
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
     while (x.m == m) {
-      Item y;
-      next(y);
+      Item z;
+      next(z);
       add(x, acc[m]);
       x = y;
+      y = z;
     }
   }
 }
@@ -779,8 +778,9 @@ ProjScratch proj_scratch(int rows, int dim, int rank, bool x_f32) {
 hipError_t launch_project(const ProjArgs &a, hipStream_t stream) {
   const int subs = (a.rows + kSub - 1) / kSub;
   if (a.adapters > 0 || a.xp) {
-    const int split = a.xp ? (int)(((int64_t)a.rows * (a.dim / 8) + kSub * kInnerThreads - 1) / (kSub * kInnerThreads)) : 0;
-    const dim3 grid(subs + 1 + (split > 1024 ? 1024 : split), kSub);
+    const int slots = a.adapters < 1 ? 1 : a.adapters < kSub ? a.adapters : kSub;
+    const int64_t split = a.xp ? ((int64_t)a.rows * (a.dim / 8) + slots * kInnerThreads - 1) / (slots * kInnerThreads) : 0;
+    const dim3 grid(subs + 1 + (unsigned)(split > 1024 ? 1024 : split), slots, a.rank > 0 ? (a.rank + kSub - 1) / kSub : 1);
     if (a.x_f32) proj_inner_kernel<true><<<grid, kInnerThreads, 0, stream>>>(a);
     else proj_inner_kernel<false><<<grid, kInnerThreads, 0, stream>>>(a);
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
