@@ -372,11 +372,13 @@ __device__ __forceinline__ void add_adapters(const ProjArgs &a, const Tile<MT> &
 #pragma unroll
     for (int t = 0; t < NT; ++t)
       it.b[t] = b_ranks(b + (int64_t)min(n0 + 16 * t + (lane & 15), a.out_dim - 1) * a.b_stride, r0 + 8 * oct, used);
+    // (rows of other adapters are left out: an address a lane is what a load costs)
     const uint16_t *h = a.hp + (int64_t)l.row[16 * it.m + (lane & 15)] * 3 * a.rank + r0 + 8 * oct;
+    const bool user = (it.users >> (lane & 15)) & 1u;
 #pragma unroll
     for (int j = 0; j < 3; ++j) {
       const int piece = n <= 8 ? q : n <= 16 ? 2 * j + (q >> 1) : j;
-      it.h[j] = j < it.products && piece < 3 && r0 + 8 * oct < a.rank ? *reinterpret_cast<const u32x4 *>(h + piece * a.rank) : none;
+      it.h[j] = user && j < it.products && piece < 3 && r0 + 8 * oct < used ? *reinterpret_cast<const u32x4 *>(h + piece * a.rank) : none;
     }
   };
   auto add = [&](const Item &it, f32x4 (&sum)[NT]) __attribute__((always_inline)) {
