@@ -46,6 +46,8 @@ const char *check_projection(const sas_projection *p) {
   if (p->softcap < 0.0f || !std::isfinite(p->softcap)) return "softcap must be finite and >= 0";
   if (p->adapters > 0 && (p->rank < 8 || p->rank > SAS_MAX_RANK || p->rank % 8 != 0))
     return "rank must be a multiple of 8 in [8, SAS_MAX_RANK]";
+  // (a block an output tile of 16 x 16 at most)
+  if ((((int64_t)p->rows + 15) / 16) * (((int64_t)p->out_dim + 15) / 16) > INT32_MAX) return "rows * out_dim is too large";
   if (p->rows == 0) return nullptr;
   if (!p->x || !p->out) return "x and out are required";
   if (p->x_stride < p->dim || p->x_stride % (p->x_type == SAS_TYPE_F32 ? 4 : 8) != 0)
@@ -75,6 +77,8 @@ const char *check_filter_rows(const sas_filter_rows *r) {
   if (r->rows < 0) return "rows must be >= 0";
   if (r->vocab < 1 || r->vocab > SAS_MAX_VOCAB) return "vocab must be in [1, SAS_MAX_VOCAB]";
   if (r->logits_type < SAS_TYPE_F32 || r->logits_type > SAS_TYPE_F16) return "logits_type must be one of SAS_TYPE_*";
+  // (a block 2,048 ids at least)
+  if ((int64_t)r->rows * (((int64_t)r->vocab + 2047) / 2048) > INT32_MAX) return "rows * vocab is too large";
   if (r->rows == 0) return nullptr;
   if (!r->logits || !r->out_ids) return "logits and out_ids are required";
   if (r->logits_stride < r->vocab) return "logits_stride < vocab";
@@ -195,8 +199,8 @@ int sas_sample_filtered(sas_sampler *s, const sas_filter_rows *r, void *stream) 
 int sas_reserve_filtered(sas_sampler *s, int32_t rows, int32_t vocab) {
   return guarded(s, [&]() -> int {
     if (!s) return fail(nullptr, SAS_ERR_INVALID, "sas_reserve_filtered: handle is NULL");
-    if (rows < 0 || vocab < 1 || vocab > SAS_MAX_VOCAB)
-      return fail(s, SAS_ERR_INVALID, "sas_reserve_filtered: rows must be >= 0 and vocab in [1, SAS_MAX_VOCAB]");
+    if (rows < 0 || vocab < 1 || vocab > SAS_MAX_VOCAB || (int64_t)rows * (((int64_t)vocab + 2047) / 2048) > INT32_MAX)
+      return fail(s, SAS_ERR_INVALID, "sas_reserve_filtered: rows must be >= 0, vocab in [1, SAS_MAX_VOCAB], rows * vocab below 2^42");
     if (int rc = set_device(s)) return rc;
     // fewer rows may be cut into more parts (from 2 cus rows on no longer)
     size_t bytes = 0;
