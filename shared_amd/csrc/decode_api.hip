@@ -189,6 +189,7 @@ int sas_sample_filtered(sas_sampler *s, const sas_filter_rows *r, void *stream) 
     a.shift = 62 - log2_ceil(r->vocab);
     a.span = filter_span(r->rows, r->vocab, 2 * s->cus);
     a.parts = (r->vocab + a.span - 1) / a.span;
+    a.log_list = filter_log_list(a.parts);
     if (int rc = grow(s, &s->filt, &s->filt_cap, filter_scratch_bytes(r->rows, a.parts), stream, "sas_sample_filtered")) return rc;
     filter_scratch(s->filt, &a);
     hipError_t e = launch_filter(a, pick_stream(s, stream));

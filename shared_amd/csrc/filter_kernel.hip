@@ -196,14 +196,10 @@ __device__ __forceinline__ void span_values(const FilterArgs &a, const sas_filte
   }
 }
 
-// Ids a part of `ids` lists: 4,096 a row of 262,144.
-constexpr int list_size(int ids) { return ids / 64; }
-
 template <int kType, bool kSoft, int kT, int Q>
 __global__ __launch_bounds__(kT) void filter_parts_kernel(const FilterArgs a) {
   constexpr int kIds = 4 * Q * kT, kW = kT / 64;
-  constexpr int kList = list_size(kIds);
-  static_assert(kList <= kFilterList && kList >= 8, "the list holds them");
+  const int kList = 1 << a.log_list;
   __shared__ double tab[kTab];
   __shared__ uint32_t count[kIds / 2];
   __shared__ unsigned long long mass[kFilterRanges];
@@ -319,7 +315,7 @@ __global__ __launch_bounds__(kT) void filter_parts_kernel(const FilterArgs a) {
     // The ranges leave room in the list and top-k may reach below them: down to
     // a value that half a list of ids reaches, the smallest of the waves' J-th
     // largest of their lanes' maxima; or to the largest, if that is too far.
-    constexpr int J = kList / 2 / kW;
+    const int J = kList / 2 / kW;
     float mine = neg;
 #pragma unroll
     for (int j = 0; j < Q; ++j) mine = fmaxf(mine, fmaxf(fmaxf(v[j][0], v[j][1]), fmaxf(v[j][2], v[j][3])));
@@ -1105,7 +1101,7 @@ __device__ __forceinline__ int merge_bin(float d) {
 template <int kType, bool kSoft, int Q>
 __global__ __launch_bounds__(kThreads) void filter_merge_kernel(const FilterArgs a) {
   constexpr int kIds = 4 * Q * kThreads;
-  constexpr int kList = list_size(kIds);
+  const int kList = 1 << a.log_list;
   constexpr int kLogIds = Q == 8 ? 13 : Q == 4 ? 12 : 11;
   static_assert(kIds == 1 << kLogIds, "a power of two");
   __shared__ MergeShared l;
@@ -1191,7 +1187,7 @@ __global__ __launch_bounds__(kThreads) void filter_merge_kernel(const FilterArgs
       u[i] = 0ull;
       if (at >= slots) continue;
       const float v = fkey((uint32_t)(e[i] >> 32)), d = mrange - range_of(v, g);
-      const bool in = at % kList < max(parts[at / kList].listed, 0) && (uint32_t)(e[i] >> 32) >= edge;
+      const bool in = (at & (kList - 1)) < max(parts[at >> a.log_list].listed, 0) && (uint32_t)(e[i] >> 32) >= edge;
       e[i] = in ? e[i] : 0ull;
       if (!in) continue;
       u[i] = units(mass_at((double)v));
@@ -1558,6 +1554,14 @@ void filter_scratch(void *base, FilterArgs *a) {
   a->left = reinterpret_cast<FilterLeft *>(at += (size_t)a->rows * kEntries * 8);
   a->found = reinterpret_cast<uint32_t *>(at += (size_t)a->rows * sizeof(FilterLeft));
   a->nleft = reinterpret_cast<uint32_t *>(at + (size_t)a->rows * 4);
+}
+
+// Ids a part lists: as many as keep a row's within what the merge takes, at
+// most kFilterList (at 25 parts of 2,048 ids 32 a part left top-k 200 short).
+int filter_log_list(int parts) {
+  int log = 7;
+  while (log > 5 && (parts << log) > kMergeMost) --log;
+  return log;
 }
 
 hipError_t launch_filter(const FilterArgs &a, hipStream_t stream) {

@@ -253,7 +253,7 @@ struct FilterArgs {
   struct FilterPart *part;
   uint64_t *range_mass;  // [rows][parts][kFilterRanges]
   uint32_t *range_count;
-  uint64_t *list;        // [rows][parts][span / 64]
+  uint64_t *list;        // [rows][parts][1 << log_list]
   // The rows that the merge leaves to the rest kernel, their number, and per row
   // how many ids of its planned ranges were found, and which.
   struct FilterLeft *left;
@@ -266,6 +266,7 @@ struct FilterArgs {
   int32_t shift;  // masses are integers of 2^-shift
   int32_t span;   // ids a part, a power of two
   int32_t parts;
+  int32_t log_list;
 };
 
 constexpr int kFilterRanges = 128;
@@ -290,6 +291,7 @@ constexpr int kFilterShift = 50;
 // Ids a part: 8,192, or fewer (at least 2,048) where the grid would hold
 // fewer than `min_blocks` blocks.
 int filter_span(int rows, int vocab, int min_blocks);
+int filter_log_list(int parts);
 size_t filter_scratch_bytes(int rows, int parts);
 void filter_scratch(void *base, FilterArgs *a);
 hipError_t launch_filter(const FilterArgs &a, hipStream_t stream);
