@@ -2,15 +2,30 @@
 // top-k of any size, top-p and min-p (gfx950).
 //
 // A row's candidates in the order (value descending, id ascending) are cut to
-// a prefix; the prefix ends inside the ids that share one value, the edge:
-// every id of a larger value is kept, and of the edge's the first `take` in
-// ascending order.  No ids are sorted: the edge is found by counts and masses
-// of value ranges, and the draw walks the kept ids in ascending order.
+// a prefix, and the draw walks the kept ids in ascending order.  No ids are
+// sorted: where the prefix ends is found from the counts and masses of value
+// ranges, then among the ids of one range.
 //
-// Masses exp((v - m) / T) are summed as 64-bit integers of 2^-shift: sums of
-// any order, atomic ones too, are the same bits.  2^shift * vocab <= 2^62, so
-// no sum overflows; rounding one mass is off by 2^-(shift + 1) of the largest
-// at most (2^-45 for 262,144 ids).
+// Masses exp((v - m) / T) are summed in doubles in a fixed order, or as 64-bit
+// integers of 2^-shift, whose sums of any order, atomic ones too, are the same
+// bits.  2^shift * vocab <= 2^62, so no sum overflows; rounding one mass is off
+// by 2^-(shift + 1) of the largest at most (2^-45 for 262,144 ids).
+//
+// Four launches:
+//   1. filter_parts_kernel, a block a part (8,192 ids, fewer in small batches):
+//      reads the logits once; leaves the part's largest value, its mass, the
+//      masses and counts of 128 ranges below its largest value, and its best
+//      ids.  Bound by the double exponentials (16 instructions a value) and, in
+//      rows that are cut, by a block's chain of barriers: 256 rows x 262,144
+//      f32, nothing cut, 79 us (3.4 TB/s); 128 rows under a grammar 66 us.
+//   2. filter_merge_kernel, four waves a row: the ends of the prefixes among
+//      the lists' ids, kept in registers, and the draw; 10 to 30 us, a chain of
+//      dependent steps.  (One kernel of 1,024 threads for every row: 24 to 30.)
+//   3. filter_gather_kernel, the whole chip: the ids of the ranges in which the
+//      ends lie, for rows whose lists do not reach them (wide nuclei).
+//   4. filter_rest_kernel, a block a row left: the ends among those ids, 33 to
+//      52 us; or, for values out of the ranges' scope, by rereading the row.
+//      Launches 3 and 4 end at once where no row was left (4 us together).
 #include "sas_device.h"
 #include "sas_exp.h"
 #include "sas_launch.h"

@@ -8,11 +8,27 @@
 //      pieces (8 + 8 + 8 bits of the f32 significand, cut, not rounded: their
 //      sum is the f32 value); f32 hidden states are stored as three pieces
 //      too.  Products of bf16 pieces are exact in the f32 sums of the matrix
-//      instructions, so f32 inputs keep all their bits.
+//      instructions, so f32 inputs keep all their bits (two pieces would be
+//      2e-6 off, one 2e-3).  One block puts the rows in the order of their
+//      adapters, so that a tile of rows meets few of them.
 //   2. proj_wide_kernel or proj_split_kernel: the rows' products with W, then
 //      with B of each adapter among a tile's rows, each adapter in sums of its
 //      own that only its rows add: a value that is not finite stays with its
 //      adapter.
+//
+// What bounds it, and what it measured (MI355X, a call):
+//   - up to about 128 rows W's stream from memory: 16 f32 rows x 2,560 x
+//     151,936 160 us (5.0 TB/s), 128 rows x 2,560 x 262,144, capped, 16
+//     adapters, 364 us (4.4 TB/s; 320 without adapters, 235 of it without the
+//     134 MB of results).  What carried it: weight rows in whole lines,
+//     nontemporal; loads kept several runs ahead of their use against the
+//     compiler's order; results in whole lines past the caches.
+//   - more rows the matrix instructions' operands in LDS, each wave reading all
+//     of a tile's hidden states: 2,048 x 4,096 x 4,096 97 us (0.72 PFLOP/s, the
+//     product 86 us of it; a library's 60), 200 f32 rows x 2,048 x 50,257 209
+//     us (three products each: 0.6 PFLOP/s).
+//   - an adapter a row (61 rows, ranks up to 64, 4,096 x 11,007: 115 us) the
+//     addresses of B's and h's loads, 16 bytes a lane.
 #include <utility>
 
 #include "sas_device.h"
