@@ -515,8 +515,9 @@ int sas_reserve_project(sas_sampler *s, int32_t rows, int32_t dim, int32_t rank)
  * and the token is the first kept id, in ascending order, whose running mass
  * exceeds U times the kept mass.  temperature <= 0 (or NaN) keeps the first
  * candidate alone.  Masses are summed as integers of 2^-s, s = 62 -
- * ceil(log2 vocab), so no sum depends on its order; an id whose mass is below
- * half of 2^-s is not drawn.  The reference's sample()
+ * ceil(log2 vocab), and as doubles over parts of the row in a fixed order, so
+ * equal calls give equal bits; an id whose mass is below half of 2^-s is not
+ * drawn.  The reference's sample()
  * cuts to top_k <= 128 first and has no min-p (tokenizer.js:151-178). */
 typedef struct sas_filter_params {
   double temperature;

@@ -27,7 +27,6 @@
 //      52 us; or, for values out of the ranges' scope, by rereading the row.
 //      Launches 3 and 4 end at once where no row was left (4 us together).
 #include "sas_device.h"
-#include "sas_exp.h"
 #include "sas_launch.h"
 
 namespace sas {
@@ -139,12 +138,10 @@ constexpr float kFar = 4194304.0f;
 constexpr double kUnit = (double)(1ull << kFilterShift);
 
 // Masses are powers of two counted in 256ths of an octave.  2^(j / 256), j = 0
-// .. 255, within 1 ulp, a thread an entry (the block's first 256).
+// .. 255, within 1 ulp, computed once a block, a thread an entry (its first 256).
 constexpr int kTab = 256;
 __device__ __forceinline__ void fill_tab(double *tab) {
-  const int j = threadIdx.x & 3;
-  const double c = j == 0 ? 1.0 : j == 1 ? 0x1.00b1afa5abcbfp+0 : j == 2 ? 0x1.0163da9fb3335p+0 : 0x1.02168143b0281p+0;
-  if (threadIdx.x < kTab) tab[threadIdx.x] = kExp2Tab[threadIdx.x >> 2].x * c;
+  if (threadIdx.x < kTab) tab[threadIdx.x] = exp2((double)threadIdx.x * (1.0 / 256.0));
 }
 // 2^(y / 256), -32768 <= y <= 256: the table's 2^(k / 256) times a Taylor series
 // in |r| <= 1/2 (2^(r / 256) to degree 4, 4e-17 short), the exponent added as
@@ -400,21 +397,23 @@ __device__ __forceinline__ int bin_of(uint32_t key, const Scale &s) {
   const double t = d * s.per_bin;
   return key == okey((float)s.m) ? 0 : t < (double)(kBins - 1) ? (int)t : kBins - 1;  // (NaN: the rest)
 }
-__device__ __forceinline__ double mass_of(uint32_t key, const Scale &s, const ExpTab &tab) {
+// e^x, x <= 0; of -inf and NaN: 0.
+__device__ __forceinline__ double mass_exp(double x) { return exp(fmax(x, -1100.0)); }
+__device__ __forceinline__ double mass_of(uint32_t key, const Scale &s) {
   const float v = fkey(key);
-  return v == (float)s.m ? 1.0 : exp_sum(((double)v - s.m) * s.inv_t, tab);
+  return v == (float)s.m ? 1.0 : mass_exp(((double)v - s.m) * s.inv_t);
 }
 __device__ __forceinline__ uint64_t units_of(double mass, const Scale &s) {
   return (uint64_t)__builtin_rint(__builtin_amdgcn_ldexp(mass, s.shift));
 }
 
 // The smallest key whose mass reaches min_p (the mass falls with the key).
-__device__ __forceinline__ uint32_t least_key(double min_p, uint32_t top, const Scale &s, const ExpTab &tab) {
+__device__ __forceinline__ uint32_t least_key(double min_p, uint32_t top, const Scale &s) {
   const double least = fmin(min_p, 1.0);
   uint32_t lo = kNegInf, hi = top;  // hi reaches it, lo does not (or is no candidate's)
   while (hi - lo > 1) {
     const uint32_t mid = lo + (hi - lo) / 2;
-    if (mass_of(mid, s, tab) >= least) hi = mid;
+    if (mass_of(mid, s) >= least) hi = mid;
     else lo = mid;
   }
   return hi;
@@ -427,7 +426,6 @@ struct Edge {
 };
 
 struct RowShared {
-  ExpTab tab;
   uint32_t count[kSpan / 2];  // history counts of a span's ids, 16 bits each
   unsigned long long mass[kBins];
   uint32_t cnt[kBins];
@@ -578,7 +576,7 @@ struct Row {
       each([&](uint32_t k) {
         if (k && (k & above) == top && bin_of(k, s) == bin) {
           const int d = 255 - (int)((k >> sh) & 0xFFu);
-          atomicAdd(&l.mass[d], (unsigned long long)units_of(mass_of(k, s, l.tab), s));
+          atomicAdd(&l.mass[d], (unsigned long long)units_of(mass_of(k, s), s));
           atomicAdd(&l.cnt[d], 1u);
         }
       });
@@ -588,7 +586,7 @@ struct Row {
       c0 += c1;
       top |= (uint32_t)(255 - d) << sh;
     }
-    const uint64_t unit = units_of(mass_of(top, s, l.tab), s);
+    const uint64_t unit = units_of(mass_of(top, s), s);
     const uint32_t n = l.cnt[255 - (top & 0xFFu)];
     uint64_t take = by_count ? need - c0 : unit ? (need - m0 + unit - 1) / unit : 1;
     take = min(max(take, (uint64_t)1), (uint64_t)n);
@@ -610,7 +608,7 @@ struct Row {
     each([&](uint32_t k) {
       if (!k || k <= end.key) return;
       const int b = bin_of(k, s);
-      const uint64_t u = by_count ? 0ull : units_of(mass_of(k, s, l.tab), s);
+      const uint64_t u = by_count ? 0ull : units_of(mass_of(k, s), s);
       if (b == kBins - 1) {
         rest += u;
         ++nrest;
@@ -625,7 +623,7 @@ struct Row {
       l.cnt[kBins - 1] = (uint32_t)nrest;
       if (end.key) {
         const int b = bin_of(end.key, s);
-        l.mass[b] += end.take * units_of(mass_of(end.key, s, l.tab), s);
+        l.mass[b] += end.take * units_of(mass_of(end.key, s), s);
         l.cnt[b] += end.take;
       }
     }
@@ -687,12 +685,12 @@ __device__ __forceinline__ void row_by_values(Row<kType, kSoft> &R, const Filter
     if (!e.key || f.key > e.key || (f.key == e.key && f.take < e.take)) e = f;
   }
   if (p.min_p > 0.0) {
-    const uint32_t hi = least_key(p.min_p, top, R.s, l.tab);
+    const uint32_t hi = least_key(p.min_p, top, R.s);
     if (hi > e.key) e = Edge{hi, ~0u};
   }
   // what is kept of each span; the edge's ids count in ascending order
   uint64_t total = 0, kept = 0, ties = 0;
-  const uint64_t unit = e.key ? units_of(mass_of(e.key, R.s, l.tab), R.s) : 0;
+  const uint64_t unit = e.key ? units_of(mass_of(e.key, R.s), R.s) : 0;
   for (int q = 0; q < R.spans(); ++q) {
     uint32_t key[kQuads][4];
     R.keys(q, key);
@@ -703,7 +701,7 @@ __device__ __forceinline__ void row_by_values(Row<kType, kSoft> &R, const Filter
       for (int i = 0; i < 4; ++i) {
         const uint32_t k = key[j][i];
         if (k > e.key) {
-          m += units_of(mass_of(k, R.s, l.tab), R.s);
+          m += units_of(mass_of(k, R.s), R.s);
           c += 1;
         } else if (k && k == e.key) {
           c += 1ull << 32;
@@ -754,7 +752,7 @@ __device__ __forceinline__ void row_by_values(Row<kType, kSoft> &R, const Filter
       const uint32_t k = key[j][i];
       bool in = k > e.key;
       if (k && k == e.key) in = tie++ < e.take;
-      mine[i] = in ? units_of(mass_of(k, R.s, l.tab), R.s) : 0;
+      mine[i] = in ? units_of(mass_of(k, R.s), R.s) : 0;
       m += mine[i];
     }
     uint64_t run = before + block_scan(l, m, &all) - m;
@@ -762,7 +760,7 @@ __device__ __forceinline__ void row_by_values(Row<kType, kSoft> &R, const Filter
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if (run <= goal && goal < run + mine[i])
-          done((uint32_t)(R.id0(q, j) + i), mass_of(key[j][i], R.s, l.tab) / __builtin_amdgcn_ldexp((double)total, -a.shift), kept);
+          done((uint32_t)(R.id0(q, j) + i), mass_of(key[j][i], R.s) / __builtin_amdgcn_ldexp((double)total, -a.shift), kept);
         run += mine[i];
       }
     }
@@ -888,7 +886,7 @@ __device__ __forceinline__ bool row_by_parts(Row<kType, kSoft> &R, const FilterA
   const bool by_k = p.top_k > 0 && (uint64_t)p.top_k < n, by_p = p.top_p < 1.0, by_min = p.min_p > 0.0;
   const bool cut = by_k || by_p || by_min;
   // a part's factor to the row's units
-  auto scale_of = [&](const FilterPart &f) { return exp_sum(((double)f.top / (double)g.inv_width - R.s.m) * R.s.inv_t, l.tab); };
+  auto scale_of = [&](const FilterPart &f) { return mass_exp(((double)f.top / (double)g.inv_width - R.s.m) * R.s.inv_t); };
   uint64_t all = 0;
   for (int i = tid; i < a.parts; i += kRowThreads) {
     const FilterPart f = parts[i];
@@ -946,14 +944,14 @@ __device__ __forceinline__ bool row_by_parts(Row<kType, kSoft> &R, const FilterA
       havem += l.mass[i];
     }
     block_sum2(l, have, havem);
-    const uint32_t least = by_min ? least_key(p.min_p, top, R.s, l.tab) : 0u;
+    const uint32_t least = by_min ? least_key(p.min_p, top, R.s) : 0u;
     // the ids of the planned ranges
     entries = (int)a.found[row];
     if (entries > kEntries) return false;
     for (int i = tid; i < entries; i += kRowThreads) {
       const uint64_t e = a.ids[(int64_t)row * kEntries + i];
       l.ent[i] = e;
-      l.entm[i] = units_of(mass_of((uint32_t)(e >> 32), R.s, l.tab), R.s);
+      l.entm[i] = units_of(mass_of((uint32_t)(e >> 32), R.s), R.s);
     }
     __syncthreads();
     auto planned = [&](int bin) { return bin < kFilterRanges && ((x.ranges[bin >> 5] >> (bin & 31)) & 1u) != 0u; };
@@ -1032,7 +1030,7 @@ __device__ __forceinline__ bool row_by_parts(Row<kType, kSoft> &R, const FilterA
       const int at = 4 * (j * kRowThreads + tid) + i;
       const uint32_t key = okey(v[j][i]);
       const bool in = at < a.span && v[j][i] > -__builtin_inff() && ((uint64_t)key << 32 | (uint32_t) ~(uint32_t)(id0 + at)) >= last;
-      u[j][i] = in ? units_of(mass_of(key, R.s, l.tab), R.s) : 0ull;
+      u[j][i] = in ? units_of(mass_of(key, R.s), R.s) : 0ull;
       sum += u[j][i];
     }
     run[j] = sums + block_scan(l, sum, &of_all) - sum;
@@ -1045,7 +1043,7 @@ __device__ __forceinline__ bool row_by_parts(Row<kType, kSoft> &R, const FilterA
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if (run[j] <= target && target < run[j] + u[j][i])
-        done((uint32_t)(id0 + 4 * (j * kRowThreads + tid) + i), mass_of(okey(v[j][i]), R.s, l.tab) / whole, kept);
+        done((uint32_t)(id0 + 4 * (j * kRowThreads + tid) + i), mass_of(okey(v[j][i]), R.s) / whole, kept);
       run[j] += u[j][i];
     }
   return true;
@@ -1058,8 +1056,6 @@ __global__ __launch_bounds__(kRowThreads) void filter_rest_kernel(const FilterAr
   if (blockIdx.x >= *a.nleft) return;
   const FilterLeft x = a.left[blockIdx.x];
   const int row = x.row;
-  l.tab.fill(exp_tab_entry());
-  __syncthreads();
   const sas_filter_params p = load_filter_params(a, row);
   Row<kType, kSoft> R{a, l, p, (int64_t)row * a.logits_stride, a.mask ? a.mask + (int64_t)row * a.mask_stride : nullptr,
                       history_of(a, row), Scale{}};
