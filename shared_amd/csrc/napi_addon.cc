@@ -472,6 +472,103 @@ bool read_head(napi_env env, napi_value d, sas_lm_head *hd) {
   return true;
 }
 
+// A sas_filter_rows descriptor: sample's fields (without candidates), with
+// logitsType, and params that hold minP; topK 0 is off.
+bool read_filter(napi_env env, napi_value d, sas_filter_rows *f) {
+  std::memset(f, 0, sizeof *f);
+  sas_rows r;
+  if (!read_rows(env, d, &r)) return false;
+  int64_t type = SAS_TYPE_F32, top_k = 0;
+  napi_value pv;
+  if (!get_i64(env, d, "logitsType", &type) || type < 0 || type > INT32_MAX) return false;
+  f->params.top_p = 1.0;
+  f->params.repetition_penalty = 1.0;
+  if (has(env, d, "params", &pv)) {
+    if (!get_f64(env, pv, "minP", &f->params.min_p) || !get_i64(env, pv, "topK", &top_k)) return false;
+    f->params.temperature = r.params.temperature;
+    f->params.top_p = r.params.top_p;
+    f->params.repetition_penalty = r.params.repetition_penalty;
+    f->params.presence_penalty = r.params.presence_penalty;
+    f->params.frequency_penalty = r.params.frequency_penalty;
+    f->params.softcap = r.params.softcap;
+    f->params.top_k = top_k > INT32_MAX ? INT32_MAX : (top_k < 0 ? 0 : (int32_t)top_k);
+  }
+  f->logits = r.logits;
+  f->logits_stride = r.logits_stride;
+  f->logits_type = (int32_t)type;
+  f->vocab = r.vocab;
+  f->rows = r.rows;
+  f->mask = r.mask;
+  f->mask_stride = r.mask_stride;
+  f->hist_ids = r.hist_ids;
+  f->hist_offsets = r.hist_offsets;
+  f->hist_count = r.hist_count;
+  f->uniforms = r.uniforms;
+  f->row_params = reinterpret_cast<const sas_filter_params *>(r.row_params);
+  f->out_ids = r.out_ids;
+  f->out_probs = r.out_probs;
+  f->out_counts = r.out_counts;
+  f->out_flags = r.out_flags;
+  return true;
+}
+
+napi_value SampleFiltered(napi_env env, napi_callback_info info) {
+  napi_value argv[2];
+  if (!args(env, info, 2, argv)) return throw_napi(env, "arguments");
+  HANDLE_OR_THROW(argv[0], s);
+  sas_filter_rows f;
+  if (!read_filter(env, argv[1], &f)) {
+    napi_throw_type_error(env, nullptr, "sas_napi: bad filtered sample descriptor");
+    return nullptr;
+  }
+  int rc = sas_sample_filtered(s, &f, sas_stream(s));
+  return rc == SAS_OK ? undefined(env) : throw_sas(env, s, rc);
+}
+
+// A sas_projection descriptor: the C fields in camelCase.
+bool read_projection(napi_env env, napi_value d, sas_projection *p) {
+  std::memset(p, 0, sizeof *p);
+  int64_t xt = 0, rows = 0, dim = 0, out = 0, n = 0, rank = 0, ot = 0, acc = 0;
+  double cap = 0.0;
+  const bool ok = get_ptr(env, d, "x", (void **)&p->x) && get_i64(env, d, "xStride", &p->x_stride) &&
+                  get_i64(env, d, "xType", &xt) && get_i64(env, d, "rows", &rows) &&
+                  get_ptr(env, d, "weight", (void **)&p->weight) && get_i64(env, d, "weightStride", &p->weight_stride) &&
+                  get_i64(env, d, "dim", &dim) && get_i64(env, d, "outDim", &out) && get_i64(env, d, "adapters", &n) &&
+                  get_i64(env, d, "rank", &rank) && get_ptr(env, d, "a", (void **)&p->a) &&
+                  get_i64(env, d, "aStride", &p->a_stride) && get_i64(env, d, "aAdapterStride", &p->a_adapter_stride) &&
+                  get_ptr(env, d, "b", (void **)&p->b) && get_i64(env, d, "bStride", &p->b_stride) &&
+                  get_i64(env, d, "bAdapterStride", &p->b_adapter_stride) &&
+                  get_ptr(env, d, "scales", (void **)&p->scales) && get_ptr(env, d, "ranks", (void **)&p->ranks) &&
+                  get_ptr(env, d, "rowAdapter", (void **)&p->row_adapter) && get_ptr(env, d, "out", &p->out) &&
+                  get_i64(env, d, "outStride", &p->out_stride) && get_i64(env, d, "outType", &ot) &&
+                  get_i64(env, d, "accumulate", &acc) && get_f64(env, d, "softcap", &cap);
+  for (int64_t v : {xt, rows, dim, out, n, rank, ot, acc})
+    if (v < INT32_MIN || v > INT32_MAX) return false;
+  p->x_type = (int32_t)xt;
+  p->rows = (int32_t)rows;
+  p->dim = (int32_t)dim;
+  p->out_dim = (int32_t)out;
+  p->adapters = (int32_t)n;
+  p->rank = (int32_t)rank;
+  p->out_type = (int32_t)ot;
+  p->accumulate = (int32_t)acc;
+  p->softcap = (float)cap;
+  return ok;
+}
+
+napi_value Project(napi_env env, napi_callback_info info) {
+  napi_value argv[2];
+  if (!args(env, info, 2, argv)) return throw_napi(env, "arguments");
+  HANDLE_OR_THROW(argv[0], s);
+  sas_projection p;
+  if (!read_projection(env, argv[1], &p)) {
+    napi_throw_type_error(env, nullptr, "sas_napi: bad projection descriptor");
+    return nullptr;
+  }
+  int rc = sas_project(s, &p, sas_stream(s));
+  return rc == SAS_OK ? undefined(env) : throw_sas(env, s, rc);
+}
+
 napi_value LmHeadSample(napi_env env, napi_callback_info info) {
   napi_value argv[3];
   if (!args(env, info, 3, argv)) return throw_napi(env, "arguments");
@@ -920,6 +1017,8 @@ napi_value Init(napi_env env, napi_value exports) {
       {"sampleStepAsync", nullptr, SampleStepAsync, nullptr, nullptr, nullptr, napi_enumerable, nullptr},
       {"lmHeadSample", nullptr, LmHeadSample, nullptr, nullptr, nullptr, napi_enumerable, nullptr},
       {"lmHeadSampleAsync", nullptr, LmHeadSampleAsync, nullptr, nullptr, nullptr, napi_enumerable, nullptr},
+      {"sampleFiltered", nullptr, SampleFiltered, nullptr, nullptr, nullptr, napi_enumerable, nullptr},
+      {"project", nullptr, Project, nullptr, nullptr, nullptr, napi_enumerable, nullptr},
       {"lmHeadStep", nullptr, LmHeadStep, nullptr, nullptr, nullptr, napi_enumerable, nullptr},
       {"lmHeadStepAsync", nullptr, LmHeadStepAsync, nullptr, nullptr, nullptr, napi_enumerable, nullptr},
       {"specStep", nullptr, SpecStep, nullptr, nullptr, nullptr, napi_enumerable, nullptr},

@@ -287,6 +287,10 @@ export declare class Sampler {
   /** The LM head with the sampling step fused (rows <= LMH_MAX_ROWS). */
   lmHeadSample(opts: LmHeadSampleOptions): SampleRowsResult;
   lmHeadSampleAsync(opts: LmHeadSampleOptions): Promise<SampleRowsResult>;
+  /** One token per row from the whole vocabulary: min-p, top-k of any size or off. */
+  sampleFiltered(opts: SampleFilteredOptions): SampleFilteredResult;
+  /** A shared projection with the low-rank adapters of many requests. */
+  project(opts: ProjectOptions): void;
   decodeRows(opts: SampleRowsOptions): DecodeBatchResult[];
   decodeRowsAsync(opts: SampleRowsOptions): Promise<DecodeBatchResult[]>;
   decodeSteps(opts: DecodeStepsOptions): DecodeBatchResult[];
@@ -341,3 +345,47 @@ export declare const STOP_PAD: number;
 export declare const LMH_MAX_ROWS: number;
 export declare const LMH_MAX_LDS_FLOATS: number;
 export declare const LMH_MAX_VOCAB: number;
+
+export interface FilterParams {
+  temperature?: number;
+  topP?: number;
+  minP?: number;
+  /** 0: off. */
+  topK?: number;
+  repetitionPenalty?: number;
+  presencePenalty?: number;
+  frequencyPenalty?: number;
+  softcap?: number;
+}
+
+export interface SampleFilteredOptions extends Omit<SampleRowsOptions, 'params'> {
+  params: FilterParams | FilterParams[];
+  uniforms: Float64Array;
+  logitsType?: 'f32' | 'bf16' | 'f16';
+}
+
+export interface SampleFilteredResult {
+  ids: Uint32Array;
+  /** With full: the token's share of the kept mass, the ids kept, SAS_FLAG_* bits. */
+  probs?: Float64Array;
+  counts?: Int32Array;
+  flags?: Uint32Array;
+}
+
+export interface ProjectOptions {
+  x: DeviceBuffer;
+  xType?: 'f32' | 'bf16';
+  rows: number;
+  dim: number;
+  /** bf16 [outDim][dim]; absent with accumulate: the adapters' terms alone. */
+  weight?: DeviceBuffer;
+  outDim: number;
+  out: DeviceBuffer;
+  outType?: 'f32' | 'bf16';
+  /** bf16 a [count][rank][dim], b [count][outDim][rank]. */
+  adapters?: { a: DeviceBuffer; b: DeviceBuffer; count: number; rank: number; scales?: DeviceBuffer; ranks?: DeviceBuffer };
+  /** int32 [rows], -1: none. */
+  rowAdapter?: DeviceBuffer;
+  softcap?: number;
+  accumulate?: boolean;
+}

@@ -406,6 +406,10 @@ class DeviceBuffer {
   }
 }
 
+// SAS_TYPE_* and sizeof(sas_filter_params)
+const ELEMENT_TYPES = { f32: 0, bf16: 1, f16: 2 };
+const FILTER_PARAMS_BYTES = 56;
+
 class Sampler {
   /** A sampler bound to HIP device `device`; throws when no device exists. */
   constructor(device) {
@@ -803,6 +807,104 @@ class Sampler {
       return self._worker(addon.lmHeadSampleAsync(self._handle(), r.desc, hd))
         .then(function () { return self._collect(opts, r.packed); });
     });
+  }
+
+  /**
+   * One token per row from the whole vocabulary (sas_sample_filtered): opts as
+   * sampleRows, but params hold {temperature, topK (0: off, any size), topP,
+   * minP, repetitionPenalty, presencePenalty, frequencyPenalty, softcap}, one
+   * object or one a row, and uniforms are required.  logitsType: 'f32' (the
+   * default), 'bf16' or 'f16' of a DeviceBuffer.  Returns {ids[, probs (the
+   * token's share of the kept mass), counts (ids kept), flags]}.
+   */
+  sampleFiltered(opts) {
+    this._idle('sampleFiltered');
+    const rows = opts.rows;
+    const ps = Array.isArray(opts.params) ? opts.params : [opts.params || {}];
+    if (ps.length !== 1 && ps.length !== rows) throw new RangeError('params must have one entry per row');
+    const type = orDefault(opts.logitsType, 'f32');
+    if (!Object.prototype.hasOwnProperty.call(ELEMENT_TYPES, type)) throw new RangeError('logitsType must be f32, bf16 or f16');
+    if (type !== 'f32' && !(opts.logits instanceof DeviceBuffer)) throw new TypeError('bf16 and f16 logits must be a DeviceBuffer');
+    if (!(opts.uniforms instanceof Float64Array) || opts.uniforms.length < rows) {
+      throw new TypeError('uniforms must be a Float64Array[rows]');
+    }
+    const words = Math.ceil(opts.vocab / 32);
+    const span = (rows - 1) * orDefault(opts.stride, opts.vocab) + opts.vocab;
+    const held = opts.logits instanceof DeviceBuffer ? opts.logits.bytes : opts.logits && opts.logits.byteLength;
+    if (!(held >= span * (type === 'f32' ? 4 : 2))) throw new RangeError('logits hold fewer than their rows');
+    if (opts.mask instanceof Uint32Array && opts.mask.length !== words && opts.mask.length < rows * words) {
+      throw new RangeError('mask holds fewer than rows * ceil(vocab / 32) words');
+    }
+    // logits, mask, history, uniforms and ids as sampleRows has them
+    const d = this._describe(Object.assign({}, opts, { params: { temperature: 1 }, full: false })).desc;
+    d.logitsType = ELEMENT_TYPES[type];
+    const full = ps.map(function (p) {
+      return { temperature: orDefault(p.temperature, 0), topP: orDefault(p.topP, 1), minP: orDefault(p.minP, 0),
+        repetitionPenalty: orDefault(p.repetitionPenalty, 1), presencePenalty: orDefault(p.presencePenalty, 0),
+        frequencyPenalty: orDefault(p.frequencyPenalty, 0), softcap: orDefault(p.softcap, 0), topK: orDefault(p.topK, 0) };
+    });
+    d.params = full[0];
+    if (full.length > 1) {
+      const view = new DataView(new ArrayBuffer(rows * FILTER_PARAMS_BYTES));
+      full.forEach(function (p, r) {
+        const at = r * FILTER_PARAMS_BYTES;
+        [p.temperature, p.topP, p.minP, p.repetitionPenalty, p.presencePenalty, p.frequencyPenalty].forEach(function (v, i) {
+          view.setFloat64(at + 8 * i, v, true);
+        });
+        view.setFloat32(at + 48, p.softcap, true);
+        view.setInt32(at + 52, Math.max(0, Math.min(0x7FFFFFFF, p.topK)), true);
+      });
+      d.rowParams = this._buf('filterParams', view.byteLength).upload(new Uint8Array(view.buffer)).ptr;
+    }
+    if (opts.full) {
+      d.outProbs = this._buf('probs', rows * 8).ptr;
+      d.outCounts = this._buf('counts', rows * 4).ptr;
+      d.outFlags = this._buf('flags', rows * 4).ptr;
+    }
+    addon.sampleFiltered(this._handle(), d);
+    const out = { ids: this._scratch.ids.download(new Uint32Array(rows)) };
+    if (opts.full) {
+      out.probs = this._scratch.probs.download(new Float64Array(rows));
+      out.counts = this._scratch.counts.download(new Int32Array(rows));
+      out.flags = this._scratch.flags.download(new Uint32Array(rows));
+    }
+    return out;
+  }
+
+  /**
+   * A shared projection with the low-rank adapters of many requests
+   * (sas_project) over DeviceBuffers: {x, xType?, rows, dim, weight, outDim,
+   * out, outType?, adapters?: {a, b, count, rank, scales?, ranks?},
+   * rowAdapter?, softcap?, accumulate?}, contiguous; x 'f32' (the default) or
+   * 'bf16', out alike.  The result is in `out` when the sampler's stream gets
+   * there (synchronize(), or a download).
+   */
+  project(opts) {
+    this._idle('project');
+    const ptr = function (b, name, bytes) {
+      if (b === undefined || b === null) return undefined;
+      if (!(b instanceof DeviceBuffer)) throw new TypeError(name + ' must be a DeviceBuffer');
+      if (!(b.bytes >= bytes)) throw new RangeError(name + ' holds fewer than its ' + bytes + ' bytes');
+      return b.ptr;
+    };
+    const xType = orDefault(opts.xType, 'f32');
+    const outType = orDefault(opts.outType, 'f32');
+    if (!Object.prototype.hasOwnProperty.call(ELEMENT_TYPES, xType)) throw new RangeError('xType must be f32 or bf16');
+    if (!Object.prototype.hasOwnProperty.call(ELEMENT_TYPES, outType)) throw new RangeError('outType must be f32 or bf16');
+    if (xType === 'f16' || outType === 'f16') throw new RangeError('xType and outType must be f32 or bf16');
+    const size = function (type) { return type === 'f32' ? 4 : 2; };
+    const d = { x: ptr(opts.x, 'x', opts.rows * opts.dim * size(xType)), xStride: opts.dim, xType: ELEMENT_TYPES[xType], rows: opts.rows, dim: opts.dim,
+      weight: ptr(opts.weight, 'weight', opts.outDim * opts.dim * 2), weightStride: opts.dim, outDim: opts.outDim, out: ptr(opts.out, 'out', opts.rows * opts.outDim * size(outType)),
+      outStride: opts.outDim, outType: ELEMENT_TYPES[outType], softcap: orDefault(opts.softcap, 0),
+      accumulate: opts.accumulate ? 1 : 0 };
+    const p = opts.adapters;
+    if (p) {
+      Object.assign(d, { a: ptr(p.a, 'adapters.a', p.count * p.rank * opts.dim * 2), aStride: opts.dim, aAdapterStride: p.rank * opts.dim,
+        b: ptr(p.b, 'adapters.b', p.count * opts.outDim * p.rank * 2), bStride: p.rank, bAdapterStride: opts.outDim * p.rank, adapters: p.count, rank: p.rank,
+        scales: ptr(p.scales, 'adapters.scales', p.count * 4), ranks: ptr(p.ranks, 'adapters.ranks', p.count * 4),
+        rowAdapter: ptr(opts.rowAdapter, 'rowAdapter', opts.rows * 4) });
+    }
+    addon.project(this._handle(), d);
   }
 
   // decodeBatch's per-row result for one step (model.js:727-741,
