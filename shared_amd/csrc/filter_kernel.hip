@@ -1180,11 +1180,14 @@ __global__ __launch_bounds__(kThreads) void filter_merge_kernel(const FilterArgs
   auto units = [&](double mass) { return (uint64_t)__builtin_rint(__builtin_amdgcn_ldexp(mass, a.shift)); };
   const bool by_k = p.top_k > 0 && (uint64_t)p.top_k < n, by_p = p.top_p < 1.0, by_min = p.min_p > 0.0;
   const bool cut = by_k || by_p || by_min;
-  // the parts' masses in the row's units
+  // The parts' masses in the row's units.  Where nothing is cut the draw goes by
+  // them, then by the units of the chosen part's ids: a part whose largest value
+  // rounds to none has no id to draw, though its sum may round to many.
   uint64_t all = 0;
   for (int i = tid; i < a.parts; i += kThreads) {
     const FilterPart f = parts[i];
-    const uint64_t u = f.listed < 0 ? 0ull : units(f.mass * mass_of_ref(f.top));
+    const bool none = f.listed < 0 || (!cut && units(mass_at((double)f.max)) == 0ull);
+    const uint64_t u = none ? 0ull : units(f.mass * mass_of_ref(f.top));
     l.part[i] = cut ? 0ull : u;
     all += u;
   }
