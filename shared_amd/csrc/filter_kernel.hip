@@ -133,6 +133,10 @@ __device__ __forceinline__ Grid grid_of(double temperature) {
 // A value's range; exact below 2^22 ranges from zero (kFar otherwise).
 __device__ __forceinline__ float range_of(float v, const Grid &g) { return __builtin_floorf(v * g.inv_width); }
 constexpr float kFar = 4194304.0f;
+// A part's ranges are kept where its largest value lies within kFar.  A part below
+// that counts for nothing in its row, so a row's largest value has to lie 2,048
+// ranges above: 128 T at least, masses below 2^-184.
+constexpr float kNear = 2048.0f - kFar;
 // A part's ranges sum masses as integers of 2^-kFilterShift: 8,192 of at most
 // e^(1/8) stay below 2^64.
 constexpr double kUnit = (double)(1ull << kFilterShift);
@@ -1172,7 +1176,7 @@ __global__ __launch_bounds__(kThreads) void filter_merge_kernel(const FilterArgs
   const uint32_t top = (uint32_t)(best >> 32);
   const Grid g = grid_of(p.temperature);
   const float mrange = range_of(fkey(top), g);
-  if (!g.plain || !(fabsf(mrange) < kFar)) return leave();
+  if (!g.plain || !(mrange >= kNear && mrange < kFar)) return leave();
   // the mass of a value, and of a part's reference
   const double m = (double)fkey(top) * g.per;
   auto mass_at = [&](double v) { return exp256(fmax(fma(v, g.per, -m), kLeast), l.tab); };
