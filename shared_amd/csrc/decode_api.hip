@@ -203,14 +203,14 @@ int sas_reserve_filtered(sas_sampler *s, int32_t rows, int32_t vocab) {
     if (rows < 0 || vocab < 1 || vocab > SAS_MAX_VOCAB || (int64_t)rows * (((int64_t)vocab + 2047) / 2048) > INT32_MAX)
       return fail(s, SAS_ERR_INVALID, "sas_reserve_filtered: rows must be >= 0, vocab in [1, SAS_MAX_VOCAB], rows * vocab below 2^42");
     if (int rc = set_device(s)) return rc;
-    // fewer rows may be cut into more parts (from 2 cus rows on no longer)
+    // fewer rows, and smaller vocabularies, may be cut into more parts (from
+    // 2 cus rows on no longer)
     size_t bytes = 0;
-    auto shape = [&](int n) {
-      const int span = filter_span(n, vocab, 2 * s->cus);
-      bytes = std::max(bytes, filter_scratch_bytes(n, (vocab + span - 1) / span));
+    auto most = [&](int n) {
+      bytes = std::max(bytes, filter_scratch_bytes(n, filter_most_parts(n, vocab, 2 * s->cus)));
     };
-    for (int n = 1; n <= std::min(rows, 2 * s->cus); ++n) shape(n);
-    if (rows > 0) shape(rows);
+    for (int n = 1; n <= std::min(rows, 2 * s->cus); ++n) most(n);
+    if (rows > 0) most(rows);
     return grow(s, &s->filt, &s->filt_cap, bytes, nullptr, "sas_reserve_filtered");
   });
 }

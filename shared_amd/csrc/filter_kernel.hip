@@ -26,6 +26,8 @@
 //   4. filter_rest_kernel, a block a row left: the ends among those ids, 33 to
 //      52 us; or, for values out of the ranges' scope, by rereading the row.
 //      Launches 3 and 4 end at once where no row was left (4 us together).
+#include <algorithm>
+
 #include "sas_device.h"
 #include "sas_launch.h"
 
@@ -1553,6 +1555,18 @@ int filter_span(int rows, int vocab, int min_blocks) {
   int span = 8192;
   while (span > 2048 && (int64_t)rows * ((vocab + span - 1) / span) < min_blocks) span /= 2;
   return span;
+}
+
+// The most parts that a row of at most `vocab` ids may have in a batch of `rows`:
+// a length of part has the most at the largest vocabulary that is cut so.  2,048
+// and 4,096 ids are for rows of fewer than min_blocks / rows parts of twice that.
+int filter_most_parts(int rows, int vocab, int min_blocks) {
+  int64_t most = ((int64_t)vocab + 8191) / 8192;
+  for (int64_t span = 4096; span >= 2048; span /= 2) {
+    const int64_t v = std::min((int64_t)vocab, 2 * span * ((min_blocks - 1) / rows));
+    most = std::max(most, (v + span - 1) / span);
+  }
+  return (int)most;
 }
 
 // The parts, their lists, the masses and counts of their ranges.

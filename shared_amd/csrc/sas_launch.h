@@ -291,6 +291,8 @@ constexpr int kFilterShift = 50;
 // Ids a part: 8,192, or fewer (at least 2,048) where the grid would hold
 // fewer than `min_blocks` blocks.
 int filter_span(int rows, int vocab, int min_blocks);
+// The most parts of a row over vocabularies of at most `vocab` ids.
+int filter_most_parts(int rows, int vocab, int min_blocks);
 int filter_log_list(int parts);
 size_t filter_scratch_bytes(int rows, int parts);
 void filter_scratch(void *base, FilterArgs *a);
