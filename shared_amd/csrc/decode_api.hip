@@ -113,7 +113,7 @@ int sas_project(sas_sampler *s, const sas_projection *p, void *stream) {
     const bool pieces = p->x_type == SAS_TYPE_F32 && p->weight;
     const int rank = p->adapters > 0 ? p->rank : 0;
     const ProjScratch at = proj_scratch(p->rows, p->dim, rank, pieces);
-    if (int rc = grow(s, &s->proj, &s->proj_cap, at.bytes, stream, who)) return rc;
+    if (int rc = grow(s, &s->proj, &s->proj_cap, at.bytes, stream, who, "sas_reserve_project")) return rc;
     char *scratch = static_cast<char *>(s->proj);
     ProjArgs a{};
     a.x = p->x;
@@ -190,7 +190,9 @@ int sas_sample_filtered(sas_sampler *s, const sas_filter_rows *r, void *stream) 
     a.span = filter_span(r->rows, r->vocab, 2 * s->cus);
     a.parts = (r->vocab + a.span - 1) / a.span;
     a.log_list = filter_log_list(a.parts);
-    if (int rc = grow(s, &s->filt, &s->filt_cap, filter_scratch_bytes(r->rows, a.parts), stream, "sas_sample_filtered")) return rc;
+    if (int rc = grow(s, &s->filt, &s->filt_cap, filter_scratch_bytes(r->rows, a.parts), stream, "sas_sample_filtered",
+                      "sas_reserve_filtered"))
+      return rc;
     filter_scratch(s->filt, &a);
     hipError_t e = launch_filter(a, pick_stream(s, stream));
     return e == hipSuccess ? SAS_OK : hip_fail(s, e, "sas_sample_filtered launch");

@@ -60,14 +60,16 @@ inline bool capturing(void *stream) {
 // is retired, not freed: launches queued on any stream, and graphs that
 // recorded them, keep a valid address; sas_destroy frees it.  Capacities
 // at least double, so retired buffers hold less than the live one.  Under
-// stream capture nothing is allocated: the call fails and names the fix.
-inline int grow(sas_sampler *s, void **buf, size_t *cap, size_t need, void *stream, const char *who) {
+// stream capture nothing is allocated: the call fails and names the fix,
+// `reserve` (the entry that sizes this buffer) or an eager call.
+inline int grow(sas_sampler *s, void **buf, size_t *cap, size_t need, void *stream, const char *who,
+                const char *reserve = "sas_reserve_for") {
   if (need <= *cap) return SAS_OK;
   if (capturing(stream))
     return fail(s, SAS_ERR_INVALID,
                 std::string(who) + ": the handle's scratch is too small for this call and the stream is being "
-                                   "captured: size it before the capture (sas_reserve_for, or one eager call "
-                                   "of this shape)");
+                                   "captured: size it before the capture (" + reserve + ", or one eager call of "
+                                   "this shape)");
   size_t bytes = (need + 255) & ~size_t(255);
   if (*cap && bytes < 2 * *cap) bytes = 2 * *cap;
   void *fresh = nullptr;

@@ -48,3 +48,21 @@ def test_smaller_calls_are_captured(rows, vocab, smaller):
                 torch.cuda.synchronize()
                 assert torch.equal(ids, want)
                 v.normal_().mul_(3)
+
+
+def test_a_call_out_of_reserve_names_the_way_out():
+    import torch
+    from shared_amd import SasError
+    v = torch.zeros((4, 30000), device="cuda")
+    u = torch.zeros(4, dtype=torch.float64, device="cuda")
+    ids = torch.zeros(4, dtype=torch.int32, device="cuda")
+    x, w = torch.zeros((4, 64), device="cuda"), torch.zeros((32, 64), dtype=torch.bfloat16, device="cuda")
+    y = torch.zeros((4, 32), device="cuda")
+    with Sampler(0) as s:
+        for call, name in ((lambda: s.sample_filtered_into(v, ids, uniforms=u, params=FilterParams(temperature=1.0)),
+                            "sas_reserve_filtered"), (lambda: s.project_into(x, w, y), "sas_reserve_project")):
+            g = torch.cuda.CUDAGraph()
+            with pytest.raises(SasError, match=name):
+                with torch.cuda.graph(g):
+                    call()
+            torch.cuda.synchronize()
