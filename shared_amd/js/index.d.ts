@@ -356,6 +356,8 @@ export interface FilterParams {
   presencePenalty?: number;
   frequencyPenalty?: number;
   softcap?: number;
+  /** The draw is among these ids (none or empty: all); not beside a mask. */
+  allowedTokenIds?: Uint32Array;
 }
 
 export interface SampleFilteredOptions extends Omit<SampleRowsOptions, 'params'> {

@@ -812,10 +812,11 @@ class Sampler {
   /**
    * One token per row from the whole vocabulary (sas_sample_filtered): opts as
    * sampleRows, but params hold {temperature, topK (0: off, any size), topP,
-   * minP, repetitionPenalty, presencePenalty, frequencyPenalty, softcap}, one
-   * object or one a row, and uniforms are required.  logitsType: 'f32' (the
-   * default), 'bf16' or 'f16' of a DeviceBuffer.  Returns {ids[, probs (the
-   * token's share of the kept mass), counts (ids kept), flags]}.
+   * minP, repetitionPenalty, presencePenalty, frequencyPenalty, softcap,
+   * allowedTokenIds (as sampleRows')}, one object or one a row, and uniforms
+   * are required.  logitsType: 'f32' (the default), 'bf16' or 'f16' of a
+   * DeviceBuffer.  Returns {ids[, probs (the token's share of the kept mass),
+   * counts (ids kept), flags]}.
    */
   sampleFiltered(opts) {
     this._idle('sampleFiltered');
@@ -835,8 +836,11 @@ class Sampler {
     if (opts.mask instanceof Uint32Array && opts.mask.length !== words && opts.mask.length < rows * words) {
       throw new RangeError('mask holds fewer than rows * ceil(vocab / 32) words');
     }
-    // logits, mask, history, uniforms and ids as sampleRows has them
-    const d = this._describe(Object.assign({}, opts, { params: { temperature: 1 }, full: false })).desc;
+    // logits, mask, allowedTokenIds, history, uniforms and ids as sampleRows has them
+    const listed = ps.map(function (p) { return { temperature: 1, allowedTokenIds: p.allowedTokenIds }; });
+    const lists = listed.some(function (p) { return p.allowedTokenIds; });
+    const d = this._describe(Object.assign({}, opts, { params: lists && ps.length > 1 ? listed : listed[0], full: false })).desc;
+    delete d.rowParams;  // (sampleRows' own)
     d.logitsType = ELEMENT_TYPES[type];
     const full = ps.map(function (p) {
       return { temperature: orDefault(p.temperature, 0), topP: orDefault(p.topP, 1), minP: orDefault(p.minP, 0),
