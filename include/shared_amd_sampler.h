@@ -451,7 +451,9 @@ int sas_lm_head_sample_step(sas_sampler *s, const sas_lm_head *head, const sas_r
  * are f32: bf16 products are exact in f32, f32 hidden states and the inner
  * products A x (scaled) are carried as three bf16 pieces, 24 bits in all.
  * A value that is not finite stays in its own row, weight row or adapter.
- * cap(y) = softcap * tanh(y / softcap) in f32 when softcap > 0.
+ * cap(y) = softcap * tanh(y / softcap) in f32 when softcap > 0 (tanh within
+ * 3.2 ulp; sas_params' softcap has it correctly rounded, so the two may differ
+ * in the last bits).
  * No counterpart in the reference, whose head is one row's
  * (lib/webgpu-llm/model.js:466-471). */
 #define SAS_TYPE_F32 0
