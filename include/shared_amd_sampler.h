@@ -450,7 +450,9 @@ int sas_lm_head_sample_step(sas_sampler *s, const sas_lm_head *head, const sas_r
  * what lies behind them is never used, whatever it holds.  Products and sums
  * are f32: bf16 products are exact in f32, f32 hidden states and the inner
  * products A x (scaled) are carried as three bf16 pieces, 24 bits in all.
- * A value that is not finite stays in its own row, weight row or adapter.
+ * A value that is not finite stays in its own row, weight row or adapter; an
+ * infinite weight that meets a piece of zero (f32 hidden states), or an infinite
+ * element of B, makes NaN there.
  * cap(y) = softcap * tanh(y / softcap) in f32 when softcap > 0 (tanh within
  * 3.2 ulp; sas_params' softcap has it correctly rounded, so the two may differ
  * in the last bits).
@@ -495,7 +497,8 @@ typedef struct sas_projection {
 } sas_projection;
 
 /* Stream-ordered on `stream`; no host synchronisation.  out must not overlap
- * an input. */
+ * an input.  As everywhere, a handle must not run two calls concurrently: its
+ * calls share scratch, so the caller orders those on different streams. */
 int sas_project(sas_sampler *s, const sas_projection *p, void *stream);
 
 /* Pre-size the handle's scratch for sas_project calls of at most these rows,
@@ -553,7 +556,8 @@ typedef struct sas_filter_rows {
   uint32_t *out_flags;         /* device [rows] or NULL: SAS_FLAG_EMPTY_ROW */
 } sas_filter_rows;
 
-/* Samples one token per row, stream-ordered like sas_sample. */
+/* Samples one token per row, stream-ordered like sas_sample (calls of a handle
+ * on different streams are ordered by the caller). */
 int sas_sample_filtered(sas_sampler *s, const sas_filter_rows *rows, void *stream);
 
 /* Pre-size the handle's scratch for sas_sample_filtered calls of at most
