@@ -845,19 +845,14 @@ __device__ __forceinline__ uint64_t end_of(const R &row, RowShared &l, int c, In
   }
 }
 
-// The row by what its parts left; false where that does not tell (*top, *n:
-// its best key and its candidates).
-template <int kType, bool kSoft>
-__device__ __forceinline__ bool row_by_parts(Row<kType, kSoft> &R, const FilterArgs &a, RowShared &l, const sas_filter_params &p, const FilterLeft &x, int row,
-                                             uint32_t *top_key, uint64_t *candidates, const Result &done) {
-  const int tid = threadIdx.x;
+// The row's largest key, from its parts' maxima; *candidates: how many there are.
+__device__ __forceinline__ uint32_t row_top(const FilterArgs &a, RowShared &l, int row, uint64_t *candidates) {
   const FilterPart *parts = a.part + (int64_t)row * a.parts;
-  // the best candidate, and how many there are
-  uint64_t best = 0, n = 0, zero = 0;
-  for (int i = tid; i < a.parts; i += kRowThreads) {
+  uint64_t best = 0, n = 0;
+  for (int i = threadIdx.x; i < a.parts; i += kRowThreads) {
     const FilterPart f = parts[i];
     if (f.max > -__builtin_inff()) {
-      best = max(best, (uint64_t)okey(f.max) << 32 | (uint32_t)~f.id);
+      best = max(best, (uint64_t)okey(f.max));
       n += (uint64_t)f.count;
     }
   }
@@ -866,9 +861,9 @@ __device__ __forceinline__ bool row_by_parts(Row<kType, kSoft> &R, const FilterA
     best = max(best, shfl_xor64(best, s));
     n += shfl_xor64(n, s);
   }
-  if ((tid & 63) == 0) {
-    l.red[tid >> 6][0] = best;
-    l.red[tid >> 6][1] = n;
+  if ((threadIdx.x & 63) == 0) {
+    l.red[threadIdx.x >> 6][0] = best;
+    l.red[threadIdx.x >> 6][1] = n;
   }
   __syncthreads();
   n = 0;
@@ -877,146 +872,139 @@ __device__ __forceinline__ bool row_by_parts(Row<kType, kSoft> &R, const FilterA
     best = max(best, (uint64_t)l.red[w][0]);
     n += l.red[w][1];
   }
-  if (best == 0 || greedy_row(p)) {
-    if (tid == 0) done(best ? ~(uint32_t)best : SAS_NO_TOKEN, best ? 1.0 : 0.0, best ? 1 : 0);
-    return true;
-  }
-  const uint32_t top = (uint32_t)(best >> 32);
-  const float m = fkey(top);
-  *top_key = top;
   *candidates = n;
-  R.s = Scale{(double)m, 1.0 / p.temperature, 8.0 / p.temperature, a.shift};
+  return (uint32_t)best;
+}
+
+// A cut row by what its parts left, where the merge planned its ranges (x.planned)
+// and `n` candidates reach down from key `top`; false where that does not tell.
+template <int kType, bool kSoft>
+__device__ __forceinline__ bool row_by_parts(Row<kType, kSoft> &R, const FilterArgs &a, RowShared &l, const sas_filter_params &p, const FilterLeft &x, int row,
+                                             uint32_t top, uint64_t n, const Result &done) {
+  const int tid = threadIdx.x;
+  const FilterPart *parts = a.part + (int64_t)row * a.parts;
+  uint64_t zero = 0;
   const Grid g = grid_of(p.temperature);
-  const float mrange = range_of(m, g);
-  if (!x.planned) return false;
+  const float mrange = range_of(fkey(top), g);
   const bool by_k = p.top_k > 0 && (uint64_t)p.top_k < n, by_p = p.top_p < 1.0, by_min = p.min_p > 0.0;
-  const bool cut = by_k || by_p || by_min;
   // a part's factor to the row's units
   auto scale_of = [&](const FilterPart &f) { return mass_exp(((double)f.top / (double)g.inv_width - R.s.m) * R.s.inv_t); };
   uint64_t all = 0;
   for (int i = tid; i < a.parts; i += kRowThreads) {
     const FilterPart f = parts[i];
-    uint64_t u = 0;
-    if (f.listed >= 0) u = (uint64_t)__builtin_rint(__builtin_amdgcn_ldexp(f.mass * scale_of(f), a.shift));
-    l.part[i] = u;
-    all += u;
+    if (f.listed >= 0) all += (uint64_t)__builtin_rint(__builtin_amdgcn_ldexp(f.mass * scale_of(f), a.shift));
   }
-  zero = 0;
   block_sum2(l, all, zero);
   uint64_t last = 0;      // every id whose (key, ~id) reaches it is kept
-  uint64_t total = all, kept = n;
-  int entries = 0;        // what l.ent holds
   const int log_span = 31 - __builtin_clz(a.span);
-  if (cut) {
-    // the ranges of all parts, in the row's units
-    for (int i = tid; i < kFilterRanges; i += kRowThreads) {
-      l.mass[i] = 0ull;
-      l.cnt[i] = 0u;
-    }
-    __syncthreads();
-    // fn(part, range, count, mass in the row's units) of every range that has ids, four
-    // ranges' loads in flight together
-    auto each_range = [&](auto fn) {
-      for (int i0 = tid; i0 < a.parts * kFilterRanges; i0 += 4 * kRowThreads) {
-        uint32_t c[4];
-        uint64_t w[4];
-        FilterPart f[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int i = min(i0 + k * kRowThreads, a.parts * kFilterRanges - 1);
-          const int64_t at = (int64_t)row * a.parts * kFilterRanges + i;
-          c[k] = a.range_count[at];
-          w[k] = a.range_mass[at];
-          f[k] = parts[i / kFilterRanges];
-        }
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int i = i0 + k * kRowThreads;
-          const int d = (int)mrange - f[k].top + i % kFilterRanges;
-          if (i >= a.parts * kFilterRanges || f[k].listed < 0 || !(f[k].max > -__builtin_inff()) || c[k] == 0u || d >= kFilterRanges) continue;
-          fn(i / kFilterRanges, d, c[k],
-             (uint64_t)__builtin_rint(__builtin_amdgcn_ldexp((double)w[k] * scale_of(f[k]), a.shift - kFilterShift)));
-        }
-      }
-    };
-    each_range([&](int, int d, uint32_t c, uint64_t u) {
-      atomicAdd(&l.cnt[d], c);
-      atomicAdd(&l.mass[d], (unsigned long long)u);
-    });
-    __syncthreads();
-    uint64_t have = 0, havem = 0;
-    for (int i = tid; i < kFilterRanges; i += kRowThreads) {
-      have += l.cnt[i];
-      havem += l.mass[i];
-    }
-    block_sum2(l, have, havem);
-    const uint32_t least = by_min ? least_key(p.min_p, top, R.s) : 0u;
-    // the ids of the planned ranges
-    entries = (int)a.found[row];
-    if (entries > kEntries) return false;
-    for (int i = tid; i < entries; i += kRowThreads) {
-      const uint64_t e = a.ids[(int64_t)row * kEntries + i];
-      l.ent[i] = e;
-      l.entm[i] = units_of(mass_of((uint32_t)(e >> 32), R.s), R.s);
-    }
-    __syncthreads();
-    auto planned = [&](int bin) { return bin < kFilterRanges && ((x.ranges[bin >> 5] >> (bin & 31)) & 1u) != 0u; };
-    auto bin_of_entry = [&](uint64_t e) { return (int)(mrange - range_of(fkey((uint32_t)(e >> 32)), g)); };
-    // the ends of the prefixes of top-k and top-p
-    bool known = true;
-    auto prefix = [&](bool by_count, uint64_t need, uint64_t *mass) {
-      if (need > (by_count ? have : havem)) {
-        known = false;
-        return;
-      }
-      uint64_t m0, c0, m1, c1;
-      const int bin = R.find(kFilterRanges, by_count, need, &m0, &c0);
-      known = planned(bin);
-      if (!known) return;
-      // (the range's mass was rounded as a whole, its ids' one by one)
-      uint64_t sum = 0;
-      zero = 0;
-      for (int i = tid; i < entries; i += kRowThreads) sum += bin_of_entry(l.ent[i]) == bin ? l.entm[i] : 0ull;
-      block_sum2(l, sum, zero);
-      known = sum > 0;
-      if (!known) return;
-      last = max(last, end_of(R, l, entries, [&](uint64_t e) { return bin_of_entry(e) == bin; }, by_count,
-                              by_count ? need - c0 : min(need - m0, sum), &m1, &c1));
-      *mass = m0 + m1;
-    };
-    uint64_t mass = all;
-    if (by_k) prefix(true, (uint64_t)p.top_k, &mass);
-    if (known && by_p) {
-      const uint64_t need = (uint64_t)ceil(fmax(p.top_p, 0.0) * (double)mass);
-      prefix(false, min(max(need, (uint64_t)1), mass), &mass);
-    }
-    if (known && by_min && (uint64_t)least << 32 > last) {
-      last = (uint64_t)least << 32;
-      known = mrange - range_of(fkey(least), g) < (float)kFilterRanges;
-    }
-    if (!known) return false;
-    // what is kept of each part: of the ranges above the end's all, of its own
-    // by its ids
-    const int bin = (int)(mrange - range_of(fkey((uint32_t)(last >> 32)), g));
-    if (!planned(bin)) return false;
-    total = kept = 0;
-    for (int i = tid; i < a.parts; i += kRowThreads) l.part[i] = 0ull;
-    __syncthreads();
-    each_range([&](int part, int d, uint32_t c, uint64_t u) {
-      if (d >= bin) return;
-      total += u;
-      kept += c;
-      atomicAdd(&l.part[part], (unsigned long long)u);
-    });
-    __syncthreads();
-    for (int i = tid; i < entries; i += kRowThreads)
-      if (l.ent[i] >= last && bin_of_entry(l.ent[i]) == bin) {
-        total += l.entm[i];
-        ++kept;
-        atomicAdd(&l.part[~(uint32_t)l.ent[i] >> log_span], l.entm[i]);
-      }
-    block_sum2(l, total, kept);
+  // the ranges of all parts, in the row's units
+  for (int i = tid; i < kFilterRanges; i += kRowThreads) {
+    l.mass[i] = 0ull;
+    l.cnt[i] = 0u;
   }
+  __syncthreads();
+  // fn(part, range, count, mass in the row's units) of every range that has ids, four
+  // ranges' loads in flight together
+  auto each_range = [&](auto fn) {
+    for (int i0 = tid; i0 < a.parts * kFilterRanges; i0 += 4 * kRowThreads) {
+      uint32_t c[4];
+      uint64_t w[4];
+      FilterPart f[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int i = min(i0 + k * kRowThreads, a.parts * kFilterRanges - 1);
+        const int64_t at = (int64_t)row * a.parts * kFilterRanges + i;
+        c[k] = a.range_count[at];
+        w[k] = a.range_mass[at];
+        f[k] = parts[i / kFilterRanges];
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int i = i0 + k * kRowThreads;
+        const int d = (int)mrange - f[k].top + i % kFilterRanges;
+        if (i >= a.parts * kFilterRanges || f[k].listed < 0 || !(f[k].max > -__builtin_inff()) || c[k] == 0u || d >= kFilterRanges) continue;
+        fn(i / kFilterRanges, d, c[k],
+           (uint64_t)__builtin_rint(__builtin_amdgcn_ldexp((double)w[k] * scale_of(f[k]), a.shift - kFilterShift)));
+      }
+    }
+  };
+  each_range([&](int, int d, uint32_t c, uint64_t u) {
+    atomicAdd(&l.cnt[d], c);
+    atomicAdd(&l.mass[d], (unsigned long long)u);
+  });
+  __syncthreads();
+  uint64_t have = 0, havem = 0;
+  for (int i = tid; i < kFilterRanges; i += kRowThreads) {
+    have += l.cnt[i];
+    havem += l.mass[i];
+  }
+  block_sum2(l, have, havem);
+  const uint32_t least = by_min ? least_key(p.min_p, top, R.s) : 0u;
+  // the ids of the planned ranges
+  const int entries = (int)a.found[row];
+  if (entries > kEntries) return false;
+  for (int i = tid; i < entries; i += kRowThreads) {
+    const uint64_t e = a.ids[(int64_t)row * kEntries + i];
+    l.ent[i] = e;
+    l.entm[i] = units_of(mass_of((uint32_t)(e >> 32), R.s), R.s);
+  }
+  __syncthreads();
+  auto planned = [&](int bin) { return bin < kFilterRanges && ((x.ranges[bin >> 5] >> (bin & 31)) & 1u) != 0u; };
+  auto bin_of_entry = [&](uint64_t e) { return (int)(mrange - range_of(fkey((uint32_t)(e >> 32)), g)); };
+  // the ends of the prefixes of top-k and top-p
+  bool known = true;
+  auto prefix = [&](bool by_count, uint64_t need, uint64_t *mass) {
+    if (need > (by_count ? have : havem)) {
+      known = false;
+      return;
+    }
+    uint64_t m0, c0, m1, c1;
+    const int bin = R.find(kFilterRanges, by_count, need, &m0, &c0);
+    known = planned(bin);
+    if (!known) return;
+    // (the range's mass was rounded as a whole, its ids' one by one)
+    uint64_t sum = 0;
+    zero = 0;
+    for (int i = tid; i < entries; i += kRowThreads) sum += bin_of_entry(l.ent[i]) == bin ? l.entm[i] : 0ull;
+    block_sum2(l, sum, zero);
+    known = sum > 0;
+    if (!known) return;
+    last = max(last, end_of(R, l, entries, [&](uint64_t e) { return bin_of_entry(e) == bin; }, by_count,
+                            by_count ? need - c0 : min(need - m0, sum), &m1, &c1));
+    *mass = m0 + m1;
+  };
+  uint64_t mass = all;
+  if (by_k) prefix(true, (uint64_t)p.top_k, &mass);
+  if (known && by_p) {
+    const uint64_t need = (uint64_t)ceil(fmax(p.top_p, 0.0) * (double)mass);
+    prefix(false, min(max(need, (uint64_t)1), mass), &mass);
+  }
+  if (known && by_min && (uint64_t)least << 32 > last) {
+    last = (uint64_t)least << 32;
+    known = mrange - range_of(fkey(least), g) < (float)kFilterRanges;
+  }
+  if (!known) return false;
+  // what is kept of each part: of the ranges above the end's all, of its own
+  // by its ids
+  const int bin = (int)(mrange - range_of(fkey((uint32_t)(last >> 32)), g));
+  if (!planned(bin)) return false;
+  uint64_t total = 0, kept = 0;
+  for (int i = tid; i < a.parts; i += kRowThreads) l.part[i] = 0ull;
+  __syncthreads();
+  each_range([&](int part, int d, uint32_t c, uint64_t u) {
+    if (d >= bin) return;
+    total += u;
+    kept += c;
+    atomicAdd(&l.part[part], (unsigned long long)u);
+  });
+  __syncthreads();
+  for (int i = tid; i < entries; i += kRowThreads)
+    if (l.ent[i] >= last && bin_of_entry(l.ent[i]) == bin) {
+      total += l.entm[i];
+      ++kept;
+      atomicAdd(&l.part[~(uint32_t)l.ent[i] >> log_span], l.entm[i]);
+    }
+  block_sum2(l, total, kept);
   // the draw: the part, then the id
   uint64_t goal = (uint64_t)fmax(a.uniforms[row] * (double)total, 0.0), before;
   goal = min(goal, total - 1);
@@ -1055,7 +1043,7 @@ __device__ __forceinline__ bool row_by_parts(Row<kType, kSoft> &R, const FilterA
   return true;
 }
 
-// The rows that the merge left.
+// The rows that the merge left: each has a candidate, and none is greedy.
 template <int kType, bool kSoft>
 __global__ __launch_bounds__(kRowThreads) void filter_rest_kernel(const FilterArgs a) {
   __shared__ RowShared l;
@@ -1066,9 +1054,11 @@ __global__ __launch_bounds__(kRowThreads) void filter_rest_kernel(const FilterAr
   Row<kType, kSoft> R{a, l, p, (int64_t)row * a.logits_stride, a.mask ? a.mask + (int64_t)row * a.mask_stride : nullptr,
                       history_of(a, row), Scale{}};
   const Result done{a, row};
-  uint32_t top = 0;
-  uint64_t n = 0;
-  if (!row_by_parts<kType, kSoft>(R, a, l, p, x, row, &top, &n, done)) row_by_values<kType, kSoft>(R, a, l, p, row, top, n, done);
+  uint64_t n;
+  const uint32_t top = row_top(a, l, row, &n);
+  R.s = Scale{(double)fkey(top), 1.0 / p.temperature, 8.0 / p.temperature, a.shift};
+  if (!x.planned || !row_by_parts<kType, kSoft>(R, a, l, p, x, row, top, n, done))
+    row_by_values<kType, kSoft>(R, a, l, p, row, top, n, done);
 }
 
 // ----------------------------------------------------------------- merge --
