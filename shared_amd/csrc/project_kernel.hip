@@ -764,7 +764,15 @@ void launch_rows(const ProjArgs &a, hipStream_t stream) {
   const int subs = (a.rows + kSub - 1) / kSub;
   // subtiles a tile of the wide kernel: as few tiles as 8 allow, evenly
   const int tiles = (subs + 7) / 8, mt = (subs + tiles - 1) / tiles;
-  if ((int64_t)tiles * ((a.out_dim + 255) / 256) >= a.cus) {
+  // The wide kernel takes few, long blocks: from 3/8 of a tile of 256 outputs a CU
+  // on (up to 32 bf16 rows: from one).  Over 1,826 shapes (1 to 4,096 rows, 512 to
+  // 80,000 outputs of 512 to 8,192 values) that is 2 % off the faster kernel in the
+  // mean, 2.1 times at worst; one tile a CU for all was 8 %, and 9.4 times at worst.
+  // bf16 rows x 4,096 values, wide / split: 64 rows x 11,007 (43 tiles) 55 / 47 us,
+  // 512 x 4,096 (64) 67 / 88, 512 x 8,192 (128) 68 / 170, 1,920 x 4,096 (240) 76 / 334;
+  // 16 x 32,768 (128) 52 / 49, 16 x 65,536 (256) 96 / 130.
+  const bool few = P == 1 && subs <= 2;
+  if ((int64_t)tiles * ((a.out_dim + 255) / 256) * 8 >= (int64_t)a.cus * (few ? 8 : 3)) {
     switch (mt) {
       case 1: return launch_wide<1, 1, P>(a, stream);
       case 2: return launch_wide<2, 1, P>(a, stream);
