@@ -139,8 +139,8 @@ constexpr float kFar = 4194304.0f;
 // that counts for nothing in its row, so a row's largest value has to lie 2,048
 // ranges above: 128 T at least, masses below 2^-184.
 constexpr float kNear = 2048.0f - kFar;
-// A part's ranges sum masses as integers of 2^-kFilterShift: 8,192 of at most
-// e^(1/8) stay below 2^64.
+// A part's ranges sum masses as integers of 2^-kFilterShift: 8,192 of at most 1
+// stay below 2^64.
 constexpr double kUnit = (double)(1ull << kFilterShift);
 
 // Masses are powers of two counted in 256ths of an octave.  2^(j / 256), j = 0
@@ -261,9 +261,9 @@ __global__ __launch_bounds__(kT) void filter_parts_kernel(const FilterArgs a) {
   const float top = range_of(m, g);
   const bool greedy = greedy_row(p), ranged = !greedy && g.plain && fabsf(top) < kFar && m > neg;
   const bool list = ranged && filters(p);
-  // Masses are relative to the lower edge of max's range.  (The edge's place is
-  // rounded as 256ths of an octave; the merge's arithmetic rounds it alike.)
-  const double ref = (double)top / (double)g.inv_width * g.per;
+  // Masses are relative to the part's largest value: the difference is exact, so
+  // equal values weigh exactly 1, and n of them exactly n.
+  const double md = (double)m;
   double sum[4] = {0.0, 0.0, 0.0, 0.0};
   uint32_t n = 0, best = ~0u;
 #pragma unroll
@@ -284,7 +284,7 @@ __global__ __launch_bounds__(kT) void filter_parts_kernel(const FilterArgs a) {
       double u[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        u[i] = exp256(fmax(fma((double)v[j][i], g.per, -ref), kLeast), tab);
+        u[i] = exp256(fmax(((double)v[j][i] - md) * g.per, kLeast), tab);
         sum[i] += u[i];
       }
       if (fmaxf(fmaxf(v[j][0], v[j][1]), fmaxf(v[j][2], v[j][3])) >= hot) {
@@ -888,7 +888,7 @@ __device__ __forceinline__ bool row_by_parts(Row<kType, kSoft> &R, const FilterA
   const float mrange = range_of(fkey(top), g);
   const bool by_k = p.top_k > 0 && (uint64_t)p.top_k < n, by_p = p.top_p < 1.0, by_min = p.min_p > 0.0;
   // a part's factor to the row's units
-  auto scale_of = [&](const FilterPart &f) { return mass_exp(((double)f.top / (double)g.inv_width - R.s.m) * R.s.inv_t); };
+  auto scale_of = [&](const FilterPart &f) { return mass_of(okey(f.max), R.s); };
   uint64_t all = 0;
   for (int i = tid; i < a.parts; i += kRowThreads) {
     const FilterPart f = parts[i];
@@ -1169,10 +1169,9 @@ __global__ __launch_bounds__(kThreads) void filter_merge_kernel(const FilterArgs
   const Grid g = grid_of(p.temperature);
   const float mrange = range_of(fkey(top), g);
   if (!g.plain || !(mrange >= kNear && mrange < kFar)) return leave();
-  // the mass of a value, and of a part's reference
-  const double m = (double)fkey(top) * g.per;
-  auto mass_at = [&](double v) { return exp256(fmax(fma(v, g.per, -m), kLeast), l.tab); };
-  auto mass_of_ref = [&](int t) { return exp256(fmax((double)t / (double)g.inv_width * g.per - m, kLeast), l.tab); };
+  // the mass of a value (of a part's largest: what its own masses count in)
+  const double m = (double)fkey(top);
+  auto mass_at = [&](double v) { return exp256(fmax((v - m) * g.per, kLeast), l.tab); };
   auto units = [&](double mass) { return (uint64_t)__builtin_rint(__builtin_amdgcn_ldexp(mass, a.shift)); };
   const bool by_k = p.top_k > 0 && (uint64_t)p.top_k < n, by_p = p.top_p < 1.0, by_min = p.min_p > 0.0;
   const bool cut = by_k || by_p || by_min;
@@ -1183,7 +1182,7 @@ __global__ __launch_bounds__(kThreads) void filter_merge_kernel(const FilterArgs
   for (int i = tid; i < a.parts; i += kThreads) {
     const FilterPart f = parts[i];
     const bool none = f.listed < 0 || (!cut && units(mass_at((double)f.max)) == 0ull);
-    const uint64_t u = none ? 0ull : units(f.mass * mass_of_ref(f.top));
+    const uint64_t u = none ? 0ull : units(f.mass * mass_at((double)f.max));
     l.part[i] = cut ? 0ull : u;
     all += u;
   }
@@ -1305,7 +1304,7 @@ __global__ __launch_bounds__(kThreads) void filter_merge_kernel(const FilterArgs
         const int d = (int)mrange - f.top + i % kFilterRanges;
         if (f.listed < 0 || !(f.max > -__builtin_inff()) || c == 0u || d >= kFilterRanges) continue;
         atomicAdd(&l.cnt[d], c);
-        atomicAdd(&l.mass[d], (unsigned long long)__builtin_rint(__builtin_amdgcn_ldexp((double)w * mass_of_ref(f.top), a.shift - kFilterShift)));
+        atomicAdd(&l.mass[d], (unsigned long long)__builtin_rint(__builtin_amdgcn_ldexp((double)w * mass_at((double)f.max), a.shift - kFilterShift)));
       }
       __syncthreads();
       if (wave > 0) return;

@@ -278,7 +278,7 @@ struct FilterPart {
   int32_t listed;   // ids in the list, -1: the part's values are out of the ranges' scope
   float edge;       // every candidate of at least this value is listed
   int32_t top;      // the range of max: floor(max / width)
-  double mass;      // of all candidates, relative to e^(top width / T), the range's lower edge
+  double mass;      // of all candidates, relative to max's
 };
 // A row left: by the ids of these of its ranges (planned), or by its values.
 struct FilterLeft {
