@@ -538,8 +538,10 @@ class Sampler:
 
     def project(self, x, weight, *, out_dtype=None, stream=None, **kw):
         """Allocate out (float32 unless out_dtype is torch.bfloat16) and run
-        project_into; returns it."""
+        project_into; returns it.  A fresh out holds nothing to accumulate on."""
         import torch
+        if weight is None or kw.get("accumulate"):
+            raise ValueError("project needs a weight and cannot accumulate: its out is new (project_into takes one)")
         with _on(stream):
             out = torch.empty((x.shape[0], weight.shape[0]), dtype=out_dtype or torch.float32, device=x.device)
         self.project_into(x, weight, out, stream=stream, **kw)
