@@ -15,17 +15,22 @@
 //   1. filter_parts_kernel, a block a part (8,192 ids, fewer in small batches):
 //      reads the logits once; leaves the part's largest value, its mass, the
 //      masses and counts of 128 ranges below its largest value, and its best
-//      ids.  Bound by the double exponentials (16 instructions a value) and, in
-//      rows that are cut, by a block's chain of barriers: 256 rows x 262,144
-//      f32, nothing cut, 79 us (3.4 TB/s); 128 rows under a grammar 66 us.
+//      ids.  Bound by the issue of vector instructions: 256 rows x 262,144 f32,
+//      nothing cut, 78 us (3.4 TB/s), 41 an id, 13 of them double, 88 % of what
+//      the units issue (the LDS that holds the exponential's table is busy 18 %
+//      of the time, half of it conflicts); 128 rows under a grammar 67 us, 69 an
+//      id, 83 %; 64 bf16 rows x 151,936 with min-p 26 us, 71 an id, 57 %, the
+//      rest waits of 2.4 blocks a CU.
 //   2. filter_merge_kernel, four waves a row: the ends of the prefixes among
 //      the lists' ids, kept in registers, and the draw; 10 to 30 us, a chain of
 //      dependent steps.  (One kernel of 1,024 threads for every row: 24 to 30.)
 //   3. filter_gather_kernel, the whole chip: the ids of the ranges in which the
 //      ends lie, for rows whose lists do not reach them (wide nuclei).
-//   4. filter_rest_kernel, a block a row left: the ends among those ids, 33 to
-//      52 us; or, for values out of the ranges' scope, by rereading the row.
-//      Launches 3 and 4 end at once where no row was left (4 us together).
+//   4. filter_rest_kernel, a block a row left: the ends among those ids, 34 to
+//      54 us; or by rereading the row, where a value is out of the ranges' scope,
+//      an end lies below the 128 ranges (8 to 16 T) or its ranges hold more than
+//      4,096 ids: 0.5 ms at 151,936 ids, 0.95 at 262,144, 1.5 with two ends.
+//      Launches 3 and 4 end at once where no row was left (4 to 9 us together).
 #include <algorithm>
 
 #include "sas_device.h"
@@ -149,10 +154,10 @@ constexpr int kTab = 256;
 __device__ __forceinline__ void fill_tab(double *tab) {
   if (threadIdx.x < kTab) tab[threadIdx.x] = exp2((double)threadIdx.x * (1.0 / 256.0));
 }
-// 2^(y / 256), -32768 <= y <= 256: the table's 2^(k / 256) times a Taylor series
+// 2^(y / 256), -32768 <= y <= 0: the table's 2^(k / 256) times a Taylor series
 // in |r| <= 1/2 (2^(r / 256) to degree 4, 4e-17 short), the exponent added as
-// an integer; within 3 ulp.  14 instructions a value, most of what the parts
-// kernel computes.
+// an integer; within 3 ulp of y's.  14 instructions a value, a third of what the
+// parts kernel issues where nothing is cut.
 __device__ __forceinline__ double exp256(double y, const double *tab) {
   const double magic = 6755399441055744.0;
   const double kf = y + magic;

@@ -19,13 +19,13 @@
 // What bounds it, and what it measured (MI355X, a call):
 //   - up to about 128 rows W's stream from memory: 16 f32 rows x 2,560 x
 //     151,936 160 us (5.0 TB/s), 128 rows x 2,560 x 262,144, capped, 16
-//     adapters, 364 us (4.4 TB/s; 320 without adapters, 235 of it without the
+//     adapters, 355 to 368 us (4.4 TB/s; 320 without adapters, 235 of it without the
 //     134 MB of results).  What carried it: weight rows in whole lines,
 //     nontemporal; loads kept several runs ahead of their use against the
 //     compiler's order; results in whole lines past the caches.
 //   - more rows the matrix instructions' operands in LDS, each wave reading all
-//     of a tile's hidden states: 2,048 x 4,096 x 4,096 97 us (0.72 PFLOP/s, the
-//     product 86 us of it; a library's 60), 200 f32 rows x 2,048 x 50,257 209
+//     of a tile's hidden states: 2,048 x 4,096 x 4,096 98 us (0.71 PFLOP/s, the
+//     product 89 us of it; a library's 60), 200 f32 rows x 2,048 x 50,257 209
 //     us (three products each: 0.6 PFLOP/s).
 //   - an adapter a row (61 rows, ranks up to 64, 4,096 x 11,007: 115 us) the
 //     addresses of B's and h's loads, 16 bytes a lane.

@@ -360,7 +360,7 @@ export interface FilterParams {
   allowedTokenIds?: Uint32Array;
 }
 
-export interface SampleFilteredOptions extends Omit<SampleRowsOptions, 'params'> {
+export interface SampleFilteredOptions extends Omit<SampleRowsOptions, 'params' | 'defaults' | 'iteration'> {
   params: FilterParams | FilterParams[];
   uniforms: Float64Array;
   logitsType?: 'f32' | 'bf16' | 'f16';
