@@ -20,7 +20,7 @@
 //      the units issue (the LDS that holds the exponential's table is busy 18 %
 //      of the time, half of it conflicts); 128 rows under a grammar 67 us, 69 an
 //      id, 83 %; 64 bf16 rows x 151,936 with min-p 26 us, 71 an id, 57 %, the
-//      rest waits of 2.4 blocks a CU.
+//      rest waits of 4.75 blocks a CU.
 //   2. filter_merge_kernel, four waves a row: the ends of the prefixes among
 //      the lists' ids, kept in registers, and the draw; 10 to 30 us, a chain of
 //      dependent steps.  (One kernel of 1,024 threads for every row: 24 to 30.)
