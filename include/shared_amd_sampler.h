@@ -493,7 +493,7 @@ typedef struct sas_projection {
   int64_t out_stride;         /* elements: >= out_dim */
   int32_t out_type;           /* SAS_TYPE_F32 or SAS_TYPE_BF16 (rounded once, to nearest even) */
   int32_t accumulate;         /* nonzero: y is added to what out holds (before the cap) */
-  float softcap;              /* 0 = off */
+  float softcap;              /* 0 = off, else a positive normal number */
 } sas_projection;
 
 /* Stream-ordered on `stream`; no host synchronisation.  out must not overlap

@@ -6,6 +6,7 @@
 #include <cmath>
 #include <cstdint>
 #include <exception>
+#include <limits>
 #include <string>
 
 #include "sas_handle.h"
@@ -44,6 +45,8 @@ const char *check_projection(const sas_projection *p) {
   if (p->adapters < 0) return "adapters must be >= 0";
   if (!p->weight && !p->accumulate) return "weight may be NULL only with accumulate";
   if (p->softcap < 0.0f || !std::isfinite(p->softcap)) return "softcap must be finite and >= 0";
+  // (its reciprocal has to be finite)
+  if (p->softcap > 0.0f && p->softcap < std::numeric_limits<float>::min()) return "softcap must be 0 or a normal number";
   if (p->adapters > 0 && (p->rank < 8 || p->rank > SAS_MAX_RANK || p->rank % 8 != 0))
     return "rank must be a multiple of 8 in [8, SAS_MAX_RANK]";
   // (a block an output tile of 16 x 16 at most)

@@ -3,6 +3,8 @@ place."""
 import numpy as np
 import pytest
 
+from shared_amd import SasError
+
 pytestmark = pytest.mark.gpu
 
 
@@ -46,6 +48,15 @@ def test_ends(sampler):
     got = capped(sampler, x, 30.0)
     assert np.array_equal(got[:2], [0, 0]) and np.array_equal(got[2:4], [30, -30]) and np.array_equal(got[6:8], [30, -30])
     assert np.isnan(capped(sampler, np.array([np.nan], np.float32), 30.0)).all()
+
+
+def test_least_cap(sampler):
+    # 1 / cap is finite from the smallest normal number on; below it 0 gave NaN
+    least = float(np.finfo(np.float32).tiny)
+    got = capped(sampler, np.array([0.0, 1.0, -1e30], np.float32), least)
+    assert np.array_equal(got, np.array([0.0, least, -least], np.float32))
+    with pytest.raises(SasError, match="softcap"):
+        capped(sampler, np.zeros(1, np.float32), least / 2)
 
 
 def test_cap_of_thirty(sampler):
