@@ -412,17 +412,24 @@ int sas_spec_step(sas_sampler *s, const sas_spec_rows *r, const sas_spec_state *
 #define SAS_HEAD_Q8_0 1
 #define SAS_HEAD_Q4_0 2
 #define SAS_HEAD_Q6_K 3
+/* SAS_HEAD_MX4: the table of sas_mx4 below (codes and scales).  The logits are
+ * sas_project_mx4's of f32 hidden states: every bit of them is kept, the sums
+ * are f32 in an order of the kernel's own (fixed for a shape). */
+#define SAS_HEAD_MX4 4
 
 typedef struct sas_lm_head {
   const float *hidden;        /* device [rows][hidden_stride] fp32: final-normed hidden states */
   int64_t hidden_stride;      /* >= dim */
-  const void *weight;         /* device [vocab] rows, 16-byte aligned: bf16 bits, or GGUF blocks */
+  const void *weight;         /* device [vocab] rows, 16-byte aligned: bf16 bits, GGUF blocks, or
+                                 MX4 codes */
   int64_t weight_stride;      /* between rows: elements (bf16: >= dim, a multiple of 8) or bytes
                                  (GGUF: >= the row's bytes; Q8_0 / Q4_0 a multiple of 4,
-                                 Q6_K of 2) */
+                                 Q6_K of 2; MX4: as codes_stride of sas_mx4) */
   int32_t dim;                /* a multiple of 256; rows * dim <= SAS_LMH_MAX_LDS_FLOATS */
   float *out_logits;          /* device [rows][vocab] or NULL: also write the logits */
   int32_t format;             /* SAS_HEAD_* (0: bf16) */
+  const void *scales;         /* MX4 alone (the other formats never read it): scales of sas_mx4 */
+  int64_t scales_stride;      /* MX4 alone: scales_stride of sas_mx4 */
 } sas_lm_head;
 
 /* Samples rows->rows rows (<= SAS_LMH_MAX_ROWS, vocab <= SAS_LMH_MAX_VOCAB)
@@ -505,6 +512,87 @@ int sas_project(sas_sampler *s, const sas_projection *p, void *stream);
  * dim and rank (rank 0: without adapters), so that they allocate nothing and
  * can be captured into a HIP graph. */
 int sas_reserve_project(sas_sampler *s, int32_t rows, int32_t dim, int32_t rank);
+
+/* ---- values in microscaled 4-bit floating point (MXFP4) ----
+ *
+ * A row's values in blocks of 32 (the last one may be cut short by dim), as
+ * the OCP Microscaling Formats specification 1.0 has them: an element is a sign,
+ * two bits of exponent and one of mantissa (0 0.5 1 1.5 2 3 4 6), a block has a
+ * scale 2^(s - 127), s a byte, and a value is their product; s = 255 makes the
+ * whole block NaN, and 253 and 254 values that may pass f32's range.  Codes
+ * lie 16 bytes a block, the first of a byte's two values in its low half, and
+ * codes past dim in a row's last block are 0.  A table of them is a head that
+ * takes 0.53 bytes a value, the embeddings of a tied one, or the hidden states
+ * of a batch, whose products then run on the 4-bit matrix instructions.
+ * No counterpart in the reference, whose 4-bit heads are GGUF blocks. */
+#define SAS_MX4_BLOCK 32
+#define SAS_TYPE_MX4 3
+/* Largest codes_stride and scales_stride. */
+#define SAS_MAX_MX4_STRIDE (1 << 24)
+
+typedef struct sas_mx4 {
+  void *codes;                /* device [rows][codes_stride], 16-byte aligned */
+  int64_t codes_stride;       /* bytes: >= 16 ceil(dim / 32), a multiple of 16 */
+  void *scales;               /* device [rows][scales_stride], 4-byte aligned */
+  int64_t scales_stride;      /* bytes: >= ceil(dim / 32), a multiple of 4 */
+} sas_mx4;
+
+/* Rounds rows to MXFP4.  A block's scale is 2^(floor(log2 max |x|) - 2), at
+ * least 2^-127 (also where every x is 0); x / scale is rounded to the nearest
+ * element, ties to the even one, and past 6 to 6.  A block that holds NaN or an
+ * infinity becomes NaN (s = 255, codes 0).  Every byte of the rows' blocks is
+ * written, codes past dim 0, and so are the scale bytes that pad a row to a
+ * multiple of four; nothing behind them. */
+typedef struct sas_mx4_quantization {
+  const void *x;              /* device [rows][x_stride], aligned to its elements */
+  int64_t x_stride;           /* elements between rows, >= dim */
+  int32_t x_type;             /* SAS_TYPE_F32, SAS_TYPE_BF16 or SAS_TYPE_F16 */
+  int32_t rows;               /* >= 0; rows * ceil(dim / 128) below 2^31 */
+  int32_t dim;                /* >= 1 */
+  sas_mx4 out;
+} sas_mx4_quantization;
+
+/* Reads rows of a table: out[i] = table[ids[i]].  An id past the table (a
+ * stopped row's SAS_STOP_PAD, SAS_NO_TOKEN) gives zeros. */
+typedef struct sas_mx4_lookup {
+  sas_mx4 table;
+  int32_t table_rows;         /* >= 0 */
+  int32_t dim;                /* >= 1 */
+  const uint32_t *ids;        /* device [rows], or NULL: the rows in order */
+  int32_t rows;               /* >= 0 (without ids <= table_rows); rows * ceil(dim / 128) below 2^31 */
+  void *out;                  /* device [rows][out_stride], aligned to its elements */
+  int64_t out_stride;         /* elements: >= dim */
+  int32_t out_type;           /* SAS_TYPE_F32, SAS_TYPE_BF16 (both exact) or SAS_TYPE_F16 (rounded,
+                                 to nearest even) */
+} sas_mx4_lookup;
+
+/* y[r] = cap(W x[r]), W a table: with f32 hidden states (carried as three bf16
+ * pieces, 24 bits in all), bf16, or rows of MXFP4 themselves.  Products are
+ * exact, sums are f32.  accumulate, softcap and out are sas_project's, whose
+ * adapters' terms can be added behind it (its weight NULL).  A value that is
+ * not finite stays in its row or weight row. */
+typedef struct sas_mx4_projection {
+  const void *x;              /* SAS_TYPE_F32, _BF16: device [rows][x_stride], 16-byte aligned */
+  int64_t x_stride;           /* elements between rows: >= dim, a multiple of 8 (f32: of 4) */
+  sas_mx4 x4;                 /* SAS_TYPE_MX4: the hidden states (x is unused) */
+  int32_t x_type;             /* SAS_TYPE_F32, SAS_TYPE_BF16 or SAS_TYPE_MX4 */
+  int32_t rows;               /* >= 0, <= SAS_MAX_PROJECT_ROWS */
+  sas_mx4 weight;             /* out_dim rows */
+  int32_t dim;                /* >= 1; f32 and bf16 hidden states: a multiple of 8 */
+  int32_t out_dim;            /* >= 1 */
+  void *out;                  /* device [rows][out_stride], aligned to its elements */
+  int64_t out_stride;         /* elements: >= out_dim */
+  int32_t out_type;           /* SAS_TYPE_F32 or SAS_TYPE_BF16 (rounded once, to nearest even) */
+  int32_t accumulate;         /* nonzero: y is added to what out holds (before the cap) */
+  float softcap;              /* 0 = off, else a positive normal number */
+} sas_mx4_projection;
+
+/* Stream-ordered on `stream`; no host synchronisation, no scratch, so that any
+ * of them can be captured without a reservation.  Outputs must not overlap an
+ * input. */
+int sas_quantize_mx4(sas_sampler *s, const sas_mx4_quantization *q, void *stream);
+int sas_lookup_mx4(sas_sampler *s, const sas_mx4_lookup *l, void *stream);
+int sas_project_mx4(sas_sampler *s, const sas_mx4_projection *p, void *stream);
 
 /* ---- sampling over the whole vocabulary: top-k, top-p, min-p ----
  *

@@ -39,9 +39,9 @@ STOP_PAD = 0xFFFFFFFF
 OK, ERR_INVALID, ERR_HIP, ERR_NOMEM = 0, 1, 2, 3
 FLAG_EMPTY_ROW, FLAG_TOPP_EDGE, FLAG_DRAW_EDGE, FLAG_SLOW_SELECT = 1, 2, 4, 8
 HINT_NO_SOFTCAP = 1
-HEAD_BF16, HEAD_Q8_0, HEAD_Q4_0, HEAD_Q6_K = 0, 1, 2, 3
+HEAD_BF16, HEAD_Q8_0, HEAD_Q4_0, HEAD_Q6_K, HEAD_MX4 = 0, 1, 2, 3, 4
 MASK_ALL, MASK_ALLOW, MASK_DENY = 0, 1, 2
-TYPE_F32, TYPE_BF16, TYPE_F16 = 0, 1, 2
+TYPE_F32, TYPE_BF16, TYPE_F16, TYPE_MX4 = 0, 1, 2, 3
 MAX_RANK = _header_define("SAS_MAX_RANK")
 MAX_PROJECT_ROWS = _header_define("SAS_MAX_PROJECT_ROWS")
 
@@ -169,6 +169,8 @@ class SasLmHead(ctypes.Structure):
         ("dim", c_int32),
         ("out_logits", c_void_p),
         ("format", c_int32),
+        ("scales", c_void_p),
+        ("scales_stride", c_int64),
     ]
 
 
@@ -193,6 +195,57 @@ class SasProjection(ctypes.Structure):
         ("scales", c_void_p),
         ("ranks", c_void_p),
         ("row_adapter", c_void_p),
+        ("out", c_void_p),
+        ("out_stride", c_int64),
+        ("out_type", c_int32),
+        ("accumulate", c_int32),
+        ("softcap", c_float),
+    ]
+
+
+class SasMx4(ctypes.Structure):
+    _fields_ = [
+        ("codes", c_void_p),
+        ("codes_stride", c_int64),
+        ("scales", c_void_p),
+        ("scales_stride", c_int64),
+    ]
+
+
+class SasMx4Quantization(ctypes.Structure):
+    _fields_ = [
+        ("x", c_void_p),
+        ("x_stride", c_int64),
+        ("x_type", c_int32),
+        ("rows", c_int32),
+        ("dim", c_int32),
+        ("out", SasMx4),
+    ]
+
+
+class SasMx4Lookup(ctypes.Structure):
+    _fields_ = [
+        ("table", SasMx4),
+        ("table_rows", c_int32),
+        ("dim", c_int32),
+        ("ids", c_void_p),
+        ("rows", c_int32),
+        ("out", c_void_p),
+        ("out_stride", c_int64),
+        ("out_type", c_int32),
+    ]
+
+
+class SasMx4Projection(ctypes.Structure):
+    _fields_ = [
+        ("x", c_void_p),
+        ("x_stride", c_int64),
+        ("x4", SasMx4),
+        ("x_type", c_int32),
+        ("rows", c_int32),
+        ("weight", SasMx4),
+        ("dim", c_int32),
+        ("out_dim", c_int32),
         ("out", c_void_p),
         ("out_stride", c_int64),
         ("out_type", c_int32),
@@ -254,6 +307,9 @@ SIGNATURES = {
     "sas_lm_head_sample_step": (c_int, [c_void_p, POINTER(SasLmHead), POINTER(SasRows), POINTER(SasStep), c_void_p]),
     "sas_project": (c_int, [c_void_p, POINTER(SasProjection), c_void_p]),
     "sas_reserve_project": (c_int, [c_void_p, c_int32, c_int32, c_int32]),
+    "sas_quantize_mx4": (c_int, [c_void_p, POINTER(SasMx4Quantization), c_void_p]),
+    "sas_lookup_mx4": (c_int, [c_void_p, POINTER(SasMx4Lookup), c_void_p]),
+    "sas_project_mx4": (c_int, [c_void_p, POINTER(SasMx4Projection), c_void_p]),
     "sas_sample_filtered": (c_int, [c_void_p, POINTER(SasFilterRows), c_void_p]),
     "sas_reserve_filtered": (c_int, [c_void_p, c_int32, c_int32]),
     "sas_clamp_params": (c_int, [POINTER(SasParams), POINTER(SasParams)]),

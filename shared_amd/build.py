@@ -22,7 +22,7 @@ LIB = os.path.join(PKG, "libshared_amd_sampler.so")
 NAPI = os.path.join(PKG, "js", "sas_napi.node")
 PROBE = os.path.join(PKG, "libsas_probe.so")
 HIP_SOURCES = ["capi.hip", "sample_kernel.hip", "verify_kernel.hip", "lmhead_kernel.hip", "decode_api.hip",
-               "project_kernel.hip", "filter_kernel.hip"]
+               "project_kernel.hip", "filter_kernel.hip", "mx4_api.hip", "mx4_kernel.hip"]
 PROBE_SOURCES = ["probe_kernel.hip"]
 
 # -ffp-contract=off: the double-precision tail must round like a JS engine.

@@ -262,7 +262,7 @@ int lm_head_on(sas_sampler *s, const sas_lm_head *h, const sas_rows *r, const sa
     if (const char *m = check_step(r, st)) return fail(s, SAS_ERR_INVALID, w + ": " + m);
   if (r->rows > SAS_LMH_MAX_ROWS) return fail(s, SAS_ERR_INVALID, w + ": rows must be <= SAS_LMH_MAX_ROWS");
   if (r->vocab > SAS_LMH_MAX_VOCAB) return fail(s, SAS_ERR_INVALID, w + ": vocab must be <= SAS_LMH_MAX_VOCAB");
-  if (h->format < SAS_HEAD_BF16 || h->format > SAS_HEAD_Q6_K)
+  if (h->format < SAS_HEAD_BF16 || h->format > SAS_HEAD_MX4)
     return fail(s, SAS_ERR_INVALID, w + ": format must be one of SAS_HEAD_*");
   if (r->rows == 0) return SAS_OK;
   if (!h->hidden || !h->weight) return fail(s, SAS_ERR_INVALID, w + ": hidden and weight are required");
@@ -273,6 +273,10 @@ int lm_head_on(sas_sampler *s, const sas_lm_head *h, const sas_rows *r, const sa
   if (h->format == SAS_HEAD_BF16) {
     if (h->weight_stride < h->dim || h->weight_stride % 8 != 0)
       return fail(s, SAS_ERR_INVALID, w + ": weight_stride must be >= dim and a multiple of 8");
+  } else if (h->format == SAS_HEAD_MX4) {
+    if (!h->scales) return fail(s, SAS_ERR_INVALID, w + ": an MX4 head needs its scales");
+    if (const char *m = sas::check_mx4(h->weight, h->weight_stride, h->scales, h->scales_stride, h->dim))
+      return fail(s, SAS_ERR_INVALID, w + ": " + m);
   } else {
     const int64_t rb = head_row_bytes(h->format, h->dim);
     if (h->weight_stride < rb || h->weight_stride % (h->format == SAS_HEAD_Q6_K ? 2 : 4) != 0)
@@ -307,6 +311,11 @@ int lm_head_on(sas_sampler *s, const sas_lm_head *h, const sas_rows *r, const sa
   a.vocab = r->vocab;
   a.rows = r->rows;
   a.blocks = sas::lmh_blocks(r->vocab, s->cus);
+  a.cus = s->cus;
+  if (h->format == SAS_HEAD_MX4) {
+    a.scales = h->scales;
+    a.scales_stride = h->scales_stride;
+  }
   hipError_t e = sas::launch_lm_head(a, pick_stream(s, stream));
   if (e != hipSuccess) return hip_fail(s, e, (w + " launch").c_str());
   sas_rows lr = *r;

@@ -5,7 +5,6 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
-#include <exception>
 #include <limits>
 #include <string>
 
@@ -16,23 +15,6 @@
 using namespace sas;
 
 namespace {
-
-// Runs f, turning what it throws (out of host memory, in a message or the
-// list of retired buffers) into an error code: nothing leaves a C entry.
-template <typename F>
-int guarded(sas_sampler *s, F f) noexcept {
-  try {
-    return f();
-  } catch (const std::exception &e) {
-    try {
-      return fail(s, SAS_ERR_NOMEM, e.what());
-    } catch (...) {
-      return SAS_ERR_NOMEM;
-    }
-  }
-}
-
-bool aligned(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
 const char *check_projection(const sas_projection *p) {
   if (!p) return "descriptor is NULL";

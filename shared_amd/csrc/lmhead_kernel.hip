@@ -25,8 +25,7 @@
 // 4,096, one row, 91.7 -> 31.2 us; Q6_K 248,320 x 2,560, three rows, 129.2
 // -> 117.9 us; bf16 262,144 x 2,560, one row, 217.1 -> 208.8 us, 7.0 TB/s
 // in this kernel.)
-#include "sas_device.h"
-#include "sas_launch.h"
+#include "mx4_product.h"
 
 namespace sas {
 
@@ -539,8 +538,28 @@ static hipError_t launch_format(const LmhArgs &a, hipStream_t stream) {
   }
 }
 
+void launch_mx4_few(const Mx4ProjArgs &a, hipStream_t stream) { launch_split<1, 2, SAS_TYPE_F32>(a, stream); }
+
 hipError_t launch_lm_head(const LmhArgs &a, hipStream_t stream) {
   switch (a.format) {
+    case SAS_HEAD_MX4: {
+      Mx4ProjArgs p{};
+      p.x = a.hidden;
+      p.x_stride = a.hidden_stride;
+      p.x_type = SAS_TYPE_F32;
+      p.w = static_cast<const uint8_t *>(a.weight);
+      p.w_stride = a.weight_stride;
+      p.w_scales = static_cast<const uint8_t *>(a.scales);
+      p.w_scales_stride = a.scales_stride;
+      p.out = a.logits;
+      p.out_stride = a.logits_stride;
+      p.rows = a.rows;
+      p.dim = a.dim;
+      p.out_dim = a.vocab;
+      p.cus = a.cus;
+      launch_mx4_few(p, stream);
+      return hipGetLastError();
+    }
     case SAS_HEAD_Q8_0: return launch_format<SAS_HEAD_Q8_0>(a, stream);
     case SAS_HEAD_Q4_0: return launch_format<SAS_HEAD_Q4_0>(a, stream);
     case SAS_HEAD_Q6_K: return launch_format<SAS_HEAD_Q6_K>(a, stream);

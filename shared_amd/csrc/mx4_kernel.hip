@@ -1,0 +1,199 @@
+// mx4_kernel.hip - values in microscaled 4-bit floating point (MXFP4):
+// quantisation, lookup of a table's rows, and products (gfx950).
+//
+// A row's values lie in blocks of 32: 16 bytes of elements (a sign, two bits of
+// exponent, one of mantissa: 0 0.5 1 1.5 2 3 4 6; the first of a byte in its low
+// half) and a byte s, the block's scale 2^(s - 127); 255 is NaN.
+#include "mx4_product.h"
+
+namespace sas {
+namespace {
+
+constexpr int kUnit = 4 * kBlock;  // values that 16 lanes handle, 8 each
+
+// 8 consecutive values of a row as f32, those from `left` on zero.
+template <int kType, bool kWide>
+__device__ __forceinline__ void load8(const void *row, int64_t k, int left, float (&v)[8]) {
+  if constexpr (kType == SAS_TYPE_F32) {
+    const float *p = static_cast<const float *>(row) + k;
+    if (kWide && left >= 8) {
+      const f32x4 a = *reinterpret_cast<const f32x4 *>(p), b = *reinterpret_cast<const f32x4 *>(p + 4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = a[i], v[4 + i] = b[i];
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < left ? p[i] : 0.0f;
+  } else {
+    const uint16_t *p = static_cast<const uint16_t *>(row) + k;
+    uint16_t h[8];
+    if (kWide && left >= 8) {
+      const u32x4 a = *reinterpret_cast<const u32x4 *>(p);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) h[2 * i] = (uint16_t)a[i], h[2 * i + 1] = (uint16_t)(a[i] >> 16);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) h[i] = i < left ? p[i] : (uint16_t)0;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      v[i] = kType == SAS_TYPE_BF16 ? __uint_as_float((uint32_t)h[i] << 16) : (float)__builtin_bit_cast(_Float16, h[i]);
+  }
+}
+
+// Units of 4 blocks, 16 lanes each, a lane 8 values.
+template <int kType, bool kWide>
+__global__ __launch_bounds__(kThreads) void mx4_quantize_kernel(const Mx4QuantizeArgs a) {
+  const int e = threadIdx.x & 15;
+  const uint32_t units = (uint32_t)a.rows * (uint32_t)a.row_units;
+  const uint32_t u = blockIdx.x * (kThreads / 16) + (threadIdx.x >> 4);
+  if (u >= units) return;  // (16 lanes together)
+  const uint32_t row = u / (uint32_t)a.row_units, k = (u - row * (uint32_t)a.row_units) * kUnit + 8 * e;
+  float v[8];
+  const int left = a.dim - (int)k;
+  const int64_t size = kType == SAS_TYPE_F32 ? 4 : 2;
+  load8<kType, kWide>(static_cast<const char *>(a.x) + (int64_t)row * a.x_stride * size, k, left, v);
+  // the largest magnitude's bits order as it does, NaN above infinity
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+  top = max(top, dppx<kDppQuad1032>(top));
+  top = max(top, dppx<kDppQuad2301>(top));
+  const bool finite = top < 0x7F800000u;
+  // 2^(s - 127) = 2^(floor(log2 top) - 2), at least 2^-127
+  const uint32_t s = finite ? (uint32_t)max((int)(top >> 23) - 2, 0) : 255u;
+  // x / 2^(s - 127) is exact, below 8; the conversion rounds it to the nearest
+  // element, ties to the even one, and stops at 6
+  const float by = __uint_as_float((254u - (finite ? s : 127u)) << 23);
+  uint32_t c = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float p = v[2 * i] * by, q = v[2 * i + 1] * by;
+    switch (i) {
+      case 0: c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, p, q, 1.0f, 0); break;
+      case 1: c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, p, q, 1.0f, 1); break;
+      case 2: c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, p, q, 1.0f, 2); break;
+      default: c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, p, q, 1.0f, 3); break;
+    }
+  }
+  if (!finite) c = 0;
+  // (a block that the row has no value of is left alone)
+  const int b = (int)k / kBlock, blocks = (a.dim + kBlock - 1) / kBlock;
+  if (b < blocks) *reinterpret_cast<uint32_t *>(a.codes + (int64_t)row * a.codes_stride + k / 2) = c;
+  uint32_t four = (b < blocks ? s : 0u) << (8 * (e >> 2));
+  four |= dppx<kDppRowRor4>(four);
+  four |= dppx<kDppRowRor8>(four);
+  if (e == 0) *reinterpret_cast<uint32_t *>(a.scales + (int64_t)row * a.scales_stride + k / kBlock) = four;
+}
+
+template <int kType, bool kWide>
+__global__ __launch_bounds__(kThreads) void mx4_lookup_kernel(const Mx4LookupArgs a) {
+  const int e = threadIdx.x & 15;
+  const uint32_t units = (uint32_t)a.rows * (uint32_t)a.row_units;
+  const uint32_t u = blockIdx.x * (kThreads / 16) + (threadIdx.x >> 4);
+  if (u >= units) return;
+  const uint32_t row = u / (uint32_t)a.row_units, k = (u - row * (uint32_t)a.row_units) * kUnit + 8 * e;
+  const int left = a.dim - (int)k;
+  if (left <= 0) return;
+  const uint32_t id = a.ids ? a.ids[row] : row;
+  const bool in = id < (uint32_t)a.table_rows;
+  const uint32_t c = in ? *reinterpret_cast<const uint32_t *>(a.codes + (int64_t)id * a.codes_stride + k / 2) : 0u;
+  const uint32_t s = in ? a.scales[(int64_t)id * a.scales_stride + k / kBlock] : 127u;
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f32x2 p;
+    switch (i) {
+      case 0: p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, scale_of(s), 0); break;
+      case 1: p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, scale_of(s), 1); break;
+      case 2: p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, scale_of(s), 2); break;
+      default: p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, scale_of(s), 3); break;
+    }
+    v[2 * i] = p[0];
+    v[2 * i + 1] = p[1];
+  }
+  const int64_t at = (int64_t)row * a.out_stride + k;
+  if constexpr (kType == SAS_TYPE_F32) {
+    float *o = static_cast<float *>(a.out) + at;
+    if (kWide && left >= 8) {
+      *reinterpret_cast<f32x4 *>(o) = f32x4{v[0], v[1], v[2], v[3]};
+      *reinterpret_cast<f32x4 *>(o + 4) = f32x4{v[4], v[5], v[6], v[7]};
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < left) o[i] = v[i];
+    }
+  } else {
+    uint16_t *o = static_cast<uint16_t *>(a.out) + at;
+    uint16_t h[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) h[i] = kType == SAS_TYPE_BF16 ? bf16_of(v[i]) : __builtin_bit_cast(uint16_t, (_Float16)v[i]);
+    if (kWide && left >= 8) {
+      u32x4 p;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[i] = (uint32_t)h[2 * i] | ((uint32_t)h[2 * i + 1] << 16);
+      *reinterpret_cast<u32x4 *>(o) = p;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < left) o[i] = h[i];
+    }
+  }
+}
+
+template <int kX>
+void launch_products(const Mx4ProjArgs &a, hipStream_t stream) {
+  if (kX == SAS_TYPE_F32 && a.rows <= kMx4Few) return launch_mx4_few(a, stream);
+  if (a.rows <= 16) return launch_split<1, 2, kX>(a, stream);
+  launch_split<4, 2, kX>(a, stream);
+}
+
+template <int kType>
+void launch_quantize_of(const Mx4QuantizeArgs &a, bool wide, unsigned blocks, hipStream_t stream) {
+  if (wide) mx4_quantize_kernel<kType, true><<<blocks, kThreads, 0, stream>>>(a);
+  else mx4_quantize_kernel<kType, false><<<blocks, kThreads, 0, stream>>>(a);
+}
+
+template <int kType>
+void launch_lookup_of(const Mx4LookupArgs &a, bool wide, unsigned blocks, hipStream_t stream) {
+  if (wide) mx4_lookup_kernel<kType, true><<<blocks, kThreads, 0, stream>>>(a);
+  else mx4_lookup_kernel<kType, false><<<blocks, kThreads, 0, stream>>>(a);
+}
+
+// Whether rows may be read or written in 16-byte pieces.
+bool in_pieces(const void *p, int64_t stride, int type) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % (type == SAS_TYPE_F32 ? 4 : 8) == 0;
+}
+
+}  // namespace
+
+hipError_t launch_mx4_quantize(const Mx4QuantizeArgs &in, hipStream_t stream) {
+  Mx4QuantizeArgs a = in;
+  a.row_units = (a.dim + kUnit - 1) / kUnit;
+  const unsigned blocks = (unsigned)(((int64_t)a.rows * a.row_units + kThreads / 16 - 1) / (kThreads / 16));
+  const bool wide = in_pieces(a.x, a.x_stride, a.x_type);
+  if (a.x_type == SAS_TYPE_F32) launch_quantize_of<SAS_TYPE_F32>(a, wide, blocks, stream);
+  else if (a.x_type == SAS_TYPE_BF16) launch_quantize_of<SAS_TYPE_BF16>(a, wide, blocks, stream);
+  else launch_quantize_of<SAS_TYPE_F16>(a, wide, blocks, stream);
+  return hipGetLastError();
+}
+
+hipError_t launch_mx4_lookup(const Mx4LookupArgs &in, hipStream_t stream) {
+  Mx4LookupArgs a = in;
+  a.row_units = (a.dim + kUnit - 1) / kUnit;
+  const unsigned blocks = (unsigned)(((int64_t)a.rows * a.row_units + kThreads / 16 - 1) / (kThreads / 16));
+  const bool wide = in_pieces(a.out, a.out_stride, a.out_type);
+  if (a.out_type == SAS_TYPE_F32) launch_lookup_of<SAS_TYPE_F32>(a, wide, blocks, stream);
+  else if (a.out_type == SAS_TYPE_BF16) launch_lookup_of<SAS_TYPE_BF16>(a, wide, blocks, stream);
+  else launch_lookup_of<SAS_TYPE_F16>(a, wide, blocks, stream);
+  return hipGetLastError();
+}
+
+hipError_t launch_mx4_project(const Mx4ProjArgs &a, hipStream_t stream) {
+  if (a.x_type == SAS_TYPE_F32) launch_products<SAS_TYPE_F32>(a, stream);
+  else if (a.x_type == SAS_TYPE_BF16) launch_products<SAS_TYPE_BF16>(a, stream);
+  else launch_products<SAS_TYPE_MX4>(a, stream);
+  return hipGetLastError();
+}
+
+}  // namespace sas

@@ -29,61 +29,10 @@
 //     us (three products each: 0.6 PFLOP/s).
 //   - an adapter a row (61 rows, ranks up to 64, 4,096 x 11,007: 115 us) the
 //     addresses of B's and h's loads, 16 bytes a lane.
-#include <utility>
-
-#include "sas_device.h"
-#include "sas_launch.h"
+#include "sas_product.h"
 
 namespace sas {
 namespace {
-
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
-typedef u16x4 u16x4u __attribute__((aligned(2)));
-
-constexpr int kSub = 16;  // rows, outputs or ranks of one matrix instruction
-
-__device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
-
-// An f32 value as three bf16 pieces whose sum it is (values below 2^-110
-// lose bits that no product of theirs keeps).  Not finite: the first piece
-// alone.
-__device__ __forceinline__ void pieces_of(float x, uint16_t (&p)[3]) {
-  const uint32_t u = __float_as_uint(x);
-  if ((u & 0x7F800000u) == 0x7F800000u) {
-    p[0] = (uint16_t)((u >> 16) | ((u & 0x7FFFFFu) ? 0x40u : 0u));
-    p[1] = p[2] = 0;
-    return;
-  }
-  p[0] = (uint16_t)(u >> 16);
-  const float r1 = x - __uint_as_float(u & 0xFFFF0000u);
-  const uint32_t u1 = __float_as_uint(r1);
-  p[1] = (uint16_t)(u1 >> 16);
-  const float r2 = r1 - __uint_as_float(u1 & 0xFFFF0000u);
-  p[2] = (uint16_t)(__float_as_uint(r2) >> 16);
-}
-
-__device__ __forceinline__ uint16_t bf16_of(float x) {
-  uint32_t u = __float_as_uint(x);
-  if (x != x) return (uint16_t)((u >> 16) | 0x40u);
-  return (uint16_t)((u + 0x7FFFu + ((u >> 16) & 1u)) >> 16);
-}
-
-// 8 consecutive f32 values as three bf16 operands.
-__device__ __forceinline__ void split8(const float *src, u32x4 (&p)[3]) {
-  const f32x4 v0 = *reinterpret_cast<const f32x4 *>(src), v1 = *reinterpret_cast<const f32x4 *>(src + 4);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    uint16_t a[3], b[3];
-    pieces_of(i < 2 ? v0[2 * i] : v1[2 * i - 4], a);
-    pieces_of(i < 2 ? v0[2 * i + 1] : v1[2 * i - 3], b);
-#pragma unroll
-    for (int k = 0; k < 3; ++k) p[k][i] = (uint32_t)a[k] | ((uint32_t)b[k] << 16);
-  }
-}
 
 // The adapter of row `row`, -1 for none.
 __device__ __forceinline__ int adapter_of(const ProjArgs &a, int row) {
@@ -250,62 +199,6 @@ __device__ __forceinline__ u32x4 b_ranks(const uint16_t *row, int r, int used) {
   return w;
 }
 
-// tanh within 3.2 ulp by its roundings (1 ulp of the instructions' exp2 and
-// reciprocal), 1.58 at worst over half a million values (at 0.627); below the split
-// 0.72.  The method is Cody and Waite's (Software Manual for the Elementary
-// Functions, 1980): below a split, here 0.625, x + x^3 P(x^2), P fitted to the
-// relative error (8.6e-9 at most), above it 1 - 2 / (e^2|x| + 1).  A third of
-// tanhf's instructions: 34 million capped values took 30 us of a call's 440.
-__device__ __forceinline__ float tanh_fast(float x) {
-  const float ax = fabsf(x), u = x * x;
-  float p = -0.005704975221306086f;
-  p = __builtin_fmaf(p, u, 0.020639074966311455f);
-  p = __builtin_fmaf(p, u, -0.05373971164226532f);
-  p = __builtin_fmaf(p, u, 0.13331441581249237f);
-  p = __builtin_fmaf(p, u, -0.3333328068256378f);
-  const float small = __builtin_fmaf(x * u, p, x);
-  const float e = __builtin_amdgcn_exp2f(fminf(ax, 16.0f) * 2.8853900817779268f);  // e^2|x|
-  const float large = copysignf(__builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(e + 1.0f), 1.0f), x);
-  return x != x ? x : ax < 0.625f ? small : large;
-}
-
-// The last steps of four sums of row `row`, outputs n .. n + 3: added to what
-// is there, capped, rounded, stored.  Nontemporal: the result is not read here
-// (128 x 262,144 f32: 312 -> 281 us a call, 268 with whole lines a row).
-__device__ __forceinline__ void finish4(const ProjArgs &a, int row, int n, f32x4 v) {
-  if (n >= a.out_dim) return;
-  const bool whole = n + 4 <= a.out_dim;
-  const int64_t at = (int64_t)row * a.out_stride + n;
-  float *of = static_cast<float *>(a.out) + at;
-  uint16_t *ob = static_cast<uint16_t *>(a.out) + at;
-  if (a.accumulate) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (n + i < a.out_dim) v[i] += a.out_bf16 ? __uint_as_float((uint32_t)ob[i] << 16) : of[i];
-  }
-  if (a.softcap > 0.0f) {
-    const float inv = 1.0f / a.softcap;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = a.softcap * tanh_fast(v[i] * inv);
-  }
-  if (a.out_bf16) {
-    const u16x4 p = {bf16_of(v[0]), bf16_of(v[1]), bf16_of(v[2]), bf16_of(v[3])};
-    if (whole) {
-      __builtin_nontemporal_store(p, reinterpret_cast<u16x4u *>(ob));
-    } else {
-#pragma unroll
-      for (int i = 0; i < 3; ++i)
-        if (n + i < a.out_dim) ob[i] = p[i];
-    }
-  } else if (whole) {
-    __builtin_nontemporal_store(v, reinterpret_cast<f32x4u *>(of));
-  } else {
-#pragma unroll
-    for (int i = 0; i < 3; ++i)
-      if (n + i < a.out_dim) of[i] = v[i];
-  }
-}
-
 // A tile of 16 MT rows (positions tile0 .. of the order in a.perm): its rows,
 // and its pairs (subtile, adapter) with the subtile's rows that use it.
 template <int MT>
@@ -434,22 +327,6 @@ __device__ __forceinline__ void add_adapters(const ProjArgs &a, const Tile<MT> &
       y = z;
     }
   }
-}
-
-// Blocks in runs that one XCD's L2 serves: block i runs on XCD i % 8.
-__device__ __forceinline__ int xcd_run(int i, int n) {
-  const int per = n / 8, left = n % 8, x = i % 8;
-  return x * per + min(x, left) + i / 8;
-}
-
-// f(integral_constant 0) .. f(integral_constant N - 1).
-template <int N, typename F, int... I>
-__device__ __forceinline__ void each_const_of(F f, std::integer_sequence<int, I...>) {
-  (f(std::integral_constant<int, I>{}), ...);
-}
-template <int N, typename F>
-__device__ __forceinline__ void each_const(F f) {
-  each_const_of<N>(f, std::make_integer_sequence<int, N>{});
 }
 
 // An operand of 16 rows x 64 values (2 KB): loaded eight lanes a row, whole

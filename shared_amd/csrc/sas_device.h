@@ -238,6 +238,7 @@ __device__ __forceinline__ uint32_t dppx(uint32_t x) {
 }
 constexpr int kDppQuad1032 = 0xB1, kDppQuad2301 = 0x4E, kDppRowHalfMirror = 0x141, kDppRowMirror = 0x140;
 constexpr int kDppRowShr1 = 0x111, kDppRowShr2 = 0x112, kDppRowShr4 = 0x114, kDppRowShr8 = 0x118;
+constexpr int kDppRowRor4 = 0x124, kDppRowRor8 = 0x128;
 constexpr int kDppRowBcast15 = 0x142, kDppRowBcast31 = 0x143;
 
 

@@ -4,6 +4,8 @@
 #include <hip/hip_runtime.h>
 
 #include <cstddef>
+#include <cstdint>
+#include <exception>
 #include <string>
 #include <vector>
 
@@ -84,6 +86,38 @@ inline int grow(sas_sampler *s, void **buf, size_t *cap, size_t need, void *stre
 inline int set_device(sas_sampler *s) {
   hipError_t e = hipSetDevice(s->device);
   return e == hipSuccess ? SAS_OK : hip_fail(s, e, "hipSetDevice");
+}
+
+// Runs f, turning what it throws (out of host memory, in a message or the
+// list of retired buffers) into an error code: nothing leaves a C entry.
+template <typename F>
+int guarded(sas_sampler *s, F f) noexcept {
+  try {
+    return f();
+  } catch (const std::exception &e) {
+    try {
+      return fail(s, SAS_ERR_NOMEM, e.what());
+    } catch (...) {
+      return SAS_ERR_NOMEM;
+    }
+  }
+}
+
+inline bool aligned(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+inline int64_t mx4_blocks(int32_t dim) { return ((int64_t)dim + SAS_MX4_BLOCK - 1) / SAS_MX4_BLOCK; }
+
+// What is wrong with a table of MXFP4 rows (sas_mx4), or null.
+inline const char *check_mx4(const void *codes, int64_t codes_stride, const void *scales, int64_t scales_stride,
+                             int32_t dim) {
+  if (!codes || !scales) return "codes and scales are required";
+  if (!aligned(codes, 16)) return "codes must be 16-byte aligned";
+  if (!aligned(scales, 4)) return "scales must be 4-byte aligned";
+  if (codes_stride < 16 * mx4_blocks(dim) || codes_stride % 16 != 0 || codes_stride > SAS_MAX_MX4_STRIDE)
+    return "codes_stride must be >= 16 ceil(dim / 32), a multiple of 16 and <= SAS_MAX_MX4_STRIDE";
+  if (scales_stride < mx4_blocks(dim) || scales_stride % 4 != 0 || scales_stride > SAS_MAX_MX4_STRIDE)
+    return "scales_stride must be >= ceil(dim / 32), a multiple of 4 and <= SAS_MAX_MX4_STRIDE";
+  return nullptr;
 }
 
 }  // namespace sas

@@ -140,8 +140,8 @@ hipError_t launch_pad_rows(const float *src, int64_t stride, int vocab, int rows
 struct LmhArgs {
   const float *hidden;
   int64_t hidden_stride;
-  const void *weight;     // bf16 bits, or GGUF blocks (format)
-  int64_t weight_stride;  // elements (bf16) or bytes (GGUF) between rows
+  const void *weight;     // bf16 bits, GGUF blocks, or MX4 codes (format)
+  int64_t weight_stride;  // elements (bf16) or bytes (GGUF, MX4) between rows
   float *logits;          // [rows][logits_stride]: out_logits, or the handle's scratch
   int64_t logits_stride;
   int32_t format;         // SAS_HEAD_*
@@ -149,6 +149,9 @@ struct LmhArgs {
   int32_t vocab;
   int32_t rows;           // 1..SAS_LMH_MAX_ROWS
   int32_t blocks;         // lmh_blocks
+  int32_t cus;
+  const void *scales;     // MX4
+  int64_t scales_stride;
 };
 
 // Blocks of the head launch.
@@ -231,6 +234,60 @@ struct ProjScratch {
 };
 ProjScratch proj_scratch(int rows, int dim, int rank, bool x_f32);
 hipError_t launch_project(const ProjArgs &a, hipStream_t stream);
+
+// ------------------------------------------------------------------- mx4 --
+struct Mx4QuantizeArgs {
+  const void *x;
+  int64_t x_stride;
+  uint8_t *codes;
+  int64_t codes_stride;
+  uint8_t *scales;
+  int64_t scales_stride;
+  int32_t x_type;
+  int32_t rows;
+  int32_t dim;
+  int32_t row_units;  // set by the launch
+};
+struct Mx4LookupArgs {
+  const uint8_t *codes;
+  int64_t codes_stride;
+  const uint8_t *scales;
+  int64_t scales_stride;
+  const uint32_t *ids;
+  void *out;
+  int64_t out_stride;
+  int32_t out_type;
+  int32_t table_rows;
+  int32_t rows;
+  int32_t dim;
+  int32_t row_units;  // set by the launch
+};
+struct Mx4ProjArgs {
+  const void *x;           // f32, bf16, or codes
+  int64_t x_stride;        // elements, or bytes between rows of codes
+  const uint8_t *x_scales; // SAS_TYPE_MX4
+  int64_t x_scales_stride;
+  const uint8_t *w;
+  int64_t w_stride;
+  const uint8_t *w_scales;
+  int64_t w_scales_stride;
+  void *out;
+  int64_t out_stride;
+  int32_t x_type;
+  int32_t rows;
+  int32_t dim;
+  int32_t out_dim;
+  float softcap;
+  bool out_bf16;
+  bool accumulate;
+  int32_t cus;
+};
+hipError_t launch_mx4_quantize(const Mx4QuantizeArgs &a, hipStream_t stream);
+hipError_t launch_mx4_lookup(const Mx4LookupArgs &a, hipStream_t stream);
+// Up to kMx4Few rows of f32 hidden states (lmhead_kernel.hip).
+constexpr int kMx4Few = 5;
+void launch_mx4_few(const Mx4ProjArgs &a, hipStream_t stream);
+hipError_t launch_mx4_project(const Mx4ProjArgs &a, hipStream_t stream);
 
 // ---------------------------------------------------------------- filter --
 struct FilterArgs {

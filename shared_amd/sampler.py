@@ -13,8 +13,8 @@ from typing import Optional, Sequence
 import numpy as np
 
 from . import _capi
-from ._capi import (SasFilterParams, SasFilterRows, SasLmHead, SasParams, SasProjection, SasRows, SasSpecRows,
-                    SasVerifyRows, check, load)
+from ._capi import (SasFilterParams, SasFilterRows, SasLmHead, SasMx4, SasMx4Lookup, SasMx4Projection,
+                    SasMx4Quantization, SasParams, SasProjection, SasRows, SasSpecRows, SasVerifyRows, check, load)
 
 
 @dataclass
@@ -94,6 +94,49 @@ class Adapters:
 
     def __len__(self) -> int:
         return self.a.shape[0]
+
+
+class Mx4:
+    """Rows of MXFP4 values (sas_mx4): codes, uint8 [rows][>= 16 ceil(dim / 32)],
+    two values a byte, and scales, uint8 [rows][>= ceil(dim / 32)], a byte a block
+    of 32, device tensors with unit element stride whose rows lie a multiple of
+    16 and of 4 bytes apart."""
+
+    def __init__(self, codes, scales, dim: int):
+        blocks = (int(dim) + 31) // 32
+        for name, t, n in (("codes", codes, 16 * blocks), ("scales", scales, blocks)):
+            if t.dim() != 2 or str(t.dtype) != "torch.uint8" or t.stride(1) != 1 or not t.is_cuda:
+                raise ValueError(f"{name} must be a 2-D uint8 device tensor with unit element stride")
+            if t.shape[1] < n:
+                raise ValueError(f"{name} must hold {n} bytes a row for dim {dim}")
+        if codes.shape[0] != scales.shape[0]:
+            raise ValueError("codes and scales must hold the same rows")
+        if dim < 1:
+            raise ValueError("dim must be >= 1")
+        self.codes, self.scales, self.dim = codes, scales, int(dim)
+
+    @classmethod
+    def empty(cls, rows: int, dim: int, device="cuda") -> "Mx4":
+        """Rows whose bytes are not set, as quantize_mx4_into takes them."""
+        import torch
+        blocks = (int(dim) + 31) // 32
+        return cls(torch.empty((rows, 16 * blocks), dtype=torch.uint8, device=device),
+                   torch.empty((rows, (blocks + 3) // 4 * 4), dtype=torch.uint8, device=device), dim)
+
+    @property
+    def shape(self):
+        return (self.codes.shape[0], self.dim)
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    def to_c(self) -> SasMx4:
+        blocks = (self.dim + 31) // 32
+        # (a table of one row may have any stride)
+        one = self.codes.shape[0] <= 1
+        return SasMx4(self.codes.data_ptr(), 16 * blocks if one else self.codes.stride(0), self.scales.data_ptr(),
+                      (blocks + 3) // 4 * 4 if one else self.scales.stride(0))
 
 
 PARAMS_DTYPE = np.dtype([("temperature", "<f8"), ("top_p", "<f8"), ("repetition_penalty", "<f8"),
@@ -429,6 +472,20 @@ class Sampler:
     def _head(hidden, weight, dim, out_logits, fmt):
         if hidden.dtype.itemsize != 4 or hidden.stride(1) != 1:
             raise ValueError("hidden must be fp32 with unit element stride")
+        if isinstance(weight, Mx4):
+            if fmt not in (_capi.HEAD_BF16, _capi.HEAD_MX4):
+                raise ValueError("an Mx4 weight has the format HEAD_MX4")
+            c = weight.to_c()
+            h = SasLmHead()
+            h.weight, h.weight_stride, h.scales, h.scales_stride = c.codes, c.codes_stride, c.scales, c.scales_stride
+            h.hidden, h.hidden_stride = hidden.data_ptr(), hidden.stride(0)
+            h.dim = int(dim if dim is not None else hidden.shape[1])
+            if h.dim != weight.dim:
+                raise ValueError("the hidden states' dim differs from the head's")
+            h.out_logits, h.format = _ptr(out_logits, "f32", "out_logits"), _capi.HEAD_MX4
+            return h
+        if fmt == _capi.HEAD_MX4:
+            raise ValueError("the format HEAD_MX4 needs an Mx4 weight")
         if fmt == _capi.HEAD_BF16:
             if weight.dtype.itemsize != 2 or weight.stride(1) != 1:
                 raise ValueError("a bf16 head holds bf16 bits (2 bytes) with unit element stride")
@@ -449,8 +506,8 @@ class Sampler:
         """sas_lm_head_sample: the LM head (hidden [rows][>= dim] fp32 times
         weight: [vocab][>= dim] bf16 bits as an int16/uint16 tensor, or with
         fmt = HEAD_Q8_0 / HEAD_Q4_0 / HEAD_Q6_K the GGUF blocks as a
-        [vocab][row bytes] uint8 tensor) with the sampling step behind
-        it; kw as for sample_into."""
+        [vocab][row bytes] uint8 tensor, or an Mx4) with the sampling step
+        behind it; kw as for sample_into."""
         vocab = int(vocab if vocab is not None else weight.shape[0])
         h = self._head(hidden, weight, dim, out_logits, fmt)
         d = rows_descriptor(hidden, out_ids, vocab=vocab, **kw)
@@ -545,6 +602,97 @@ class Sampler:
         with _on(stream):
             out = torch.empty((x.shape[0], weight.shape[0]), dtype=out_dtype or torch.float32, device=x.device)
         self.project_into(x, weight, out, stream=stream, **kw)
+        return out
+
+    def quantize_mx4_into(self, x, out: Mx4, *, stream=None) -> None:
+        """sas_quantize_mx4: rounds x [rows][dim] (float32, bfloat16 or float16)
+        into out's first rows."""
+        types = {"torch.float32": _capi.TYPE_F32, "torch.bfloat16": _capi.TYPE_BF16, "torch.float16": _capi.TYPE_F16}
+        if x.dim() != 2 or x.stride(1) != 1 or not x.is_cuda or str(x.dtype) not in types:
+            raise ValueError("x must be a 2-D float32, bfloat16 or float16 device tensor with unit element stride")
+        if out.shape[0] < x.shape[0] or out.dim != x.shape[1]:
+            raise ValueError("out must hold x's rows of x's dim")
+        d = SasMx4Quantization()
+        d.x, d.x_type = x.data_ptr(), types[str(x.dtype)]
+        d.rows, d.dim = x.shape
+        d.x_stride = x.stride(0) if x.shape[0] > 1 else x.shape[1]
+        d.out = out.to_c()
+        check(self._lib.sas_quantize_mx4(self._h, ctypes.byref(d), _stream(stream)), self._h)
+
+    def quantize_mx4(self, x, *, stream=None) -> Mx4:
+        """Allocate an Mx4 and run quantize_mx4_into; returns it."""
+        if x.dim() != 2:
+            raise ValueError("x must be a 2-D float32, bfloat16 or float16 device tensor with unit element stride")
+        with _on(stream):
+            out = Mx4.empty(x.shape[0], x.shape[1], x.device)
+        self.quantize_mx4_into(x, out, stream=stream)
+        return out
+
+    def lookup_mx4_into(self, table: Mx4, out, ids=None, *, stream=None) -> None:
+        """sas_lookup_mx4: out [rows][dim] (float32, bfloat16 or float16) = the
+        table's rows ids (4-byte integers; one past the table gives zeros), or its
+        first rows in order."""
+        types = {"torch.float32": _capi.TYPE_F32, "torch.bfloat16": _capi.TYPE_BF16, "torch.float16": _capi.TYPE_F16}
+        if out.dim() != 2 or out.stride(1) != 1 or not out.is_cuda or str(out.dtype) not in types:
+            raise ValueError("out must be a 2-D float32, bfloat16 or float16 device tensor with unit element stride")
+        if out.shape[1] != table.dim:
+            raise ValueError("out's dim differs from the table's")
+        if ids is not None and (ids.dim() != 1 or ids.shape[0] != out.shape[0]):
+            raise ValueError("ids must hold one id per row of out")
+        d = SasMx4Lookup()
+        d.table, d.table_rows, d.dim = table.to_c(), table.shape[0], table.dim
+        d.ids, d.rows = _ptr(ids, "i32", "ids"), out.shape[0]
+        d.out, d.out_type = out.data_ptr(), types[str(out.dtype)]
+        d.out_stride = out.stride(0) if out.shape[0] > 1 else out.shape[1]
+        check(self._lib.sas_lookup_mx4(self._h, ctypes.byref(d), _stream(stream)), self._h)
+
+    def lookup_mx4(self, table: Mx4, ids=None, *, out_dtype=None, stream=None):
+        """Allocate out (float32 unless out_dtype) for every id, or the whole
+        table, and run lookup_mx4_into; returns it."""
+        import torch
+        with _on(stream):
+            out = torch.empty((table.shape[0] if ids is None else ids.shape[0], table.dim),
+                              dtype=out_dtype or torch.float32, device=table.device)
+        self.lookup_mx4_into(table, out, ids, stream=stream)
+        return out
+
+    def project_mx4_into(self, x, weight: Mx4, out, *, softcap: float = 0.0, accumulate: bool = False,
+                         stream=None) -> None:
+        """sas_project_mx4: out [rows][out] (float32 or bfloat16) = x [rows][dim]
+        (float32, bfloat16 or an Mx4) times weight, capped."""
+        types = {"torch.float32": _capi.TYPE_F32, "torch.bfloat16": _capi.TYPE_BF16}
+        four = isinstance(x, Mx4)
+        for name, t in (("x", x), ("out", out)):
+            if name == "x" and four:
+                continue
+            if t.dim() != 2 or t.stride(1) != 1 or not t.is_cuda or str(t.dtype) not in types:
+                raise ValueError(f"{name} must be a 2-D float32 or bfloat16 device tensor with unit element stride")
+        rows, dim = x.shape
+        if out.shape[0] != rows or tuple(weight.shape) != (out.shape[1], dim):
+            raise ValueError("x [rows][dim], weight [out][dim] and out [rows][out] do not fit together")
+        d = SasMx4Projection()
+        if four:
+            d.x4, d.x_type = x.to_c(), _capi.TYPE_MX4
+        else:
+            # (a tensor of one row may have any stride; its row is the whole of it)
+            d.x, d.x_stride, d.x_type = x.data_ptr(), x.stride(0) if rows > 1 else (dim + 7) // 8 * 8, types[str(x.dtype)]
+        d.rows, d.dim, d.out_dim = rows, dim, out.shape[1]
+        d.weight = weight.to_c()
+        d.out, d.out_type = out.data_ptr(), types[str(out.dtype)]
+        d.out_stride = out.stride(0) if rows > 1 else out.shape[1]
+        d.softcap = float(softcap)
+        d.accumulate = 1 if accumulate else 0
+        check(self._lib.sas_project_mx4(self._h, ctypes.byref(d), _stream(stream)), self._h)
+
+    def project_mx4(self, x, weight: Mx4, *, out_dtype=None, stream=None, **kw):
+        """Allocate out (float32 unless out_dtype is torch.bfloat16) and run
+        project_mx4_into; returns it.  A fresh out holds nothing to accumulate on."""
+        import torch
+        if kw.get("accumulate"):
+            raise ValueError("project_mx4 cannot accumulate: its out is new (project_mx4_into takes one)")
+        with _on(stream):
+            out = torch.empty((x.shape[0], weight.shape[0]), dtype=out_dtype or torch.float32, device=x.device)
+        self.project_mx4_into(x, weight, out, stream=stream, **kw)
         return out
 
     def reserve_project(self, rows: int, dim: int, *, rank: int = 0) -> None:
