@@ -144,6 +144,17 @@ __global__ __launch_bounds__(kThreads) void mx4_lookup_kernel(const Mx4LookupArg
 template <int kX>
 void launch_products(const Mx4ProjArgs &a, hipStream_t stream) {
   if (kX == SAS_TYPE_F32 && a.rows <= kMx4Few) return launch_mx4_few(a, stream);
+  const int64_t work = (int64_t)((a.rows + 127) / 128) * ((a.out_dim + 255) / 256);
+  if (work * 8 >= a.cus * 3 && a.x_stride < (1 << 21)) {
+    if (a.rows <= 16) {
+      if (kX != SAS_TYPE_F32 && stream_fits<1, kX, false>(a)) return launch_stream<1, 1, kX, false>(a, stream);
+      return launch_wide<1, 1, 2, kX>(a, stream);
+    }
+    if (a.rows <= 32) return launch_wide<2, 1, 2, kX>(a, stream);
+    if (a.rows <= 64) return launch_wide<4, 1, 2, kX>(a, stream);
+    if constexpr (kX == SAS_TYPE_F32) return launch_wide<4, 1, 2, kX>(a, stream);
+    else return launch_wide<4, 2, 4, kX>(a, stream);
+  }
   if (a.rows <= 16) return launch_split<1, 2, kX>(a, stream);
   launch_split<4, 2, kX>(a, stream);
 }

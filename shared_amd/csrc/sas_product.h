@@ -25,13 +25,9 @@ __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
 // alone.
 __device__ __forceinline__ void pieces_of(float x, uint16_t (&p)[3]) {
   const uint32_t u = __float_as_uint(x);
-  if ((u & 0x7F800000u) == 0x7F800000u) {
-    p[0] = (uint16_t)((u >> 16) | ((u & 0x7FFFFFu) ? 0x40u : 0u));
-    p[1] = p[2] = 0;
-    return;
-  }
-  p[0] = (uint16_t)(u >> 16);
-  const float r1 = x - __uint_as_float(u & 0xFFFF0000u);
+  const bool finite = (u & 0x7F800000u) != 0x7F800000u;
+  p[0] = (uint16_t)((u | (x != x ? 0x400000u : 0u)) >> 16);
+  const float r1 = finite ? x - __uint_as_float(u & 0xFFFF0000u) : 0.0f;
   const uint32_t u1 = __float_as_uint(r1);
   p[1] = (uint16_t)(u1 >> 16);
   const float r2 = r1 - __uint_as_float(u1 & 0xFFFF0000u);
@@ -44,17 +40,22 @@ __device__ __forceinline__ uint16_t bf16_of(float x) {
   return (uint16_t)((u + 0x7FFFu + ((u >> 16) & 1u)) >> 16);
 }
 
-// 8 consecutive f32 values (4-byte aligned) as three bf16 operands.
-__device__ __forceinline__ void split8(const float *src, u32x4 (&p)[3]) {
-  const f32x4 v0 = *reinterpret_cast<const f32x4u *>(src), v1 = *reinterpret_cast<const f32x4u *>(src + 4);
+// 8 f32 values as three bf16 operands.
+__device__ __forceinline__ void split_f32(const float (&v)[8], u32x4 (&p)[3]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     uint16_t a[3], b[3];
-    pieces_of(i < 2 ? v0[2 * i] : v1[2 * i - 4], a);
-    pieces_of(i < 2 ? v0[2 * i + 1] : v1[2 * i - 3], b);
+    pieces_of(v[2 * i], a);
+    pieces_of(v[2 * i + 1], b);
 #pragma unroll
     for (int k = 0; k < 3; ++k) p[k][i] = (uint32_t)a[k] | ((uint32_t)b[k] << 16);
   }
+}
+// The same of 8 consecutive ones in memory (4-byte aligned).
+__device__ __forceinline__ void split8(const float *src, u32x4 (&p)[3]) {
+  const f32x4 v0 = *reinterpret_cast<const f32x4u *>(src), v1 = *reinterpret_cast<const f32x4u *>(src + 4);
+  const float v[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+  split_f32(v, p);
 }
 
 // tanh within 3.2 ulp by its roundings (1 ulp of the instructions' exp2 and
