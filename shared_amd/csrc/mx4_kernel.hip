@@ -141,21 +141,47 @@ __global__ __launch_bounds__(kThreads) void mx4_lookup_kernel(const Mx4LookupArg
   }
 }
 
+// The outputs a wave of the wide kernel takes, in 16s: as few rounds of blocks as
+// that leaves, a round's cost being its products and half of 16 outputs more.
+int wide_nt(const Mx4ProjArgs &a, int mt, int most) {
+  int best = 1;
+  int64_t cost = INT64_MAX;
+  for (int nt = 1; nt <= most; ++nt) {
+    const int64_t blocks = (int64_t)((a.rows + 16 * mt - 1) / (16 * mt)) * ((a.out_dim + 128 * nt - 1) / (128 * nt));
+    const int64_t c = (blocks + a.cus - 1) / a.cus * (2 * nt + 1);
+    if (c <= cost) {
+      cost = c;
+      best = nt;
+    }
+  }
+  return best;
+}
+
 template <int kX>
 void launch_products(const Mx4ProjArgs &a, hipStream_t stream) {
   if (kX == SAS_TYPE_F32 && a.rows <= kMx4Few) return launch_mx4_few(a, stream);
-  const int64_t work = (int64_t)((a.rows + 127) / 128) * ((a.out_dim + 255) / 256);
-  if (work * 8 >= a.cus * 3 && a.x_stride < (1 << 21)) {
+  if (a.x_stride < (1 << 21) && a.out_stride < kMaxOutStride && (int64_t)a.out_dim * ((a.rows + 63) / 64) >= 4096) {
+    if constexpr (kX == SAS_TYPE_MX4) {
+      if (a.rows > 32 && a.rows <= 64 && stream_fits<4, kX, false>(a)) return launch_stream<4, 1, kX, false>(a, stream);
+      if (a.rows > 16 && a.rows <= 32 && stream_fits<2, kX, false>(a)) return launch_stream<2, 1, kX, false>(a, stream);
+    }
     if (a.rows <= 16) {
       if (kX != SAS_TYPE_F32 && stream_fits<1, kX, false>(a)) return launch_stream<1, 1, kX, false>(a, stream);
-      return launch_wide<1, 1, 2, kX>(a, stream);
+      switch (wide_nt(a, 1, 3)) {
+        case 1: return launch_wide<1, 1, kX>(a, stream);
+        case 2: return launch_wide<1, 2, kX>(a, stream);
+        default: return launch_wide<1, 3, kX>(a, stream);
+      }
     }
-    if (a.rows <= 32) return launch_wide<2, 1, 2, kX>(a, stream);
-    if (a.rows <= 64) return launch_wide<4, 1, 2, kX>(a, stream);
-    if constexpr (kX == SAS_TYPE_F32) return launch_wide<4, 1, 2, kX>(a, stream);
-    else return launch_wide<4, 2, 4, kX>(a, stream);
+    if (a.rows <= 32) return wide_nt(a, 2, 2) == 1 ? launch_wide<2, 1, kX>(a, stream) : launch_wide<2, 2, kX>(a, stream);
+    if (a.rows <= 64 || kX == SAS_TYPE_F32) return wide_nt(a, 4, 2) == 1 ? launch_wide<4, 1, kX>(a, stream) : launch_wide<4, 2, kX>(a, stream);
+    if constexpr (kX != SAS_TYPE_F32) return wide_nt(a, 8, 2) == 1 ? launch_wide<8, 1, kX>(a, stream) : launch_wide<8, 2, kX>(a, stream);
   }
-  if (a.rows <= 16) return launch_split<1, 2, kX>(a, stream);
+  if (a.rows <= 16) {
+    if (a.out_dim <= 32 * a.cus) return launch_split<1, 1, kX>(a, stream);
+    return launch_split<1, 2, kX>(a, stream);
+  }
+  if (a.rows <= 32) return launch_split<2, 2, kX>(a, stream);
   launch_split<4, 2, kX>(a, stream);
 }
 

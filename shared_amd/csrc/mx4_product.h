@@ -8,6 +8,7 @@ namespace sas {
 namespace {
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef u32x4 u32x4a4 __attribute__((aligned(4)));
@@ -46,121 +47,36 @@ __device__ __forceinline__ f32x4 mfma4(u32x4 w, uint32_t ws, u32x4 x, uint32_t x
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 4, 4, kByte, (int)ws, kByte, (int)xs);
 }
 
-// A lane's scales of a super-run: of the row's 16 bytes from block 16 s on, byte
-// q of each dword (blocks q, 4 + q, 8 + q, 12 + q).
-struct Scales {
-  u32x4 d;
-};
-__device__ __forceinline__ Scales load_scales(const uint8_t *row, int s, int blocks) {
-  Scales v;
-  const int last = (blocks - 1) / 4;  // the dwords behind it are not the row's
-  if (4 * s + 3 <= last) {
-    v.d = *reinterpret_cast<const u32x4a4 *>(row + 16 * s);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v.d[i] = *reinterpret_cast<const uint32_t *>(row + 4 * min(4 * s + i, last));
-  }
-  return v;
+// A lane's scales of a super-run (blocks 16 s ..): lane l loads the l / 16-th of
+// its row's four dwords; exchanged among the row's four lanes, each keeps byte
+// l / 16 of every one, in the order of the runs.  No branches: the loops that
+// use them stay one block, or the compiler moves all products behind the loads.
+// (run: the first of the four)
+__device__ __forceinline__ uint32_t load_scales_of(const uint8_t *row, int run, int blocks) {
+  // (the dwords behind the last block's are not the row's)
+  return *reinterpret_cast<const uint32_t *>(row + 4 * min(run + (int)((threadIdx.x & 63) >> 4), (blocks - 1) / 4));
 }
-// Bytes past the row's last block become 127 (1): what is there may be NaN.
-__device__ __forceinline__ uint32_t pack_scales(const Scales &v, int q, int s, int blocks) {
-  const uint32_t sel = 0x0C0C0400u + 0x0101u * (uint32_t)q;
-  const uint32_t lo = __builtin_amdgcn_perm(v.d[1], v.d[0], sel), hi = __builtin_amdgcn_perm(v.d[3], v.d[2], sel);
-  uint32_t p = lo | (hi << 16);
-  if (16 * s + 16 > blocks) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (16 * s + 4 * j + q >= blocks) p = (p & ~(0xFFu << (8 * j))) | (0x7Fu << (8 * j));
-  }
-  return p;
+template <bool kTail = true>
+__device__ __forceinline__ uint32_t load_scales(const uint8_t *row, int s, int blocks) {
+  if constexpr (!kTail) return *reinterpret_cast<const uint32_t *>(row + 16 * s + ((threadIdx.x & 63) >> 4 << 2));
+  return load_scales_of(row, 4 * s, blocks);
 }
-
-// Eight waves split dim for the same 16 NT outputs of 16 MT rows; their sums
-// meet in LDS in a fixed order.
-constexpr int kSplitWaves = 8;
-
-template <int MT, int NT, int kX>
-__global__ __launch_bounds__(64 * kSplitWaves) void mx4_split_kernel(const Mx4ProjArgs a) {
-  __shared__ f32x4 part[kSplitWaves][MT * NT][64];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int r = lane & 15, q = lane >> 4;
-  const int mtiles = (a.rows + 16 * MT - 1) / (16 * MT);
-  const int pos = xcd_run((int)blockIdx.x, (int)gridDim.x);
-  const int m0 = (pos % mtiles) * 16 * MT, n0 = (pos / mtiles) * 16 * NT;
-  const u32x4 none = {0u, 0u, 0u, 0u};
-  const int blocks = (a.dim + kBlock - 1) / kBlock, runs = (blocks + 3) / 4;
-  const int g0 = runs * wave / kSplitWaves, g1 = runs * (wave + 1) / kSplitWaves;
-  f32x4 acc[MT][NT];
-#pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
-    for (int t = 0; t < NT; ++t) acc[m][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  for (int g = g0; g < g1; ++g) {
-    const int b = 4 * g + q;
-    const bool in = b < blocks;
-    u32x4 w[NT];
-    uint32_t ws[NT];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const int64_t row = min(n0 + 16 * t + r, a.out_dim - 1);
-      w[t] = in ? *reinterpret_cast<const u32x4 *>(a.w + row * a.w_stride + 16 * b) : none;
-      ws[t] = in ? a.w_scales[row * a.w_scales_stride + b] : 127u;
-    }
-    if constexpr (kX == SAS_TYPE_MX4) {
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        const int64_t row = min(m0 + 16 * m + r, a.rows - 1);
-        const u32x4 x = in ? *reinterpret_cast<const u32x4 *>(static_cast<const uint8_t *>(a.x) + row * a.x_stride + 16 * b) : none;
-        const uint32_t xs = in ? a.x_scales[row * a.x_scales_stride + b] : 127u;
-#pragma unroll
-        for (int t = 0; t < NT; ++t) acc[m][t] = mfma4<0>(w[t], ws[t], x, xs, acc[m][t]);
-      }
-    } else {
-      u32x4 wide[NT][4];
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) wide[t][i] = widen(w[t][i], scale_of(ws[t]));
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        const int64_t row = min(m0 + 16 * m + r, a.rows - 1);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int k = kBlock * b + 8 * i;
-          if constexpr (kX == SAS_TYPE_F32) {
-            u32x4 x[3] = {none, none, none};
-            if (k < a.dim) split8(static_cast<const float *>(a.x) + row * a.x_stride + k, x);
-#pragma unroll
-            for (int p = 0; p < 3; ++p)
-#pragma unroll
-              for (int t = 0; t < NT; ++t) acc[m][t] = mfma(wide[t][i], x[p], acc[m][t]);
-          } else {
-            const u32x4 x = k < a.dim ? *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(a.x) + row * a.x_stride + k) : none;
-#pragma unroll
-            for (int t = 0; t < NT; ++t) acc[m][t] = mfma(wide[t][i], x, acc[m][t]);
-          }
-        }
-      }
-    }
-  }
-#pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
-    for (int t = 0; t < NT; ++t) part[wave][m * NT + t][lane] = acc[m][t];
-  __syncthreads();
-  for (int i = wave; i < MT * NT; i += kSplitWaves) {
-    f32x4 v = part[0][i][lane];
-#pragma unroll
-    for (int w = 1; w < kSplitWaves; ++w) v = v + part[w][i][lane];
-    const int row = m0 + 16 * (i / NT) + r;
-    if (row < a.rows) finish4(a, row, n0 + 16 * (i % NT) + 4 * q, v);
-  }
+// The bytes of a lane's runs that the row has blocks for.
+__device__ __forceinline__ uint32_t scale_mask_of(int run, int blocks) {
+  const int q = (threadIdx.x & 63) >> 4, n = min(max((blocks - 4 * run - q + 3) >> 2, 0), 4);
+  return n == 4 ? 0xFFFFFFFFu : (1u << (8 * n)) - 1u;
 }
-
-template <int MT, int NT, int kX>
-void launch_split(const Mx4ProjArgs &a, hipStream_t stream) {
-  const int blocks = ((a.rows + 16 * MT - 1) / (16 * MT)) * ((a.out_dim + 16 * NT - 1) / (16 * NT));
-  mx4_split_kernel<MT, NT, kX><<<blocks, 64 * kSplitWaves, 0, stream>>>(a);
+__device__ __forceinline__ uint32_t scale_mask(int s, int blocks) { return scale_mask_of(4 * s, blocks); }
+// The others become 127 (1): what is there may be NaN.
+template <bool kTail = true>
+__device__ __forceinline__ uint32_t pack_scales(uint32_t mine, uint32_t mask) {
+  const uint32_t q = (threadIdx.x & 63) >> 4, sel = 0x0C0C0400u + 0x0101u * q;
+  const auto half = __builtin_amdgcn_permlane32_swap(mine, mine, false, false);
+  const auto lo = __builtin_amdgcn_permlane16_swap(half[0], half[0], false, false);
+  const auto hi = __builtin_amdgcn_permlane16_swap(half[1], half[1], false, false);
+  const uint32_t a = __builtin_amdgcn_perm(lo[1], lo[0], sel), b = __builtin_amdgcn_perm(hi[1], hi[0], sel);
+  const uint32_t p = __builtin_amdgcn_perm(b, a, 0x05040100u);
+  return kTail ? (p & mask) | (0x7F7F7F7Fu & ~mask) : p;
 }
 
 // ---- the hidden states in LDS ----
@@ -205,62 +121,114 @@ template <int kX>
 struct XPart {  // what a lane loads: an octet, or a block
   u32x4 v[kX == SAS_TYPE_F32 ? 2 : 1];
 };
-// From `at` on, of `size` values (bytes) a row has; zeros past them.
+// A part, at p.
 template <int kX>
-__device__ __forceinline__ XPart<kX> x_load(const void *row, int at, int size) {
-  XPart<kX> p;
-  const u32x4 none = {0u, 0u, 0u, 0u};
+__device__ __forceinline__ XPart<kX> x_load(const char *p) {
+  XPart<kX> v;
+  const u32x4a4 *src = reinterpret_cast<const u32x4a4 *>(p);
   if constexpr (kX == SAS_TYPE_F32) {
-    const u32x4a4 *src = reinterpret_cast<const u32x4a4 *>(static_cast<const float *>(row) + at);
-    p.v[0] = at < size ? src[0] : none;
-    p.v[1] = at < size ? src[1] : none;
-  } else if constexpr (kX == SAS_TYPE_BF16) {
-    p.v[0] = at < size ? *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(row) + at) : none;
+    v.v[0] = src[0];
+    v.v[1] = src[1];
   } else {
-    p.v[0] = at < size ? *reinterpret_cast<const u32x4 *>(static_cast<const uint8_t *>(row) + at) : none;
+    v.v[0] = *reinterpret_cast<const u32x4 *>(p);
   }
-  return p;
+  return v;
 }
-// The bf16 operands of a part: itself, or its three pieces.
 template <int kX>
-__device__ __forceinline__ void x_pieces(const XPart<kX> &p, u32x4 (&o)[XOperand<kX>::kPieces]) {
+constexpr int kXSize = kX == SAS_TYPE_F32 ? 4 : kX == SAS_TYPE_BF16 ? 2 : 1;  // bytes
+// Of `size` values (bytes) a row has, the part from `at` on is read here: its last
+// one past them (no branch; x_pieces makes zeros of it).
+template <int kX>
+__device__ __forceinline__ int x_within(int at, int size) {
+  return min(at, size - (kX == SAS_TYPE_MX4 ? 16 : 8));
+}
+// The operands of a part: itself, or its three pieces; zeros from `size` on.
+template <int kX>
+__device__ __forceinline__ void x_pieces(const XPart<kX> &p, int at, int size, u32x4 (&o)[XOperand<kX>::kPieces]) {
+  const u32x4 none = {0u, 0u, 0u, 0u};
   if constexpr (kX == SAS_TYPE_F32) {
     float v[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(p.v[i / 4][i % 4]);
+    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(at < size ? p.v[i / 4][i % 4] : 0u);
     split_f32(v, o);
   } else {
-    o[0] = p.v[0];
+    o[0] = at < size ? p.v[0] : none;
   }
 }
 
-// The sums of 16 rows x 16 NT outputs from the matrix layout to whole runs of a
-// row's outputs, through LDS of the wave's own: f(row, column, 4 sums).
+// The sums of 16 rows x 16 NT outputs go out as whole runs of a row's outputs:
+// from the matrix layout through LDS of the wave's own (kStage<NT> floats), 4 NT
+// lanes a row.  n0: the first output; row0: the first row; value(row, col): the
+// four sums.  (Addresses are a uniform base and 32 bits a lane: what is spent on
+// them here is as much as on the products of 512 values.)
 template <int NT>
-constexpr int kStage = 16 * (16 * NT + 4);  // floats
+constexpr int kStage = 16 * (16 * NT + 4);
+constexpr int64_t kMaxOutStride = 1 << 25;  // elements: 16 rows are within 32 bits
 template <int NT, typename F>
-__device__ __forceinline__ void by_rows(float *stage, const f32x4 (&acc)[NT], F f) {
+__device__ __forceinline__ void put_rows(const Mx4ProjArgs &a, int row0, int n0, F value) {
   const int lane = threadIdx.x & 63;
-  constexpr int kPitch = 16 * NT + 4, kLanes = 4 * NT;
-  wave_lds_sync();
-#pragma unroll
-  for (int t = 0; t < NT; ++t) *reinterpret_cast<f32x4 *>(stage + (lane & 15) * kPitch + 16 * t + 4 * (lane >> 4)) = acc[t];
-  wave_lds_sync();
+  constexpr int kLanes = 4 * NT;
+  const uint32_t size = a.out_bf16 ? 2u : 4u;
+  char *base = static_cast<char *>(a.out) + ((int64_t)row0 * a.out_stride + n0) * size;
+  const float inv = a.softcap > 0.0f ? 1.0f / a.softcap : 0.0f;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    const int i = 64 * n + lane, row = i / kLanes, col = 4 * (i % kLanes);
-    f(row, col, *reinterpret_cast<const f32x4 *>(stage + row * kPitch + col));
+    const int i = 64 * n + lane, row = i / kLanes, col = 4 * (i % kLanes), left = a.out_dim - n0 - col;
+    if (row0 + row >= a.rows || left <= 0) continue;
+    f32x4 v = value(row, col);
+    char *at = base + ((uint32_t)row * (uint32_t)a.out_stride + (uint32_t)col) * size;
+    float *of = reinterpret_cast<float *>(at);
+    uint16_t *ob = reinterpret_cast<uint16_t *>(at);
+    if (a.accumulate) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (k < left) v[k] += a.out_bf16 ? __uint_as_float((uint32_t)ob[k] << 16) : of[k];
+    }
+    if (a.softcap > 0.0f) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = a.softcap * tanh_fast(v[k] * inv);
+    }
+    // (nontemporal: the result is not read here)
+    if (a.out_bf16) {
+      const u16x4 p = __builtin_bit_cast(u16x4, __builtin_convertvector(v, bf16x4));
+      if (left >= 4) {
+        __builtin_nontemporal_store(p, reinterpret_cast<u16x4u *>(ob));
+      } else {
+#pragma unroll
+        for (int k = 0; k < 3; ++k)
+          if (k < left) ob[k] = p[k];
+      }
+    } else if (left >= 4) {
+      __builtin_nontemporal_store(v, reinterpret_cast<f32x4u *>(of));
+    } else {
+#pragma unroll
+      for (int k = 0; k < 3; ++k)
+        if (k < left) of[k] = v[k];
+    }
   }
+}
+template <int NT>
+__device__ __forceinline__ void stage_rows(float *stage, const f32x4 (&acc)[NT]) {
+  const int lane = threadIdx.x & 63;
+  wave_lds_sync();
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+    *reinterpret_cast<f32x4 *>(stage + (lane & 15) * (16 * NT + 4) + 16 * t + 4 * (lane >> 4)) = acc[t];
+  wave_lds_sync();
+}
+template <int NT>
+__device__ __forceinline__ f32x4 staged(const float *stage, int row, int col) {
+  return *reinterpret_cast<const f32x4 *>(stage + row * (16 * NT + 4) + col);
 }
 
 // Weight rows.  A super-run of 16 rows is 4 KB: loaded eight lanes a row, whole
 // 128-byte lines (load k: rows 8 (k % 2) .., line k / 2 of the super-run), and
-// turned into the matrix layout through LDS of the wave's own, laid out as a bf16
-// operand's 16-byte slots are.
+// turned into the matrix layout, a line of each row at a time, through LDS of the
+// wave's own, laid out as a bf16 operand's 16-byte slots are.
 template <int NT>
 struct WSuper {
   u32x4 c[4][NT];
-  Scales s[NT];
+  uint32_t s[NT];
 };
 template <int NT>
 struct WRows {
@@ -268,7 +236,6 @@ struct WRows {
   const uint8_t *scales[NT];
   uint32_t at[NT][2];         // the lane's rows of a load, its chunk
   uint32_t scale_at[NT];      // the lane's row
-  template <bool kDirect = false>
   __device__ __forceinline__ void set(const Mx4ProjArgs &a, int n0) {
     const int lane = threadIdx.x & 63;
 #pragma unroll
@@ -278,55 +245,47 @@ struct WRows {
       scales[t] = a.w_scales + (int64_t)first * a.w_scales_stride;
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        at[t][h] = (uint32_t)(min(n + (kDirect ? lane & 15 : 8 * h + (lane >> 3)), a.out_dim - 1) - first) * (uint32_t)a.w_stride;
+        at[t][h] = (uint32_t)(min(n + 8 * h + (lane >> 3), a.out_dim - 1) - first) * (uint32_t)a.w_stride;
       scale_at[t] = (uint32_t)(min(n + (lane & 15), a.out_dim - 1) - first) * (uint32_t)a.w_scales_stride;
     }
   }
-  // The same straight into the matrix layout: lane l block l / 16 of run k of row
-  // l % 16 (half lines: for products that the matrix instructions bound).
-  __device__ __forceinline__ void load_direct(WSuper<NT> &b, int s, int blocks) const {
-#pragma unroll
-    for (int t = 0; t < NT; ++t) b.s[t] = load_scales(scales[t] + scale_at[t], s, blocks);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) load_direct_run(b, k, s, blocks);
-  }
-  __device__ __forceinline__ void load_direct_run(WSuper<NT> &b, int k, int s, int blocks) const {
-    const uint32_t chunk = 16u * (uint32_t)min(16 * s + 4 * k + (int)((threadIdx.x & 63) >> 4), blocks - 1);
-#pragma unroll
-    for (int t = 0; t < NT; ++t) b.c[k][t] = *reinterpret_cast<const u32x4 *>(codes[t] + (at[t][0] + chunk));
-  }
   // kOnce: no other wave reads these rows (nontemporal loads then)
-  template <bool kOnce>
+  template <bool kOnce, bool kTail = true>
   __device__ __forceinline__ void load(WSuper<NT> &b, int s, int blocks) const {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int t = 0; t < NT; ++t) b.s[t] = load_scales(scales[t] + scale_at[t], s, blocks);
+    const uint32_t lane = threadIdx.x & 63;
+    load_s<kTail>(b.s, s, blocks);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const uint32_t chunk = 16u * (uint32_t)min(16 * s + 8 * (k >> 1) + (lane & 7), blocks - 1);
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        const u32x4 *src = reinterpret_cast<const u32x4 *>(codes[t] + (at[t][k & 1] + chunk));
+        const uint8_t *p = kTail ? codes[t] + (at[t][k & 1] + 16u * (uint32_t)min(16 * s + 8 * (k >> 1) + (int)(lane & 7), blocks - 1))
+                                 : codes[t] + 256 * s + (at[t][k & 1] + 16u * (lane & 7)) + 128 * (k >> 1);
+        const u32x4 *src = reinterpret_cast<const u32x4 *>(p);
         b.c[k][t] = kOnce ? __builtin_nontemporal_load(src) : *src;
       }
     }
   }
+  template <bool kTail>
+  __device__ __forceinline__ void load_s(uint32_t (&v)[NT], int s, int blocks) const {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) v[t] = load_scales<kTail>(scales[t] + scale_at[t], s, blocks);
+  }
 };
-constexpr int kWSlots = 256;  // of a tile's super-run
+constexpr int kWSlots = 128;  // of a tile's line
 template <int NT>
-__device__ __forceinline__ void w_put(u32x4 *ws, const WSuper<NT> &b) {
+__device__ __forceinline__ void w_put(u32x4 *ws, const WSuper<NT> &b, int line) {
   const int lane = threadIdx.x & 63;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const int r = 8 * (k & 1) + (lane >> 3);
+  for (int h = 0; h < 2; ++h) {
+    const int r = 8 * h + (lane >> 3);
 #pragma unroll
-    for (int t = 0; t < NT; ++t) ws[kWSlots * t + 128 * (k >> 1) + 8 * r + ((lane & 7) ^ (r >> 1))] = b.c[k][t];
+    for (int t = 0; t < NT; ++t) ws[kWSlots * t + 8 * r + ((lane & 7) ^ (r >> 1))] = b.c[2 * line + h][t];
   }
 }
 // Lane l: block l / 16 of run j of row l % 16.
 __device__ __forceinline__ int w_get(int j) {
   const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
-  return 128 * (j >> 1) + 8 * r + ((4 * (j & 1) + q) ^ (r >> 1));
+  return 8 * r + ((4 * (j & 1) + q) ^ (r >> 1));
 }
 
 // Adds a run's products: c the tiles' blocks, ws their packed scales, x the run's
@@ -361,16 +320,138 @@ __device__ __forceinline__ void add_run(const u32x4 (&c)[NT], const uint32_t (&w
   }
 }
 
+// Few outputs: eight waves split dim for the same 16 NT outputs of 16 MT rows, all
+// operands straight from memory, kFlight runs' loads together; their sums meet in
+// LDS in a fixed order.
+constexpr int kSplitWaves = 8;
+
+template <int MT, int NT, int kX>
+__global__ __launch_bounds__(64 * kSplitWaves, 2) void mx4_split_kernel(const Mx4ProjArgs a) {
+  using X = XOperand<kX>;
+  constexpr int P = X::kPieces, kOctets = kX == SAS_TYPE_MX4 ? 1 : 4;
+  constexpr int kFlight = kX == SAS_TYPE_MX4 ? 4 : MT == 1 && kX == SAS_TYPE_BF16 ? 4 : MT == 1 ? 2 : 1;
+  __shared__ f32x4 part[kSplitWaves][MT * NT][64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r = lane & 15, q = lane >> 4;
+  const int mtiles = (a.rows + 16 * MT - 1) / (16 * MT);
+  const int pos = xcd_run((int)blockIdx.x, (int)gridDim.x);
+  const int m0 = (pos % mtiles) * 16 * MT, n0 = (pos / mtiles) * 16 * NT;
+  const int blocks = (a.dim + kBlock - 1) / kBlock, runs = (blocks + 3) / 4;
+  const int g0 = runs * wave / kSplitWaves, g1 = runs * (wave + 1) / kSplitWaves;
+  const int size = kX == SAS_TYPE_MX4 ? 16 * blocks : a.dim;
+  const uint8_t *wr[NT], *wsr[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int64_t row = min(n0 + 16 * t + r, a.out_dim - 1);
+    wr[t] = a.w + row * a.w_stride;
+    wsr[t] = a.w_scales + row * a.w_scales_stride;
+  }
+  const char *xr[MT];
+  const uint8_t *xsr[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    const int64_t row = min(m0 + 16 * m + r, a.rows - 1);
+    xr[m] = static_cast<const char *>(a.x) + row * a.x_stride * kXSize<kX>;
+    xsr[m] = kX == SAS_TYPE_MX4 ? a.x_scales + row * a.x_scales_stride : nullptr;
+  }
+  f32x4 acc[MT][NT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int t = 0; t < NT; ++t) acc[m][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int g4 = g0; g4 < g1; g4 += 4) {
+  uint32_t ws[NT], xs[MT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) ws[t] = load_scales_of(wsr[t], g4, blocks);
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+    if constexpr (kX == SAS_TYPE_MX4) xs[m] = load_scales_of(xsr[m], g4, blocks);
+  each_const<4 / kFlight>([&](auto part_of) __attribute__((always_inline)) {
+    const int g = g4 + kFlight * decltype(part_of)::value;
+    u32x4 w[kFlight][NT];
+    XPart<kX> x[kFlight][MT][kOctets];
+#pragma unroll
+    for (int u = 0; u < kFlight; ++u) {
+      // (past the wave's last run, and the row's last block, what is there again:
+      // x_pieces makes zeros of the hidden states)
+      const int b = min(4 * min(g + u, g1 - 1) + q, blocks - 1);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) w[u][t] = *reinterpret_cast<const u32x4 *>(wr[t] + 16 * b);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+#pragma unroll
+        for (int i = 0; i < kOctets; ++i) {
+          const int at = kX == SAS_TYPE_MX4 ? 16 * b : kBlock * b + 8 * i;
+          x[u][m][i] = x_load<kX>(xr[m] + (int64_t)x_within<kX>(at, size) * kXSize<kX>);
+        }
+      }
+    }
+    if constexpr (decltype(part_of)::value == 0) {
+      const uint32_t mask = scale_mask_of(g4, blocks);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) ws[t] = pack_scales(ws[t], mask);
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+        if constexpr (kX == SAS_TYPE_MX4) xs[m] = pack_scales(xs[m], mask);
+    }
+    each_const<kFlight>([&](auto ut) __attribute__((always_inline)) {
+      constexpr int u = decltype(ut)::value, j = kFlight * decltype(part_of)::value + u;
+      const int b = 4 * (g + u) + q;
+      const bool in = g + u < g1 && b < blocks;
+#pragma unroll
+      for (int i = 0; i < kOctets; ++i) {
+        u32x4 wv[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          if constexpr (kX == SAS_TYPE_MX4) wv[t] = w[u][t];
+          else wv[t] = widen(w[u][t][i], scale_byte<j>(ws[t]));
+        }
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          u32x4 o[P];
+          x_pieces<kX>(x[u][m][i], in ? (kX == SAS_TYPE_MX4 ? 16 * b : kBlock * b + 8 * i) : size, size, o);
+#pragma unroll
+          for (int p = 0; p < P; ++p)
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+              if constexpr (kX == SAS_TYPE_MX4) acc[m][t] = mfma4<j>(wv[t], ws[t], o[p], xs[m], acc[m][t]);
+              else acc[m][t] = mfma(wv[t], o[p], acc[m][t]);
+            }
+        }
+      }
+    });
+  });
+  }
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int t = 0; t < NT; ++t) part[wave][m * NT + t][lane] = acc[m][t];
+  __syncthreads();
+  for (int i = wave; i < MT * NT; i += kSplitWaves) {
+    f32x4 v = part[0][i][lane];
+#pragma unroll
+    for (int k = 1; k < kSplitWaves; ++k) v = v + part[k][i][lane];
+    const int row = m0 + 16 * (i / NT) + r;
+    if (row < a.rows) finish4(a, row, n0 + 16 * (i % NT) + 4 * q, v);
+  }
+}
+
+template <int MT, int NT, int kX>
+void launch_split(const Mx4ProjArgs &a, hipStream_t stream) {
+  const int blocks = ((a.rows + 16 * MT - 1) / (16 * MT)) * ((a.out_dim + 16 * NT - 1) / (16 * NT));
+  mx4_split_kernel<MT, NT, kX><<<blocks, 64 * kSplitWaves, 0, stream>>>(a);
+}
+
 // Few rows, hidden states that fit in LDS: every block holds all of them, and its
 // waves take 16 NT outputs after another, their weight rows two super-runs
 // ahead in registers; no barrier after the first.
 // kPack: up to kMx4Few rows of f32, whose pieces are rows of one operand (row r's
 // piece p is row kMx4Few p + r): a third of the products.
-constexpr int kStreamWaves = 8;
-constexpr int kStreamSlots = 128 * 1024 / 16;
+constexpr int kStreamWaves = 12;
+constexpr int kStreamSlots = 136 * 1024 / 16;
 
 template <int MT, int NT, int kX, bool kPack>
-__global__ __launch_bounds__(64 * kStreamWaves, 2) void mx4_stream_kernel(const Mx4ProjArgs a) {
+__global__ __launch_bounds__(64 * kStreamWaves, 3) void mx4_stream_kernel(const Mx4ProjArgs a) {
   using X = XOperand<kX>;
   constexpr int P = kPack ? 1 : X::kPieces, kSubs = MT * P;
   // the hidden states (MX4: then their scales, [super-run][subtile][lane])
@@ -385,11 +466,10 @@ __global__ __launch_bounds__(64 * kStreamWaves, 2) void mx4_stream_kernel(const 
   const int groups = (a.out_dim + 16 * NT - 1) / (16 * NT);
   const int total = gw < groups ? (groups - gw + waves - 1) / waves * supers : 0;
   WRows<NT> w;
-  int lg = gw, ls = 0;  // the next super-run to load
+  int lg = gw, ls = 0;  // the super-run to load
   w.set(a, 16 * NT * lg);
   // (past the last super-run the last again)
-  auto load = [&](WSuper<NT> &b) __attribute__((always_inline)) {
-    w.template load<true>(b, ls, blocks);
+  auto advance = [&] {
     if (++ls == supers) {
       if (lg + waves < groups) {
         lg += waves;
@@ -401,21 +481,23 @@ __global__ __launch_bounds__(64 * kStreamWaves, 2) void mx4_stream_kernel(const 
     }
   };
   WSuper<NT> b0, b1;
-  load(b0);
-  load(b1);
-  // the hidden states, zeros past dim and the last row
+  w.template load<true>(b0, ls, blocks);
+  advance();
+  w.template load<true>(b1, ls, blocks);
+  // the hidden states, zeros past dim (rows past the last: the last again)
   {
     const int size = kX == SAS_TYPE_MX4 ? 16 * blocks : a.dim;
-    const int64_t bytes = a.x_stride * (kX == SAS_TYPE_F32 ? 4 : kX == SAS_TYPE_BF16 ? 2 : 1);
+    const int64_t bytes = a.x_stride * kXSize<kX>;
     constexpr int kRunSize = kX == SAS_TYPE_MX4 ? 64 : kRun;
     for (int i = wave; i < MT * X::kLoads * runs; i += kStreamWaves) {
       const int f = i % X::kLoads, m = i / X::kLoads % MT, run = i / X::kLoads / MT;
       const int xr = x_row<kX>(f), row = 16 * m + xr;
       if (kPack && (f & 1)) continue;
-      const XPart<kX> p = x_load<kX>(static_cast<const char *>(a.x) + (int64_t)min(row, a.rows - 1) * bytes, kRunSize * run + x_at<kX>(f),
-                                     row < a.rows ? size : 0);
+      const int at = kRunSize * run + x_at<kX>(f);
+      const XPart<kX> p = x_load<kX>(static_cast<const char *>(a.x) + (int64_t)min(row, a.rows - 1) * bytes +
+                                     (int64_t)x_within<kX>(at, size) * kXSize<kX>);
       u32x4 o[X::kPieces];
-      x_pieces<kX>(p, o);
+      x_pieces<kX>(p, at, size, o);
 #pragma unroll
       for (int k = 0; k < X::kPieces; ++k) {
         if constexpr (kPack) {
@@ -431,7 +513,7 @@ __global__ __launch_bounds__(64 * kStreamWaves, 2) void mx4_stream_kernel(const 
     if constexpr (kX == SAS_TYPE_MX4) {
       for (int i = wave; i < MT * supers; i += kStreamWaves) {
         const int m = i % MT, s = i / MT, row = min(16 * m + r, a.rows - 1);
-        xsc[i * 64 + lane] = pack_scales(load_scales(a.x_scales + (int64_t)row * a.x_scales_stride, s, blocks), q, s, blocks);
+        xsc[i * 64 + lane] = pack_scales(load_scales(a.x_scales + (int64_t)row * a.x_scales_stride, s, blocks), scale_mask(s, blocks));
       }
     }
   }
@@ -448,17 +530,23 @@ __global__ __launch_bounds__(64 * kStreamWaves, 2) void mx4_stream_kernel(const 
   u32x4 *wl = wls[wave];
   // a super-run out of b, which then takes the one two ahead
   auto compute = [&](WSuper<NT> &b) __attribute__((always_inline)) {
+    advance();  // (not behind a product: see the wide kernel)
     uint32_t ws[NT];
+    const uint32_t mask = scale_mask(s, blocks);
 #pragma unroll
-    for (int t = 0; t < NT; ++t) ws[t] = pack_scales(b.s[t], q, s, blocks);
-    wave_lds_sync();
-    w_put<NT>(wl, b);
-    __builtin_amdgcn_sched_barrier(0);
-    load(b);
-    wave_lds_sync();
-    __builtin_amdgcn_sched_barrier(0);
+    for (int t = 0; t < NT; ++t) ws[t] = pack_scales(b.s[t], mask);
     each_const<4>([&](auto jt) __attribute__((always_inline)) {
       constexpr int j = decltype(jt)::value;
+      if constexpr (j % 2 == 0) {
+        wave_lds_sync();
+        w_put<NT>(wl, b, j / 2);
+        if constexpr (j == 2) {
+          __builtin_amdgcn_sched_barrier(0);
+          w.template load<true>(b, ls, blocks);
+        }
+        wave_lds_sync();
+        __builtin_amdgcn_sched_barrier(0);
+      }
       u32x4 c[NT];
 #pragma unroll
       for (int t = 0; t < NT; ++t) c[t] = wl[kWSlots * t + w_get(j)];
@@ -469,15 +557,11 @@ __global__ __launch_bounds__(64 * kStreamWaves, 2) void mx4_stream_kernel(const 
       float *stage = reinterpret_cast<float *>(wl);
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
-        by_rows<NT>(stage, acc[m], [&](int row, int col, f32x4 v) __attribute__((always_inline)) {
-          if constexpr (kPack) {
-            if (row >= a.rows) return;
-            const float *st = stage + row * (16 * NT + 4) + col;
-            const f32x4 v1 = *reinterpret_cast<const f32x4 *>(st + kMx4Few * (16 * NT + 4));
-            const f32x4 v2 = *reinterpret_cast<const f32x4 *>(st + 2 * kMx4Few * (16 * NT + 4));
-            v = (v2 + v1) + v;
-          }
-          if (16 * m + row < a.rows) finish4(a, 16 * m + row, n0 + col, v);
+        stage_rows<NT>(stage, acc[m]);
+        put_rows<NT>(a, 16 * m, n0, [&](int row, int col) __attribute__((always_inline)) {
+          f32x4 v = staged<NT>(stage, row, col);
+          if constexpr (kPack) v = (staged<NT>(stage, row + 2 * kMx4Few, col) + staged<NT>(stage, row + kMx4Few, col)) + v;
+          return v;
         });
 #pragma unroll
         for (int t = 0; t < NT; ++t) acc[m][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -509,36 +593,53 @@ void launch_stream(const Mx4ProjArgs &a, hipStream_t stream) {
   mx4_stream_kernel<MT, NT, kX, kPack><<<blocks, 64 * kStreamWaves, 0, stream>>>(a);
 }
 
-// Many outputs: WM x WN waves, a wave 16 MT rows x 16 NT outputs; the hidden
-// states' chunks of kChunk runs in LDS, the next one on its way in registers,
-// weight rows one super-run ahead in registers.
+// Many outputs: eight waves share the hidden states of 16 MT rows and take 16 NT
+// outputs each; the hidden states' chunks of kChunk runs in LDS, the next one on
+// its way in registers, weight rows one super-run ahead in registers.  kOnce: one
+// tile has all rows, and a block takes one group of outputs after another, its
+// loads going on across them.
+// A step is one operand of each subtile: its products come with the reads of the
+// next step's operands, so that no product waits for LDS; the next chunk is
+// stored half-way, and the barrier that shows it stands before the last step.
 constexpr int kWideWaves = 8;
-template <int MT, int WM, int NT, int kX>
+template <int MT, int NT, int kX>
 struct Wide4 {
-  static constexpr int kWN = kWideWaves / WM, kRows = 16 * MT * WM, kOuts = 16 * NT * kWN;
-  static constexpr int S = MT * WM, P = XOperand<kX>::kPieces, kSubs = S * P;
+  static constexpr int kRows = 16 * MT, kOuts = 16 * NT * kWideWaves;
+  static constexpr int P = XOperand<kX>::kPieces, kSubs = MT * P;
   static constexpr int kChunk = kX == SAS_TYPE_MX4 ? 4 : kSubs <= 2 ? 4 : kSubs <= 4 ? 2 : 1;
   static constexpr int kXSlots = 2 * kChunk * kSubs * XOperand<kX>::kSlots;
-  // Rows that bound the matrix instructions (WM > 1) take their weights straight.
-  static constexpr bool kDirect = WM > 1;
-  static constexpr int kWave = kDirect ? kStage<NT> / 4 : NT * kWSlots;  // 16-byte slots of a wave
-  static constexpr int kLoads = S * XOperand<kX>::kLoads * kChunk;
+  static constexpr int kWave = NT * kWSlots + kStage<NT> / 4;  // 16-byte slots of a wave: weight rows, sums
+  static constexpr int kLoads = MT * XOperand<kX>::kLoads * kChunk;
   static constexpr int kMine = (kLoads + kWideWaves - 1) / kWideWaves;
+  static constexpr int kRunSteps = kX == SAS_TYPE_MX4 ? 1 : 4;   // operands of a run
+  static constexpr int kChunkSteps = kChunk * kRunSteps;
 };
 
-template <int MT, int WM, int NT, int kX, bool kOnce>
+constexpr int kTileRows = 4;
+
+template <int MT, int NT, int kX, bool kOnce, bool kTail>
 __global__ __launch_bounds__(64 * kWideWaves, 2) void mx4_wide_kernel(const Mx4ProjArgs a) {
   using X = XOperand<kX>;
-  using C = Wide4<MT, WM, NT, kX>;
-  constexpr int P = C::P, S = C::S, kChunk = C::kChunk;
+  using C = Wide4<MT, NT, kX>;
+  constexpr int P = C::P, kChunk = C::kChunk, kRunSteps = C::kRunSteps, kChunkSteps = C::kChunkSteps;
   __shared__ u32x4 xs[C::kXSlots];
   __shared__ u32x4 wls[kWideWaves][C::kWave];
-  __shared__ uint32_t xsc[kX == SAS_TYPE_MX4 ? 2 * S * 64 : 1];
+  __shared__ uint32_t xsc[kX == SAS_TYPE_MX4 ? 2 * MT * 64 : 1];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int r = lane & 15, q = lane >> 4, wm = wave % WM, wn = wave / WM;
+  const int r = lane & 15;
+  const int groups = (a.out_dim + C::kOuts - 1) / C::kOuts;
   const int mtiles = kOnce ? 1 : (a.rows + C::kRows - 1) / C::kRows;
-  const int pos = xcd_run((int)blockIdx.x, (int)gridDim.x);
-  const int m0 = (pos % mtiles) * C::kRows, n0 = (pos / mtiles) * C::kOuts + wn * 16 * NT;
+  const int pos = kOnce ? (int)blockIdx.x : xcd_run((int)blockIdx.x, (int)gridDim.x);
+  // tiles in the order of kTileRows of them by all groups: the 32 blocks that an
+  // XCD runs at a time share rows and weights out of its L2
+  int mt = 0, g = pos;
+  if constexpr (!kOnce) {
+    const int band = pos / (kTileRows * groups), at = pos % (kTileRows * groups);
+    const int rows = min(mtiles - kTileRows * band, kTileRows);
+    mt = kTileRows * band + at % rows;
+    g = at / rows;
+  }
+  const int m0 = mt * C::kRows, gstep = kOnce ? (int)gridDim.x : groups;
   const int blocks = (a.dim + kBlock - 1) / kBlock, supers = (blocks + 15) / 16, chunks = supers * (4 / kChunk);
   f32x4 acc[MT][NT];
 #pragma unroll
@@ -546,18 +647,30 @@ __global__ __launch_bounds__(64 * kWideWaves, 2) void mx4_wide_kernel(const Mx4P
 #pragma unroll
     for (int t = 0; t < NT; ++t) acc[m][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   WRows<NT> w;
-  w.template set<C::kDirect>(a, n0);
+  int lg = g, ls = 0;  // the super-run to load
+  w.set(a, lg * C::kOuts + wave * 16 * NT);
+  // (past the last one the last group's first again)
+  auto advance = [&] {
+    if (++ls == supers) {
+      ls = 0;
+      if (lg + gstep < groups) {
+        lg += gstep;
+        w.set(a, lg * C::kOuts + wave * 16 * NT);
+      }
+    }
+  };
   // This wave's loads of a chunk: load i = wave + 8 n is load f of operand (run,
   // subtile), in the order f, subtile, run (a subtile's f and, where a run has
   // as many loads as there are waves, its subtile are the wave's).
-  static_assert(S == 1 || S == 2 || S == 4 || S == 8, "a power of two");
+  static_assert(MT == 1 || MT == 2 || MT == 4 || MT == 8, "a power of two");
   constexpr int kFirst = X::kLoads == 4 ? 2 : 8;  // subtiles that the waves take together
   const int size = kX == SAS_TYPE_MX4 ? 16 * blocks : a.dim;
-  constexpr int kSize = kX == SAS_TYPE_F32 ? 4 : kX == SAS_TYPE_BF16 ? 2 : 1, kRunSize = kX == SAS_TYPE_MX4 ? 64 : kRun;
-  const int f = wave % X::kLoads, i0 = wave / X::kLoads;
-  auto sub_of = [&](int n) { return (i0 + kFirst * n) % S; };
-  auto run_of = [&](int n) { return (i0 + kFirst * n) / S; };
-  constexpr int kXRows = S <= kFirst ? 1 : S / kFirst;  // different subtiles of a wave
+  constexpr int kSize = kXSize<kX>, kRunSize = kX == SAS_TYPE_MX4 ? 64 : kRun;
+  // (fewer loads than waves: the same again)
+  const int f = wave % X::kLoads, i0 = wave % C::kLoads / X::kLoads;
+  auto sub_of = [&](int n) { return (i0 + kFirst * n) % MT; };
+  auto run_of = [&](int n) { return (i0 + kFirst * n) / MT; };
+  constexpr int kXRows = MT <= kFirst ? 1 : MT / kFirst;  // different subtiles of a wave
   const char *xbase = static_cast<const char *>(a.x) + (int64_t)m0 * a.x_stride * kSize;
   uint32_t xrow[kXRows];
 #pragma unroll
@@ -565,87 +678,145 @@ __global__ __launch_bounds__(64 * kWideWaves, 2) void mx4_wide_kernel(const Mx4P
     xrow[n] = (uint32_t)min(16 * sub_of(n) + x_row<kX>(f), a.rows - 1 - m0) * ((uint32_t)a.x_stride * kSize);
   const int xput = x_put<kX>(f, x_row<kX>(f));
   XPart<kX> x[C::kMine];
-  Scales xsv;
-  const uint8_t *xscale_row = kX == SAS_TYPE_MX4 ? a.x_scales + (int64_t)min(m0 + 16 * (wave % S) + r, a.rows - 1) * a.x_scales_stride : nullptr;
+  uint32_t xsv = 0;
+  const uint8_t *xscale_row = kX == SAS_TYPE_MX4 ? a.x_scales + (int64_t)min(m0 + 16 * (wave % MT) + r, a.rows - 1) * a.x_scales_stride : nullptr;
+  auto x_first = [&](int chunk, int n) { return kRunSize * (chunk * kChunk + run_of(n)) + x_at<kX>(f); };
   auto load_x = [&](int chunk) __attribute__((always_inline)) {
 #pragma unroll
     for (int n = 0; n < C::kMine; ++n)
-      x[n] = x_load<kX>(xbase + xrow[n % kXRows], kRunSize * (chunk * kChunk + run_of(n)) + x_at<kX>(f), size);
-    if constexpr (kX == SAS_TYPE_MX4) {
-      if (wave < S) xsv = load_scales(xscale_row, chunk, blocks);
-    }
+      x[n] = kTail ? x_load<kX>(xbase + (xrow[n % kXRows] + (uint32_t)(x_within<kX>(x_first(chunk, n), size) * kSize)))
+                   : x_load<kX>(xbase + (int64_t)chunk * (kRunSize * kChunk * kSize) + (xrow[n % kXRows] + (uint32_t)(x_first(0, n) * kSize)));
+    if constexpr (kX == SAS_TYPE_MX4) xsv = load_scales<kTail>(xscale_row, chunk, blocks);
   };
   auto store_x = [&](int buf, int chunk) __attribute__((always_inline)) {
 #pragma unroll
     for (int n = 0; n < C::kMine; ++n) {
-      if (C::kLoads % kWideWaves != 0 && wave + kWideWaves * n >= C::kLoads) continue;
       u32x4 o[X::kPieces];
-      x_pieces<kX>(x[n], o);
+      x_pieces<kX>(x[n], kTail ? x_first(chunk, n) : 0, kTail ? size : 1, o);
 #pragma unroll
       for (int p = 0; p < P; ++p) xs[((buf * kChunk + run_of(n)) * C::kSubs + P * sub_of(n) + p) * X::kSlots + xput] = o[p];
     }
-    if constexpr (kX == SAS_TYPE_MX4) {
-      if (wave < S) xsc[(buf * S + wave) * 64 + lane] = pack_scales(xsv, q, chunk, blocks);
-    }
+    if constexpr (kX == SAS_TYPE_MX4) xsc[(buf * MT + wave % MT) * 64 + lane] = pack_scales<kTail>(xsv, scale_mask(chunk, blocks));
   };
+  auto after = [&](int chunk) { return chunk + 1 == chunks ? 0 : chunk + 1; };
   int get[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) get[i] = x_get<kX>(i);
-  WSuper<NT> b;
-  load_x(0);
-  if constexpr (C::kDirect) w.load_direct(b, 0, blocks);
-  else w.template load<kOnce>(b, 0, blocks);
-  store_x(0, 0);
-  lds_barrier();
   u32x4 *wl = wls[wave];
-  for (int s = 0; s < supers; ++s) {
-    uint32_t ws[NT];
+  // the operands of the next step, as they are read: hidden states, a run's
+  // weights, MX4: a super-run's scales of the hidden states
+  u32x4 xf[P * MT], c[NT];
+  uint32_t xscale[MT];
+  auto read_x = [&](int buf, int run, int i, int n) __attribute__((always_inline)) {
+    xf[n] = xs[((buf * kChunk + run) * C::kSubs + n) * X::kSlots + get[i]];
+  };
+  auto read_c = [&](int j) __attribute__((always_inline)) {
 #pragma unroll
-    for (int t = 0; t < NT; ++t) ws[t] = pack_scales(b.s[t], q, s, blocks);
-    const int ns = min(s + 1, supers - 1);
-    if constexpr (C::kDirect) {
+    for (int t = 0; t < NT; ++t) c[t] = wl[kWSlots * t + w_get(j)];
+  };
+  // A line of the weight rows into LDS, and the next super-run's loads once the
+  // second one is there.
+  WSuper<NT> b;
+  auto line = [&](int l) __attribute__((always_inline)) {
+    wave_lds_sync();
+    w_put<NT>(wl, b, l);
+    if (l == 1) w.template load<kOnce, kTail>(b, ls, blocks);
+    wave_lds_sync();
+  };
+  load_x(0);
+  w.template load<kOnce, kTail>(b, ls, blocks);
+  store_x(0, 0);
+  load_x(after(0));
+  lds_barrier();
 #pragma unroll
-      for (int t = 0; t < NT; ++t) b.s[t] = load_scales(w.scales[t] + w.scale_at[t], ns, blocks);
-    } else {
-      wave_lds_sync();
-      w_put<NT>(wl, b);
-      __builtin_amdgcn_sched_barrier(0);
-      load_x(min(s * (4 / kChunk) + 1, chunks - 1));
-      w.template load<kOnce>(b, ns, blocks);
-      wave_lds_sync();
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    each_const<4>([&](auto jt) __attribute__((always_inline)) {
-      constexpr int j = decltype(jt)::value;
-      const int chunk = s * (4 / kChunk) + j / kChunk, buf = chunk & 1;
-      if constexpr ((C::kDirect || j != 0) && j % kChunk == 0) load_x(min(chunk + 1, chunks - 1));
-      u32x4 c[NT];
+  for (int n = 0; n < P * MT; ++n) read_x(0, 0, 0, n);
+  if constexpr (kX == SAS_TYPE_MX4) {
 #pragma unroll
-      for (int t = 0; t < NT; ++t) c[t] = C::kDirect ? b.c[j][t] : wl[kWSlots * t + w_get(j)];
-      if constexpr (C::kDirect) w.load_direct_run(b, j, ns, blocks);
-      add_run<MT, NT, kX, P, j>(c, ws, xs + ((buf * kChunk + j % kChunk) * C::kSubs + P * MT * wm) * X::kSlots, get,
-                                xsc + (buf * S + MT * wm) * 64 + lane, acc);
-      if constexpr (j % kChunk == kChunk - 1) {
-        __builtin_amdgcn_sched_barrier(0);
-        store_x(buf ^ 1, min(chunk + 1, chunks - 1));
-        lds_barrier();
-      }
-    });
+    for (int m = 0; m < MT; ++m) xscale[m] = xsc[m * 64 + lane];
   }
+  line(0);
+  read_c(0);
+  int first = 0;  // the buffer of the super-run's first chunk
+  for (; g < groups; g += gstep) {
+    for (int s = 0; s < supers; ++s) {
+      // (here: behind the products, its branch would have the compiler move them
+      // past it, and all their operands would have to wait in registers)
+      advance();
+      uint32_t ws[NT];
+      const uint32_t mask = scale_mask(s, blocks);
 #pragma unroll
-  for (int m = 0; m < MT; ++m)
-    by_rows<NT>(reinterpret_cast<float *>(wl), acc[m], [&](int row, int col, f32x4 v) __attribute__((always_inline)) {
-      const int at = m0 + 16 * (MT * wm + m) + row;
-      if (at < a.rows) finish4(a, at, n0 + col, v);
-    });
+      for (int t = 0; t < NT; ++t) ws[t] = pack_scales<kTail>(b.s[t], mask);
+      each_const<4 * kRunSteps>([&](auto st) __attribute__((always_inline)) {
+        // step i of run j, the e-th of its chunk; the next one: step i2 of run j2
+        constexpr int step = decltype(st)::value, j = step / kRunSteps, i = step % kRunSteps, e = step % kChunkSteps;
+        constexpr int j2 = (step + 1) / kRunSteps % 4, i2 = (step + 1) % kRunSteps;
+        const int buf = (first + j / kChunk) & 1, chunk = s * (4 / kChunk) + j / kChunk;
+        // the chunk after this one is in registers: into the other buffer, whose
+        // last reads lie before the barrier of the chunk before
+        if constexpr (e == kChunkSteps / 2 - 1) {
+          const int next = after(chunk);
+          store_x(buf ^ 1, next);
+          load_x(after(next));
+        }
+        u32x4 wv[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          if constexpr (kX == SAS_TYPE_MX4) wv[t] = c[t];
+          else wv[t] = widen(c[t][i], scale_byte<j>(ws[t]));
+        }
+        if constexpr (i2 == 0) {
+          if constexpr (j2 % 2 == 0) line(j2 / 2);
+          read_c(j2);
+        }
+        const int buf2 = e == kChunkSteps - 1 ? buf ^ 1 : buf;
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          uint32_t xv = 0;
+          if constexpr (kX == SAS_TYPE_MX4) {
+            xv = xscale[m];
+            if constexpr (step == 3) xscale[m] = xsc[(buf2 * MT + m) * 64 + lane];
+          }
+#pragma unroll
+          for (int p = 0; p < P; ++p) {
+            const u32x4 o = xf[P * m + p];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+              if constexpr (kX == SAS_TYPE_MX4) acc[m][t] = mfma4<j>(wv[t], ws[t], o, xv, acc[m][t]);
+              else acc[m][t] = mfma(wv[t], o, acc[m][t]);
+            }
+            read_x(buf2, j2 % kChunk, i2, P * m + p);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (e == kChunkSteps - 2) lds_barrier();
+      });
+      first = (first + 4 / kChunk) & 1;
+    }
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      float *stage = reinterpret_cast<float *>(wl + NT * kWSlots);
+      stage_rows<NT>(stage, acc[m]);
+      put_rows<NT>(a, m0 + 16 * m, g * C::kOuts + wave * 16 * NT,
+                   [&](int row, int col) __attribute__((always_inline)) { return staged<NT>(stage, row, col); });
+#pragma unroll
+      for (int t = 0; t < NT; ++t) acc[m][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+  }
 }
 
-template <int MT, int WM, int NT, int kX>
+template <int MT, int NT, int kX>
 void launch_wide(const Mx4ProjArgs &a, hipStream_t stream) {
-  using C = Wide4<MT, WM, NT, kX>;
-  const int mtiles = (a.rows + C::kRows - 1) / C::kRows, blocks = mtiles * ((a.out_dim + C::kOuts - 1) / C::kOuts);
-  if (mtiles == 1) mx4_wide_kernel<MT, WM, NT, kX, true><<<blocks, 64 * kWideWaves, 0, stream>>>(a);
-  else mx4_wide_kernel<MT, WM, NT, kX, false><<<blocks, 64 * kWideWaves, 0, stream>>>(a);
+  using C = Wide4<MT, NT, kX>;
+  const int mtiles = (a.rows + C::kRows - 1) / C::kRows, groups = (a.out_dim + C::kOuts - 1) / C::kOuts;
+  const int blocks = mtiles > 1 ? mtiles * groups : groups < a.cus ? groups : a.cus;
+  // whole super-runs have no blocks to mask
+  if (a.dim % kSuper == 0) {
+    if (mtiles == 1) mx4_wide_kernel<MT, NT, kX, true, false><<<blocks, 64 * kWideWaves, 0, stream>>>(a);
+    else mx4_wide_kernel<MT, NT, kX, false, false><<<blocks, 64 * kWideWaves, 0, stream>>>(a);
+  } else {
+    if (mtiles == 1) mx4_wide_kernel<MT, NT, kX, true, true><<<blocks, 64 * kWideWaves, 0, stream>>>(a);
+    else mx4_wide_kernel<MT, NT, kX, false, true><<<blocks, 64 * kWideWaves, 0, stream>>>(a);
+  }
 }
 
 }  // namespace

@@ -102,41 +102,47 @@ class Mx4:
     of 32, device tensors with unit element stride whose rows lie a multiple of
     16 and of 4 bytes apart."""
 
+    __slots__ = ("codes", "scales", "dim", "shape")
+
     def __init__(self, codes, scales, dim: int):
-        blocks = (int(dim) + 31) // 32
+        dim = int(dim)
+        if dim < 1:
+            raise ValueError("dim must be >= 1")
+        blocks = (dim + 31) // 32
         for name, t, n in (("codes", codes, 16 * blocks), ("scales", scales, blocks)):
-            if t.dim() != 2 or str(t.dtype) != "torch.uint8" or t.stride(1) != 1 or not t.is_cuda:
+            size = t.shape
+            if len(size) != 2 or t.element_size() != 1 or str(t.dtype) != "torch.uint8" or t.stride(1) != 1 or not t.is_cuda:
                 raise ValueError(f"{name} must be a 2-D uint8 device tensor with unit element stride")
-            if t.shape[1] < n:
+            if size[1] < n:
                 raise ValueError(f"{name} must hold {n} bytes a row for dim {dim}")
         if codes.shape[0] != scales.shape[0]:
             raise ValueError("codes and scales must hold the same rows")
-        if dim < 1:
-            raise ValueError("dim must be >= 1")
-        self.codes, self.scales, self.dim = codes, scales, int(dim)
+        self.codes, self.scales, self.dim, self.shape = codes, scales, dim, (codes.shape[0], dim)
 
     @classmethod
     def empty(cls, rows: int, dim: int, device="cuda") -> "Mx4":
         """Rows whose bytes are not set, as quantize_mx4_into takes them."""
         import torch
-        blocks = (int(dim) + 31) // 32
-        return cls(torch.empty((rows, 16 * blocks), dtype=torch.uint8, device=device),
-                   torch.empty((rows, (blocks + 3) // 4 * 4), dtype=torch.uint8, device=device), dim)
-
-    @property
-    def shape(self):
-        return (self.codes.shape[0], self.dim)
+        dim = int(dim)
+        if dim < 1:
+            raise ValueError("dim must be >= 1")
+        blocks = (dim + 31) // 32
+        new = cls.__new__(cls)
+        new.codes = torch.empty((rows, 16 * blocks), dtype=torch.uint8, device=device)
+        new.scales = torch.empty((rows, (blocks + 3) // 4 * 4), dtype=torch.uint8, device=device)
+        new.dim, new.shape = dim, (int(rows), dim)
+        return new
 
     @property
     def device(self):
         return self.codes.device
 
     def to_c(self) -> SasMx4:
-        blocks = (self.dim + 31) // 32
+        if self.shape[0] > 1:
+            return SasMx4(self.codes.data_ptr(), self.codes.stride(0), self.scales.data_ptr(), self.scales.stride(0))
         # (a table of one row may have any stride)
-        one = self.codes.shape[0] <= 1
-        return SasMx4(self.codes.data_ptr(), 16 * blocks if one else self.codes.stride(0), self.scales.data_ptr(),
-                      (blocks + 3) // 4 * 4 if one else self.scales.stride(0))
+        blocks = (self.dim + 31) // 32
+        return SasMx4(self.codes.data_ptr(), 16 * blocks, self.scales.data_ptr(), (blocks + 3) // 4 * 4)
 
 
 PARAMS_DTYPE = np.dtype([("temperature", "<f8"), ("top_p", "<f8"), ("repetition_penalty", "<f8"),
@@ -221,6 +227,17 @@ def _ptr(t, kind: Optional[str] = None, name: str = "tensor") -> Optional[int]:
             raise ValueError(f"{name} must hold {want} elements (got {t.dtype})")
         _seen[kind, t.dtype] = True
     return t.data_ptr()
+
+
+_types: dict = {}  # torch dtype -> SAS_TYPE_*
+
+
+def _type_of(t) -> Optional[int]:
+    """SAS_TYPE_* of a tensor's elements; None for any other."""
+    if not _types:
+        import torch
+        _types.update({torch.float32: _capi.TYPE_F32, torch.bfloat16: _capi.TYPE_BF16, torch.float16: _capi.TYPE_F16})
+    return _types.get(t.dtype)
 
 
 _current_stream = None
@@ -607,16 +624,14 @@ class Sampler:
     def quantize_mx4_into(self, x, out: Mx4, *, stream=None) -> None:
         """sas_quantize_mx4: rounds x [rows][dim] (float32, bfloat16 or float16)
         into out's first rows."""
-        types = {"torch.float32": _capi.TYPE_F32, "torch.bfloat16": _capi.TYPE_BF16, "torch.float16": _capi.TYPE_F16}
-        if x.dim() != 2 or x.stride(1) != 1 or not x.is_cuda or str(x.dtype) not in types:
+        size, kind = x.shape, _type_of(x)
+        if len(size) != 2 or kind is None or x.stride(1) != 1 or not x.is_cuda:
             raise ValueError("x must be a 2-D float32, bfloat16 or float16 device tensor with unit element stride")
-        if out.shape[0] < x.shape[0] or out.dim != x.shape[1]:
+        rows, dim = size
+        if out.shape[0] < rows or out.dim != dim:
             raise ValueError("out must hold x's rows of x's dim")
-        d = SasMx4Quantization()
-        d.x, d.x_type = x.data_ptr(), types[str(x.dtype)]
-        d.rows, d.dim = x.shape
-        d.x_stride = x.stride(0) if x.shape[0] > 1 else x.shape[1]
-        d.out = out.to_c()
+        # (a tensor of one row may have any stride; its row is the whole of it)
+        d = SasMx4Quantization(x.data_ptr(), x.stride(0) if rows > 1 else dim, kind, rows, dim, out.to_c())
         check(self._lib.sas_quantize_mx4(self._h, ctypes.byref(d), _stream(stream)), self._h)
 
     def quantize_mx4(self, x, *, stream=None) -> Mx4:
@@ -632,18 +647,16 @@ class Sampler:
         """sas_lookup_mx4: out [rows][dim] (float32, bfloat16 or float16) = the
         table's rows ids (4-byte integers; one past the table gives zeros), or its
         first rows in order."""
-        types = {"torch.float32": _capi.TYPE_F32, "torch.bfloat16": _capi.TYPE_BF16, "torch.float16": _capi.TYPE_F16}
-        if out.dim() != 2 or out.stride(1) != 1 or not out.is_cuda or str(out.dtype) not in types:
+        size, kind = out.shape, _type_of(out)
+        if len(size) != 2 or kind is None or out.stride(1) != 1 or not out.is_cuda:
             raise ValueError("out must be a 2-D float32, bfloat16 or float16 device tensor with unit element stride")
-        if out.shape[1] != table.dim:
+        rows, dim = size
+        if dim != table.dim:
             raise ValueError("out's dim differs from the table's")
-        if ids is not None and (ids.dim() != 1 or ids.shape[0] != out.shape[0]):
+        if ids is not None and (ids.dim() != 1 or ids.shape[0] != rows):
             raise ValueError("ids must hold one id per row of out")
-        d = SasMx4Lookup()
-        d.table, d.table_rows, d.dim = table.to_c(), table.shape[0], table.dim
-        d.ids, d.rows = _ptr(ids, "i32", "ids"), out.shape[0]
-        d.out, d.out_type = out.data_ptr(), types[str(out.dtype)]
-        d.out_stride = out.stride(0) if out.shape[0] > 1 else out.shape[1]
+        d = SasMx4Lookup(table.to_c(), table.shape[0], dim, _ptr(ids, "i32", "ids"), rows, out.data_ptr(),
+                         out.stride(0) if rows > 1 else dim, kind)
         check(self._lib.sas_lookup_mx4(self._h, ctypes.byref(d), _stream(stream)), self._h)
 
     def lookup_mx4(self, table: Mx4, ids=None, *, out_dtype=None, stream=None):
@@ -660,39 +673,38 @@ class Sampler:
                          stream=None) -> None:
         """sas_project_mx4: out [rows][out] (float32 or bfloat16) = x [rows][dim]
         (float32, bfloat16 or an Mx4) times weight, capped."""
-        types = {"torch.float32": _capi.TYPE_F32, "torch.bfloat16": _capi.TYPE_BF16}
         four = isinstance(x, Mx4)
-        for name, t in (("x", x), ("out", out)):
+        x_kind, kind = None if four else _type_of(x), _type_of(out)
+        for name, t, k in (("x", x, x_kind), ("out", out, kind)):
             if name == "x" and four:
                 continue
-            if t.dim() != 2 or t.stride(1) != 1 or not t.is_cuda or str(t.dtype) not in types:
+            if k is None or k == _capi.TYPE_F16 or len(t.shape) != 2 or t.stride(1) != 1 or not t.is_cuda:
                 raise ValueError(f"{name} must be a 2-D float32 or bfloat16 device tensor with unit element stride")
-        rows, dim = x.shape
-        if out.shape[0] != rows or tuple(weight.shape) != (out.shape[1], dim):
+        (rows, dim), (out_rows, out_dim) = x.shape, out.shape
+        if out_rows != rows or weight.shape != (out_dim, dim):
             raise ValueError("x [rows][dim], weight [out][dim] and out [rows][out] do not fit together")
         d = SasMx4Projection()
         if four:
             d.x4, d.x_type = x.to_c(), _capi.TYPE_MX4
         else:
             # (a tensor of one row may have any stride; its row is the whole of it)
-            d.x, d.x_stride, d.x_type = x.data_ptr(), x.stride(0) if rows > 1 else (dim + 7) // 8 * 8, types[str(x.dtype)]
-        d.rows, d.dim, d.out_dim = rows, dim, out.shape[1]
+            d.x, d.x_stride, d.x_type = x.data_ptr(), x.stride(0) if rows > 1 else (dim + 7) // 8 * 8, x_kind
+        d.rows, d.dim, d.out_dim = rows, dim, out_dim
         d.weight = weight.to_c()
-        d.out, d.out_type = out.data_ptr(), types[str(out.dtype)]
-        d.out_stride = out.stride(0) if rows > 1 else out.shape[1]
-        d.softcap = float(softcap)
+        d.out, d.out_stride, d.out_type = out.data_ptr(), out.stride(0) if rows > 1 else out_dim, kind
+        d.softcap = softcap
         d.accumulate = 1 if accumulate else 0
         check(self._lib.sas_project_mx4(self._h, ctypes.byref(d), _stream(stream)), self._h)
 
-    def project_mx4(self, x, weight: Mx4, *, out_dtype=None, stream=None, **kw):
+    def project_mx4(self, x, weight: Mx4, *, out_dtype=None, softcap: float = 0.0, accumulate: bool = False, stream=None):
         """Allocate out (float32 unless out_dtype is torch.bfloat16) and run
         project_mx4_into; returns it.  A fresh out holds nothing to accumulate on."""
         import torch
-        if kw.get("accumulate"):
+        if accumulate:
             raise ValueError("project_mx4 cannot accumulate: its out is new (project_mx4_into takes one)")
         with _on(stream):
             out = torch.empty((x.shape[0], weight.shape[0]), dtype=out_dtype or torch.float32, device=x.device)
-        self.project_mx4_into(x, weight, out, stream=stream, **kw)
+        self.project_mx4_into(x, weight, out, softcap=softcap, stream=stream)
         return out
 
     def reserve_project(self, rows: int, dim: int, *, rank: int = 0) -> None:
