@@ -141,8 +141,11 @@ __global__ __launch_bounds__(kThreads) void mx4_lookup_kernel(const Mx4LookupArg
   }
 }
 
-// The outputs a wave of the wide kernel takes, in 16s: as few rounds of blocks as
-// that leaves, a round's cost being its products and half of 16 outputs more.
+// The outputs a wave of the wide kernel takes, in 16s: the fewest rounds of blocks,
+// a round counted as its products and half of 16 outputs more.  One / two of
+// them, us: bf16, 64 rows x 4,096 x 32,768 (one round either way) 27 / 36; 32 x
+// 4,096 x 65,536 (two rounds, one) 34 / 31; 128 x 2,560 x 262,144 227 / 175; f32,
+// 16 x 2,560 x 151,936 65 / 69, three 64.
 int wide_nt(const Mx4ProjArgs &a, int mt, int most) {
   int best = 1;
   int64_t cost = INT64_MAX;
@@ -160,29 +163,31 @@ int wide_nt(const Mx4ProjArgs &a, int mt, int most) {
 template <int kX>
 void launch_products(const Mx4ProjArgs &a, hipStream_t stream) {
   if (kX == SAS_TYPE_F32 && a.rows <= kMx4Few) return launch_mx4_few(a, stream);
-  if (a.x_stride < (1 << 21) && a.out_stride < kMaxOutStride && (int64_t)a.out_dim * ((a.rows + 63) / 64) >= 4096) {
-    if constexpr (kX == SAS_TYPE_MX4) {
-      if (a.rows > 32 && a.rows <= 64 && stream_fits<4, kX, false>(a)) return launch_stream<4, 1, kX, false>(a, stream);
-      if (a.rows > 16 && a.rows <= 32 && stream_fits<2, kX, false>(a)) return launch_stream<2, 1, kX, false>(a, stream);
-    }
-    if (a.rows <= 16) {
-      if (kX != SAS_TYPE_F32 && stream_fits<1, kX, false>(a)) return launch_stream<1, 1, kX, false>(a, stream);
-      switch (wide_nt(a, 1, 3)) {
-        case 1: return launch_wide<1, 1, kX>(a, stream);
-        case 2: return launch_wide<1, 2, kX>(a, stream);
-        default: return launch_wide<1, 3, kX>(a, stream);
-      }
-    }
-    if (a.rows <= 32) return wide_nt(a, 2, 2) == 1 ? launch_wide<2, 1, kX>(a, stream) : launch_wide<2, 2, kX>(a, stream);
-    if (a.rows <= 64 || kX == SAS_TYPE_F32) return wide_nt(a, 4, 2) == 1 ? launch_wide<4, 1, kX>(a, stream) : launch_wide<4, 2, kX>(a, stream);
-    if constexpr (kX != SAS_TYPE_F32) return wide_nt(a, 8, 2) == 1 ? launch_wide<8, 1, kX>(a, stream) : launch_wide<8, 2, kX>(a, stream);
-  }
+  // (rows further apart than the other kernels' 32-bit offsets reach)
+  const bool far = a.x_stride >= kMaxXStride || a.out_stride >= kMaxOutStride;
   if (a.rows <= 16) {
-    if (a.out_dim <= 32 * a.cus) return launch_split<1, 1, kX>(a, stream);
-    return launch_split<1, 2, kX>(a, stream);
+    if (far || split_fits<1, 1>(a)) return launch_split<1, 1, kX>(a, stream);
+    if (kX != SAS_TYPE_F32 && stream_fits<1, kX, false>(a)) return launch_stream<1, 1, kX, false>(a, stream);
+    switch (wide_nt(a, 1, 3)) {
+      case 1: return launch_wide<1, 1, kX>(a, stream);
+      case 2: return launch_wide<1, 2, kX>(a, stream);
+      default: return launch_wide<1, 3, kX>(a, stream);
+    }
   }
-  if (a.rows <= 32) return launch_split<2, 2, kX>(a, stream);
-  launch_split<4, 2, kX>(a, stream);
+  if (a.rows <= 32) {
+    if (far || split_fits<2, 2>(a)) return launch_split<2, 2, kX>(a, stream);
+    if constexpr (kX == SAS_TYPE_MX4)
+      if (stream_fits<2, kX, false>(a)) return launch_stream<2, 1, kX, false>(a, stream);
+    return wide_nt(a, 2, 2) == 1 ? launch_wide<2, 1, kX>(a, stream) : launch_wide<2, 2, kX>(a, stream);
+  }
+  if (far || split_fits<4, 2>(a)) return launch_split<4, 2, kX>(a, stream);
+  if constexpr (kX == SAS_TYPE_MX4)
+    if (a.rows <= 64 && stream_fits<4, kX, false>(a)) return launch_stream<4, 1, kX, false>(a, stream);
+  // (128 rows of f32 pieces do not fit in LDS)
+  if (a.rows <= 64 || kX == SAS_TYPE_F32)
+    return wide_nt(a, 4, 2) == 1 ? launch_wide<4, 1, kX>(a, stream) : launch_wide<4, 2, kX>(a, stream);
+  if constexpr (kX != SAS_TYPE_F32)
+    return wide_nt(a, 8, 2) == 1 ? launch_wide<8, 1, kX>(a, stream) : launch_wide<8, 2, kX>(a, stream);
 }
 
 template <int kType>

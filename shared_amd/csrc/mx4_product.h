@@ -163,7 +163,8 @@ __device__ __forceinline__ void x_pieces(const XPart<kX> &p, int at, int size, u
 // them here is as much as on the products of 512 values.)
 template <int NT>
 constexpr int kStage = 16 * (16 * NT + 4);
-constexpr int64_t kMaxOutStride = 1 << 25;  // elements: 16 rows are within 32 bits
+constexpr int64_t kMaxOutStride = 1 << 25;  // elements: 16 rows of 4 bytes within 32 bits
+constexpr int64_t kMaxXStride = 1 << 23;    // elements (MXFP4: bytes): 128 rows of 2 bytes, or 64 of 4
 template <int NT, typename F>
 __device__ __forceinline__ void put_rows(const Mx4ProjArgs &a, int row0, int n0, F value) {
   const int lane = threadIdx.x & 63;
@@ -434,6 +435,18 @@ __global__ __launch_bounds__(64 * kSplitWaves, 2) void mx4_split_kernel(const Mx
     const int row = m0 + 16 * (i / NT) + r;
     if (row < a.rows) finish4(a, row, n0 + 16 * (i % NT) + 4 * q, v);
   }
+}
+
+// Few outputs: the split kernel, where it fills the chip once at most and dim is
+// more than two super-runs; then the waves of a block share dim, and all of a
+// call's loads are one latency.  The wide kernel's blocks walk along dim.  Over
+// 440 shapes (8 to 2,048 rows, 256 to 32,768 outputs of 512 to 8,192 values),
+// split / wide, us: bf16, 16 rows x 2,560 x 4,096 7 / 8, x 16,384 15 / 10; 128 x
+// 2,560 x 4,096 23 / 27, x 8,192 43 / 27; 128 x 8,192 x 4,096 41 / 76; 64 x 512 x
+// 4,096 11 / 7; MXFP4, 64 x 8,192 x 4,096 17 / 23, x 16,384 34 / 30.
+template <int MT, int NT>
+inline bool split_fits(const Mx4ProjArgs &a) {
+  return a.dim > 2 * kSuper && (int64_t)((a.rows + 16 * MT - 1) / (16 * MT)) * ((a.out_dim + 16 * NT - 1) / (16 * NT)) <= a.cus;
 }
 
 template <int MT, int NT, int kX>

@@ -22,6 +22,7 @@
 #include <cmath>
 #include <cstdint>
 #include <cstring>
+#include <initializer_list>
 #include <mutex>
 #include <string>
 
@@ -456,7 +457,8 @@ napi_value SampleStep(napi_env env, napi_callback_info info) {
 }
 
 // A sas_lm_head descriptor: {hidden, hiddenStride, weight, weightStride,
-// dim, outLogits?, format?} of device addresses (BigInt) and sizes.
+// dim, outLogits?, format?, scales?, scalesStride?} of device addresses (BigInt)
+// and sizes.
 bool read_head(napi_env env, napi_value d, sas_lm_head *hd) {
   std::memset(hd, 0, sizeof *hd);
   int64_t dim = 0;
@@ -465,7 +467,8 @@ bool read_head(napi_env env, napi_value d, sas_lm_head *hd) {
                   get_i64(env, d, "hiddenStride", &hd->hidden_stride) &&
                   get_ptr(env, d, "weight", (void **)&hd->weight) &&
                   get_i64(env, d, "weightStride", &hd->weight_stride) && get_i64(env, d, "dim", &dim) &&
-                  get_ptr(env, d, "outLogits", (void **)&hd->out_logits) && get_i64(env, d, "format", &format);
+                  get_ptr(env, d, "outLogits", (void **)&hd->out_logits) && get_i64(env, d, "format", &format) &&
+                  get_ptr(env, d, "scales", (void **)&hd->scales) && get_i64(env, d, "scalesStride", &hd->scales_stride);
   if (!ok || dim < INT32_MIN || dim > INT32_MAX || format < INT32_MIN || format > INT32_MAX) return false;
   hd->dim = (int32_t)dim;
   hd->format = (int32_t)format;
@@ -566,6 +569,95 @@ napi_value Project(napi_env env, napi_callback_info info) {
     return nullptr;
   }
   int rc = sas_project(s, &p, sas_stream(s));
+  return rc == SAS_OK ? undefined(env) : throw_sas(env, s, rc);
+}
+
+// A table of MXFP4 rows: `prefix`Codes, `prefix`CodesStride, `prefix`Scales,
+// `prefix`ScalesStride.
+bool read_mx4(napi_env env, napi_value d, const std::string &prefix, sas_mx4 *t) {
+  return get_ptr(env, d, (prefix + "Codes").c_str(), &t->codes) &&
+         get_i64(env, d, (prefix + "CodesStride").c_str(), &t->codes_stride) &&
+         get_ptr(env, d, (prefix + "Scales").c_str(), &t->scales) &&
+         get_i64(env, d, (prefix + "ScalesStride").c_str(), &t->scales_stride);
+}
+
+bool fit_i32(std::initializer_list<int64_t> vs) {
+  for (int64_t v : vs)
+    if (v < INT32_MIN || v > INT32_MAX) return false;
+  return true;
+}
+
+napi_value QuantizeMx4(napi_env env, napi_callback_info info) {
+  napi_value argv[2];
+  if (!args(env, info, 2, argv)) return throw_napi(env, "arguments");
+  HANDLE_OR_THROW(argv[0], s);
+  sas_mx4_quantization q;
+  std::memset(&q, 0, sizeof q);
+  int64_t type = 0, rows = 0, dim = 0;
+  const bool ok = get_ptr(env, argv[1], "x", (void **)&q.x) && get_i64(env, argv[1], "xStride", &q.x_stride) &&
+                  get_i64(env, argv[1], "xType", &type) && get_i64(env, argv[1], "rows", &rows) &&
+                  get_i64(env, argv[1], "dim", &dim) && read_mx4(env, argv[1], "out", &q.out);
+  if (!ok || !fit_i32({type, rows, dim})) {
+    napi_throw_type_error(env, nullptr, "sas_napi: bad quantization descriptor");
+    return nullptr;
+  }
+  q.x_type = (int32_t)type;
+  q.rows = (int32_t)rows;
+  q.dim = (int32_t)dim;
+  int rc = sas_quantize_mx4(s, &q, sas_stream(s));
+  return rc == SAS_OK ? undefined(env) : throw_sas(env, s, rc);
+}
+
+napi_value LookupMx4(napi_env env, napi_callback_info info) {
+  napi_value argv[2];
+  if (!args(env, info, 2, argv)) return throw_napi(env, "arguments");
+  HANDLE_OR_THROW(argv[0], s);
+  sas_mx4_lookup l;
+  std::memset(&l, 0, sizeof l);
+  int64_t type = 0, rows = 0, dim = 0, table = 0;
+  const bool ok = read_mx4(env, argv[1], "table", &l.table) && get_i64(env, argv[1], "tableRows", &table) &&
+                  get_i64(env, argv[1], "dim", &dim) && get_ptr(env, argv[1], "ids", (void **)&l.ids) &&
+                  get_i64(env, argv[1], "rows", &rows) && get_ptr(env, argv[1], "out", &l.out) &&
+                  get_i64(env, argv[1], "outStride", &l.out_stride) && get_i64(env, argv[1], "outType", &type);
+  if (!ok || !fit_i32({type, rows, dim, table})) {
+    napi_throw_type_error(env, nullptr, "sas_napi: bad lookup descriptor");
+    return nullptr;
+  }
+  l.table_rows = (int32_t)table;
+  l.dim = (int32_t)dim;
+  l.rows = (int32_t)rows;
+  l.out_type = (int32_t)type;
+  int rc = sas_lookup_mx4(s, &l, sas_stream(s));
+  return rc == SAS_OK ? undefined(env) : throw_sas(env, s, rc);
+}
+
+napi_value ProjectMx4(napi_env env, napi_callback_info info) {
+  napi_value argv[2];
+  if (!args(env, info, 2, argv)) return throw_napi(env, "arguments");
+  HANDLE_OR_THROW(argv[0], s);
+  sas_mx4_projection p;
+  std::memset(&p, 0, sizeof p);
+  int64_t xt = 0, rows = 0, dim = 0, out = 0, ot = 0, acc = 0;
+  double cap = 0.0;
+  const bool ok = get_ptr(env, argv[1], "x", (void **)&p.x) && get_i64(env, argv[1], "xStride", &p.x_stride) &&
+                  read_mx4(env, argv[1], "x", &p.x4) && get_i64(env, argv[1], "xType", &xt) &&
+                  get_i64(env, argv[1], "rows", &rows) && read_mx4(env, argv[1], "weight", &p.weight) &&
+                  get_i64(env, argv[1], "dim", &dim) && get_i64(env, argv[1], "outDim", &out) &&
+                  get_ptr(env, argv[1], "out", &p.out) && get_i64(env, argv[1], "outStride", &p.out_stride) &&
+                  get_i64(env, argv[1], "outType", &ot) && get_i64(env, argv[1], "accumulate", &acc) &&
+                  get_f64(env, argv[1], "softcap", &cap);
+  if (!ok || !fit_i32({xt, rows, dim, out, ot, acc})) {
+    napi_throw_type_error(env, nullptr, "sas_napi: bad projection descriptor");
+    return nullptr;
+  }
+  p.x_type = (int32_t)xt;
+  p.rows = (int32_t)rows;
+  p.dim = (int32_t)dim;
+  p.out_dim = (int32_t)out;
+  p.out_type = (int32_t)ot;
+  p.accumulate = (int32_t)acc;
+  p.softcap = (float)cap;
+  int rc = sas_project_mx4(s, &p, sas_stream(s));
   return rc == SAS_OK ? undefined(env) : throw_sas(env, s, rc);
 }
 
@@ -1019,6 +1111,9 @@ napi_value Init(napi_env env, napi_value exports) {
       {"lmHeadSampleAsync", nullptr, LmHeadSampleAsync, nullptr, nullptr, nullptr, napi_enumerable, nullptr},
       {"sampleFiltered", nullptr, SampleFiltered, nullptr, nullptr, nullptr, napi_enumerable, nullptr},
       {"project", nullptr, Project, nullptr, nullptr, nullptr, napi_enumerable, nullptr},
+      {"quantizeMx4", nullptr, QuantizeMx4, nullptr, nullptr, nullptr, napi_enumerable, nullptr},
+      {"lookupMx4", nullptr, LookupMx4, nullptr, nullptr, nullptr, napi_enumerable, nullptr},
+      {"projectMx4", nullptr, ProjectMx4, nullptr, nullptr, nullptr, napi_enumerable, nullptr},
       {"lmHeadStep", nullptr, LmHeadStep, nullptr, nullptr, nullptr, napi_enumerable, nullptr},
       {"lmHeadStepAsync", nullptr, LmHeadStepAsync, nullptr, nullptr, nullptr, napi_enumerable, nullptr},
       {"specStep", nullptr, SpecStep, nullptr, nullptr, nullptr, napi_enumerable, nullptr},

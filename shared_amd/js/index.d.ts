@@ -140,14 +140,14 @@ export interface SampleRowsOptions {
 /** The LM head of lmHeadSample: logits[row][id] = sum over k of
  * weight[id][k] * hidden[row][k]: a bf16 head widened to f32, or a GGUF
  * head (Q8_0 / Q4_0 / Q6_K blocks) against the Q8_1-quantized hidden
- * state, summed in the library's fixed order. */
-export type LmHeadFormat = 'bf16' | 'q8_0' | 'q4_0' | 'q6_k';
+ * state, summed in the library's fixed order, or an MXFP4 table. */
+export type LmHeadFormat = 'bf16' | 'q8_0' | 'q4_0' | 'q6_k' | 'mx4';
 
 export interface LmHead {
   /** [rows][hiddenStride] f32 final-normed hidden states. */
   hidden: DeviceBuffer | Float32Array;
-  /** [vocab] rows, device-resident: bf16 bits, or GGUF blocks. */
-  weight: DeviceBuffer;
+  /** [vocab] rows, device-resident: bf16 bits, GGUF blocks, or ('mx4') an Mx4Table. */
+  weight: DeviceBuffer | Mx4Table;
   /** Default 'bf16'. */
   format?: LmHeadFormat;
   /** A multiple of 256; rows * dim <= LMH_MAX_LDS_FLOATS. */
@@ -291,6 +291,14 @@ export declare class Sampler {
   sampleFiltered(opts: SampleFilteredOptions): SampleFilteredResult;
   /** A shared projection with the low-rank adapters of many requests. */
   project(opts: ProjectOptions): void;
+  /** Device memory of MXFP4 rows (not set). */
+  allocMx4(rows: number, dim: number): Mx4Table;
+  /** Rounds rows to MXFP4; returns `out` or a new table. */
+  quantizeMx4(opts: QuantizeMx4Options): Mx4Table;
+  /** A table's rows by id, or its first rows in order. */
+  lookupMx4(opts: LookupMx4Options): void;
+  /** out [rows][weight.rows] = x times a table's rows. */
+  projectMx4(opts: ProjectMx4Options): void;
   decodeRows(opts: SampleRowsOptions): DecodeBatchResult[];
   decodeRowsAsync(opts: SampleRowsOptions): Promise<DecodeBatchResult[]>;
   decodeSteps(opts: DecodeStepsOptions): DecodeBatchResult[];
@@ -372,6 +380,50 @@ export interface SampleFilteredResult {
   probs?: Float64Array;
   counts?: Int32Array;
   flags?: Uint32Array;
+}
+
+/** MXFP4 rows in device memory: values in blocks of 32, 4 bits each, a scale a block. */
+export declare class Mx4Table {
+  readonly rows: number;
+  readonly dim: number;
+  /** [rows][codesStride] bytes. */
+  readonly codes: DeviceBuffer;
+  readonly codesStride: number;
+  /** [rows][scalesStride] bytes. */
+  readonly scales: DeviceBuffer;
+  readonly scalesStride: number;
+  free(): void;
+}
+
+export interface QuantizeMx4Options {
+  /** [rows][dim]. */
+  x: DeviceBuffer;
+  xType?: 'f32' | 'bf16' | 'f16';
+  rows: number;
+  dim: number;
+  out?: Mx4Table;
+}
+
+export interface LookupMx4Options {
+  table: Mx4Table;
+  /** u32 [rows]; an id past the table gives zeros. */
+  ids?: DeviceBuffer;
+  rows: number;
+  /** [rows][table.dim]. */
+  out: DeviceBuffer;
+  outType?: 'f32' | 'bf16' | 'f16';
+}
+
+export interface ProjectMx4Options {
+  /** [rows][weight.dim], or MXFP4 rows. */
+  x: DeviceBuffer | Mx4Table;
+  xType?: 'f32' | 'bf16';
+  rows: number;
+  weight: Mx4Table;
+  out: DeviceBuffer;
+  outType?: 'f32' | 'bf16';
+  softcap?: number;
+  accumulate?: boolean;
 }
 
 export interface ProjectOptions {

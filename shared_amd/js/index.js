@@ -240,12 +240,14 @@ function packedToolMask(constraint, raw, parseArguments, builder) {
  * top-p 0.95, a random seed, and eos only when eosId is given.
  */
 // LM head formats (sas_lm_head.format): bf16, and the GGUF block types the
-// reference loads (gguf/parser.js:29-36) with their values and bytes per block.
+// reference loads (gguf/parser.js:29-36) with their values and bytes per block;
+// then MXFP4 tables.
 const HEAD_FORMATS = {
   bf16: { id: 0, values: 1, bytesPer: 0 },
   q8_0: { id: 1, values: 32, bytesPer: 34 },
   q4_0: { id: 2, values: 32, bytesPer: 18 },
   q6_k: { id: 3, values: 256, bytesPer: 210 },
+  mx4: { id: 4, values: 32, bytesPer: 16 },  // an Mx4Table's codes, its scales beside them
 };
 
 const PACKER_DEFAULTS = {
@@ -403,6 +405,33 @@ class DeviceBuffer {
   free() {
     if (this.ptr !== null && this.sampler._h !== null) addon.free(this.sampler._idle('free'), this.ptr);
     this.ptr = null;
+  }
+}
+
+/** MXFP4 rows in device memory (sas_mx4), contiguous: codes 16 bytes a block of
+ * 32 values, scales a byte a block, their rows padded to a multiple of four. */
+class Mx4Table {
+  constructor(sampler, rows, dim) {
+    if (!Number.isInteger(rows) || rows < 0 || !Number.isInteger(dim) || dim < 1) throw new RangeError('rows and dim must be whole numbers');
+    const blocks = Math.ceil(dim / 32);
+    this.rows = rows;
+    this.dim = dim;
+    this.codesStride = 16 * blocks;
+    this.scalesStride = 4 * Math.ceil(blocks / 4);
+    this.codes = sampler.alloc(Math.max(16, rows * this.codesStride));
+    this.scales = sampler.alloc(Math.max(16, rows * this.scalesStride));
+  }
+  _fields(prefix) {
+    const f = {};
+    f[prefix + 'Codes'] = this.codes.ptr;
+    f[prefix + 'CodesStride'] = this.codesStride;
+    f[prefix + 'Scales'] = this.scales.ptr;
+    f[prefix + 'ScalesStride'] = this.scalesStride;
+    return f;
+  }
+  free() {
+    this.codes.free();
+    this.scales.free();
   }
 }
 
@@ -752,7 +781,7 @@ class Sampler {
   // hiddenStride?, weightStride?, outLogits?}.  format: 'bf16' (default:
   // bits [vocab][weightStride elements]) or a GGUF type, 'q8_0', 'q4_0',
   // 'q6_k' (blocks [vocab][weightStride bytes], the row's bytes by
-  // default).  The head must be device-resident; the hidden states may be a
+  // default), or 'mx4' (weight an Mx4Table).  The head must be device-resident; the hidden states may be a
   // host Float32Array [rows][hiddenStride], staged up per call.
   _describeHead(opts) {
     const h = opts.head;
@@ -775,8 +804,16 @@ class Sampler {
     } else {
       throw new TypeError('head.hidden must be a DeviceBuffer or a Float32Array');
     }
-    if (!(h.weight instanceof DeviceBuffer)) throw new TypeError('head.weight must be a DeviceBuffer');
-    hd.weight = h.weight.ptr;
+    if (fmt === 'mx4') {
+      if (!(h.weight instanceof Mx4Table)) throw new TypeError('head.weight must be an Mx4Table');
+      if (h.weight.dim !== dim) throw new RangeError('head.dim differs from the table\'s');
+      if (h.weight.rows < opts.vocab) throw new RangeError('head.weight holds fewer than vocab rows');
+      Object.assign(hd, { weight: h.weight.codes.ptr, weightStride: h.weight.codesStride, scales: h.weight.scales.ptr,
+        scalesStride: h.weight.scalesStride });
+    } else {
+      if (!(h.weight instanceof DeviceBuffer)) throw new TypeError('head.weight must be a DeviceBuffer');
+      hd.weight = h.weight.ptr;
+    }
     if (h.outLogits !== undefined && h.outLogits !== null) {
       if (!(h.outLogits instanceof DeviceBuffer)) throw new TypeError('head.outLogits must be a DeviceBuffer');
       hd.outLogits = h.outLogits.ptr;
@@ -909,6 +946,84 @@ class Sampler {
         rowAdapter: ptr(opts.rowAdapter, 'rowAdapter', opts.rows * 4) });
     }
     addon.project(this._handle(), d);
+  }
+
+  /** Device memory of `rows` MXFP4 rows of `dim` values (not set). */
+  allocMx4(rows, dim) {
+    return new Mx4Table(this, rows, dim);
+  }
+
+  // A DeviceBuffer's address, checked for its size.
+  _room(b, name, bytes) {
+    if (!(b instanceof DeviceBuffer)) throw new TypeError(name + ' must be a DeviceBuffer');
+    if (!(b.bytes >= bytes)) throw new RangeError(name + ' holds fewer than its ' + bytes + ' bytes');
+    return b.ptr;
+  }
+
+  _elements(type, name, half) {
+    if (!Object.prototype.hasOwnProperty.call(ELEMENT_TYPES, type) || (type === 'f16' && !half)) {
+      throw new RangeError(name + ' must be f32' + (half ? ', bf16 or f16' : ' or bf16'));
+    }
+    return { id: ELEMENT_TYPES[type], size: type === 'f32' ? 4 : 2 };
+  }
+
+  _table(t, name) {
+    if (!(t instanceof Mx4Table)) throw new TypeError(name + ' must be an Mx4Table');
+    return t;
+  }
+
+  /**
+   * Rounds x [rows][dim] (a DeviceBuffer, xType 'f32', the default, 'bf16' or
+   * 'f16') to MXFP4 (sas_quantize_mx4): {x, xType?, rows, dim, out?}.  Returns
+   * the table, `out` or a new one.
+   */
+  quantizeMx4(opts) {
+    this._idle('quantizeMx4');
+    const type = this._elements(orDefault(opts.xType, 'f32'), 'xType', true);
+    const x = this._room(opts.x, 'x', opts.rows * opts.dim * type.size);
+    const fresh = opts.out === undefined || opts.out === null;
+    const out = fresh ? this.allocMx4(opts.rows, opts.dim) : this._table(opts.out, 'out');
+    if (out.dim !== opts.dim || out.rows < opts.rows) throw new RangeError('out must hold x\'s rows of x\'s dim');
+    addon.quantizeMx4(this._handle(), Object.assign({ x: x, xStride: opts.dim, xType: type.id, rows: opts.rows, dim: opts.dim },
+      out._fields('out')));
+    return out;
+  }
+
+  /**
+   * Rows of a table (sas_lookup_mx4): {table, ids? (a DeviceBuffer of u32; one
+   * past the table gives zeros), rows, out, outType? ('f32', 'bf16' or
+   * 'f16')}; without ids the table's first rows.
+   */
+  lookupMx4(opts) {
+    this._idle('lookupMx4');
+    const t = this._table(opts.table, 'table');
+    const type = this._elements(orDefault(opts.outType, 'f32'), 'outType', true);
+    const d = Object.assign({ tableRows: t.rows, dim: t.dim, rows: opts.rows, out: this._room(opts.out, 'out', opts.rows * t.dim * type.size),
+      outStride: t.dim, outType: type.id }, t._fields('table'));
+    if (opts.ids !== undefined && opts.ids !== null) d.ids = this._room(opts.ids, 'ids', opts.rows * 4);
+    addon.lookupMx4(this._handle(), d);
+  }
+
+  /**
+   * out [rows][outDim] = x times a table's rows (sas_project_mx4): {x (a
+   * DeviceBuffer, xType 'f32' or 'bf16', or an Mx4Table), rows, weight (an
+   * Mx4Table), out, outType?, softcap?, accumulate?}, contiguous.
+   */
+  projectMx4(opts) {
+    this._idle('projectMx4');
+    const w = this._table(opts.weight, 'weight');
+    const out = this._elements(orDefault(opts.outType, 'f32'), 'outType', false);
+    const d = Object.assign({ rows: opts.rows, dim: w.dim, outDim: w.rows, out: this._room(opts.out, 'out', opts.rows * w.rows * out.size),
+      outStride: w.rows, outType: out.id, softcap: orDefault(opts.softcap, 0), accumulate: opts.accumulate ? 1 : 0 },
+    w._fields('weight'));
+    if (opts.x instanceof Mx4Table) {
+      if (opts.x.dim !== w.dim || opts.x.rows < opts.rows) throw new RangeError('x must hold rows of the weight\'s dim');
+      Object.assign(d, { xType: 3 }, opts.x._fields('x'));
+    } else {
+      const type = this._elements(orDefault(opts.xType, 'f32'), 'xType', false);
+      Object.assign(d, { x: this._room(opts.x, 'x', opts.rows * w.dim * type.size), xStride: w.dim, xType: type.id });
+    }
+    addon.projectMx4(this._handle(), d);
   }
 
   // decodeBatch's per-row result for one step (model.js:727-741,
@@ -1476,6 +1591,7 @@ class Sampler {
 module.exports = {
   Sampler: Sampler,
   DeviceBuffer: DeviceBuffer,
+  Mx4Table: Mx4Table,
   PenaltyWindow: PenaltyWindow,
   MaskBuilder: MaskBuilder,
   packedToolMask: packedToolMask,

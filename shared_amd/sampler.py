@@ -486,12 +486,14 @@ class Sampler:
         return out if full else out["ids"]
 
     @staticmethod
-    def _head(hidden, weight, dim, out_logits, fmt):
+    def _head(hidden, weight, dim, out_logits, fmt, vocab):
         if hidden.dtype.itemsize != 4 or hidden.stride(1) != 1:
             raise ValueError("hidden must be fp32 with unit element stride")
         if isinstance(weight, Mx4):
             if fmt not in (_capi.HEAD_BF16, _capi.HEAD_MX4):
                 raise ValueError("an Mx4 weight has the format HEAD_MX4")
+            if vocab > weight.shape[0]:
+                raise ValueError("vocab exceeds the head's rows")
             c = weight.to_c()
             h = SasLmHead()
             h.weight, h.weight_stride, h.scales, h.scales_stride = c.codes, c.codes_stride, c.scales, c.scales_stride
@@ -526,7 +528,7 @@ class Sampler:
         [vocab][row bytes] uint8 tensor, or an Mx4) with the sampling step
         behind it; kw as for sample_into."""
         vocab = int(vocab if vocab is not None else weight.shape[0])
-        h = self._head(hidden, weight, dim, out_logits, fmt)
+        h = self._head(hidden, weight, dim, out_logits, fmt, vocab)
         d = rows_descriptor(hidden, out_ids, vocab=vocab, **kw)
         d.logits = None
         d.logits_stride = 0
@@ -541,7 +543,7 @@ class Sampler:
         if kw.get("hist_ids") is not None:
             raise ValueError("a decode step's history is its ring")
         vocab = int(vocab if vocab is not None else weight.shape[0])
-        h = self._head(hidden, weight, dim, out_logits, fmt)
+        h = self._head(hidden, weight, dim, out_logits, fmt, vocab)
         d = rows_descriptor(hidden, out_ids, vocab=vocab, **kw)
         d.logits = None
         d.logits_stride = 0
@@ -647,6 +649,8 @@ class Sampler:
         """sas_lookup_mx4: out [rows][dim] (float32, bfloat16 or float16) = the
         table's rows ids (4-byte integers; one past the table gives zeros), or its
         first rows in order."""
+        if not isinstance(table, Mx4):
+            raise ValueError("table must be an Mx4")
         size, kind = out.shape, _type_of(out)
         if len(size) != 2 or kind is None or out.stride(1) != 1 or not out.is_cuda:
             raise ValueError("out must be a 2-D float32, bfloat16 or float16 device tensor with unit element stride")
@@ -673,6 +677,8 @@ class Sampler:
                          stream=None) -> None:
         """sas_project_mx4: out [rows][out] (float32 or bfloat16) = x [rows][dim]
         (float32, bfloat16 or an Mx4) times weight, capped."""
+        if not isinstance(weight, Mx4):
+            raise ValueError("weight must be an Mx4")
         four = isinstance(x, Mx4)
         x_kind, kind = None if four else _type_of(x), _type_of(out)
         for name, t, k in (("x", x, x_kind), ("out", out, kind)):

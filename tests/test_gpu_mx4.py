@@ -447,6 +447,10 @@ def test_refusals(sampler):
         sampler.lm_head_sample(hid, table(10, 256), fmt=W.HEAD_Q6_K, params=Params())
     with pytest.raises(SasError, match="scales_stride"):
         sampler.lm_head_sample(hid, Mx4(u8(10, 128), u8(10, 9), 256), params=Params())
+    with pytest.raises(ValueError, match="vocab exceeds"):
+        sampler.lm_head_sample(hid, table(10, 256), vocab=11, params=Params())
+    with pytest.raises(ValueError, match="must be an Mx4"):
+        sampler.project_mx4(x, torch.zeros((10, 64), device="cuda"))
     # nothing of no rows
     assert sampler.project_mx4(x[:0], t).shape == (0, 10)
     assert sampler.quantize_mx4(x[:0]).shape == (0, 64)
@@ -550,6 +554,63 @@ def test_head_in_a_captured_decode_loop(sampler):
     with Sampler(0) as s:
         s.reserve(rows=rows, vocab=vocab, lm_head_rows=rows, hist_ids=rows * 512)
         assert np.array_equal(run(s, True), want)
+
+
+def test_offsets_past_32_bits(sampler):
+    """Tables and hidden states of more than 4 GiB: the last rows are what they are
+    alone."""
+    import torch
+    rows, dim = 3_400_000, 2560
+    small = table(300, dim, seed=4)
+    big = Mx4(torch.zeros((rows, 1280), dtype=torch.uint8, device="cuda"), torch.zeros((rows, 80), dtype=torch.uint8, device="cuda"), dim)
+    big.codes[-300:], big.scales[-300:] = small.codes, small.scales
+    ids = torch.tensor([rows - 1, 0, rows - 300, rows], dtype=torch.int32, device="cuda")
+    got, want = sampler.lookup_mx4(big, ids), sampler.lookup_mx4(small)
+    assert torch.equal(got[0], want[299]) and torch.equal(got[2], want[0]) and not got[1].any() and not got[3].any()
+    for n, kind in ((2, torch.float32), (12, torch.bfloat16), (70, torch.bfloat16)):
+        x = torch.randn((n, dim), device="cuda").to(kind)
+        y = sampler.project_mx4(x, big, out_dtype=torch.bfloat16)
+        p = Product.__new__(Product)
+        p.x, p.value, p.weight = x, x.double(), torch.from_numpy(table_values(small)).cuda()
+        p.check(y[:, -300:])
+        assert not y[:, :-300].any()
+        del y
+    del big
+    x = torch.zeros((rows // 4, dim), device="cuda")     # 8.7 GB of f32
+    x[-3:] = torch.randn((3, dim), device="cuda")
+    q, alone = sampler.quantize_mx4(x), sampler.quantize_mx4(x[-3:])
+    assert torch.equal(q.codes[-3:], alone.codes) and torch.equal(q.scales[-3:], alone.scales)
+    assert not q.codes[:-3].any() and not q.scales[:-3].any()
+
+
+@pytest.mark.parametrize("rows", [3, 20, 50])
+def test_rows_far_apart(sampler, rows):
+    """Strides that pass the kernels' 32-bit offsets within a tile."""
+    import torch
+    dim, out = 64, 9000
+    p = Product(rows, dim, out, "bfloat16", seed=rows)
+    want = sampler.project_mx4(p.x, p.w)
+    far = torch.empty(((rows - 1) << 24) + dim, dtype=torch.bfloat16, device="cuda").as_strided((rows, dim), (1 << 24, 1))
+    far.copy_(p.x)
+    p.check(sampler.project_mx4(far, p.w))
+    there = torch.empty(((rows - 1) << 25) + out, device="cuda").as_strided((rows, out), (1 << 25, 1))
+    sampler.project_mx4_into(p.x, p.w, there)
+    p.check(there)
+    assert (there - want).abs().max() <= 2.0 ** -18 * want.abs().max() + 1e-3
+
+
+def test_accumulate_then_cap_and_nan_in_bf16(sampler):
+    import torch
+    for rows, out in ((2, 9000), (40, 64), (40, 40000)):
+        for kind in ("float32", "bfloat16", "mx4"):
+            p = Product(rows, 256, out, kind, seed=out)
+            held = torch.randn((rows, out), device="cuda")
+            got = held.clone()
+            sampler.project_mx4_into(p.x, p.w, got, accumulate=True, softcap=10.0)
+            p.check(got, cap=10.0, extra=held.double())
+            p.w.scales[7, 2] = 255
+            y = sampler.project_mx4(p.x, p.w, out_dtype=torch.bfloat16, softcap=10.0)
+            assert y[:, 7].isnan().all() and y[:, :7].isfinite().all() and y[:, 8:].isfinite().all()
 
 
 def test_other_streams(sampler):
