@@ -81,11 +81,18 @@ __device__ __forceinline__ uint32_t pack_scales(uint32_t mine, uint32_t mask) {
 
 // ---- the hidden states in LDS ----
 //
-// An operand: 16 rows x 128 values of bf16 (4 KB) in two halves of 64 values,
-// value octet o of row r in 16-byte slot 8 r + (o ^ r / 2) of its half; or 16 rows
-// x 64 bytes of codes (1 KB), block c of row r in slot 4 r + (c ^ r / 4).  The
-// lanes that write a row, and the 16 rows that read an octet or a block, meet
-// every bank once.
+// An operand: 16 rows x 128 values of bf16 (4 KB) in two halves of 64 values, a
+// row's octets in the eight 16-byte slots from 8 r of its half on; or 16 rows x 64
+// bytes of codes (1 KB), a row's blocks in the four slots from 4 r on.  LDS serves
+// a 16-byte read 16 lanes at a time: lanes 0 .. 3, 12 .. 15, 20 .. 23 and 24 .. 27
+// together, then the other 16 of the first 32, the upper half alike.  In these
+// orders each such set meets every bank once.  (With octet o at o ^ r / 2, right
+// for 16 lanes after another, SQ_LDS_BANK_CONFLICT was 40 % of the LDS's cycles.)
+__device__ __forceinline__ int octet_slot(int o, int r) { return 8 * r + (((o & 3) << 1 | o >> 2) ^ (r >> 1)); }
+__device__ __forceinline__ int block_slot(int c, int r) {
+  const int t = r >> 2;  // 0 2 3 1
+  return 4 * r + (c ^ ((t & 1) << 1) ^ (t >> 1) * 3);
+}
 template <int kX>
 struct XOperand {
   static constexpr int kSlots = kX == SAS_TYPE_MX4 ? 64 : 256;
@@ -96,8 +103,8 @@ struct XOperand {
 template <int kX>
 __device__ __forceinline__ int x_get(int i) {
   const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
-  if constexpr (kX == SAS_TYPE_MX4) return 4 * r + (q ^ (r >> 2));
-  return 128 * (q >> 1) + 8 * r + ((4 * (q & 1) + i) ^ (r >> 1));
+  if constexpr (kX == SAS_TYPE_MX4) return block_slot(q, r);
+  return 128 * (q >> 1) + octet_slot(4 * (q & 1) + i, r);
 }
 // Load f of an operand: the lane's row, its first value (or byte) in the run, and
 // the slot it goes to.
@@ -114,8 +121,8 @@ __device__ __forceinline__ int x_at(int f) {
 template <int kX>
 __device__ __forceinline__ int x_put(int f, int r) {
   const int lane = threadIdx.x & 63;
-  if constexpr (kX == SAS_TYPE_MX4) return 4 * r + ((lane & 3) ^ (r >> 2));
-  return 128 * (f >> 1) + 8 * r + ((lane & 7) ^ (r >> 1));
+  if constexpr (kX == SAS_TYPE_MX4) return block_slot(lane & 3, r);
+  return 128 * (f >> 1) + octet_slot(lane & 7, r);
 }
 template <int kX>
 struct XPart {  // what a lane loads: an octet, or a block
