@@ -3,7 +3,9 @@
 //
 // A row's values lie in blocks of 32: 16 bytes of elements (a sign, two bits of
 // exponent, one of mantissa: 0 0.5 1 1.5 2 3 4 6; the first of a byte in its low
-// half) and a byte s, the block's scale 2^(s - 127); 255 is NaN.
+// half) and a byte s, the block's scale 2^(s - 127); 255 is NaN.  Quantisation
+// rounds x / 2^(s - 127), which is exact, once.  The products are in
+// mx4_product.h; here is which kernel takes a call.
 #include "mx4_product.h"
 
 namespace sas {

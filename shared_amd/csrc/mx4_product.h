@@ -1,5 +1,30 @@
 // mx4_product.h - products with rows of MXFP4 values (gfx950): the kernels that
 // sas_project_mx4 and the fused head share.
+//
+//   y[r][n] = cap(sum over k of x[r][k] w[n][k] (+ y[r][n]))
+//
+// A weight is element x scale, exact in bf16 (v_cvt_scalef32_pk_bf16_fp4 makes
+// two of them), so its product with a bf16 value is exact in the matrix
+// instructions' f32 sums; f32 hidden states are three bf16 pieces, 24 bits,
+// three products.  Hidden states of MXFP4 take the scaled 4-bit matrix
+// instruction: 128 values at the cost of bf16's 32, no conversions.
+//
+// Three kernels:
+//   - mx4_split_kernel: few outputs.  Eight waves split dim, every load of a
+//     call in flight together (1 x 2,560 x 2,560 5.0 us).
+//   - mx4_stream_kernel: few rows, hidden states that fit in LDS.  Bound by the
+//     weights' stream: one f32 row x 2,560 x 262,144 60 us (357 MB, 6.0 TB/s), 16
+//     bf16 rows x 151,936 42, 16 MXFP4 rows 39, 61 MXFP4 rows x 4,096 x 11,007 12.5.
+//   - mx4_wide_kernel: the rest.  2,048 x 4,096 x 4,096 bf16 58 us (1.19 PFLOP/s),
+//     8,192 x 4,096 x 11,008 607 (1.22), the same of MXFP4 289 (2.6): a wave reads
+//     all of a tile's hidden states from LDS, and waits for what it read; 128
+//     bf16 rows x 2,560 x 262,144 164 us (1.05 PFLOP/s; 129 without loads and
+//     results), 16 f32 rows x 151,936 66 (52).
+// What carried them: weight rows in whole 128-byte lines, nontemporal (half lines
+// in the matrix layout: nontemporal 469 MB fetched for 357, 84 us for a head's
+// row; cached 66; whole lines through LDS 60); one tile of 16 rows at a time, so
+// that what a wave asks for lies together (two tiles 77 us, four 88); operands read
+// a step ahead; one block of code a loop; bands of tiles for the L2.
 #pragma once
 
 #include "sas_product.h"
@@ -14,10 +39,9 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef u32x4 u32x4a4 __attribute__((aligned(4)));
 
 constexpr int kBlock = SAS_MX4_BLOCK;
+
 // The f32 scale of byte s as the conversions take it.
 __device__ __forceinline__ float scale_of(uint32_t s) { return __uint_as_float(s << 23); }
-
-// --------------------------------------------------------------- products --
 
 constexpr int kRun = 4 * kBlock;   // values of dim a step: a block a lane
 constexpr int kSuper = 4 * kRun;   // values whose scales are loaded together
@@ -368,67 +392,67 @@ __global__ __launch_bounds__(64 * kSplitWaves, 2) void mx4_split_kernel(const Mx
 #pragma unroll
     for (int t = 0; t < NT; ++t) acc[m][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   for (int g4 = g0; g4 < g1; g4 += 4) {
-  uint32_t ws[NT], xs[MT];
+    uint32_t ws[NT], xs[MT];
 #pragma unroll
-  for (int t = 0; t < NT; ++t) ws[t] = load_scales_of(wsr[t], g4, blocks);
+    for (int t = 0; t < NT; ++t) ws[t] = load_scales_of(wsr[t], g4, blocks);
 #pragma unroll
-  for (int m = 0; m < MT; ++m)
-    if constexpr (kX == SAS_TYPE_MX4) xs[m] = load_scales_of(xsr[m], g4, blocks);
-  each_const<4 / kFlight>([&](auto part_of) __attribute__((always_inline)) {
-    const int g = g4 + kFlight * decltype(part_of)::value;
-    u32x4 w[kFlight][NT];
-    XPart<kX> x[kFlight][MT][kOctets];
+    for (int m = 0; m < MT; ++m)
+      if constexpr (kX == SAS_TYPE_MX4) xs[m] = load_scales_of(xsr[m], g4, blocks);
+    each_const<4 / kFlight>([&](auto part_of) __attribute__((always_inline)) {
+      const int g = g4 + kFlight * decltype(part_of)::value;
+      u32x4 w[kFlight][NT];
+      XPart<kX> x[kFlight][MT][kOctets];
 #pragma unroll
-    for (int u = 0; u < kFlight; ++u) {
-      // (past the wave's last run, and the row's last block, what is there again:
-      // x_pieces makes zeros of the hidden states)
-      const int b = min(4 * min(g + u, g1 - 1) + q, blocks - 1);
+      for (int u = 0; u < kFlight; ++u) {
+        // (past the wave's last run, and the row's last block, what is there again:
+        // x_pieces makes zeros of the hidden states)
+        const int b = min(4 * min(g + u, g1 - 1) + q, blocks - 1);
 #pragma unroll
-      for (int t = 0; t < NT; ++t) w[u][t] = *reinterpret_cast<const u32x4 *>(wr[t] + 16 * b);
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-#pragma unroll
-        for (int i = 0; i < kOctets; ++i) {
-          const int at = kX == SAS_TYPE_MX4 ? 16 * b : kBlock * b + 8 * i;
-          x[u][m][i] = x_load<kX>(xr[m] + (int64_t)x_within<kX>(at, size) * kXSize<kX>);
-        }
-      }
-    }
-    if constexpr (decltype(part_of)::value == 0) {
-      const uint32_t mask = scale_mask_of(g4, blocks);
-#pragma unroll
-      for (int t = 0; t < NT; ++t) ws[t] = pack_scales(ws[t], mask);
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-        if constexpr (kX == SAS_TYPE_MX4) xs[m] = pack_scales(xs[m], mask);
-    }
-    each_const<kFlight>([&](auto ut) __attribute__((always_inline)) {
-      constexpr int u = decltype(ut)::value, j = kFlight * decltype(part_of)::value + u;
-      const int b = 4 * (g + u) + q;
-      const bool in = g + u < g1 && b < blocks;
-#pragma unroll
-      for (int i = 0; i < kOctets; ++i) {
-        u32x4 wv[NT];
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          if constexpr (kX == SAS_TYPE_MX4) wv[t] = w[u][t];
-          else wv[t] = widen(w[u][t][i], scale_byte<j>(ws[t]));
-        }
+        for (int t = 0; t < NT; ++t) w[u][t] = *reinterpret_cast<const u32x4 *>(wr[t] + 16 * b);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-          u32x4 o[P];
-          x_pieces<kX>(x[u][m][i], in ? (kX == SAS_TYPE_MX4 ? 16 * b : kBlock * b + 8 * i) : size, size, o);
 #pragma unroll
-          for (int p = 0; p < P; ++p)
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-              if constexpr (kX == SAS_TYPE_MX4) acc[m][t] = mfma4<j>(wv[t], ws[t], o[p], xs[m], acc[m][t]);
-              else acc[m][t] = mfma(wv[t], o[p], acc[m][t]);
-            }
+          for (int i = 0; i < kOctets; ++i) {
+            const int at = kX == SAS_TYPE_MX4 ? 16 * b : kBlock * b + 8 * i;
+            x[u][m][i] = x_load<kX>(xr[m] + (int64_t)x_within<kX>(at, size) * kXSize<kX>);
+          }
         }
       }
+      if constexpr (decltype(part_of)::value == 0) {
+        const uint32_t mask = scale_mask_of(g4, blocks);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) ws[t] = pack_scales(ws[t], mask);
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+          if constexpr (kX == SAS_TYPE_MX4) xs[m] = pack_scales(xs[m], mask);
+      }
+      each_const<kFlight>([&](auto ut) __attribute__((always_inline)) {
+        constexpr int u = decltype(ut)::value, j = kFlight * decltype(part_of)::value + u;
+        const int b = 4 * (g + u) + q;
+        const bool in = g + u < g1 && b < blocks;
+#pragma unroll
+        for (int i = 0; i < kOctets; ++i) {
+          u32x4 wv[NT];
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            if constexpr (kX == SAS_TYPE_MX4) wv[t] = w[u][t];
+            else wv[t] = widen(w[u][t][i], scale_byte<j>(ws[t]));
+          }
+#pragma unroll
+          for (int m = 0; m < MT; ++m) {
+            u32x4 o[P];
+            x_pieces<kX>(x[u][m][i], in ? (kX == SAS_TYPE_MX4 ? 16 * b : kBlock * b + 8 * i) : size, size, o);
+#pragma unroll
+            for (int p = 0; p < P; ++p)
+#pragma unroll
+              for (int t = 0; t < NT; ++t) {
+                if constexpr (kX == SAS_TYPE_MX4) acc[m][t] = mfma4<j>(wv[t], ws[t], o[p], xs[m], acc[m][t]);
+                else acc[m][t] = mfma(wv[t], o[p], acc[m][t]);
+              }
+          }
+        }
+      });
     });
-  });
   }
 #pragma unroll
   for (int m = 0; m < MT; ++m)
@@ -467,6 +491,8 @@ void launch_split(const Mx4ProjArgs &a, hipStream_t stream) {
 // ahead in registers; no barrier after the first.
 // kPack: up to kMx4Few rows of f32, whose pieces are rows of one operand (row r's
 // piece p is row kMx4Few p + r): a third of the products.
+// (Twelve waves against eight: 16 bf16 rows x 2,560 x 151,936 42.9 / 44.8 us, a
+// head's row 59.8 / 60.6.)
 constexpr int kStreamWaves = 12;
 constexpr int kStreamSlots = 136 * 1024 / 16;
 
@@ -620,10 +646,14 @@ void launch_stream(const Mx4ProjArgs &a, hipStream_t stream) {
 // loads going on across them.
 // A step is one operand of each subtile: its products come with the reads of the
 // next step's operands, so that no product waits for LDS; the next chunk is
-// stored half-way, and the barrier that shows it stands before the last step.
+// stored half-way, and the barrier that shows it stands before the last step
+// (2,048 x 4,096 x 4,096 bf16 67 -> 59 us, with the loop free of branches, cheap
+// addresses and bands of tiles; MXFP4 115 -> 27).  A matrix instruction leaves room
+// for two others beside it (16 cycles, or 8 and 4 for each of them): the
+// conversions are one, what goes beyond costs.
 constexpr int kWideWaves = 8;
 template <int MT, int NT, int kX>
-struct Wide4 {
+struct Mx4Wide {
   static constexpr int kRows = 16 * MT, kOuts = 16 * NT * kWideWaves;
   static constexpr int P = XOperand<kX>::kPieces, kSubs = MT * P;
   static constexpr int kChunk = kX == SAS_TYPE_MX4 ? 4 : kSubs <= 2 ? 4 : kSubs <= 4 ? 2 : 1;
@@ -635,12 +665,14 @@ struct Wide4 {
   static constexpr int kChunkSteps = kChunk * kRunSteps;
 };
 
+// (8,192 x 4,096 x 11,008, MXFP4: bands of 4 tiles 283 us, 8 301, all rows 313;
+// bf16: 4 613, 8 623, all rows 680)
 constexpr int kTileRows = 4;
 
 template <int MT, int NT, int kX, bool kOnce, bool kTail>
 __global__ __launch_bounds__(64 * kWideWaves, 2) void mx4_wide_kernel(const Mx4ProjArgs a) {
   using X = XOperand<kX>;
-  using C = Wide4<MT, NT, kX>;
+  using C = Mx4Wide<MT, NT, kX>;
   constexpr int P = C::P, kChunk = C::kChunk, kRunSteps = C::kRunSteps, kChunkSteps = C::kChunkSteps;
   __shared__ u32x4 xs[C::kXSlots];
   __shared__ u32x4 wls[kWideWaves][C::kWave];
@@ -826,7 +858,7 @@ __global__ __launch_bounds__(64 * kWideWaves, 2) void mx4_wide_kernel(const Mx4P
 
 template <int MT, int NT, int kX>
 void launch_wide(const Mx4ProjArgs &a, hipStream_t stream) {
-  using C = Wide4<MT, NT, kX>;
+  using C = Mx4Wide<MT, NT, kX>;
   const int mtiles = (a.rows + C::kRows - 1) / C::kRows, groups = (a.out_dim + C::kOuts - 1) / C::kOuts;
   const int blocks = mtiles > 1 ? mtiles * groups : groups < a.cus ? groups : a.cus;
   // whole super-runs have no blocks to mask
