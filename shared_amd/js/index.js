@@ -807,7 +807,7 @@ class Sampler {
     if (fmt === 'mx4') {
       if (!(h.weight instanceof Mx4Table)) throw new TypeError('head.weight must be an Mx4Table');
       if (h.weight.dim !== dim) throw new RangeError('head.dim differs from the table\'s');
-      if (h.weight.rows < opts.vocab) throw new RangeError('head.weight holds fewer than vocab rows');
+      if (!(h.weight.rows >= opts.vocab)) throw new RangeError('head.weight holds fewer than vocab rows');
       Object.assign(hd, { weight: h.weight.codes.ptr, weightStride: h.weight.codesStride, scales: h.weight.scales.ptr,
         scalesStride: h.weight.scalesStride });
     } else {
@@ -1204,7 +1204,7 @@ class Sampler {
     const st = this._stepState(opts, r.packed, k);
     const next = this._scratch.stNext;
     for (let i = 0; i < k; i++) {
-      const hd = this._describeHead({ rows: opts.rows, head: Object.assign({}, opts.head, { hidden: opts.hidden(i, next) }) });
+      const hd = this._describeHead({ rows: opts.rows, vocab: opts.vocab, head: Object.assign({}, opts.head, { hidden: opts.hidden(i, next) }) });
       addon.lmHeadStep(this._handle(), r.desc, hd, st);
     }
     return this._stepResults(opts, r.packed, k);
@@ -1223,7 +1223,7 @@ class Sampler {
       let chain = Promise.resolve();
       for (let i = 0; i < k; i++) {
         chain = chain.then(function () { return opts.hidden(i, next); }).then(function (h) {
-          const hd = self._describeHead({ rows: opts.rows, head: Object.assign({}, opts.head, { hidden: h }) });
+          const hd = self._describeHead({ rows: opts.rows, vocab: opts.vocab, head: Object.assign({}, opts.head, { hidden: h }) });
           return self._worker(addon.lmHeadStepAsync(self._handle(), r.desc, hd, st));
         });
       }

@@ -37,6 +37,11 @@ try {
   const r = s.lmHeadSample({ rows: m.rows, vocab: m.vocab, params: { temperature: 0.9, topK: 40, topP: 0.95 }, uniforms: uniforms,
     head: { hidden: x, weight: head, dim: m.dim, format: 'mx4' } });
   write('ids.out', r.ids);
+  const steps = function (vocab) {
+    return s.decodeStepsWithHead({ rows: m.rows, vocab: vocab, k: 2, params: { temperature: 0 }, hidden: function () { return x; },
+      head: { weight: head, dim: m.dim, format: 'mx4' } });
+  };
+  write('greedy.out', Uint32Array.from(steps(m.vocab).map(function (row) { return row.ids[1]; })));
   let refused = 0;
   for (const f of [
     function () { s.quantizeMx4({ x: x, xType: 'f64', rows: 1, dim: 8 }); },
@@ -50,10 +55,11 @@ try {
     function () { s.projectMx4({ x: x, rows: m.rows, weight: head, out: s.alloc(16) }); },
     function () { s.lmHeadSample({ rows: 1, vocab: m.vocab, params: {}, head: { hidden: x, weight: logits, dim: m.dim, format: 'mx4' } }); },
     function () { s.lmHeadSample({ rows: 1, vocab: m.vocab + 1, params: {}, head: { hidden: x, weight: head, dim: m.dim, format: 'mx4' } }); },
+    function () { steps(m.vocab + 1); },
   ]) {
     try { f(); } catch (e) { refused++; }
   }
-  if (refused !== 11) throw new Error('refusals: ' + refused);
+  if (refused !== 12) throw new Error('refusals: ' + refused);
   console.log('[node] mx4 done');
 } finally {
   s.close();

@@ -42,3 +42,4 @@ def test_node_mx4(tmp_path, sampler):
     assert np.array_equal(f32("rows.f32", n, dim), sampler.lookup_mx4(head, dev(ids.view(np.int32))).cpu().numpy())
     got = sampler.lm_head_sample(dev(x), head, uniforms=dev(u), params=Params(temperature=0.9, top_k=40, top_p=0.95))
     assert np.array_equal(np.fromfile(tmp_path / "ids.out", np.int32), got.cpu().numpy())
+    assert np.array_equal(np.fromfile(tmp_path / "greedy.out", np.int32), sampler.lm_head_sample(dev(x), head, params=Params()).cpu().numpy())
