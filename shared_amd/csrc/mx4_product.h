@@ -217,8 +217,16 @@ __device__ __forceinline__ void put_rows(const Mx4ProjArgs &a, int row0, int n0,
         if (k < left) v[k] += a.out_bf16 ? __uint_as_float((uint32_t)ob[k] << 16) : of[k];
     }
     if (a.softcap > 0.0f) {
+      const f32x4 u = v * inv;
+      // (logits lie far below the cap as a rule: then half of tanh is all of it)
+      // (of NaN it is NaN)
+      if (__any(fmaxf(fmaxf(fabsf(u[0]), fabsf(u[1])), fmaxf(fabsf(u[2]), fabsf(u[3]))) >= 0.625f)) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = a.softcap * tanh_fast(v[k] * inv);
+        for (int k = 0; k < 4; ++k) v[k] = a.softcap * tanh_fast(u[k]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = a.softcap * tanh_small(u[k]);
+      }
     }
     // (nontemporal: the result is not read here)
     if (a.out_bf16) {

@@ -64,14 +64,17 @@ __device__ __forceinline__ void split8(const float *src, u32x4 (&p)[3]) {
 // Functions, 1980): below a split, here 0.625, x + x^3 P(x^2), P fitted to the
 // relative error (8.6e-9 at most), above it 1 - 2 / (e^2|x| + 1).  A third of
 // tanhf's instructions: 34 million capped values took 30 us of a call's 440.
-__device__ __forceinline__ float tanh_fast(float x) {
-  const float ax = fabsf(x), u = x * x;
+__device__ __forceinline__ float tanh_small(float x) {  // below the split
+  const float u = x * x;
   float p = -0.005704975221306086f;
   p = __builtin_fmaf(p, u, 0.020639074966311455f);
   p = __builtin_fmaf(p, u, -0.05373971164226532f);
   p = __builtin_fmaf(p, u, 0.13331441581249237f);
   p = __builtin_fmaf(p, u, -0.3333328068256378f);
-  const float small = __builtin_fmaf(x * u, p, x);
+  return __builtin_fmaf(x * u, p, x);
+}
+__device__ __forceinline__ float tanh_fast(float x) {
+  const float ax = fabsf(x), small = tanh_small(x);
   const float e = __builtin_amdgcn_exp2f(fminf(ax, 16.0f) * 2.8853900817779268f);  // e^2|x|
   const float large = copysignf(__builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(e + 1.0f), 1.0f), x);
   return x != x ? x : ax < 0.625f ? small : large;
