@@ -6,6 +6,8 @@
 // half) and a byte s, the block's scale 2^(s - 127); 255 is NaN.  Quantisation
 // rounds x / 2^(s - 127), which is exact, once.  The products are in
 // mx4_product.h; here is which kernel takes a call.
+#include <algorithm>
+
 #include "mx4_product.h"
 
 namespace sas {
@@ -50,38 +52,39 @@ template <int kType, bool kWide>
 __global__ __launch_bounds__(kThreads) void mx4_quantize_kernel(const Mx4QuantizeArgs a) {
   const int e = threadIdx.x & 15;
   const uint32_t units = (uint32_t)a.rows * (uint32_t)a.row_units;
-  const uint32_t u = blockIdx.x * (kThreads / 16) + (threadIdx.x >> 4);
-  if (u >= units) return;  // (16 lanes together)
-  const uint32_t row = u / (uint32_t)a.row_units, k = (u - row * (uint32_t)a.row_units) * kUnit + 8 * e;
-  float v[8];
-  const int left = a.dim - (int)k;
-  const int64_t size = kType == SAS_TYPE_F32 ? 4 : 2;
-  load8<kType, kWide>(static_cast<const char *>(a.x) + (int64_t)row * a.x_stride * size, k, left, v);
-  // the largest magnitude's bits order as it does, NaN above infinity
-  uint32_t top = 0;
+  // (16 lanes together)
+  for (uint32_t u = blockIdx.x * (kThreads / 16) + (threadIdx.x >> 4); u < units; u += gridDim.x * (kThreads / 16)) {
+    const uint32_t row = u / (uint32_t)a.row_units, k = (u - row * (uint32_t)a.row_units) * kUnit + 8 * e;
+    float v[8];
+    const int left = a.dim - (int)k;
+    const int64_t size = kType == SAS_TYPE_F32 ? 4 : 2;
+    load8<kType, kWide>(static_cast<const char *>(a.x) + (int64_t)row * a.x_stride * size, k, left, v);
+    // the largest magnitude's bits order as it does, NaN above infinity
+    uint32_t top = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-  top = max(top, dppx<kDppQuad1032>(top));
-  top = max(top, dppx<kDppQuad2301>(top));
-  const bool finite = top < 0x7F800000u;
-  // 2^(s - 127) = 2^(floor(log2 top) - 2), at least 2^-127
-  const uint32_t s = finite ? (uint32_t)max((int)(top >> 23) - 2, 0) : 255u;
-  // x / 2^(s - 127) is exact, below 8; the conversion rounds it to the nearest
-  // element, ties to the even one, and stops at 6
-  const float by = __uint_as_float((254u - (finite ? s : 127u)) << 23);
-  uint32_t c = 0;
-  each_const<4>([&](auto it) __attribute__((always_inline)) {
-    constexpr int i = decltype(it)::value;
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[2 * i] * by, v[2 * i + 1] * by, 1.0f, i);
-  });
-  if (!finite) c = 0;
-  // (a block that the row has no value of is left alone)
-  const int b = (int)k / kBlock, blocks = (a.dim + kBlock - 1) / kBlock;
-  if (b < blocks) *reinterpret_cast<uint32_t *>(a.codes + (int64_t)row * a.codes_stride + k / 2) = c;
-  uint32_t four = (b < blocks ? s : 0u) << (8 * (e >> 2));
-  four |= dppx<kDppRowRor4>(four);
-  four |= dppx<kDppRowRor8>(four);
-  if (e == 0) *reinterpret_cast<uint32_t *>(a.scales + (int64_t)row * a.scales_stride + k / kBlock) = four;
+    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+    top = max(top, dppx<kDppQuad1032>(top));
+    top = max(top, dppx<kDppQuad2301>(top));
+    const bool finite = top < 0x7F800000u;
+    // 2^(s - 127) = 2^(floor(log2 top) - 2), at least 2^-127
+    const uint32_t s = finite ? (uint32_t)max((int)(top >> 23) - 2, 0) : 255u;
+    // x / 2^(s - 127) is exact, below 8; the conversion rounds it to the nearest
+    // element, ties to the even one, and stops at 6
+    const float by = __uint_as_float((254u - (finite ? s : 127u)) << 23);
+    uint32_t c = 0;
+    each_const<4>([&](auto it) __attribute__((always_inline)) {
+      constexpr int i = decltype(it)::value;
+      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[2 * i] * by, v[2 * i + 1] * by, 1.0f, i);
+    });
+    if (!finite) c = 0;
+    // (a block that the row has no value of is left alone)
+    const int b = (int)k / kBlock, blocks = (a.dim + kBlock - 1) / kBlock;
+    if (b < blocks) *reinterpret_cast<uint32_t *>(a.codes + (int64_t)row * a.codes_stride + k / 2) = c;
+    uint32_t four = (b < blocks ? s : 0u) << (8 * (e >> 2));
+    four |= dppx<kDppRowRor4>(four);
+    four |= dppx<kDppRowRor8>(four);
+    if (e == 0) *reinterpret_cast<uint32_t *>(a.scales + (int64_t)row * a.scales_stride + k / kBlock) = four;
+  }
 }
 
 // Units of 4 blocks, a lane 16 bytes of the result, so that a wave's store is whole
@@ -94,48 +97,48 @@ __global__ __launch_bounds__(kThreads) void mx4_lookup_kernel(const Mx4LookupArg
   constexpr int V = kLookup<kType>, kLanes = kUnit / V;
   const int e = threadIdx.x % kLanes;
   const uint32_t units = (uint32_t)a.rows * (uint32_t)a.row_units;
-  const uint32_t u = blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;
-  if (u >= units) return;
-  const uint32_t row = u / (uint32_t)a.row_units, k = (u - row * (uint32_t)a.row_units) * kUnit + V * e;
-  const int left = a.dim - (int)k;
-  if (left <= 0) return;
-  const uint32_t id = a.ids ? a.ids[row] : row;
-  const bool in = id < (uint32_t)a.table_rows;
-  const uint8_t *at4 = a.codes + (int64_t)id * a.codes_stride + k / 2;
-  uint32_t c = 0u;
-  if (in) c = V == 8 ? *reinterpret_cast<const uint32_t *>(at4) : *reinterpret_cast<const uint16_t *>(at4);
-  const float by = scale_of(in ? a.scales[(int64_t)id * a.scales_stride + k / kBlock] : 127u);
-  float v[V];
-  each_const<V / 2>([&](auto it) __attribute__((always_inline)) {
-    constexpr int i = decltype(it)::value;
-    const f32x2 p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, by, i);
-    v[2 * i] = p[0];
-    v[2 * i + 1] = p[1];
-  });
-  const int64_t at = (int64_t)row * a.out_stride + k;
-  if constexpr (kType == SAS_TYPE_F32) {
-    float *o = static_cast<float *>(a.out) + at;
-    if (kWide && left >= V) {
-      __builtin_nontemporal_store(f32x4{v[0], v[1], v[2], v[3]}, reinterpret_cast<f32x4 *>(o));
+  for (uint32_t u = blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes; u < units; u += gridDim.x * (kThreads / kLanes)) {
+    const uint32_t row = u / (uint32_t)a.row_units, k = (u - row * (uint32_t)a.row_units) * kUnit + V * e;
+    const int left = a.dim - (int)k;
+    if (left <= 0) continue;
+    const uint32_t id = a.ids ? a.ids[row] : row;
+    const bool in = id < (uint32_t)a.table_rows;
+    const uint8_t *at4 = a.codes + (int64_t)id * a.codes_stride + k / 2;
+    uint32_t c = 0u;
+    if (in) c = V == 8 ? *reinterpret_cast<const uint32_t *>(at4) : *reinterpret_cast<const uint16_t *>(at4);
+    const float by = scale_of(in ? a.scales[(int64_t)id * a.scales_stride + k / kBlock] : 127u);
+    float v[V];
+    each_const<V / 2>([&](auto it) __attribute__((always_inline)) {
+      constexpr int i = decltype(it)::value;
+      const f32x2 p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, by, i);
+      v[2 * i] = p[0];
+      v[2 * i + 1] = p[1];
+    });
+    const int64_t at = (int64_t)row * a.out_stride + k;
+    if constexpr (kType == SAS_TYPE_F32) {
+      float *o = static_cast<float *>(a.out) + at;
+      if (kWide && left >= V) {
+        __builtin_nontemporal_store(f32x4{v[0], v[1], v[2], v[3]}, reinterpret_cast<f32x4 *>(o));
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          if (i < left) o[i] = v[i];
+      }
     } else {
+      uint16_t *o = static_cast<uint16_t *>(a.out) + at;
+      uint16_t h[V];
 #pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (i < left) o[i] = v[i];
-    }
-  } else {
-    uint16_t *o = static_cast<uint16_t *>(a.out) + at;
-    uint16_t h[V];
+      for (int i = 0; i < V; ++i) h[i] = kType == SAS_TYPE_BF16 ? bf16_of(v[i]) : __builtin_bit_cast(uint16_t, (_Float16)v[i]);
+      if (kWide && left >= V) {
+        u32x4 p;
 #pragma unroll
-    for (int i = 0; i < V; ++i) h[i] = kType == SAS_TYPE_BF16 ? bf16_of(v[i]) : __builtin_bit_cast(uint16_t, (_Float16)v[i]);
-    if (kWide && left >= V) {
-      u32x4 p;
+        for (int i = 0; i < 4; ++i) p[i] = (uint32_t)h[2 * i] | ((uint32_t)h[2 * i + 1] << 16);
+        __builtin_nontemporal_store(p, reinterpret_cast<u32x4 *>(o));
+      } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) p[i] = (uint32_t)h[2 * i] | ((uint32_t)h[2 * i + 1] << 16);
-      __builtin_nontemporal_store(p, reinterpret_cast<u32x4 *>(o));
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (i < left) o[i] = h[i];
+        for (int i = 0; i < V; ++i)
+          if (i < left) o[i] = h[i];
+      }
     }
   }
 }
@@ -201,6 +204,10 @@ void launch_lookup_of(const Mx4LookupArgs &a, bool wide, unsigned blocks, hipStr
   else mx4_lookup_kernel<kType, false><<<blocks, kThreads, 0, stream>>>(a);
 }
 
+// Blocks for `units` of them, `per` a block: a launch holds fewer than 2^32
+// threads, so that past 2^22 blocks they go round.
+unsigned unit_blocks(int64_t units, int per) { return (unsigned)std::min<int64_t>((units + per - 1) / per, 1 << 22); }
+
 // Whether rows may be read or written in 16-byte pieces.
 bool in_pieces(const void *p, int64_t stride, int type) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % (type == SAS_TYPE_F32 ? 4 : 8) == 0;
@@ -211,7 +218,7 @@ bool in_pieces(const void *p, int64_t stride, int type) {
 hipError_t launch_mx4_quantize(const Mx4QuantizeArgs &in, hipStream_t stream) {
   Mx4QuantizeArgs a = in;
   a.row_units = (a.dim + kUnit - 1) / kUnit;
-  const unsigned blocks = (unsigned)(((int64_t)a.rows * a.row_units + kThreads / 16 - 1) / (kThreads / 16));
+  const unsigned blocks = unit_blocks((int64_t)a.rows * a.row_units, kThreads / 16);
   const bool wide = in_pieces(a.x, a.x_stride, a.x_type);
   if (a.x_type == SAS_TYPE_F32) launch_quantize_of<SAS_TYPE_F32>(a, wide, blocks, stream);
   else if (a.x_type == SAS_TYPE_BF16) launch_quantize_of<SAS_TYPE_BF16>(a, wide, blocks, stream);
@@ -223,7 +230,7 @@ hipError_t launch_mx4_lookup(const Mx4LookupArgs &in, hipStream_t stream) {
   Mx4LookupArgs a = in;
   a.row_units = (a.dim + kUnit - 1) / kUnit;
   const int per = kThreads / (a.out_type == SAS_TYPE_F32 ? kUnit / kLookup<SAS_TYPE_F32> : kUnit / kLookup<SAS_TYPE_BF16>);
-  const unsigned blocks = (unsigned)(((int64_t)a.rows * a.row_units + per - 1) / per);
+  const unsigned blocks = unit_blocks((int64_t)a.rows * a.row_units, per);
   const bool wide = in_pieces(a.out, a.out_stride, a.out_type);
   if (a.out_type == SAS_TYPE_F32) launch_lookup_of<SAS_TYPE_F32>(a, wide, blocks, stream);
   else if (a.out_type == SAS_TYPE_BF16) launch_lookup_of<SAS_TYPE_BF16>(a, wide, blocks, stream);

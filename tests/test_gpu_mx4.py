@@ -583,6 +583,23 @@ def test_offsets_past_32_bits(sampler):
     assert not q.codes[:-3].any() and not q.scales[:-3].any()
 
 
+def test_more_rows_than_a_launch_has_threads_for(sampler):
+    """2^28 rows and more of one value: 16 lanes each would be 2^32 threads."""
+    import torch
+    rows = (1 << 28) + 77
+    x = torch.zeros((rows, 1), dtype=torch.bfloat16, device="cuda")
+    x[0], x[-1], x[rows // 2], x[1 << 26] = 3.0, -0.75, 5.0, 1.5
+    q = sampler.quantize_mx4(x)
+    out = torch.full_like(x, 7.0)
+    sampler.lookup_mx4_into(q, out)
+    want = sampler.lookup_mx4(sampler.quantize_mx4(x[rows // 2:rows // 2 + 1]), out_dtype=torch.bfloat16)
+    x[rows // 2] = want[0]
+    assert torch.equal(out, x)
+    f32 = torch.full((rows, 1), 7.0, device="cuda")
+    sampler.lookup_mx4_into(q, f32)
+    assert torch.equal(f32, x.float())
+
+
 @pytest.mark.parametrize("rows", [3, 20, 50])
 def test_rows_far_apart(sampler, rows):
     """Strides that pass the kernels' 32-bit offsets within a tile."""
