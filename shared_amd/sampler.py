@@ -486,13 +486,13 @@ class Sampler:
         return out if full else out["ids"]
 
     @staticmethod
-    def _head(hidden, weight, dim, out_logits, fmt, vocab):
+    def _head(hidden, weight, dim, out_logits, fmt, vocab=None):
         if hidden.dtype.itemsize != 4 or hidden.stride(1) != 1:
             raise ValueError("hidden must be fp32 with unit element stride")
         if isinstance(weight, Mx4):
             if fmt not in (_capi.HEAD_BF16, _capi.HEAD_MX4):
                 raise ValueError("an Mx4 weight has the format HEAD_MX4")
-            if vocab > weight.shape[0]:
+            if vocab is not None and vocab > weight.shape[0]:
                 raise ValueError("vocab exceeds the head's rows")
             c = weight.to_c()
             h = SasLmHead()
