@@ -46,7 +46,7 @@ __device__ __forceinline__ void load8(const void *row, int64_t k, int left, floa
 }
 
 // Units of 4 blocks, 16 lanes each, a lane 8 values: a block's largest magnitude
-// is two exchanges among four lanes.  Bound by memory: 262,144 x 2,560 bf16 286 us
+// is two exchanges among four lanes.  Bound by memory: 262,144 x 2,560 bf16 290 us
 // (5.9 TB/s of what it reads and writes), 2,048 x 4,096 5.9 us.
 template <int kType, bool kWide>
 __global__ __launch_bounds__(kThreads) void mx4_quantize_kernel(const Mx4QuantizeArgs a) {
@@ -145,9 +145,10 @@ __global__ __launch_bounds__(kThreads) void mx4_lookup_kernel(const Mx4LookupArg
 
 // The outputs a wave of the wide kernel takes, in 16s: the fewest rounds of blocks,
 // a round counted as its products and half of 16 outputs more.  One / two of
-// them, us: bf16, 64 rows x 4,096 x 32,768 (one round either way) 27 / 36; 32 x
-// 4,096 x 65,536 (two rounds, one) 34 / 31; 128 x 2,560 x 262,144 227 / 175; f32,
-// 16 x 2,560 x 151,936 65 / 69, three 64.
+// them, us: bf16, 64 rows x 4,096 x 32,768 (one round either way) 25 / 36; 32 x
+// 4,096 x 65,536 (two rounds, one) 33 / 30; 128 x 2,560 x 262,144 191 / 161; f32,
+// one / two / three, 16 x 2,560 x 32,000 17 / 24 / 31, x 128,256 52 / 47 / 63,
+// x 151,936 63 / 65 / 63; 12 x 2,048 x 200,000 67 / 66 / 70.
 int wide_nt(const Mx4ProjArgs &a, int mt, int most) {
   int best = 1;
   int64_t cost = INT64_MAX;

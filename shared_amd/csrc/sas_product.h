@@ -64,7 +64,8 @@ __device__ __forceinline__ void split8(const float *src, u32x4 (&p)[3]) {
 // Functions, 1980): below a split, here 0.625, x + x^3 P(x^2), P fitted to the
 // relative error (8.6e-9 at most), above it 1 - 2 / (e^2|x| + 1).  A third of
 // tanhf's instructions: 34 million capped values took 30 us of a call's 440.
-__device__ __forceinline__ float tanh_small(float x) {  // below the split
+// The part below the split:
+__device__ __forceinline__ float tanh_small(float x) {
   const float u = x * x;
   float p = -0.005704975221306086f;
   p = __builtin_fmaf(p, u, 0.020639074966311455f);
