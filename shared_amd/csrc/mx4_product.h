@@ -427,7 +427,9 @@ __global__ __launch_bounds__(64 * kSplitWaves, 2) void mx4_split_kernel(const Mx
         }
       }
       if constexpr (decltype(part_of)::value == 0) {
-        const uint32_t mask = scale_mask_of(g4, blocks);
+        // (of the wave's own runs: behind them are the last one's codes again, and
+        // under another block's scale they may pass bf16's range, times 0 NaN)
+        const uint32_t mask = scale_mask_of(g4, min(blocks, 4 * g1));
 #pragma unroll
         for (int t = 0; t < NT; ++t) ws[t] = pack_scales(ws[t], mask);
 #pragma unroll
