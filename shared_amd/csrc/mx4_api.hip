@@ -61,7 +61,7 @@ const char *check_mx4_projection(const sas_mx4_projection *p) {
   if (p->softcap < 0.0f || !std::isfinite(p->softcap)) return "softcap must be finite and >= 0";
   // (its reciprocal has to be finite)
   if (p->softcap > 0.0f && p->softcap < std::numeric_limits<float>::min()) return "softcap must be 0 or a normal number";
-  // (a block an output tile of 16 x 16 at most)
+  // (2^39 outputs are more than memory holds)
   if ((((int64_t)p->rows + 15) / 16) * (((int64_t)p->out_dim + 15) / 16) > INT32_MAX) return "rows * out_dim is too large";
   if (p->rows == 0) return nullptr;
   if (!p->out) return "out is required";

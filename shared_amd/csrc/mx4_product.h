@@ -487,13 +487,31 @@ __global__ __launch_bounds__(64 * kSplitWaves, 2) void mx4_split_kernel(const Mx
 // 4,096 11 / 7; MXFP4, 64 x 8,192 x 4,096 17 / 23, x 16,384 34 / 30.
 template <int MT, int NT>
 inline bool split_fits(const Mx4ProjArgs &a) {
-  return a.dim > 2 * kSuper && (int64_t)((a.rows + 16 * MT - 1) / (16 * MT)) * ((a.out_dim + 16 * NT - 1) / (16 * NT)) <= a.cus;
+  return a.dim > 2 * kSuper && (int64_t)((a.rows + 16 * MT - 1) / (16 * MT)) * (((int64_t)a.out_dim + 16 * NT - 1) / (16 * NT)) <= a.cus;
+}
+
+// A launch holds fewer than 2^32 threads, 512 a block here: launch(part, groups)
+// for parts of the outputs that take 2^22 blocks of `outs` of them at most.
+template <typename F>
+void in_parts(const Mx4ProjArgs &a, int mtiles, int outs, F launch) {
+  static_assert((SAS_MAX_PROJECT_ROWS + 15) / 16 <= 1 << 22, "a part of one block's outputs at least");
+  const int64_t most = (int64_t)((1 << 22) / mtiles) * outs;
+  for (int64_t n = 0; n < a.out_dim; n += most) {
+    Mx4ProjArgs part = a;
+    part.w += n * a.w_stride;
+    part.w_scales += n * a.w_scales_stride;
+    part.out = static_cast<char *>(a.out) + n * (a.out_bf16 ? 2 : 4);
+    part.out_dim = (int32_t)(a.out_dim - n < most ? a.out_dim - n : most);
+    launch(part, (part.out_dim + outs - 1) / outs);
+  }
 }
 
 template <int MT, int NT, int kX>
 void launch_split(const Mx4ProjArgs &a, hipStream_t stream) {
-  const int blocks = ((a.rows + 16 * MT - 1) / (16 * MT)) * ((a.out_dim + 16 * NT - 1) / (16 * NT));
-  mx4_split_kernel<MT, NT, kX><<<blocks, 64 * kSplitWaves, 0, stream>>>(a);
+  const int mtiles = (a.rows + 16 * MT - 1) / (16 * MT);
+  in_parts(a, mtiles, 16 * NT, [&](const Mx4ProjArgs &part, int groups) {
+    mx4_split_kernel<MT, NT, kX><<<mtiles * groups, 64 * kSplitWaves, 0, stream>>>(part);
+  });
 }
 
 // Few rows, hidden states that fit in LDS: every block holds all of them, and its
@@ -869,16 +887,18 @@ __global__ __launch_bounds__(64 * kWideWaves, 2) void mx4_wide_kernel(const Mx4P
 template <int MT, int NT, int kX>
 void launch_wide(const Mx4ProjArgs &a, hipStream_t stream) {
   using C = Mx4Wide<MT, NT, kX>;
-  const int mtiles = (a.rows + C::kRows - 1) / C::kRows, groups = (a.out_dim + C::kOuts - 1) / C::kOuts;
-  const int blocks = mtiles > 1 ? mtiles * groups : groups < a.cus ? groups : a.cus;
-  // whole super-runs have no blocks to mask
-  if (a.dim % kSuper == 0) {
-    if (mtiles == 1) mx4_wide_kernel<MT, NT, kX, true, false><<<blocks, 64 * kWideWaves, 0, stream>>>(a);
-    else mx4_wide_kernel<MT, NT, kX, false, false><<<blocks, 64 * kWideWaves, 0, stream>>>(a);
-  } else {
-    if (mtiles == 1) mx4_wide_kernel<MT, NT, kX, true, true><<<blocks, 64 * kWideWaves, 0, stream>>>(a);
-    else mx4_wide_kernel<MT, NT, kX, false, true><<<blocks, 64 * kWideWaves, 0, stream>>>(a);
-  }
+  const int mtiles = (a.rows + C::kRows - 1) / C::kRows;
+  in_parts(a, mtiles, C::kOuts, [&](const Mx4ProjArgs &part, int groups) {
+    const int blocks = mtiles > 1 ? mtiles * groups : groups < a.cus ? groups : a.cus;
+    // whole super-runs have no blocks to mask
+    if (a.dim % kSuper == 0) {
+      if (mtiles == 1) mx4_wide_kernel<MT, NT, kX, true, false><<<blocks, 64 * kWideWaves, 0, stream>>>(part);
+      else mx4_wide_kernel<MT, NT, kX, false, false><<<blocks, 64 * kWideWaves, 0, stream>>>(part);
+    } else {
+      if (mtiles == 1) mx4_wide_kernel<MT, NT, kX, true, true><<<blocks, 64 * kWideWaves, 0, stream>>>(part);
+      else mx4_wide_kernel<MT, NT, kX, false, true><<<blocks, 64 * kWideWaves, 0, stream>>>(part);
+    }
+  });
 }
 
 }  // namespace
