@@ -556,7 +556,7 @@ typedef struct sas_mx4_quantization {
  * stopped row's SAS_STOP_PAD, SAS_NO_TOKEN) gives zeros. */
 typedef struct sas_mx4_lookup {
   sas_mx4 table;
-  int32_t table_rows;         /* >= 0 */
+  int32_t table_rows;         /* >= 0 (0: table is not looked at) */
   int32_t dim;                /* >= 1 */
   const uint32_t *ids;        /* device [rows], or NULL: the rows in order */
   int32_t rows;               /* >= 0 (without ids <= table_rows); rows * ceil(dim / 128) below 2^31 */

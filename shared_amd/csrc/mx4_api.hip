@@ -46,6 +46,8 @@ const char *check_lookup(const sas_mx4_lookup *l) {
   if (!l->out) return "out is required";
   if (l->out_stride < l->dim) return "out_stride < dim";
   if (!aligned_to(l->out, l->out_type)) return "out must be aligned to its elements";
+  // (a table of no rows is never read: it may lie nowhere)
+  if (l->table_rows == 0) return nullptr;
   return check_mx4(l->table.codes, l->table.codes_stride, l->table.scales, l->table.scales_stride, l->dim);
 }
 

@@ -7,6 +7,16 @@ from test_gpu_mx4_scales import values
 pytestmark = pytest.mark.gpu
 
 
+@pytest.mark.parametrize("kind", ["float32", "bfloat16", "float16"])
+def test_lookup_in_a_table_of_no_rows(sampler, kind):
+    """Every id lies past it: zeros."""
+    import torch
+    ids = torch.tensor([0, -1, 5], dtype=torch.int32, device="cuda")
+    out = sampler.lookup_mx4(Mx4.empty(0, 100), ids, out_dtype=getattr(torch, kind))
+    assert out.shape == (3, 100) and not out.any()
+    assert sampler.lookup_mx4(Mx4.empty(0, 100)).shape == (0, 100)
+
+
 @pytest.mark.parametrize("rows,out,kind", [(1, (1 << 27) + 77, "bfloat16"), (3, (1 << 27) + 77, "mx4"), (20, (1 << 28) + 77, "bfloat16")])
 def test_more_outputs_than_a_launch_has_threads_for(sampler, rows, out, kind):
     """2^23 tiles of outputs and more, 512 threads each: 2^32.  Every 8 outputs in
