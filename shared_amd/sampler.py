@@ -100,7 +100,8 @@ class Mx4:
     """Rows of MXFP4 values (sas_mx4): codes, uint8 [rows][>= 16 ceil(dim / 32)],
     two values a byte, and scales, uint8 [rows][>= ceil(dim / 32)], a byte a block
     of 32, device tensors with unit element stride whose rows lie a multiple of
-    16 and of 4 bytes apart."""
+    16 and of 4 bytes apart.  (Scales are read four bytes at a time, those behind
+    a row's last block for nothing.)"""
 
     __slots__ = ("codes", "scales", "dim", "shape")
 
@@ -625,13 +626,17 @@ class Sampler:
 
     def quantize_mx4_into(self, x, out: Mx4, *, stream=None) -> None:
         """sas_quantize_mx4: rounds x [rows][dim] (float32, bfloat16 or float16)
-        into out's first rows."""
+        into out's first rows.  Scale bytes are written up to a multiple of four a
+        row, which out.scales has to hold."""
         size, kind = x.shape, _type_of(x)
         if len(size) != 2 or kind is None or x.stride(1) != 1 or not x.is_cuda:
             raise ValueError("x must be a 2-D float32, bfloat16 or float16 device tensor with unit element stride")
         rows, dim = size
         if out.shape[0] < rows or out.dim != dim:
             raise ValueError("out must hold x's rows of x's dim")
+        padded = (dim + 127) // 128 * 4
+        if out.scales.shape[1] < padded:
+            raise ValueError(f"out's scales must hold {padded} bytes a row, their padding included")
         # (a tensor of one row may have any stride; its row is the whole of it)
         d = SasMx4Quantization(x.data_ptr(), x.stride(0) if rows > 1 else dim, kind, rows, dim, out.to_c())
         check(self._lib.sas_quantize_mx4(self._h, ctypes.byref(d), _stream(stream)), self._h)

@@ -59,3 +59,26 @@ def test_reference_of_the_format():
     every = np.arange(16, dtype=np.uint8)
     v = R.values((every | every << 4)[None], np.array([[128]]), 32)
     assert v[0, ::2].tolist() == [0, 1, 2, 3, 4, 6, 8, 12, 0, -1, -2, -3, -4, -6, -8, -12]
+
+
+def test_quantisation_refuses_scales_without_their_padding():
+    """A row's scale bytes are written up to a multiple of four: a view that holds
+    fewer would have what lies beside it overwritten."""
+    import torch
+    from shared_amd import Sampler
+
+    class Device(torch.Tensor):
+        is_cuda = property(lambda self: True)
+
+    def dev(*shape, dtype=torch.uint8):
+        return torch.zeros(shape, dtype=dtype).as_subclass(Device)
+    s = Sampler.__new__(Sampler)
+    s._lib, s._h = _capi.load(), None
+    table = dev(10, 5)         # rows of 5 blocks, one behind another
+    for rows, scales in ((1, table[4:5]), (1, dev(1, 7)[:, :5]), (3, dev(3, 12)[:, :5])):
+        out = Mx4(dev(rows, 80), scales, 160)
+        with pytest.raises(ValueError, match="8 bytes a row"):
+            s.quantize_mx4_into(dev(rows, 160, dtype=torch.float32), out, stream=0)
+    # with the padding the call goes on to the library, which has no handle here
+    with pytest.raises(_capi.SasError, match="handle"):
+        s.quantize_mx4_into(dev(3, 160, dtype=torch.float32), Mx4(dev(3, 80), dev(3, 12)[:, :8], 160), stream=0)
