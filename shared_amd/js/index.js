@@ -419,7 +419,12 @@ class Mx4Table {
     this.codesStride = 16 * blocks;
     this.scalesStride = 4 * Math.ceil(blocks / 4);
     this.codes = sampler.alloc(Math.max(16, rows * this.codesStride));
-    this.scales = sampler.alloc(Math.max(16, rows * this.scalesStride));
+    try {
+      this.scales = sampler.alloc(Math.max(16, rows * this.scalesStride));
+    } catch (e) {
+      this.codes.free();
+      throw e;
+    }
   }
   _fields(prefix) {
     const f = {};
@@ -984,8 +989,13 @@ class Sampler {
     const fresh = opts.out === undefined || opts.out === null;
     const out = fresh ? this.allocMx4(opts.rows, opts.dim) : this._table(opts.out, 'out');
     if (out.dim !== opts.dim || out.rows < opts.rows) throw new RangeError('out must hold x\'s rows of x\'s dim');
-    addon.quantizeMx4(this._handle(), Object.assign({ x: x, xStride: opts.dim, xType: type.id, rows: opts.rows, dim: opts.dim },
-      out._fields('out')));
+    try {
+      addon.quantizeMx4(this._handle(), Object.assign({ x: x, xStride: opts.dim, xType: type.id, rows: opts.rows, dim: opts.dim },
+        out._fields('out')));
+    } catch (e) {
+      if (fresh) out.free();
+      throw e;
+    }
     return out;
   }
 
