@@ -810,7 +810,7 @@ class Sampler {
       throw new TypeError('head.hidden must be a DeviceBuffer or a Float32Array');
     }
     if (fmt === 'mx4') {
-      if (!(h.weight instanceof Mx4Table)) throw new TypeError('head.weight must be an Mx4Table');
+      this._table(h.weight, 'head.weight');
       if (h.weight.dim !== dim) throw new RangeError('head.dim differs from the table\'s');
       if (!(h.weight.rows >= opts.vocab)) throw new RangeError('head.weight holds fewer than vocab rows');
       Object.assign(hd, { weight: h.weight.codes.ptr, weightStride: h.weight.codesStride, scales: h.weight.scales.ptr,
@@ -961,6 +961,7 @@ class Sampler {
   // A DeviceBuffer's address, checked for its size.
   _room(b, name, bytes) {
     if (!(b instanceof DeviceBuffer)) throw new TypeError(name + ' must be a DeviceBuffer');
+    if (b.ptr === null) throw new TypeError(name + ' has been freed');
     if (!(b.bytes >= bytes)) throw new RangeError(name + ' holds fewer than its ' + bytes + ' bytes');
     return b.ptr;
   }
@@ -974,6 +975,7 @@ class Sampler {
 
   _table(t, name) {
     if (!(t instanceof Mx4Table)) throw new TypeError(name + ' must be an Mx4Table');
+    if (t.codes.ptr === null || t.scales.ptr === null) throw new TypeError(name + ' has been freed');
     return t;
   }
 
@@ -1027,6 +1029,7 @@ class Sampler {
       outStride: w.rows, outType: out.id, softcap: orDefault(opts.softcap, 0), accumulate: opts.accumulate ? 1 : 0 },
     w._fields('weight'));
     if (opts.x instanceof Mx4Table) {
+      this._table(opts.x, 'x');
       if (opts.x.dim !== w.dim || opts.x.rows < opts.rows) throw new RangeError('x must hold rows of the weight\'s dim');
       Object.assign(d, { xType: 3 }, opts.x._fields('x'));
     } else {

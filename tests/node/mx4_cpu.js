@@ -1,14 +1,14 @@
 'use strict';
 // CPU checks of the Node layer's MXFP4 calls (no GPU): a call that fails leaves no
-// memory behind.
+// memory behind, and freed buffers are refused.
 const assert = require('assert');
 const path = require('path');
 const sas = require(process.env.SAS_JS_DIR || path.join(__dirname, '..', '..', 'shared_amd', 'js'));
 
-function buffer(bytes) {
+function buffer(bytes, freed) {
   const b = Object.create(sas.DeviceBuffer.prototype);
   b.bytes = bytes;
-  b.ptr = 4096n;
+  b.ptr = freed ? null : 4096n;
   b.free = function () { this.ptr = null; };
   return b;
 }
@@ -44,4 +44,19 @@ const left = function (s) { return s.made.filter(function (b) { return b.ptr !==
   assert.throws(function () { s.quantizeMx4({ x: buffer(1024), rows: 4, dim: 64, out: out }); });
   assert.strictEqual(left(s), 2);
   console.log('ok a quantisation that fails frees the table it made, and no other');
+}
+{
+  const s = fake(10), table = s.allocMx4(8, 64);
+  const freed = /freed/;
+  assert.throws(function () { s.lookupMx4({ table: table, ids: buffer(16, true), rows: 4, out: buffer(1024) }); }, freed);
+  assert.throws(function () { s.lookupMx4({ table: table, rows: 4, out: buffer(1024, true) }); }, freed);
+  assert.throws(function () { s.quantizeMx4({ x: buffer(1024, true), rows: 4, dim: 64 }); }, freed);
+  assert.throws(function () { s.projectMx4({ x: buffer(1024, true), rows: 4, weight: table, out: buffer(128) }); }, freed);
+  table.free();
+  assert.throws(function () { s.lookupMx4({ table: table, ids: buffer(16), rows: 4, out: buffer(1024) }); }, freed);
+  assert.throws(function () { s.projectMx4({ x: buffer(1024), rows: 4, weight: table, out: buffer(128) }); }, freed);
+  assert.throws(function () { s.projectMx4({ x: table, rows: 4, weight: s.allocMx4(8, 64), out: buffer(128) }); }, freed);
+  const head = { hidden: buffer(1024), weight: table, dim: 64, format: 'mx4' };
+  assert.throws(function () { s._describeHead({ rows: 1, vocab: 8, head: head }); }, freed);
+  console.log('ok freed buffers and tables are refused');
 }

@@ -15,4 +15,4 @@ def test_node_mx4_cpu():
         pytest.skip("the addon is not built")
     p = subprocess.run(["node", os.path.join(ROOT, "tests", "node", "mx4_cpu.js")], capture_output=True, text=True, timeout=60)
     assert p.returncode == 0, p.stdout + p.stderr
-    assert len([line for line in p.stdout.splitlines() if line.startswith("ok ")]) == 2
+    assert len([line for line in p.stdout.splitlines() if line.startswith("ok ")]) == 3
