@@ -46,6 +46,18 @@ def test_node_host_layer_under_asan_ubsan(built):
     assert p.stdout.rstrip().endswith("all ok")
 
 
+def test_a_changed_header_rebuilds_the_library():
+    """make -q answers 1 where a target would be made anew; -W takes the header as
+    changed."""
+    if shutil.which("make") is None:
+        pytest.skip("make is not installed")
+    root = os.path.dirname(os.path.dirname(HERE))
+    csrc = os.path.join(root, "shared_amd", "csrc")
+    for h in [os.path.join(csrc, h) for h in os.listdir(csrc) if h.endswith(".h")] + [os.path.join(root, "include", "shared_amd_sampler.h")]:
+        p = subprocess.run(["make", "-q", "-C", HERE, "-W", h, "_build/libsas_san.so"], stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+        assert p.returncode == 1, (h, p.stdout)
+
+
 @pytest.mark.gpu
 def test_c_abi_device_paths_under_asan_ubsan():
     """The driver built on the CPU side runs its device part here: one call
