@@ -540,7 +540,7 @@ static hipError_t launch_format(const LmhArgs &a, hipStream_t stream) {
 
 void launch_mx4_few(const Mx4ProjArgs &a, hipStream_t stream) {
   if (split_fits<1, 1>(a)) launch_split<1, 1, SAS_TYPE_F32>(a, stream);
-  else if (stream_fits<1, SAS_TYPE_F32, true>(a) && a.out_stride < kMaxOutStride) launch_stream<1, 1, SAS_TYPE_F32, true>(a, stream);
+  else if (stream_fits<1, SAS_TYPE_F32>(a) && a.out_stride < kMaxOutStride) launch_stream<1, 1, SAS_TYPE_F32>(a, stream);
   else launch_split<1, 2, SAS_TYPE_F32>(a, stream);
 }
 

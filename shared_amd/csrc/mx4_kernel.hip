@@ -170,7 +170,8 @@ void launch_products(const Mx4ProjArgs &a, hipStream_t stream) {
   const bool far = a.x_stride >= kMaxXStride || a.out_stride >= kMaxOutStride;
   if (a.rows <= 16) {
     if (far || split_fits<1, 1>(a)) return launch_split<1, 1, kX>(a, stream);
-    if (kX != SAS_TYPE_F32 && stream_fits<1, kX, false>(a)) return launch_stream<1, 1, kX, false>(a, stream);
+    if constexpr (kX != SAS_TYPE_F32)
+      if (stream_fits<1, kX>(a)) return launch_stream<1, 1, kX>(a, stream);
     switch (wide_nt(a, 1, 3)) {
       case 1: return launch_wide<1, 1, kX>(a, stream);
       case 2: return launch_wide<1, 2, kX>(a, stream);
@@ -180,12 +181,12 @@ void launch_products(const Mx4ProjArgs &a, hipStream_t stream) {
   if (a.rows <= 32) {
     if (far || split_fits<2, 2>(a)) return launch_split<2, 2, kX>(a, stream);
     if constexpr (kX == SAS_TYPE_MX4)
-      if (stream_fits<2, kX, false>(a)) return launch_stream<2, 1, kX, false>(a, stream);
+      if (stream_fits<2, kX>(a)) return launch_stream<2, 1, kX>(a, stream);
     return wide_nt(a, 2, 2) == 1 ? launch_wide<2, 1, kX>(a, stream) : launch_wide<2, 2, kX>(a, stream);
   }
   if (far || split_fits<4, 2>(a)) return launch_split<4, 2, kX>(a, stream);
   if constexpr (kX == SAS_TYPE_MX4)
-    if (a.rows <= 64 && stream_fits<4, kX, false>(a)) return launch_stream<4, 1, kX, false>(a, stream);
+    if (a.rows <= 64 && stream_fits<4, kX>(a)) return launch_stream<4, 1, kX>(a, stream);
   // (128 rows of f32 pieces do not fit in LDS)
   if (a.rows <= 64 || kX == SAS_TYPE_F32)
     return wide_nt(a, 4, 2) == 1 ? launch_wide<4, 1, kX>(a, stream) : launch_wide<4, 2, kX>(a, stream);

@@ -330,7 +330,7 @@ __device__ __forceinline__ int w_get(int j) {
 
 // Adds a run's products: c the tiles' blocks, ws their packed scales, x the run's
 // operands in LDS, get the lane's slots in one, xscale the subtiles' scales.
-template <int MT, int NT, int kX, int P, int kRunOf4>
+template <int MT, int NT, int kX, int kRunOf4>
 __device__ __forceinline__ void add_run(const u32x4 (&c)[NT], const uint32_t (&ws)[NT], const u32x4 *x, const int (&get)[4],
                                         const uint32_t *xscale, f32x4 (&acc)[MT][NT]) {
   constexpr int kSlots = XOperand<kX>::kSlots;
@@ -349,13 +349,11 @@ __device__ __forceinline__ void add_run(const u32x4 (&c)[NT], const uint32_t (&w
 #pragma unroll
       for (int t = 0; t < NT; ++t) wv[t] = widen(c[t][i], scale_byte<kRunOf4>(ws[t]));
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
+      for (int m = 0; m < MT; ++m) {
+        const u32x4 xv = x[m * kSlots + get[i]];
 #pragma unroll
-        for (int p = 0; p < P; ++p) {
-          const u32x4 xv = x[(P * m + p) * kSlots + get[i]];
-#pragma unroll
-          for (int t = 0; t < NT; ++t) acc[m][t] = mfma(wv[t], xv, acc[m][t]);
-        }
+        for (int t = 0; t < NT; ++t) acc[m][t] = mfma(wv[t], xv, acc[m][t]);
+      }
     }
   }
 }
@@ -517,25 +515,26 @@ void launch_split(const Mx4ProjArgs &a, hipStream_t stream) {
 // Few rows, hidden states that fit in LDS: every block holds all of them, and its
 // waves take 16 NT outputs after another, their weight rows two super-runs
 // ahead in registers; no barrier after the first.
-// kPack: up to kMx4Few rows of f32, whose pieces are rows of one operand (row r's
-// piece p is row kMx4Few p + r): a third of the products.
+// f32 hidden states are packed: up to kMx4Few rows, whose pieces are rows of one
+// operand (row r's piece p is row kMx4Few p + r): a third of the products.
 // (Twelve waves against eight: 16 bf16 rows x 2,560 x 151,936 42.9 / 44.8 us, a
 // head's row 59.8 / 60.6.)
 constexpr int kStreamWaves = 12;
 constexpr int kStreamSlots = 136 * 1024 / 16;
 
-template <int MT, int NT, int kX, bool kPack>
+template <int MT, int NT, int kX>
 __global__ __launch_bounds__(64 * kStreamWaves, 3) void mx4_stream_kernel(const Mx4ProjArgs a) {
   using X = XOperand<kX>;
-  constexpr int P = kPack ? 1 : X::kPieces, kSubs = MT * P;
+  constexpr bool kPack = kX == SAS_TYPE_F32;
+  static_assert(!kPack || MT == 1, "packed rows are one operand");
   // the hidden states (MX4: then their scales, [super-run][subtile][lane])
   __shared__ u32x4 xs[kStreamSlots];
   __shared__ u32x4 wls[kStreamWaves][NT * kWSlots];
   static_assert(kStage<NT> * 4 <= NT * kWSlots * 16, "the sums fit where the weight rows were");
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int r = lane & 15, q = lane >> 4;
+  const int r = lane & 15;
   const int blocks = (a.dim + kBlock - 1) / kBlock, supers = (blocks + 15) / 16, runs = 4 * supers;
-  uint32_t *xsc = reinterpret_cast<uint32_t *>(xs + runs * kSubs * X::kSlots);
+  uint32_t *xsc = reinterpret_cast<uint32_t *>(xs + runs * MT * X::kSlots);
   const int waves = (int)gridDim.x * kStreamWaves, gw = wave * (int)gridDim.x + (int)blockIdx.x;
   const int groups = (a.out_dim + 16 * NT - 1) / (16 * NT);
   const int total = gw < groups ? (groups - gw + waves - 1) / waves * supers : 0;
@@ -572,16 +571,13 @@ __global__ __launch_bounds__(64 * kStreamWaves, 3) void mx4_stream_kernel(const 
                                      (int64_t)x_within<kX>(at, size) * kXSize<kX>);
       u32x4 o[X::kPieces];
       x_pieces<kX>(p, at, size, o);
-#pragma unroll
-      for (int k = 0; k < X::kPieces; ++k) {
-        if constexpr (kPack) {
-          if (xr < kMx4Few) xs[run * X::kSlots + x_put<kX>(f, kMx4Few * k + xr)] = o[k];
-        } else {
-          xs[(run * kSubs + P * m + k) * X::kSlots + x_put<kX>(f, xr)] = o[k];
-        }
-      }
       if constexpr (kPack) {
+#pragma unroll
+        for (int k = 0; k < X::kPieces; ++k)
+          if (xr < kMx4Few) xs[run * X::kSlots + x_put<kX>(f, kMx4Few * k + xr)] = o[k];
         if (xr == kMx4Few) xs[run * X::kSlots + x_put<kX>(f, 15)] = u32x4{0u, 0u, 0u, 0u};
+      } else {
+        xs[(run * MT + m) * X::kSlots + x_put<kX>(f, xr)] = o[0];
       }
     }
     if constexpr (kX == SAS_TYPE_MX4) {
@@ -624,7 +620,7 @@ __global__ __launch_bounds__(64 * kStreamWaves, 3) void mx4_stream_kernel(const 
       u32x4 c[NT];
 #pragma unroll
       for (int t = 0; t < NT; ++t) c[t] = wl[kWSlots * t + w_get(j)];
-      add_run<MT, NT, kX, P, j>(c, ws, xs + (4 * s + j) * kSubs * X::kSlots, get, xsc + s * MT * 64 + lane, acc);
+      add_run<MT, NT, kX, j>(c, ws, xs + (4 * s + j) * MT * X::kSlots, get, xsc + s * MT * 64 + lane, acc);
     });
     if (++s == supers) {
       const int n0 = 16 * NT * g;
@@ -653,18 +649,17 @@ __global__ __launch_bounds__(64 * kStreamWaves, 3) void mx4_stream_kernel(const 
 }
 
 // Whether the stream kernel's LDS holds the hidden states.
-template <int MT, int kX, bool kPack>
+template <int MT, int kX>
 bool stream_fits(const Mx4ProjArgs &a) {
-  using X = XOperand<kX>;
   const int64_t supers = ((int64_t)a.dim + kSuper - 1) / kSuper;
-  return supers * MT * (4 * (kPack ? 1 : X::kPieces) * X::kSlots + (kX == SAS_TYPE_MX4 ? 16 : 0)) <= kStreamSlots;
+  return supers * MT * (4 * XOperand<kX>::kSlots + (kX == SAS_TYPE_MX4 ? 16 : 0)) <= kStreamSlots;
 }
 
-template <int MT, int NT, int kX, bool kPack>
+template <int MT, int NT, int kX>
 void launch_stream(const Mx4ProjArgs &a, hipStream_t stream) {
   const int groups = (a.out_dim + 16 * NT - 1) / (16 * NT);
   const int blocks = groups < a.cus ? groups : a.cus;
-  mx4_stream_kernel<MT, NT, kX, kPack><<<blocks, 64 * kStreamWaves, 0, stream>>>(a);
+  mx4_stream_kernel<MT, NT, kX><<<blocks, 64 * kStreamWaves, 0, stream>>>(a);
 }
 
 // Many outputs: eight waves share the hidden states of 16 MT rows and take 16 NT
@@ -884,20 +879,27 @@ __global__ __launch_bounds__(64 * kWideWaves, 2) void mx4_wide_kernel(const Mx4P
   }
 }
 
+// Whether calls with more rows than one tile's come here (launch_products).
+template <int MT, int kX>
+constexpr bool kManyTiles = MT == 8 || (MT == 4 && kX == SAS_TYPE_F32);
+
 template <int MT, int NT, int kX>
 void launch_wide(const Mx4ProjArgs &a, hipStream_t stream) {
   using C = Mx4Wide<MT, NT, kX>;
   const int mtiles = (a.rows + C::kRows - 1) / C::kRows;
   in_parts(a, mtiles, C::kOuts, [&](const Mx4ProjArgs &part, int groups) {
-    const int blocks = mtiles > 1 ? mtiles * groups : groups < a.cus ? groups : a.cus;
     // whole super-runs have no blocks to mask
-    if (a.dim % kSuper == 0) {
-      if (mtiles == 1) mx4_wide_kernel<MT, NT, kX, true, false><<<blocks, 64 * kWideWaves, 0, stream>>>(part);
-      else mx4_wide_kernel<MT, NT, kX, false, false><<<blocks, 64 * kWideWaves, 0, stream>>>(part);
-    } else {
-      if (mtiles == 1) mx4_wide_kernel<MT, NT, kX, true, true><<<blocks, 64 * kWideWaves, 0, stream>>>(part);
-      else mx4_wide_kernel<MT, NT, kX, false, true><<<blocks, 64 * kWideWaves, 0, stream>>>(part);
+    const bool whole = a.dim % kSuper == 0;
+    if constexpr (kManyTiles<MT, kX>) {
+      if (mtiles > 1) {
+        if (whole) mx4_wide_kernel<MT, NT, kX, false, false><<<mtiles * groups, 64 * kWideWaves, 0, stream>>>(part);
+        else mx4_wide_kernel<MT, NT, kX, false, true><<<mtiles * groups, 64 * kWideWaves, 0, stream>>>(part);
+        return;
+      }
     }
+    const int blocks = groups < a.cus ? groups : a.cus;
+    if (whole) mx4_wide_kernel<MT, NT, kX, true, false><<<blocks, 64 * kWideWaves, 0, stream>>>(part);
+    else mx4_wide_kernel<MT, NT, kX, true, true><<<blocks, 64 * kWideWaves, 0, stream>>>(part);
   });
 }
 
