@@ -93,6 +93,13 @@ static void null_handle_paths() {
   EXPECT(sas_verify(nullptr, &v, nullptr) == SAS_ERR_INVALID);
   sas_lm_head lh{};
   EXPECT(sas_lm_head_sample(nullptr, &lh, &r, nullptr) == SAS_ERR_INVALID);
+  sas_mx4_quantization mq{};
+  sas_mx4_lookup ml{};
+  sas_mx4_projection mp{};
+  EXPECT(sas_quantize_mx4(nullptr, &mq, nullptr) == SAS_ERR_INVALID && sas_quantize_mx4(nullptr, nullptr, nullptr) == SAS_ERR_INVALID);
+  EXPECT(sas_lookup_mx4(nullptr, &ml, nullptr) == SAS_ERR_INVALID && sas_lookup_mx4(nullptr, nullptr, nullptr) == SAS_ERR_INVALID);
+  EXPECT(sas_project_mx4(nullptr, &mp, nullptr) == SAS_ERR_INVALID && sas_project_mx4(nullptr, nullptr, nullptr) == SAS_ERR_INVALID);
+  EXPECT(last_error_has(nullptr, "sas_project_mx4: handle is NULL"));
   EXPECT(sas_reserve(nullptr, 1, 1) == SAS_ERR_INVALID);
   sas_reserve_desc rd{};
   rd.rows = 1;
@@ -399,6 +406,103 @@ static void device_paths(sas_sampler *s) {
     EXPECT(sas_free(s, q) == SAS_OK);
 }
 
+// The MXFP4 entries: small whole numbers, which survive quantisation, and the
+// refusals of each descriptor.
+static void mx4_paths(sas_sampler *s) {
+  const int rows = 3, out = 40, dim = 72, blocks = 3;
+  std::vector<float> w((size_t)out * dim), x((size_t)rows * dim);
+  for (size_t i = 0; i < w.size(); ++i) w[i] = (float)((int)(i * 7 % 5) - 2);
+  for (size_t i = 0; i < x.size(); ++i) x[i] = (float)((int)(i * 11 % 5) - 2);
+  float *dw = upload(s, w), *dx = upload(s, x);
+  void *codes = nullptr, *scales = nullptr, *y = nullptr, *back = nullptr;
+  EXPECT(sas_alloc(s, out * 16 * blocks, &codes) == SAS_OK && sas_alloc(s, out * 4, &scales) == SAS_OK);
+  EXPECT(sas_alloc(s, rows * out * 4, &y) == SAS_OK && sas_alloc(s, out * dim * 4, &back) == SAS_OK);
+  sas_mx4 t{};
+  t.codes = codes;
+  t.codes_stride = 16 * blocks;
+  t.scales = scales;
+  t.scales_stride = 4;
+  sas_mx4_quantization q{};
+  q.x = dw;
+  q.x_stride = dim;
+  q.x_type = SAS_TYPE_F32;
+  q.rows = out;
+  q.dim = dim;
+  q.out = t;
+  EXPECT(sas_quantize_mx4(s, &q, nullptr) == SAS_OK);
+  sas_mx4_lookup l{};
+  l.table = t;
+  l.table_rows = out;
+  l.dim = dim;
+  l.rows = out;
+  l.out = back;
+  l.out_stride = dim;
+  l.out_type = SAS_TYPE_F32;
+  EXPECT(sas_lookup_mx4(s, &l, nullptr) == SAS_OK);
+  sas_mx4_projection p{};
+  p.x = dx;
+  p.x_stride = dim;
+  p.x_type = SAS_TYPE_F32;
+  p.rows = rows;
+  p.weight = t;
+  p.dim = dim;
+  p.out_dim = out;
+  p.out = y;
+  p.out_stride = out;
+  p.out_type = SAS_TYPE_F32;
+  EXPECT(sas_project_mx4(s, &p, nullptr) == SAS_OK);
+  EXPECT(sas_synchronize(s, nullptr) == SAS_OK);
+  EXPECT(download(s, (float *)back, w.size()) == w);
+  const std::vector<float> got = download(s, (float *)y, (size_t)rows * out);
+  for (int r = 0; r < rows; ++r)
+    for (int n = 0; n < out; ++n) {
+      float sum = 0.0f;
+      for (int k = 0; k < dim; ++k) sum += x[(size_t)r * dim + k] * w[(size_t)n * dim + k];
+      EXPECT(got[(size_t)r * out + n] == sum);
+    }
+  auto bad_q = [&](auto change, const char *what) {
+    sas_mx4_quantization b = q;
+    change(b);
+    EXPECT(sas_quantize_mx4(s, &b, nullptr) == SAS_ERR_INVALID && last_error_has(s, what));
+  };
+  bad_q([](auto &b) { b.rows = -1; }, "rows");
+  bad_q([](auto &b) { b.dim = 0; }, "dim");
+  bad_q([](auto &b) { b.rows = INT32_MAX; b.dim = INT32_MAX; }, "too large");
+  bad_q([](auto &b) { b.x_type = SAS_TYPE_MX4; }, "x_type");
+  bad_q([](auto &b) { b.x = nullptr; }, "x is required");
+  bad_q([](auto &b) { b.x_stride = 71; }, "x_stride");
+  bad_q([](auto &b) { b.out.codes_stride = 40; }, "codes_stride");
+  bad_q([](auto &b) { b.out.scales_stride = SAS_MAX_MX4_STRIDE + 4; }, "scales_stride");
+  bad_q([](auto &b) { b.out.scales = nullptr; }, "scales are required");
+  auto bad_l = [&](auto change, const char *what) {
+    sas_mx4_lookup b = l;
+    change(b);
+    EXPECT(sas_lookup_mx4(s, &b, nullptr) == SAS_ERR_INVALID && last_error_has(s, what));
+  };
+  bad_l([](auto &b) { b.table_rows = -1; }, "table_rows");
+  bad_l([](auto &b) { b.rows = 41; }, "without ids");
+  bad_l([](auto &b) { b.out = nullptr; }, "out is required");
+  bad_l([](auto &b) { b.out_stride = 71; }, "out_stride");
+  bad_l([](auto &b) { b.out_type = 7; }, "out_type");
+  bad_l([](auto &b) { b.table.codes = nullptr; }, "codes");
+  auto bad_p = [&](auto change, const char *what) {
+    sas_mx4_projection b = p;
+    change(b);
+    EXPECT(sas_project_mx4(s, &b, nullptr) == SAS_ERR_INVALID && last_error_has(s, what));
+  };
+  bad_p([](auto &b) { b.rows = SAS_MAX_PROJECT_ROWS + 1; }, "SAS_MAX_PROJECT_ROWS");
+  bad_p([](auto &b) { b.rows = SAS_MAX_PROJECT_ROWS; b.out_dim = INT32_MAX; }, "too large");
+  bad_p([](auto &b) { b.dim = 68; }, "multiple of 8");
+  bad_p([](auto &b) { b.out_dim = 0; }, "out_dim");
+  bad_p([](auto &b) { b.softcap = -1.0f; }, "softcap");
+  bad_p([](auto &b) { b.softcap = 1e-40f; }, "normal");
+  bad_p([](auto &b) { b.x_type = SAS_TYPE_F16; }, "x_type");
+  bad_p([](auto &b) { b.out_stride = 39; }, "out_stride");
+  bad_p([](auto &b) { b.x_type = SAS_TYPE_MX4; }, "codes and scales");
+  bad_p([](auto &b) { b.weight.codes_stride = 16; }, "codes_stride");
+  for (void *m : {(void *)dw, (void *)dx, codes, scales, y, back}) EXPECT(sas_free(s, m) == SAS_OK);
+}
+
 int main() {
   host_helpers();
   std::printf("[host_check] host helpers done\n");
@@ -410,6 +514,7 @@ int main() {
     std::printf("[host_check] no HIP device (%s): device paths skipped\n", sas_last_error(nullptr));
   } else {
     device_paths(s);
+    mx4_paths(s);
     sas_destroy(s);
     std::printf("[host_check] device paths done\n");
   }
