@@ -413,8 +413,8 @@ int sas_spec_step(sas_sampler *s, const sas_spec_rows *r, const sas_spec_state *
 #define SAS_HEAD_Q4_0 2
 #define SAS_HEAD_Q6_K 3
 /* SAS_HEAD_MX4: the table of sas_mx4 below (codes and scales).  The logits are
- * sas_project_mx4's of f32 hidden states: every bit of them is kept, the sums
- * are f32 in an order of the kernel's own (fixed for a shape). */
+ * sas_project_mx4's of f32 hidden states: every bit of them from 2^-133 up is
+ * kept, the sums are f32 in an order of the kernel's own (fixed for a shape). */
 #define SAS_HEAD_MX4 4
 
 typedef struct sas_lm_head {
@@ -456,7 +456,8 @@ int sas_lm_head_sample_step(sas_sampler *s, const sas_lm_head *head, const sas_r
  * Adapter a uses the first ranks[a] of its `rank` rows of A and columns of B;
  * what lies behind them is never used, whatever it holds.  Products and sums
  * are f32: bf16 products are exact in f32, f32 hidden states and the inner
- * products A x (scaled) are carried as three bf16 pieces, 24 bits in all.
+ * products A x (scaled) are carried as three bf16 pieces, 24 bits in all (those
+ * below 2^-133 are cut off).
  * A value that is not finite stays in its own row, weight row or adapter; an
  * infinite weight that meets a piece of zero (f32 hidden states), or an infinite
  * element of B, makes NaN there.
@@ -567,10 +568,11 @@ typedef struct sas_mx4_lookup {
 } sas_mx4_lookup;
 
 /* y[r] = cap(W x[r]), W a table: with f32 hidden states (carried as three bf16
- * pieces, 24 bits in all), bf16, or rows of MXFP4 themselves.  Products are
- * exact, sums are f32.  accumulate, softcap and out are sas_project's, whose
- * adapters' terms can be added behind it (its weight NULL).  A value that is
- * not finite stays in its row or weight row. */
+ * pieces, 24 bits in all, those below 2^-133 cut off), bf16, or rows of MXFP4
+ * themselves.  Products of what is carried are exact, sums are f32.
+ * accumulate, softcap and out are sas_project's, whose adapters' terms can be
+ * added behind it (its weight NULL).  A value that is not finite stays in its
+ * row or weight row. */
 typedef struct sas_mx4_projection {
   const void *x;              /* SAS_TYPE_F32, _BF16: device [rows][x_stride], 16-byte aligned */
   int64_t x_stride;           /* elements between rows: >= dim, a multiple of 8 (f32: of 4) */

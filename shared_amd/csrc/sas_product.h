@@ -20,9 +20,9 @@ __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-// An f32 value as three bf16 pieces whose sum it is (values below 2^-110
-// lose bits that no product of theirs keeps).  Not finite: the first piece
-// alone.
+// An f32 value as three bf16 pieces whose sum it is, but for bits below 2^-133,
+// bf16's last, which are cut off (values under 2^-110 have such bits).  Not
+// finite: the first piece alone.
 __device__ __forceinline__ void pieces_of(float x, uint16_t (&p)[3]) {
   const uint32_t u = __float_as_uint(x);
   const bool finite = (u & 0x7F800000u) != 0x7F800000u;

@@ -81,3 +81,19 @@ def test_a_head_with_scales_near_the_top(sampler, rows, dim, vocab):
     want, size = x.double() @ weight.T, x.double().abs() @ weight.abs().T
     assert ((r["logits"].double() - want).abs() <= (3 * dim + 32) * 2.0 ** -23 * size).all()
     assert torch.equal(r["ids"].long(), r["logits"].argmax(1))
+
+
+@pytest.mark.parametrize("rows", [2, 20])
+def test_small_f32_hidden_states_keep_their_bits_down_to_bf16s_last(sampler, rows):
+    """A value alone in its sum, under a weight of 2^100: exact but for bits below
+    2^-133, which are cut off."""
+    import torch
+    codes = torch.zeros((40, 16), dtype=torch.uint8, device="cuda")
+    codes[:, 0] = 2                                                   # 1
+    w = Mx4(codes, torch.full((40, 4), 227, dtype=torch.uint8, device="cuda"), 32)
+    for e in range(-126, -99):
+        x = torch.zeros((rows, 32), device="cuda")
+        x[:, 0] = 2.0 ** e * (2 - 2.0 ** -23)
+        got = sampler.project_mx4(x, w).double()
+        want = torch.floor(x[0, 0].double() * 2.0 ** 133) * 2.0 ** -33
+        assert (got == want).all(), (e, float(got[0, 0]), float(want))
