@@ -538,6 +538,8 @@ static hipError_t launch_format(const LmhArgs &a, hipStream_t stream) {
   }
 }
 
+// (Past 4,096 values, which the stream kernel's LDS holds, the split kernel
+// whatever the outputs: right, and far from its floor, see there.)
 void launch_mx4_few(const Mx4ProjArgs &a, hipStream_t stream) {
   if (split_fits<1, 1>(a)) launch_split<1, 1, SAS_TYPE_F32>(a, stream);
   else if (stream_fits<1, SAS_TYPE_F32>(a) && a.out_stride < kMaxOutStride) launch_stream<1, 1, SAS_TYPE_F32>(a, stream);

@@ -46,8 +46,9 @@ __device__ __forceinline__ void load8(const void *row, int64_t k, int left, floa
 }
 
 // Units of 4 blocks, 16 lanes each, a lane 8 values: a block's largest magnitude
-// is two exchanges among four lanes.  Bound by memory: 262,144 x 2,560 bf16 290 us
-// (5.9 TB/s of what it reads and writes), 2,048 x 4,096 5.9 us.
+// is two exchanges among four lanes.  Bound by memory: 262,144 x 2,560 bf16 307 us
+// (5.5 TB/s of what it reads and writes), 2,048 x 4,096 6.3 us.  Rows off 16 bytes
+// load value by value: 262,144 x 2,559 746 us.
 template <int kType, bool kWide>
 __global__ __launch_bounds__(kThreads) void mx4_quantize_kernel(const Mx4QuantizeArgs a) {
   const int e = threadIdx.x & 15;
@@ -89,7 +90,8 @@ __global__ __launch_bounds__(kThreads) void mx4_quantize_kernel(const Mx4Quantiz
 
 // Units of 4 blocks, a lane 16 bytes of the result, so that a wave's store is whole
 // lines: nontemporal then (8,192 x 4,096 to bf16 21.0 -> 14.9 us, 5.7 TB/s; f32
-// in two stores of every second 16 bytes 18.2 -> 21.9 us).
+// in two stores of every second 16 bytes 18.2 -> 21.9 us).  Results off 16 bytes
+// are stored value by value: 262,144 x 2,560 bf16 354 us, x 2,559 889.
 template <int kType>
 constexpr int kLookup = kType == SAS_TYPE_F32 ? 4 : 8;  // values of a lane
 template <int kType, bool kWide>

@@ -11,15 +11,21 @@
 //
 // Three kernels:
 //   - mx4_split_kernel: few outputs.  Eight waves split dim, every load of a
-//     call in flight together (1 x 2,560 x 2,560 5.0 us).
+//     call in flight together (1 x 2,560 x 2,560 4.8 us).  Also up to five f32 rows
+//     of more than 4,096 values over wide outputs, far from their floor: one row x
+//     5,120 x 151,936 270 us (413 MB, 1.5 TB/s), x 8,192 288, x 12,288 427.  And rows
+//     further apart than the others' 32-bit offsets reach.
 //   - mx4_stream_kernel: few rows, hidden states that fit in LDS.  Bound by the
 //     weights' stream: one f32 row x 2,560 x 262,144 60 us (357 MB, 6.0 TB/s), 16
-//     bf16 rows x 151,936 42, 16 MXFP4 rows 39, 61 MXFP4 rows x 4,096 x 11,007 12.5.
-//   - mx4_wide_kernel: the rest.  2,048 x 4,096 x 4,096 bf16 58 us (1.19 PFLOP/s),
-//     8,192 x 4,096 x 11,008 607 (1.22), the same of MXFP4 289 (2.6): a wave reads
-//     all of a tile's hidden states from LDS, and waits for what it read; 128
-//     bf16 rows x 2,560 x 262,144 164 us (1.05 PFLOP/s; 129 without loads and
-//     results), 16 f32 rows x 151,936 66 (52).
+//     bf16 rows x 151,936 42, 16 MXFP4 rows 39, 61 MXFP4 rows x 4,096 x 11,007 12.7.
+//   - mx4_wide_kernel: the rest.  2,048 x 4,096 x 4,096 bf16 56 us (1.23 PFLOP/s),
+//     8,192 x 4,096 x 11,008 587 (1.26), the same of MXFP4 285 (2.6): a wave reads
+//     all of a tile's hidden states from LDS, and waits for what it read; f32, three
+//     products each, 2,048 x 4,096 x 4,096 161, 8,192 x 4,096 x 11,008 1,785; 128
+//     bf16 rows x 2,560 x 262,144, capped, 160 us (1.07 PFLOP/s; 129 without loads
+//     and results), 16 f32 rows x 151,936 63 (52).
+// (Calls queued one behind another; a launch alone under the profiler takes about
+// a tenth more, 61 MXFP4 rows 14.2 us.)
 // What carried them: weight rows in whole 128-byte lines, nontemporal (half lines
 // in the matrix layout: nontemporal 469 MB fetched for 357, 84 us for a head's
 // row; cached 66; whole lines through LDS 60); one tile of 16 rows at a time, so
@@ -479,8 +485,8 @@ __global__ __launch_bounds__(64 * kSplitWaves, 2) void mx4_split_kernel(const Mx
 // Few outputs: the split kernel, where it fills the chip once at most and dim is
 // more than two super-runs; then the waves of a block share dim, and all of a
 // call's loads are one latency.  The wide kernel's blocks walk along dim.  Over
-// 440 shapes (8 to 2,048 rows, 256 to 32,768 outputs of 512 to 8,192 values),
-// split / wide, us: bf16, 16 rows x 2,560 x 4,096 7 / 8, x 16,384 15 / 10; 128 x
+// 440 shapes (8 to 2,048 rows, 256 to 32,768 outputs of 512 to 8,192 values; up to
+// five f32 rows, which follow the same rule, were not among them), split / wide, us: bf16, 16 rows x 2,560 x 4,096 7 / 8, x 16,384 15 / 10; 128 x
 // 2,560 x 4,096 23 / 27, x 8,192 43 / 27; 128 x 8,192 x 4,096 41 / 76; 64 x 512 x
 // 4,096 11 / 7; MXFP4, 64 x 8,192 x 4,096 17 / 23, x 16,384 34 / 30.
 template <int MT, int NT>
