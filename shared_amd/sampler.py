@@ -635,7 +635,7 @@ class Sampler:
         if out.shape[0] < rows or out.dim != dim:
             raise ValueError("out must hold x's rows of x's dim")
         padded = (dim + 127) // 128 * 4
-        if out.scales.shape[1] < padded:
+        if rows and out.scales.shape[1] < padded:
             raise ValueError(f"out's scales must hold {padded} bytes a row, their padding included")
         # (a tensor of one row may have any stride; its row is the whole of it)
         d = SasMx4Quantization(x.data_ptr(), x.stride(0) if rows > 1 else dim, kind, rows, dim, out.to_c())

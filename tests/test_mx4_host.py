@@ -82,3 +82,17 @@ def test_quantisation_refuses_scales_without_their_padding():
     # with the padding the call goes on to the library, which has no handle here
     with pytest.raises(_capi.SasError, match="handle"):
         s.quantize_mx4_into(dev(3, 160, dtype=torch.float32), Mx4(dev(3, 80), dev(3, 12)[:, :8], 160), stream=0)
+
+
+def test_quantisation_of_no_rows_needs_no_padding():
+    import torch
+    from shared_amd import Sampler
+
+    class Device(torch.Tensor):
+        is_cuda = property(lambda self: True)
+    s = Sampler.__new__(Sampler)
+    s._lib, s._h = _capi.load(), None
+    u8 = lambda *shape: torch.zeros(shape, dtype=torch.uint8).as_subclass(Device)  # noqa: E731
+    # (it reaches the library, which has no handle here)
+    with pytest.raises(_capi.SasError, match="handle"):
+        s.quantize_mx4_into(torch.zeros((0, 160)).as_subclass(Device), Mx4(u8(2, 80), u8(2, 5), 160), stream=0)
